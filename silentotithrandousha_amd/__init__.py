@@ -5,7 +5,8 @@ The compute lives in libmxfp4moe.so (HIP kernels, built by __graft_entry__.build
 package is a thin host front end. Importing it does not need a GPU; creating a dispatcher
 does, and fails loudly without the library or a gfx950 device.
 """
-from ._ffi import LIB_PATH, MoeError, lib  # noqa: F401
+from ._ffi import (LIB_PATH, MOE_BF16, MOE_F32, MOE_MXFP8, GatedFfn, GatedFfnGrads, MoeError,  # noqa: F401
+                   lib)
 from .dispatcher import (DeviceBuffer, GpuMoeDispatcher, mxfp4_dequant, mxfp4_matvec,  # noqa: F401
                          mxfp4_pack, safetensors_find)
 from .beaver import GpuTripleGen32  # noqa: F401

@@ -9,8 +9,9 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmxfp4moe.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "mxfp4_moe.h")
-# every header of the library's C ABI: the MoE path and the Beaver-triple generator
-HEADER_PATHS = [HEADER_PATH, os.path.join(os.path.dirname(_HERE), "include", "beaver32.h")]
+# every header of the library's C ABI: the MoE path, the dense operators and the Beaver-triple generator
+HEADER_PATHS = [HEADER_PATH, os.path.join(os.path.dirname(_HERE), "include", "moe_dense.h"),
+                os.path.join(os.path.dirname(_HERE), "include", "beaver32.h")]
 
 MOE_OK = 0
 MOE_ERR_INVALID = 1
@@ -19,6 +20,10 @@ MOE_ERR_HIP = 3
 MOE_ERR_NO_DEVICE = 4
 MOE_ERR_OOM = 5
 MOE_ERR_IO = 6
+
+MOE_F32 = 0
+MOE_BF16 = 1
+MOE_MXFP8 = 2
 
 MOE_OPT_FUSED_DECODE = 1
 MOE_OPT_SPIN_LIMIT = 2
@@ -53,6 +58,16 @@ class ExpertRef(ctypes.Structure):
                 ("down_blocks", _vp), ("down_blocks_len", _sz),
                 ("down_scales", _vp), ("down_scales_len", _sz),
                 ("down_bias", _vp), ("down_bias_len", _sz)]
+
+
+class GatedFfn(ctypes.Structure):
+    """moe_ffn: the device pointers of a gated block's weights (biases may be None)."""
+    _fields_ = [("inter", _sz), ("gate_up", _vp), ("gate_up_bias", _vp), ("down", _vp), ("down_bias", _vp)]
+
+
+class GatedFfnGrads(ctypes.Structure):
+    """moe_ffn_grads: the device pointers that a gated block's gradients go to (None: not computed)."""
+    _fields_ = [("x", _vp), ("gate_up", _vp), ("gate_up_bias", _vp), ("down", _vp), ("down_bias", _vp)]
 
 
 # name -> (restype, argtypes)
@@ -111,6 +126,15 @@ SIGNATURES = {
     "moe_get_timing": (_int, [_vp, _int, ctypes.POINTER(ctypes.c_double),
                               ctypes.POINTER(ctypes.c_uint64)]),
     "moe_reset_timing": (_int, [_vp]),
+    # include/moe_dense.h
+    "moe_lm_head_loss_device": (_int, [_vp, _vp, _int, _vp, _sz, _sz, _vp, _vp, _vp]),
+    "moe_lm_head_loss_backward_device": (_int, [_vp, _vp, _int, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp]),
+    "moe_ffn_forward_device": (_int, [_vp, ctypes.POINTER(GatedFfn), _vp, _int, _sz, _vp, _vp, _vp]),
+    "moe_ffn_backward_device": (_int, [_vp, ctypes.POINTER(GatedFfn), _vp, _int, _vp, _int, _sz,
+                                       ctypes.POINTER(GatedFfnGrads), _vp]),
+    "moe_act8_bytes": (_sz, [_sz, _sz]),
+    "moe_act8_pack_device": (_int, [_vp, _vp, _int, _sz, _sz, _vp, _vp]),
+    "moe_act8_unpack_device": (_int, [_vp, _vp, _sz, _sz, _vp, _int, _vp]),
     # include/beaver32.h
     "beaver32_create": (_int, [_sz, _sz, ctypes.POINTER(_vp)]),
     "beaver32_destroy": (None, [_vp]),

@@ -1,0 +1,111 @@
+// Host interface of the dense operators' kernels (dense_gemm.hpp, dense.hip, act8.hip): bf16 matrix
+// products with the epilogues of the LM-head loss and of the gated feed-forward block.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <vector>
+
+namespace moe {
+
+// f32 values enter the bf16 MFMA as the sum of kPlanes bf16 values (8 significant bits each: the 24
+// of an f32 exactly, short of the subnormal range); bf16 values as one.
+constexpr int kPlanes = 3;
+constexpr int kMaxPass = 6;
+
+// Epilogues.
+enum DenseEpi {
+  DENSE_STORE = 0,   // out (+ bias) as f32 or bf16, or added to f32
+  DENSE_GATE = 1,    // rows of D are interleaved gate and up: h = act(gate, up) as bf16 planes
+  DENSE_GATE_RAW = 2,  // the same rows with their bias, as f32 (for the backward pass)
+  DENSE_DGATE = 3,   // D = dh: gate and up from DENSE_GATE_RAW give h, d(gate, up) and bias sums
+  DENSE_STATS = 4,   // D = logits: running maximum and sum of exponentials of each column's tile
+  DENSE_DLOGITS = 5  // D = logits: their gradient as bf16 planes
+};
+
+// D[m][n] = sum over passes and k of A_p[m][k] B_p[n][k], stored as [n][m] (m contiguous).
+// Layouts of an operand: K-contiguous ([rows][k], the fast case) or transposed ([k][rows]).
+// A K-contiguous operand is readable up to K rounded up to 8; a transposed one's rows up to M (N)
+// rounded up to 8.
+struct DenseArgs {
+  const uint16_t *A, *B;
+  size_t a_plane, b_plane;  // elements between planes
+  size_t lda, ldb;          // elements between rows of the stored matrix
+  int M, N, K;
+  int n_pass;
+  uint32_t pa, pb;          // planes of A and B of each pass, 4 bits each
+  int splits;               // K split (DENSE_STORE with f32 only): out + split * split_stride
+  int k_split;              // K per split, a multiple of 64
+  // DENSE_STORE
+  void *out;
+  size_t ldo, split_stride;
+  int out_mode;             // 0 bf16, 1 f32, 2 f32 added to
+  const float *bias;        // [M] or NULL
+  // gated block
+  float limit;
+  uint16_t *h;              // [planes][N][ldh] bf16
+  size_t h_plane, ldh;
+  float *gu;                // [N][M] (GATE_RAW), [N][2 M] (DGATE)
+  uint16_t *dgu;            // [planes][N][2 M]
+  size_t dgu_plane;
+  float *db_part;           // [parts][2 M] or NULL
+  int planes;
+  // loss
+  const int32_t *targets;   // [N], in the whole vocabulary
+  int v0;                   // first vocabulary row of D
+  float2 *stats;            // [parts][N]: maximum, sum of exp(l - maximum)
+  float *picked;            // [N] target logits
+  const float *lse, *dloss; // [N]
+  int vocab;                // rows of the whole vocabulary: targets at or above it are invalid
+  uint16_t *dl;             // [planes][N][ld_dl]
+  size_t dl_plane, ld_dl;
+};
+
+struct DenseShape {
+  bool at, bt;   // A / B transposed
+  DenseEpi epi;
+};
+int dense_parts(const DenseShape &s, const DenseArgs &a);  // parts of db_part / stats that a launch writes
+// K splits worth taking (none of them empty)
+int dense_splits(const DenseShape &s, const DenseArgs &a, int n_cu);
+int dense_split_count(const DenseArgs &a);  // the splits that a launch with a.splits makes (none of them empty)
+hipError_t launch_dense(const DenseShape &s, const DenseArgs &a, hipStream_t st);
+
+// x [n] f32 as kPlanes bf16 planes, `plane` elements apart.
+hipError_t launch_planes(const float *x, size_t n, uint16_t *out, size_t plane, hipStream_t s);
+// out[i] = sum over parts of part[p * stride + i] (+ bias[i % n_bias]) for i < n, in order; bf16 or f32.
+hipError_t launch_sum_parts(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias,
+                            void *out, bool bf16, hipStream_t s);
+// Column sums of x [T][H] (f32 or bf16) into parts [dense_colsum_parts(T)][H].
+int dense_colsum_parts(size_t T);
+hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *part, hipStream_t s);
+// loss and log-sum-exp of each token from the parts of DENSE_STATS.
+hipError_t launch_loss(const float2 *stats, int parts, const float *picked, const int32_t *targets, size_t T,
+                       int vocab, float *loss, float *lse, hipStream_t s);
+
+// MXFP8 activation checkpoints (act8.hip): codes [n][cols], then scales [n][cols / 32].
+hipError_t launch_act8_pack(const void *x, bool bf16, size_t n, size_t cols, uint8_t *packed, hipStream_t s);
+hipError_t launch_act8_unpack(const uint8_t *packed, size_t n, size_t cols, void *out, bool bf16, hipStream_t s);
+
+// Device workspace of the dense operators: grows at need; a buffer that a captured graph may hold is
+// kept until the context goes.
+struct DenseWork {
+  void *p = nullptr;
+  size_t cap = 0;
+  bool captured = false;  // used by a call under capture since it was allocated
+  std::vector<void *> kept;
+};
+
+// What the dense operators need of a context (moe_api.cpp).
+struct DenseCtx {
+  hipStream_t stream;  // the context's
+  size_t H;
+  float clamp;
+  const uint16_t *lm_w;  // bf16 LM head rows, NULL if none or f32
+  size_t lm_vocab;
+  int n_cu;
+  DenseWork *work;
+};
+
+}  // namespace moe

@@ -1,0 +1,512 @@
+// C ABI of the dense operators (include/moe_dense.h): checks, workspace, and the order of launches.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <initializer_list>
+
+#include "../../include/moe_dense.h"
+#include "dense.hpp"
+#include "kernels.hpp"
+
+namespace moe {
+int api_fail(int code, const char *msg);
+int dense_ctx(moe_ctx *c, DenseCtx *d);
+}  // namespace moe
+
+using namespace moe;
+
+namespace {
+
+int fail(int code, const char *fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return api_fail(code, buf);
+}
+
+#define HIP_TRY(call)                                                                          \
+  do {                                                                                         \
+    hipError_t e_ = (call);                                                                    \
+    if (e_ != hipSuccess)                                                                      \
+      return fail(e_ == hipErrorOutOfMemory ? MOE_ERR_OOM : MOE_ERR_HIP, "%s: %s (%s:%d)",     \
+                  #call, hipGetErrorString(e_), __FILE__, __LINE__);                           \
+  } while (0)
+
+#define RETURN_IF(rc)  \
+  do {                 \
+    int r_ = (rc);     \
+    if (r_) return r_; \
+  } while (0)
+
+constexpr size_t kMaxTokens = (size_t)1 << 20;  // tokens per call, as the path-level calls
+constexpr size_t kMaxInter = (size_t)1 << 20;
+
+size_t al(size_t v) { return (v + 255) / 256 * 256; }
+
+// Parts of the workspace: sized first (base NULL), then placed.
+struct Carve {
+  char *base = nullptr;
+  size_t off = 0;
+  template <class T>
+  T *take(size_t n) {
+    T *p = base ? (T *)(base + off) : nullptr;
+    off += al(n * sizeof(T));
+    return p;
+  }
+};
+
+// Grows the context's workspace to `bytes`. A call under capture marks it: a graph may hold it.
+int ensure(const DenseCtx &c, size_t bytes, hipStream_t s) {
+  DenseWork &w = *c.work;
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  HIP_TRY(hipStreamIsCapturing(s, &cap));
+  const bool capturing = cap != hipStreamCaptureStatusNone;
+  if (bytes > w.cap) {
+    if (capturing)
+      return fail(MOE_ERR_STATE, "workspace too small for this call during graph capture; run it once uncaptured first");
+    void *q = nullptr;
+    const hipError_t e = hipMalloc(&q, bytes);
+    if (e != hipSuccess) return fail(MOE_ERR_OOM, "hipMalloc(%zu): %s", bytes, hipGetErrorString(e));
+    if (w.p && w.captured)
+      w.kept.push_back(w.p);
+    else if (w.p)
+      (void)hipFree(w.p);  // waits for the launches that use it
+    w.p = q;
+    w.cap = bytes;
+    w.captured = false;
+  }
+  w.captured |= capturing;
+  return MOE_OK;
+}
+
+bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+size_t elem(int dtype) { return dtype == MOE_F32 ? 4 : 2; }
+
+int check_dtype(int dtype) {
+  if (dtype != MOE_F32 && dtype != MOE_BF16) return fail(MOE_ERR_INVALID, "dtype %d is neither MOE_F32 nor MOE_BF16", dtype);
+  return MOE_OK;
+}
+// Pointers that matrix loads and stores of 16 bytes go through.
+int check_aligned(std::initializer_list<const void *> ps) {
+  for (const void *p : ps)
+    if (!aligned(p, 16)) return fail(MOE_ERR_INVALID, "device pointer %p is not 16-byte aligned", p);
+  return MOE_OK;
+}
+int check_tokens(size_t T) {
+  if (T > kMaxTokens) return fail(MOE_ERR_INVALID, "n_tokens %zu above %zu", T, kMaxTokens);
+  return MOE_OK;
+}
+// An output that is also an input, or twice an output.
+int check_distinct(std::initializer_list<const void *> outs, std::initializer_list<const void *> ins) {
+  for (auto o = outs.begin(); o != outs.end(); ++o) {
+    if (!*o) continue;
+    for (auto p = outs.begin(); p != o; ++p)
+      if (*p == *o) return fail(MOE_ERR_INVALID, "two outputs at %p", *o);
+    for (const void *i : ins)
+      if (i == *o) return fail(MOE_ERR_INVALID, "an output is also an input (%p)", *o);
+  }
+  return MOE_OK;
+}
+
+// Rows [n][cols] as the products take them: bf16 planes.
+struct Rows {
+  const uint16_t *p = nullptr;
+  int planes = 1;
+  size_t plane = 0;  // elements between planes
+};
+
+// Products of the planes of A and B, smallest terms first; terms below 2^-24 of the result are left out.
+void set_passes(DenseArgs &a, int na, int nb) {
+  a.n_pass = 0;
+  a.pa = a.pb = 0;
+  for (int sum = kPlanes - 1; sum >= 0; sum--)
+    for (int i = 0; i <= sum; i++)
+      if (i < na && sum - i < nb) {
+        a.pa |= (uint32_t)i << 4 * a.n_pass;
+        a.pb |= (uint32_t)(sum - i) << 4 * a.n_pass;
+        a.n_pass++;
+      }
+}
+
+DenseArgs product(const uint16_t *A, size_t lda, size_t a_plane, int na, const uint16_t *B, size_t ldb, size_t b_plane, int nb,
+                  size_t M, size_t N, size_t K) {
+  DenseArgs a{};
+  a.A = A;
+  a.lda = lda;
+  a.a_plane = a_plane;
+  a.B = B;
+  a.ldb = ldb;
+  a.b_plane = b_plane;
+  a.M = (int)M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.splits = 1;
+  set_passes(a, na, nb);
+  return a;
+}
+
+// f32 rows: their planes in the workspace. bf16 rows: as they are.
+Rows plane_rows(Carve &w, const void *x, int dtype, size_t n) {
+  if (dtype == MOE_BF16) return Rows{(const uint16_t *)x, 1, 0};
+  return Rows{w.take<uint16_t>(kPlanes * n), kPlanes, n};
+}
+int fill_rows(const Rows &r, const void *x, int dtype, size_t n, hipStream_t s) {
+  if (dtype == MOE_F32) HIP_TRY(launch_planes((const float *)x, n, const_cast<uint16_t *>(r.p), r.plane, s));
+  return MOE_OK;
+}
+
+// out [N][M] (+ bias) of a product, K split where that fills the device; part: [splits][N][M] f32 then.
+int store(DenseArgs a, bool at, bool bt, int splits, float *part, const float *bias, void *out, int dtype, hipStream_t s) {
+  const DenseShape shape{at, bt, DENSE_STORE};
+  a.ldo = (size_t)a.M;
+  if (splits > 1) {
+    a.splits = splits;
+    a.split_stride = (size_t)a.M * a.N;
+    a.out = part;
+    a.out_mode = 1;
+    HIP_TRY(launch_dense(shape, a, s));
+    HIP_TRY(launch_sum_parts(part, a.split_stride, splits, a.split_stride, bias, (size_t)a.M, out, dtype == MOE_BF16, s));
+    return MOE_OK;
+  }
+  a.out = out;
+  a.out_mode = dtype == MOE_BF16 ? 0 : 1;
+  a.bias = bias;
+  HIP_TRY(launch_dense(shape, a, s));
+  return MOE_OK;
+}
+
+int zero(void *p, size_t bytes, hipStream_t s) {
+  if (p) HIP_TRY(launch_zero(p, bytes, s));
+  return MOE_OK;
+}
+
+// ------------------------------------------------------------------ loss
+
+int check_loss(const DenseCtx &c, const void *x, int dtype, const int32_t *targets, size_t T, size_t vocab) {
+  RETURN_IF(check_dtype(dtype));
+  if (!c.lm_vocab) return fail(MOE_ERR_STATE, "call init_lm_head_bf16 first");
+  if (!c.lm_w) return fail(MOE_ERR_STATE, "the loss reads the bf16 LM head; the context holds the f32 one");
+  if (!vocab || vocab > c.lm_vocab)
+    return fail(MOE_ERR_INVALID, "vocab %zu outside [1, %zu]", vocab, c.lm_vocab);
+  if (vocab > 0x7FFFFF00) return fail(MOE_ERR_INVALID, "vocab %zu too large", vocab);
+  RETURN_IF(check_tokens(T));
+  if (T && (!x || !targets)) return fail(MOE_ERR_INVALID, "null x or targets");
+  return check_aligned({x});
+}
+
+constexpr size_t kLossTokens = 16384;                 // tokens whose statistics are kept at once
+constexpr size_t kGradTokens = 8192;                  // tokens and bytes of the logits' gradient at once
+constexpr size_t kGradBytes = (size_t)512 << 20;
+
+// ------------------------------------------------------------------ gated block
+
+int check_block(const moe_ffn *b, const void *x, const void *other, size_t T) {
+  if (!b || !b->gate_up || !b->down) return fail(MOE_ERR_INVALID, "null block or weights");
+  if (!b->inter || b->inter % 8 || b->inter > kMaxInter)
+    return fail(MOE_ERR_INVALID, "inter %zu must be a positive multiple of 8, at most %zu", b->inter, kMaxInter);
+  RETURN_IF(check_tokens(T));
+  if (T && (!x || !other)) return fail(MOE_ERR_INVALID, "null rows");
+  return check_aligned({b->gate_up, b->gate_up_bias, b->down, b->down_bias, x, other});
+}
+
+}  // namespace
+
+extern "C" {
+
+int moe_lm_head_loss_device(moe_ctx *ctx, const void *x, int dtype, const int32_t *targets, size_t T, size_t vocab,
+                            float *loss, float *lse, void *stream) {
+  DenseCtx c;
+  RETURN_IF(dense_ctx(ctx, &c));
+  RETURN_IF(check_loss(c, x, dtype, targets, T, vocab));
+  if (!T) return MOE_OK;
+  if (!loss || !lse) return fail(MOE_ERR_INVALID, "null loss or lse");
+  RETURN_IF(check_distinct({loss, lse}, {x, targets, c.lm_w}));
+  const hipStream_t s = stream ? (hipStream_t)stream : c.stream;
+  const size_t H = c.H, Tc = std::min(T, kLossTokens);
+  const DenseShape shape{false, false, DENSE_STATS};
+  Carve w;
+  Rows r;
+  float2 *stats = nullptr;
+  float *picked = nullptr;
+  for (int placed = 0; placed < 2; placed++) {
+    r = plane_rows(w, x, dtype, T * H);
+    size_t most = 0;  // (the last piece of tokens may take another tile)
+    for (size_t t0 = 0; t0 < T; t0 += Tc) {
+      const size_t n = std::min(Tc, T - t0);
+      most = std::max(most, n * (size_t)dense_parts(shape, product(c.lm_w, H, 0, 1, r.p, H, r.plane, r.planes, vocab, n, H)));
+    }
+    stats = w.take<float2>(most);
+    picked = w.take<float>(Tc);
+    if (!placed) {
+      RETURN_IF(ensure(c, w.off, s));
+      w = Carve{(char *)c.work->p};
+    }
+  }
+  RETURN_IF(fill_rows(r, x, dtype, T * H, s));
+  for (size_t t0 = 0; t0 < T; t0 += Tc) {
+    const size_t n = std::min(Tc, T - t0);
+    DenseArgs a = product(c.lm_w, H, 0, 1, r.p + t0 * H, H, r.plane, r.planes, vocab, n, H);
+    a.targets = targets + t0;
+    a.stats = stats;
+    a.picked = picked;
+    HIP_TRY(launch_dense(shape, a, s));
+    HIP_TRY(launch_loss(stats, dense_parts(shape, a), picked, targets + t0, n, (int)vocab, loss + t0, lse + t0, s));
+  }
+  return MOE_OK;
+}
+
+int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, const int32_t *targets, const float *lse,
+                                     const float *dloss, size_t T, size_t vocab, void *dx, void *dw, void *stream) {
+  DenseCtx c;
+  RETURN_IF(dense_ctx(ctx, &c));
+  RETURN_IF(check_loss(c, x, dtype, targets, T, vocab));
+  RETURN_IF(check_aligned({dx, dw}));
+  const hipStream_t s = stream ? (hipStream_t)stream : c.stream;
+  const size_t H = c.H;
+  if (!T) return zero(dw, vocab * H * elem(dtype), s);
+  if (!lse || !dloss) return fail(MOE_ERR_INVALID, "null lse or dloss");
+  RETURN_IF(check_distinct({dx, dw}, {x, targets, lse, dloss, c.lm_w}));
+  if (!dx && !dw) return MOE_OK;
+  const int P = dtype == MOE_BF16 ? 1 : kPlanes;
+  const bool bf = dtype == MOE_BF16;
+  // pieces of tokens and of the vocabulary whose gradient of the logits is held at once
+  const size_t Tc = std::min(T, kGradTokens), nt = (T + Tc - 1) / Tc;
+  const size_t most = std::max<size_t>(256, kGradBytes / (2 * P * Tc) / 256 * 256), nv = (vocab + most - 1) / most;
+  const size_t Vc = std::min(vocab, ((vocab + nv - 1) / nv + 255) / 256 * 256), ld = (Vc + 7) / 8 * 8;
+  const DenseShape sx{true, false, DENSE_STORE}, sw{true, true, DENSE_STORE};
+  // few tokens: dx from K splits of every piece of the vocabulary, summed at the end; many: added up
+  const int splits = dense_splits(sx, product(c.lm_w, H, 0, 1, nullptr, ld, 0, P, H, Tc, Vc), c.n_cu);
+  const bool parts = dx && splits > 1 && nt == 1;
+  Carve w;
+  Rows r;
+  uint16_t *dl = nullptr;
+  float *dx_acc = nullptr, *dw_acc = nullptr;
+  for (int placed = 0; placed < 2; placed++) {
+    r = plane_rows(w, x, dtype, T * H);
+    dl = w.take<uint16_t>(P * Tc * ld);
+    if (parts)
+      dx_acc = w.take<float>(nv * splits * T * H);
+    else if (dx)
+      dx_acc = bf && nv > 1 ? w.take<float>(T * H) : bf ? nullptr : (float *)dx;
+    if (dw) dw_acc = bf && nt > 1 ? w.take<float>(Vc * H) : nullptr;
+    if (!placed) {
+      RETURN_IF(ensure(c, w.off, s));
+      w = Carve{(char *)c.work->p};
+    }
+  }
+  RETURN_IF(fill_rows(r, x, dtype, T * H, s));
+  int written = 0;  // parts of dx
+  for (size_t v0 = 0; v0 < vocab; v0 += Vc) {
+    const size_t nvoc = std::min(Vc, vocab - v0);
+    const uint16_t *wv = c.lm_w + v0 * H;
+    for (size_t t0 = 0; t0 < T; t0 += Tc) {
+      const size_t n = std::min(Tc, T - t0);
+      DenseArgs a = product(wv, H, 0, 1, r.p + t0 * H, H, r.plane, r.planes, nvoc, n, H);
+      a.targets = targets + t0;
+      a.lse = lse + t0;
+      a.dloss = dloss + t0;
+      a.v0 = (int)v0;
+      a.vocab = (int)vocab;
+      a.dl = dl;
+      a.dl_plane = Tc * ld;
+      a.ld_dl = ld;
+      a.planes = P;
+      HIP_TRY(launch_dense(DenseShape{false, false, DENSE_DLOGITS}, a, s));
+      if (dx) {
+        DenseArgs g = product(wv, H, 0, 1, dl, ld, Tc * ld, P, H, n, nvoc);
+        g.ldo = H;
+        if (parts) {
+          g.splits = splits;
+          g.split_stride = T * H;
+          g.out = dx_acc + (size_t)written * T * H;
+          g.out_mode = 1;
+          written += dense_split_count(g);
+        } else if (dx_acc) {
+          g.out = dx_acc + t0 * H;
+          g.out_mode = v0 ? 2 : 1;
+        } else {
+          g.out = (uint16_t *)dx + t0 * H;
+        }
+        HIP_TRY(launch_dense(sx, g, s));
+      }
+      if (dw) {
+        DenseArgs g = product(r.p + t0 * H, H, r.plane, r.planes, dl, ld, Tc * ld, P, H, nvoc, n);
+        g.ldo = H;
+        if (!bf || dw_acc) {
+          g.out = bf ? dw_acc : (float *)dw + v0 * H;
+          g.out_mode = t0 ? 2 : 1;
+        } else {
+          g.out = (uint16_t *)dw + v0 * H;
+        }
+        HIP_TRY(launch_dense(sw, g, s));
+      }
+    }
+    if (dw && dw_acc) HIP_TRY(launch_sum_parts(dw_acc, 0, 1, nvoc * H, nullptr, 1, (uint16_t *)dw + v0 * H, true, s));
+  }
+  if (parts)
+    HIP_TRY(launch_sum_parts(dx_acc, T * H, written, T * H, nullptr, 1, dx, bf, s));
+  else if (dx && dx_acc && bf)
+    HIP_TRY(launch_sum_parts(dx_acc, 0, 1, T * H, nullptr, 1, dx, true, s));
+  return MOE_OK;
+}
+
+int moe_ffn_forward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int dtype, size_t T, void *y, uint8_t *x8,
+                           void *stream) {
+  DenseCtx c;
+  RETURN_IF(dense_ctx(ctx, &c));
+  RETURN_IF(check_dtype(dtype));
+  RETURN_IF(check_block(b, x, y, T));
+  RETURN_IF(check_aligned({x8}));
+  if (!T) return MOE_OK;
+  RETURN_IF(check_distinct({y, x8}, {x, b->gate_up, b->gate_up_bias, b->down, b->down_bias}));
+  const hipStream_t s = stream ? (hipStream_t)stream : c.stream;
+  const size_t H = c.H, I = b->inter;
+  const int P = dtype == MOE_BF16 ? 1 : kPlanes;
+  Carve w;
+  Rows r, h;
+  float *part = nullptr;
+  int splits = 1;
+  for (int placed = 0; placed < 2; placed++) {
+    r = plane_rows(w, x, dtype, T * H);
+    h = Rows{w.take<uint16_t>(P * T * I), P, T * I};
+    splits = dense_splits(DenseShape{false, false, DENSE_STORE}, product(b->down, I, 0, 1, h.p, I, h.plane, P, H, T, I), c.n_cu);
+    part = splits > 1 ? w.take<float>(splits * T * H) : nullptr;
+    if (!placed) {
+      RETURN_IF(ensure(c, w.off, s));
+      w = Carve{(char *)c.work->p};
+    }
+  }
+  if (x8) HIP_TRY(launch_act8_pack(x, dtype == MOE_BF16, T, H, x8, s));
+  RETURN_IF(fill_rows(r, x, dtype, T * H, s));
+  DenseArgs g = product(b->gate_up, H, 0, 1, r.p, H, r.plane, r.planes, 2 * I, T, H);
+  g.bias = b->gate_up_bias;
+  g.limit = c.clamp;
+  g.h = const_cast<uint16_t *>(h.p);
+  g.h_plane = h.plane;
+  g.ldh = I;
+  g.planes = P;
+  HIP_TRY(launch_dense(DenseShape{false, false, DENSE_GATE}, g, s));
+  return store(product(b->down, I, 0, 1, h.p, I, h.plane, P, H, T, I), false, false, splits, part, b->down_bias, y, dtype, s);
+}
+
+int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x_type, const void *dy, int dtype, size_t T,
+                            const moe_ffn_grads *out, void *stream) {
+  DenseCtx c;
+  RETURN_IF(dense_ctx(ctx, &c));
+  RETURN_IF(check_dtype(dtype));
+  if (x_type != dtype && x_type != MOE_MXFP8)
+    return fail(MOE_ERR_INVALID, "x_type %d is neither dtype %d nor MOE_MXFP8", x_type, dtype);
+  if (!out) return fail(MOE_ERR_INVALID, "null gradients");
+  RETURN_IF(check_block(b, x, dy, T));
+  RETURN_IF(check_aligned({out->x, out->gate_up, out->gate_up_bias, out->down, out->down_bias}));
+  RETURN_IF(check_distinct({out->x, out->gate_up, out->gate_up_bias, out->down, out->down_bias},
+                           {x, dy, b->gate_up, b->gate_up_bias, b->down, b->down_bias}));
+  const hipStream_t s = stream ? (hipStream_t)stream : c.stream;
+  const size_t H = c.H, I = b->inter, el = elem(dtype);
+  if (!T) {
+    RETURN_IF(zero(out->gate_up, 2 * I * H * el, s));
+    RETURN_IF(zero(out->gate_up_bias, 2 * I * 4, s));
+    RETURN_IF(zero(out->down, H * I * el, s));
+    return zero(out->down_bias, H * 4, s);
+  }
+  const int P = dtype == MOE_BF16 ? 1 : kPlanes;
+  const bool bf = dtype == MOE_BF16;
+  const bool inner = out->x || out->gate_up || out->gate_up_bias || out->down;
+  const DenseShape sg{true, false, DENSE_DGATE}, sx{true, false, DENSE_STORE}, sw{true, true, DENSE_STORE};
+  Carve w;
+  Rows r, d, h, dgu;
+  float *gu = nullptr, *db = nullptr, *col = nullptr, *part = nullptr;
+  int nx = 1, ngu = 1, nd = 1, db_parts = 0;
+  for (int placed = 0; placed < 2; placed++) {
+    if (inner) {
+      r = x_type == MOE_MXFP8 ? Rows{w.take<uint16_t>(T * H), 1, 0} : plane_rows(w, x, dtype, T * H);
+      d = plane_rows(w, dy, dtype, T * H);
+      gu = w.take<float>(T * 2 * I);
+      h = Rows{w.take<uint16_t>(P * T * I), P, T * I};
+      dgu = Rows{w.take<uint16_t>(P * T * 2 * I), P, T * 2 * I};
+      db_parts = dense_parts(sg, product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H));
+      db = out->gate_up_bias ? w.take<float>((size_t)db_parts * 2 * I) : nullptr;
+      nx = dense_splits(sx, product(b->gate_up, H, 0, 1, dgu.p, 2 * I, dgu.plane, P, H, T, 2 * I), c.n_cu);
+      ngu = dense_splits(sw, product(r.p, H, r.plane, r.planes, dgu.p, 2 * I, dgu.plane, P, H, 2 * I, T), c.n_cu);
+      nd = dense_splits(sw, product(h.p, I, h.plane, P, d.p, H, d.plane, P, I, H, T), c.n_cu);
+      size_t most = 0;  // one after the other, so they share it
+      if (out->x && nx > 1) most = std::max(most, nx * T * H);
+      if (out->gate_up && ngu > 1) most = std::max(most, ngu * 2 * I * H);
+      if (out->down && nd > 1) most = std::max(most, nd * I * H);
+      part = w.take<float>(most);
+    }
+    col = out->down_bias ? w.take<float>(dense_colsum_parts(T) * H) : nullptr;
+    if (!placed) {
+      RETURN_IF(ensure(c, w.off, s));
+      w = Carve{(char *)c.work->p};
+    }
+  }
+  if (out->down_bias) {
+    HIP_TRY(launch_colsum(dy, bf, T, H, col, s));
+    HIP_TRY(launch_sum_parts(col, H, dense_colsum_parts(T), H, nullptr, 1, out->down_bias, false, s));
+  }
+  if (!inner) return MOE_OK;
+  if (x_type == MOE_MXFP8)
+    HIP_TRY(launch_act8_unpack((const uint8_t *)x, T, H, const_cast<uint16_t *>(r.p), true, s));
+  else
+    RETURN_IF(fill_rows(r, x, dtype, T * H, s));
+  RETURN_IF(fill_rows(d, dy, dtype, T * H, s));
+  DenseArgs g = product(b->gate_up, H, 0, 1, r.p, H, r.plane, r.planes, 2 * I, T, H);
+  g.bias = b->gate_up_bias;
+  g.gu = gu;
+  HIP_TRY(launch_dense(DenseShape{false, false, DENSE_GATE_RAW}, g, s));
+  g = product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H);
+  g.limit = c.clamp;
+  g.gu = gu;
+  g.h = const_cast<uint16_t *>(h.p);
+  g.h_plane = h.plane;
+  g.ldh = I;
+  g.dgu = const_cast<uint16_t *>(dgu.p);
+  g.dgu_plane = dgu.plane;
+  g.db_part = db;
+  g.planes = P;
+  HIP_TRY(launch_dense(sg, g, s));
+  if (db) HIP_TRY(launch_sum_parts(db, 2 * I, db_parts, 2 * I, nullptr, 1, out->gate_up_bias, false, s));
+  if (out->x)
+    RETURN_IF(store(product(b->gate_up, H, 0, 1, dgu.p, 2 * I, dgu.plane, P, H, T, 2 * I), true, false, nx, part, nullptr,
+                    out->x, dtype, s));
+  if (out->gate_up)
+    RETURN_IF(store(product(r.p, H, r.plane, r.planes, dgu.p, 2 * I, dgu.plane, P, H, 2 * I, T), true, true, ngu, part, nullptr,
+                    out->gate_up, dtype, s));
+  if (out->down)
+    RETURN_IF(store(product(h.p, I, h.plane, P, d.p, H, d.plane, P, I, H, T), true, true, nd, part, nullptr, out->down, dtype, s));
+  return MOE_OK;
+}
+
+size_t moe_act8_bytes(size_t n, size_t cols) { return cols % 32 ? 0 : n * cols + n * (cols / 32); }
+
+static int check_act8(const void *from, const void *to, int dtype, size_t n, size_t cols) {
+  RETURN_IF(check_dtype(dtype));
+  if (!cols || cols % 32 || cols > kMaxInter) return fail(MOE_ERR_INVALID, "cols %zu must be a positive multiple of 32, at most %zu", cols, kMaxInter);
+  RETURN_IF(check_tokens(n));
+  if (n && (!from || !to)) return fail(MOE_ERR_INVALID, "null argument");
+  RETURN_IF(check_aligned({from, to}));
+  return n ? check_distinct({to}, {from}) : MOE_OK;
+}
+
+int moe_act8_pack_device(moe_ctx *ctx, const void *x, int dtype, size_t n, size_t cols, uint8_t *packed, void *stream) {
+  DenseCtx c;
+  RETURN_IF(dense_ctx(ctx, &c));
+  RETURN_IF(check_act8(x, packed, dtype, n, cols));
+  HIP_TRY(launch_act8_pack(x, dtype == MOE_BF16, n, cols, packed, stream ? (hipStream_t)stream : c.stream));
+  return MOE_OK;
+}
+
+int moe_act8_unpack_device(moe_ctx *ctx, const uint8_t *packed, size_t n, size_t cols, void *out, int dtype, void *stream) {
+  DenseCtx c;
+  RETURN_IF(dense_ctx(ctx, &c));
+  RETURN_IF(check_act8(packed, out, dtype, n, cols));
+  HIP_TRY(launch_act8_unpack(packed, n, cols, out, dtype == MOE_BF16, stream ? (hipStream_t)stream : c.stream));
+  return MOE_OK;
+}
+
+}  // extern "C"

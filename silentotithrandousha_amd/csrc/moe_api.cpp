@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/mxfp4_moe.h"
+#include "dense.hpp"
 #include "kernels.hpp"
 #include "layout.hpp"
 
@@ -149,6 +150,7 @@ struct moe_ctx {
   DevBuf lm_w, lm_x, lm_y;
   size_t lm_vocab = 0;
   bool lm_bf16 = false;  // lm_w holds the checkpoint's bf16 rows (else f32)
+  DenseWork dense;       // workspace of the dense operators (dense_api.cpp)
   bool timing = false;
   bool capturing = false;
   // single-token forwards: 0 = the batch path, 1 = two decode kernels, 2 = one launch
@@ -787,6 +789,8 @@ void moe_destroy(moe_ctx *c) {
   c->lm_w.release();
   c->lm_x.release();
   c->lm_y.release();
+  for (void *p : c->dense.kept) (void)hipFree(p);
+  if (c->dense.p) (void)hipFree(c->dense.p);
   (void)hipStreamDestroy(c->stream);
   delete c;
 }
@@ -1407,14 +1411,20 @@ int moe_reset_timing(moe_ctx *c) {
 
 }  // extern "C"
 
-// For the library's other host sources (safetensors.cpp): record the failure message that
-// moe_last_error returns, and read a context's dimensions.
+// For the library's other host sources (safetensors.cpp, dense_api.cpp): record the failure message
+// that moe_last_error returns, and read a context.
 namespace moe {
 int api_fail(int code, const char *msg) { return fail(code, "%s", msg); }
 int ctx_dims(const moe_ctx *c, size_t *H, size_t *I) {
   if (!c) return fail(MOE_ERR_INVALID, "null context");
   *H = c->H;
   *I = c->I;
+  return MOE_OK;
+}
+// Makes the context's device current and describes it.
+int dense_ctx(moe_ctx *c, DenseCtx *d) {
+  RETURN_IF(use_dev(c));
+  *d = DenseCtx{c->stream, c->H, c->clamp, c->lm_bf16 ? (const uint16_t *)c->lm_w.p : nullptr, c->lm_vocab, c->n_cu, &c->dense};
   return MOE_OK;
 }
 }  // namespace moe

@@ -25,6 +25,11 @@ def _dp(b):
     return ctypes.c_void_p(b.ptr if hasattr(b, "ptr") else int(b))
 
 
+def _dpn(b):
+    """The same, None as NULL."""
+    return None if b is None else _dp(b)
+
+
 class DeviceBuffer:
     """A device allocation made through moe_device_alloc (freed on close / GC)."""
 
@@ -267,6 +272,43 @@ class GpuMoeDispatcher:
     def dispatch_lm_head_device(self, x_dev, vocab_size, logits_dev, stream=None):
         """Device pointers (DeviceBuffer or int), enqueued without synchronisation."""
         check(lib().moe_dispatch_lm_head_device(self._ctx, _dp(x_dev), vocab_size, _dp(logits_dev), stream))
+
+    # ---- dense operators (include/moe_dense.h): device pointers (DeviceBuffer or int), enqueued
+    # without synchronisation; dtype MOE_F32 or MOE_BF16
+    def lm_head_loss_device(self, x, dtype, targets, n_tokens, vocab_size, loss, lse, stream=None):
+        """Cross entropy of rows x [n_tokens, H] against targets over the resident bf16 LM head, and
+        its log-sum-exp; no logits are kept. A negative target is ignored."""
+        check(lib().moe_lm_head_loss_device(self._ctx, _dpn(x), dtype, _dpn(targets), n_tokens, vocab_size,
+                                            _dpn(loss), _dpn(lse), stream))
+
+    def lm_head_loss_backward_device(self, x, dtype, targets, lse, dloss, n_tokens, vocab_size, dx, dw, stream=None):
+        """Gradients of sum(dloss * loss): dx [n_tokens, H] and dw [vocab, H] (either may be None)."""
+        check(lib().moe_lm_head_loss_backward_device(self._ctx, _dpn(x), dtype, _dpn(targets), _dpn(lse), _dpn(dloss),
+                                                     n_tokens, vocab_size, _dpn(dx), _dpn(dw), stream))
+
+    def ffn_forward_device(self, block, x, dtype, n_tokens, y, x8=None, stream=None):
+        """y = the gated block (GatedFfn) of x; x8: also x as an 8-bit checkpoint of act8_bytes bytes."""
+        check(lib().moe_ffn_forward_device(self._ctx, ctypes.byref(block), _dpn(x), dtype, n_tokens, _dpn(y),
+                                           _dpn(x8), stream))
+
+    def ffn_backward_device(self, block, x, x_type, dy, dtype, n_tokens, grads, stream=None):
+        """The gradients (GatedFfnGrads) of the gated block from x (x_type dtype, or MOE_MXFP8: the
+        checkpoint) and dy."""
+        check(lib().moe_ffn_backward_device(self._ctx, ctypes.byref(block), _dpn(x), x_type, _dpn(dy), dtype, n_tokens,
+                                            ctypes.byref(grads), stream))
+
+    def act8_bytes(self, n_tokens, cols):
+        n = lib().moe_act8_bytes(n_tokens, cols)
+        if n == 0 and n_tokens:
+            raise ValueError("cols must be a positive multiple of 32")
+        return n
+
+    def act8_pack_device(self, x, dtype, n_tokens, cols, packed, stream=None):
+        """Rows as MXFP8: e4m3 codes, then one E8M0 scale per 32 values."""
+        check(lib().moe_act8_pack_device(self._ctx, _dpn(x), dtype, n_tokens, cols, _dpn(packed), stream))
+
+    def act8_unpack_device(self, packed, n_tokens, cols, out, dtype, stream=None):
+        check(lib().moe_act8_unpack_device(self._ctx, _dpn(packed), n_tokens, cols, _dpn(out), dtype, stream))
 
     # ---- path level
     def router_topk(self, layer, x, top_k, want_logits=False, n_experts=None):
