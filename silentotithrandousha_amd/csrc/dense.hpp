@@ -33,15 +33,17 @@ struct DenseArgs {
   size_t a_plane, b_plane;  // elements between planes
   size_t lda, ldb;          // elements between rows of the stored matrix
   int M, N, K;
+  int stack;                // planes of B that one pass takes as rows [plane][N] (N * stack <= 64), else 1
   int n_pass;
   uint32_t pa, pb;          // planes of A and B of each pass, 4 bits each
   int splits;               // K split (DENSE_STORE with f32 only): out + split * split_stride
-  int k_split;              // K per split, a multiple of 64
+  int k_split;              // K per split, a multiple of the step
   // DENSE_STORE
   void *out;
   size_t ldo, split_stride;
   int out_mode;             // 0 bf16, 1 f32, 2 f32 added to
   const float *bias;        // [M] or NULL
+  const float *scale;       // factor of the result (one value) or NULL; of the loss: what dloss is divided by
   // gated block
   float limit;
   uint16_t *h;              // [planes][N][ldh] bf16
@@ -68,7 +70,7 @@ struct DenseShape {
 };
 int dense_parts(const DenseShape &s, const DenseArgs &a);  // parts of db_part / stats that a launch writes
 // K splits worth taking (none of them empty)
-int dense_splits(const DenseShape &s, const DenseArgs &a, int n_cu);
+int dense_splits(const DenseShape &s, const DenseArgs &a);
 int dense_split_count(const DenseArgs &a);  // the splits that a launch with a.splits makes (none of them empty)
 hipError_t launch_dense(const DenseShape &s, const DenseArgs &a, hipStream_t st);
 
@@ -83,6 +85,9 @@ hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *pa
 // loss and log-sum-exp of each token from the parts of DENSE_STATS.
 hipError_t launch_loss(const float2 *stats, int parts, const float *picked, const int32_t *targets, size_t T,
                        int vocab, float *loss, float *lse, hipStream_t s);
+
+// The largest magnitude of dloss [T], 1 where that is 0 or not finite.
+hipError_t launch_dloss_scale(const float *dloss, size_t T, float *scale, hipStream_t s);
 
 // MXFP8 activation checkpoints (act8.hip): codes [n][cols], then scales [n][cols / 32].
 hipError_t launch_act8_pack(const void *x, bool bf16, size_t n, size_t cols, uint8_t *packed, hipStream_t s);
@@ -104,7 +109,6 @@ struct DenseCtx {
   float clamp;
   const uint16_t *lm_w;  // bf16 LM head rows, NULL if none or f32
   size_t lm_vocab;
-  int n_cu;
   DenseWork *work;
 };
 

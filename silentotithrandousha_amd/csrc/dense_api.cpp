@@ -133,7 +133,7 @@ void set_passes(DenseArgs &a, int na, int nb) {
 }
 
 DenseArgs product(const uint16_t *A, size_t lda, size_t a_plane, int na, const uint16_t *B, size_t ldb, size_t b_plane, int nb,
-                  size_t M, size_t N, size_t K) {
+                  size_t M, size_t N, size_t K, bool bt = false) {
   DenseArgs a{};
   a.A = A;
   a.lda = lda;
@@ -145,6 +145,11 @@ DenseArgs product(const uint16_t *A, size_t lda, size_t a_plane, int na, const u
   a.N = (int)N;
   a.K = (int)K;
   a.splits = 1;
+  a.stack = 1;
+  if (!bt && na == 1 && nb > 1 && N * nb <= 64 && b_plane == N * ldb) {  // few rows: the planes of B as its rows
+    a.stack = nb;
+    nb = 1;
+  }
   set_passes(a, na, nb);
   return a;
 }
@@ -279,14 +284,15 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
   const size_t Vc = std::min(vocab, ((vocab + nv - 1) / nv + 255) / 256 * 256), ld = (Vc + 7) / 8 * 8;
   const DenseShape sx{true, false, DENSE_STORE}, sw{true, true, DENSE_STORE};
   // few tokens: dx from K splits of every piece of the vocabulary, summed at the end; many: added up
-  const int splits = dense_splits(sx, product(c.lm_w, H, 0, 1, nullptr, ld, 0, P, H, Tc, Vc), c.n_cu);
+  const int splits = dense_splits(sx, product(c.lm_w, H, 0, 1, nullptr, ld, 0, P, H, Tc, Vc));
   const bool parts = dx && splits > 1 && nt == 1;
   Carve w;
   Rows r;
   uint16_t *dl = nullptr;
-  float *dx_acc = nullptr, *dw_acc = nullptr;
+  float *dx_acc = nullptr, *dw_acc = nullptr, *scale = nullptr;
   for (int placed = 0; placed < 2; placed++) {
     r = plane_rows(w, x, dtype, T * H);
+    scale = w.take<float>(1);
     dl = w.take<uint16_t>(P * Tc * ld);
     if (parts)
       dx_acc = w.take<float>(nv * splits * T * H);
@@ -299,6 +305,10 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
     }
   }
   RETURN_IF(fill_rows(r, x, dtype, T * H, s));
+  // The gradient of the logits is held over the largest |dloss| and the results multiplied by it: for the
+  // mean's constant dloss the entries of the targets, which weigh most, then lie next to -1 and are rounded
+  // by their p alone, where bf16(1 / n) would put one error into all of them.
+  HIP_TRY(launch_dloss_scale(dloss, T, scale, s));
   int written = 0;  // parts of dx
   for (size_t v0 = 0; v0 < vocab; v0 += Vc) {
     const size_t nvoc = std::min(Vc, vocab - v0);
@@ -309,6 +319,7 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
       a.targets = targets + t0;
       a.lse = lse + t0;
       a.dloss = dloss + t0;
+      a.scale = scale;
       a.v0 = (int)v0;
       a.vocab = (int)vocab;
       a.dl = dl;
@@ -319,6 +330,7 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
       if (dx) {
         DenseArgs g = product(wv, H, 0, 1, dl, ld, Tc * ld, P, H, n, nvoc);
         g.ldo = H;
+        g.scale = scale;
         if (parts) {
           g.splits = splits;
           g.split_stride = T * H;
@@ -334,8 +346,9 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
         HIP_TRY(launch_dense(sx, g, s));
       }
       if (dw) {
-        DenseArgs g = product(r.p + t0 * H, H, r.plane, r.planes, dl, ld, Tc * ld, P, H, nvoc, n);
+        DenseArgs g = product(r.p + t0 * H, H, r.plane, r.planes, dl, ld, Tc * ld, P, H, nvoc, n, true);
         g.ldo = H;
+        g.scale = scale;
         if (!bf || dw_acc) {
           g.out = bf ? dw_acc : (float *)dw + v0 * H;
           g.out_mode = t0 ? 2 : 1;
@@ -373,7 +386,7 @@ int moe_ffn_forward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int dt
   for (int placed = 0; placed < 2; placed++) {
     r = plane_rows(w, x, dtype, T * H);
     h = Rows{w.take<uint16_t>(P * T * I), P, T * I};
-    splits = dense_splits(DenseShape{false, false, DENSE_STORE}, product(b->down, I, 0, 1, h.p, I, h.plane, P, H, T, I), c.n_cu);
+    splits = dense_splits(DenseShape{false, false, DENSE_STORE}, product(b->down, I, 0, 1, h.p, I, h.plane, P, H, T, I));
     part = splits > 1 ? w.take<float>(splits * T * H) : nullptr;
     if (!placed) {
       RETURN_IF(ensure(c, w.off, s));
@@ -430,9 +443,9 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
       dgu = Rows{w.take<uint16_t>(P * T * 2 * I), P, T * 2 * I};
       db_parts = dense_parts(sg, product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H));
       db = out->gate_up_bias ? w.take<float>((size_t)db_parts * 2 * I) : nullptr;
-      nx = dense_splits(sx, product(b->gate_up, H, 0, 1, dgu.p, 2 * I, dgu.plane, P, H, T, 2 * I), c.n_cu);
-      ngu = dense_splits(sw, product(r.p, H, r.plane, r.planes, dgu.p, 2 * I, dgu.plane, P, H, 2 * I, T), c.n_cu);
-      nd = dense_splits(sw, product(h.p, I, h.plane, P, d.p, H, d.plane, P, I, H, T), c.n_cu);
+      nx = dense_splits(sx, product(b->gate_up, H, 0, 1, dgu.p, 2 * I, dgu.plane, P, H, T, 2 * I));
+      ngu = dense_splits(sw, product(r.p, H, r.plane, r.planes, dgu.p, 2 * I, dgu.plane, P, H, 2 * I, T, true));
+      nd = dense_splits(sw, product(h.p, I, h.plane, P, d.p, H, d.plane, P, I, H, T, true));
       size_t most = 0;  // one after the other, so they share it
       if (out->x && nx > 1) most = std::max(most, nx * T * H);
       if (out->gate_up && ngu > 1) most = std::max(most, ngu * 2 * I * H);
@@ -475,10 +488,10 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
     RETURN_IF(store(product(b->gate_up, H, 0, 1, dgu.p, 2 * I, dgu.plane, P, H, T, 2 * I), true, false, nx, part, nullptr,
                     out->x, dtype, s));
   if (out->gate_up)
-    RETURN_IF(store(product(r.p, H, r.plane, r.planes, dgu.p, 2 * I, dgu.plane, P, H, 2 * I, T), true, true, ngu, part, nullptr,
+    RETURN_IF(store(product(r.p, H, r.plane, r.planes, dgu.p, 2 * I, dgu.plane, P, H, 2 * I, T, true), true, true, ngu, part, nullptr,
                     out->gate_up, dtype, s));
   if (out->down)
-    RETURN_IF(store(product(h.p, I, h.plane, P, d.p, H, d.plane, P, I, H, T), true, true, nd, part, nullptr, out->down, dtype, s));
+    RETURN_IF(store(product(h.p, I, h.plane, P, d.p, H, d.plane, P, I, H, T, true), true, true, nd, part, nullptr, out->down, dtype, s));
   return MOE_OK;
 }
 

@@ -2,19 +2,23 @@
 // D[m][n] = sum A[m][k] B[n][k], each operand K-contiguous or transposed in memory, with the
 // operators' epilogues applied to the accumulators.
 //
-// A workgroup of WM x WN wavefronts computes a BM x BN tile in K-steps of 64 values. Both operands of
-// a step arrive by LDS-DMA in one of two LDS slots while the other is computed on; one barrier a step.
-// A K-contiguous operand lies in LDS as rows of 128 bytes whose 16-byte chunks are permuted by the
-// row (chunk ^ row % 8), so that 8 lanes reading one chunk of 8 rows touch different banks. A
-// transposed operand lies as its 64 rows of k, and the fragments are read by the transposing LDS
-// load, whose 16 lanes take 4 rows x 32 bytes: the 32-byte pieces are permuted by the row.
+// A workgroup of WM x WN wavefronts computes a BM x BN tile in K-steps of 64 values, two halves of 32.
+// Both operands of a step arrive by LDS-DMA in one of NS LDS slots (2 for the large tiles, more for the
+// small ones, which wait for memory). Fragments are read one half ahead of the MFMAs, the first half of
+// the next step included: the step's one barrier stands between its halves, where this step's reads are
+// done (its slot takes the step NS ahead) and the next step's loads have landed.
+// A K-contiguous operand lies in LDS as rows of 128 bytes (a line each, so that no line is asked for
+// twice) whose 16-byte chunks are permuted by the row (chunk ^ row % 8), so that 8 lanes reading one chunk
+// of 8 rows touch different banks. A transposed one lies as its 64 rows of k, and the fragments are read
+// by the transposing LDS load, whose 16 lanes take 4 rows x 32 bytes: the 32-byte pieces are permuted by
+// the row.
 #pragma once
 #include "dense.hpp"
 #include "stream.hpp"
 
 namespace moe {
-
 constexpr int kDenseStep = 64;  // k values per step
+constexpr int kDenseHalf = 32;  // and per half, an MFMA's
 
 __device__ __forceinline__ uint16_t dense_bf16(float v) {
   return __builtin_bit_cast(uint16_t, (__bf16)v);  // round to nearest even
@@ -52,11 +56,12 @@ struct DenseGate {
 template <int R, int W, bool TR>
 struct DenseTile {
   static constexpr int kBytes = R * 128;
-  static constexpr int kLoads = (R / 8 + W - 1) / W;  // LDS-DMAs of 1 KB per wavefront
-  static constexpr bool kEven = R / 8 % W == 0;
+  static constexpr int kDmas = R / 8;                 // LDS-DMAs of 1 KB
+  static constexpr int kLoads = (kDmas + W - 1) / W;  // per wavefront; past the last one again (the same bytes)
   static constexpr int kPairs = R / 16;               // 32-byte pieces of a transposed row
 
-  // piece of a transposed row that holds the logical piece q in row k
+  // Transposed: piece of a row that holds the logical piece q in row k. The transposing load's 16 lanes
+  // take rows k = 8g .. 8g + 3 (and + 4): their pieces go to different banks.
   static __device__ __forceinline__ int piece(int q, int k) {
     const int f = (k & 3) | ((k >> 1) & 4);
     const int mask = kPairs >= 8 ? ((q | 7) < kPairs ? 7 : (q | 3) < kPairs ? 3 : 0)
@@ -65,61 +70,56 @@ struct DenseTile {
   }
 
   uint32_t off[kLoads];  // byte offset of this lane's 16 bytes from the tile's base
-  uint32_t part[kLoads]; // K-contiguous: first k of the lane's chunk; transposed: its row k
 
+  static __device__ __forceinline__ int dma(int i, int wave) {
+    const int d = i * W + wave;
+    return kDmas % W == 0 ? d : d % kDmas;
+  }
+  // chunk c of the tile: the first k of its values if K-contiguous, its row's k if transposed
+  static __device__ __forceinline__ int k_of(int c) { return TR ? c / (R / 8) : ((c & 7) ^ ((c >> 3) & 7)) * 8; }
   // rows: valid rows from the tile's first; ld: bytes between stored rows
-  __device__ __forceinline__ void init(int wave, int lane, int rows, size_t ld) {
+  __device__ __forceinline__ void init(int wave, int lane, int rows, uint32_t ld) {
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
-      const int c = (i * W + wave) * 64 + lane;
+      const int c = dma(i, wave) * 64 + lane, k = k_of(c);
       if constexpr (!TR) {
-        const int row = c >> 3, ch = (c & 7) ^ (row & 7);
-        off[i] = (uint32_t)((size_t)min(row, rows - 1) * ld);
-        part[i] = ch * 8;
+        off[i] = (uint32_t)min(c >> 3, rows - 1) * ld + k * 2;
       } else {
-        const int k = c / (R / 8), pos = c % (R / 8);
+        const int pos = c % (R / 8);
         int col = piece(pos >> 1, k) * 16 + (pos & 1) * 8;  // the permutation is its own inverse
         if (col >= rows) col = 0;
-        off[i] = (uint32_t)(col * 2);
-        part[i] = k;
+        off[i] = (uint32_t)k * ld + col * 2;
       }
     }
   }
-  // loads the step whose first k is at `base`; left: k values left in K from there
-  __device__ __forceinline__ void load(const uint16_t *base, size_t ld, int left, uint32_t lds, int wave) const {
+  // the wavefront's load i of the step whose first k is at `base`
+  __device__ __forceinline__ void load(int i, const uint16_t *base, uint32_t lds, int wave) const {
+    str_dma16(off[i], base, lds + dma(i, wave) * 1024);
+  }
+  // for a step with fewer k values left than its 64: past them a valid place instead (zero_tail clears it)
+  __device__ __forceinline__ void clamp(int wave, int lane, uint32_t ld, int left) {
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
-      if (!kEven && (i * W + wave) * 8 >= R) continue;
-      uint32_t o = off[i];
-      if constexpr (!TR)
-        o += ((int)part[i] < left ? part[i] : 0u) * 2;
-      else
-        o += (uint32_t)min((int)part[i], left - 1) * (uint32_t)ld;
-      str_dma16(o, base, lds + (i * W + wave) * 1024);
+      const int k = k_of(dma(i, wave) * 64 + lane);
+      if (k >= left) off[i] -= TR ? (uint32_t)(k - (left - 1)) * ld : (uint32_t)k * 2;
     }
   }
   // zeroes the k values of the step past `left` (the last step of a K that is no multiple of 64)
   __device__ __forceinline__ static void zero_tail(uint8_t *lds, int left, int tid, int threads) {
-    for (int c = tid; c < R * 8; c += threads) {
-      bool past;
-      if constexpr (!TR)
-        past = (((c & 7) ^ ((c >> 3) & 7)) * 8) >= left;
-      else
-        past = c / (R / 8) >= left;
-      if (past) *(uint4 *)(lds + c * 16) = uint4{0u, 0u, 0u, 0u};
-    }
+    for (int c = tid; c < R * 8; c += threads)
+      if (k_of(c) >= left) *(uint4 *)(lds + c * 16) = uint4{0u, 0u, 0u, 0u};
   }
-  // MFMA operand of 16 rows from row0 (tile-relative), k slice kk (32 values)
-  static __device__ __forceinline__ bf16x8 frag(const uint8_t *lds, int row0, int kk, int lane) {
+  // MFMA operand of 16 rows from row0 (tile-relative), half h of the step at lds
+  static __device__ __forceinline__ bf16x8 frag(const uint8_t *lds, int row0, int h, int lane) {
     if constexpr (!TR) {
-      const int row = row0 + (lane & 15), ch = kk * 4 + (lane >> 4);
+      const int row = row0 + (lane & 15), ch = h * 4 + (lane >> 4);
       return *(const bf16x8 *)(lds + row * 128 + ((ch ^ (row & 7)) << 4));
     } else {
       typedef short s16x4 __attribute__((ext_vector_type(4)));
-      const int i = lane & 15, k = kk * 32 + (lane >> 4) * 8 + (i >> 2);
+      const int i = lane & 15, k = (lane >> 4) * 8 + (i >> 2);
       const int q = row0 >> 4;
       auto at = [&](int k) {
-        return (__attribute__((address_space(3))) s16x4 *)(lds + k * (R * 2) + piece(q, k) * 32 + (i & 3) * 8);
+        return (__attribute__((address_space(3))) s16x4 *)(lds + (h * kDenseHalf + k) * (R * 2) + piece(q, k) * 32 + (i & 3) * 8);
       };
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(k));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(k + 4));
@@ -128,38 +128,101 @@ struct DenseTile {
   }
 };
 
-template <int BM, int BN, int WM, int WN, bool AT, bool BT, int EPI>
+// The tile of workgroup b: 8 XCDs take the workgroups in turn, so each gets a contiguous share of the
+// order; in it, 8 tiles along n, then along m, so that the 32 workgroups of an XCD share the rows of
+// about 4 x 8 tiles in its L2.
+__device__ __forceinline__ void dense_tile_of(int b, int tiles_m, int tiles_n, int &tm, int &tn) {
+  const int total = tiles_m * tiles_n, x = b & 7, q = total >> 3, r = total & 7;
+  const int t = x * q + min(x, r) + (b >> 3);
+  const int group = t / (tiles_m * 8), n0 = group * 8, width = min(8, tiles_n - n0), in = t - group * tiles_m * 8;
+  tm = in / width;
+  tn = n0 + in % width;
+}
+
+// Stores 16 rows of 16-bit results of a wavefront: lane l holds the V values q[i] of row l % 16 from column
+// (4 i + l / 16) V on. They pass through LDS (`stage`, the wavefront's own, dense_stage_bytes) so that
+// a row leaves in 16-byte pieces side by side: stored from the accumulators' layout, in pieces of
+// 8 bytes over 16 rows, the gradient of the LM head ran at 2.3 TB/s.
+constexpr int dense_stage_bytes(int tm, int v) { return 16 * (tm * v * 8 + 16); }
+template <int TM, int V>
+__device__ __forceinline__ void dense_rows(uint8_t *stage, int lane, const uint16_t (&q)[TM][V], uint16_t *out, size_t ld, int rows, int cols) {
+  constexpr int kRow = TM * V * 8, kPieces = kRow / 16;  // bytes and 16-byte pieces of a row
+  typedef uint16_t vec __attribute__((ext_vector_type(V)));
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < TM; i++) *(vec *)(stage + (lane & 15) * (kRow + 16) + (4 * i + (lane >> 4)) * V * 2) = __builtin_bit_cast(vec, q[i]);
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int c = 0; c < 16 * kPieces; c += 64) {
+    const int at = c + lane, row = at / kPieces, piece = at % kPieces;
+    if (row < min(rows, 16) && piece * 8 < cols) *(uint4 *)(out + row * ld + piece * 8) = *(const uint4 *)(stage + row * (kRow + 16) + piece * 16);
+  }
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Takes the bf16 of each value, and leaves what it did not hold.
+template <int N>
+__device__ __forceinline__ void dense_take(float (&v)[N], uint16_t (&q)[N]) {
+#pragma unroll
+  for (int r = 0; r < N; r++) {
+    q[r] = dense_bf16(v[r]);
+    const float h = bf16_to_f32(q[r]);
+    v[r] = isfinite(h) ? v[r] - h : 0.0f;
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int NS, bool AT, bool BT, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   using TA = DenseTile<BM, W, AT>;
   using TB = DenseTile<BN, W, BT>;
   extern __shared__ __align__(16) uint8_t lds[];
-  constexpr int kSlot = TA::kBytes + TB::kBytes;
+  constexpr int kSlot = TA::kBytes + TB::kBytes, kLoads = TA::kLoads + TB::kLoads;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM;
-  const int tiles_m = (a.M + BM - 1) / BM;
-  const int tile = blockIdx.x;
-  const int m0 = tile % tiles_m * BM, n0 = tile / tiles_m * BN;
+  const int rows_b = a.N * a.stack;
+  const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (rows_b + BN - 1) / BN;
+  int tile_m, tile_n;
+  dense_tile_of(blockIdx.x, tiles_m, tiles_n, tile_m, tile_n);
+  const int m0 = tile_m * BM, n0 = tile_n * BN;
   const int split = blockIdx.y;
   const int k_lo = split * a.k_split, k_hi = min(a.K, k_lo + a.k_split);
   const int nk = (k_hi - k_lo + kDenseStep - 1) / kDenseStep, steps = nk * a.n_pass;
 
-  const uint32_t lds0 = str_lds(lds);
+  const uint32_t lds0 = str_lds(lds), lda = (uint32_t)a.lda * 2, ldb = (uint32_t)a.ldb * 2;
   TA la;
   TB lb;
-  la.init(wave, lane, a.M - m0, a.lda * 2);
-  lb.init(wave, lane, a.N - n0, a.ldb * 2);
-  int pass = 0, k0 = k_lo;  // of the next step to load
-  auto load = [&](int slot) {
-    const uint16_t *A = a.A + ((a.pa >> 4 * pass) & 15) * a.a_plane + (AT ? (size_t)k0 * a.lda + m0 : (size_t)m0 * a.lda + k0);
-    const uint16_t *B = a.B + ((a.pb >> 4 * pass) & 15) * a.b_plane + (BT ? (size_t)k0 * a.ldb + n0 : (size_t)n0 * a.ldb + k0);
-    la.load(A, a.lda * 2, k_hi - k0, lds0 + slot * kSlot, wave);
-    lb.load(B, a.ldb * 2, k_hi - k0, lds0 + slot * kSlot + TA::kBytes, wave);
-    k0 += kDenseStep;
-    if (k0 >= k_hi) {
-      k0 = k_lo;
+  // the step to load: its operands' addresses, k values left in its pass from there
+  int pass = 0, left = 0;
+  const uint16_t *pa = nullptr, *pb = nullptr;
+  const size_t step_a = AT ? a.lda * kDenseStep : kDenseStep, step_b = BT ? a.ldb * kDenseStep : kDenseStep;
+  auto next_load = [&]() __attribute__((always_inline)) {
+    left -= kDenseStep;
+    pa += step_a;
+    pb += step_b;
+    if (left <= 0) {
+      pa = a.A + ((a.pa >> 4 * pass) & 15) * a.a_plane + (AT ? (size_t)k_lo * a.lda + m0 : (size_t)m0 * a.lda + k_lo);
+      pb = a.B + ((a.pb >> 4 * pass) & 15) * a.b_plane + (BT ? (size_t)k_lo * a.ldb + n0 : (size_t)n0 * a.ldb + k_lo);
+      left = k_hi - k_lo;
       pass++;
+      la.init(wave, lane, a.M - m0, lda);
+      lb.init(wave, lane, rows_b - n0, ldb);
     }
+    if (left < kDenseStep) {
+      la.clamp(wave, lane, lda, left);
+      lb.clamp(wave, lane, ldb, left);
+    }
+  };
+  auto load_one = [&](int i, uint32_t slot) __attribute__((always_inline)) {
+    if (i < TA::kLoads)
+      la.load(i, pa, slot, wave);
+    else
+      lb.load(i - TA::kLoads, pb, slot + TA::kBytes, wave);
+  };
+  auto load = [&](uint32_t slot) __attribute__((always_inline)) {
+    next_load();
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) load_one(i, slot);
   };
 
   f32x4 acc[TM][TN];
@@ -167,155 +230,263 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   for (int i = 0; i < TM; i++)
 #pragma unroll
     for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  load(0);
-  int kt = 0;  // step within its pass
-  for (int s = 0; s < steps; s++) {
-    const int slot = s & 1;
-    uint8_t *sl = lds + slot * kSlot;
-    // this step's loads have landed, and the wavefront is done reading the other slot
+  // two sets of A fragments where the registers hold them, else one, whose rows take the next half as soon
+  // as their products are done
+  constexpr bool kTwoA = 4 * (TM * TN + 2 * (TM + TN)) <= 224;
+  constexpr bool kPinned = !AT || kTwoA;  // (the transposing loads' addresses take registers: 288 x 256 spilled)
+  bf16x8 fa0[TM], fa1[kTwoA ? TM : 1], fb0[TN], fb1[TN];
+  auto read_b = [&](const uint8_t *sl, int half, int j) __attribute__((always_inline)) { return TB::frag(sl + TA::kBytes, (wn * TN + j) * 16, half, lane); };
+  auto read_a = [&](const uint8_t *sl, int half, int i) __attribute__((always_inline)) { return TA::frag(sl, (wm * TM + i) * 16, half, lane); };
+  // The products of a half (fa, fb), row by row, and between the rows the reads of the half after it (`half`
+  // of sl, into na and nb, if READ) and the LDS-DMAs of the step after the next (into slot `to`, if DMA): issued in
+  // one go they held the MFMAs up, as the LDS serves 8 wavefronts' 12 reads in 768 cycles (256 x 256: 958
+  // against 1130 TFLOP/s). The reads come in the first three quarters of the rows.
+  auto multiply = [&](auto DMA, auto READ, auto &fa, const bf16x8(&fb)[TN], auto &na, bf16x8(&nb)[TN], const uint8_t *sl, int half, uint32_t to) __attribute__((always_inline)) {
+    constexpr int kReads = kTwoA ? TN + TM : TN, kOver = (3 * TM + 3) / 4, kEach = (kReads + kOver - 1) / kOver;
+    constexpr int kDma = kPinned ? (kLoads + TM - 1) / TM : kLoads;
+    if constexpr (kPinned) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      if constexpr (decltype(DMA)::value && !kPinned) {
+#pragma unroll
+        for (int l = i * kDma; l < (i + 1) * kDma && l < kLoads; l++) load_one(l, to);
+      }
+      if constexpr (decltype(READ)::value) {
+#pragma unroll
+        for (int r = i * kEach; r < (i + 1) * kEach && r < kReads; r++) {
+          if (r < TN)
+            nb[r] = read_b(sl, half, r);
+          else
+            na[r - TN] = read_a(sl, half, r - TN);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+      if constexpr (!kTwoA && decltype(READ)::value) fa[i] = read_a(sl, half, i);
+      if constexpr (decltype(DMA)::value && kPinned) {
+#pragma unroll
+        for (int l = i * kDma; l < (i + 1) * kDma && l < kLoads; l++) load_one(l, to);
+      }
+      if constexpr (kPinned) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  // this wavefront's loads have landed, up to those of the `NS - 2` steps after it if MORE are on their way,
+  // and its reads are done, and every other's
+  auto meet = [&](auto MORE) __attribute__((always_inline)) {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(vm_lgkm_wait(0));
+    __builtin_amdgcn_s_waitcnt(vm_lgkm_wait(decltype(MORE)::value ? (NS - 2) * kLoads : 0));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + 1 < steps) load(slot ^ 1);
-    const int left = k_hi - k_lo - kt * kDenseStep;
-    kt = kt + 1 == nk ? 0 : kt + 1;
-    if (left < kDenseStep) {
-      TA::zero_tail(sl, left, tid, 64 * W);
-      TB::zero_tail(sl + TA::kBytes, left, tid, 64 * W);
-      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt 0
+  };
+  int here = k_hi - k_lo;  // k values left in its pass from the next step to be read
+  auto zero = [&](uint8_t *sl) __attribute__((always_inline)) {
+    if (here < kDenseStep) {
+      TA::zero_tail(sl, here, tid, 64 * W);
+      TB::zero_tail(sl + TA::kBytes, here, tid, 64 * W);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     }
+    here -= kDenseStep;
+    if (here <= 0) here = k_hi - k_lo;
+  };
+  auto landed = [&](auto MORE, uint8_t *sl) __attribute__((always_inline)) {
+    meet(MORE);
+    zero(sl);
+  };
+  for (int t = 0; t < NS && t < steps; t++) load(lds0 + t * kSlot);
+  if (NS <= steps)  // step 0 is there
+    __builtin_amdgcn_s_waitcnt(vm_wait((NS - 1) * kLoads));
+  else
+    __builtin_amdgcn_s_waitcnt(vm_wait(0));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  zero(lds);
 #pragma unroll
-    for (int kk = 0; kk < 2; kk++) {
-      bf16x8 fb[TN];
+  for (int j = 0; j < TN; j++) fb0[j] = read_b(lds, 0, j);
 #pragma unroll
-      for (int j = 0; j < TN; j++) fb[j] = TB::frag(sl + TA::kBytes, (wn * TN + j) * 16, kk, lane);
+  for (int i = 0; i < TM; i++) fa0[i] = read_a(lds, 0, i);
+  uint32_t cur = 0;
+  auto &fa_odd = [&]() -> auto & {
+    if constexpr (kTwoA) return fa1; else return fa0;
+  }();
+  auto after = [&](uint32_t slot) __attribute__((always_inline)) {
+    const uint32_t n = slot + kSlot;
+    return n == NS * kSlot ? 0u : n;
+  };
+  int s = 0;
+  for (; s + NS < steps; s++) {
+    const uint32_t next = after(cur);
+    multiply(no, yes, fa0, fb0, fa_odd, fb1, lds + cur, 1, 0);
+    landed(yes, lds + next);
+    next_load();
+    multiply(yes, yes, fa_odd, fb1, fa0, fb0, lds + next, 0, lds0 + cur);
+    cur = next;
+  }
+  for (; s + 1 < steps; s++) {
+    const uint32_t next = after(cur);
+    multiply(no, yes, fa0, fb0, fa_odd, fb1, lds + cur, 1, 0);
+    landed(no, lds + next);
+    multiply(no, yes, fa_odd, fb1, fa0, fb0, lds + next, 0, 0);
+    cur = next;
+  }
+  multiply(no, yes, fa0, fb0, fa_odd, fb1, lds + cur, 1, 0);
+  multiply(no, no, fa_odd, fb1, fa0, fb0, lds, 0, 0);
+
+  if constexpr (BM * BN * 4 <= NS * kSlot && BN <= 64) {
+    // B's planes were stacked as rows of one pass (so that A, which few rows wait for, streams once): a
+    // column's result is the sum of its planes' columns, from the lowest terms up
+    if (a.stack > 1) {
+      __syncthreads();
+      float *o = (float *)lds;
 #pragma unroll
-      for (int i = 0; i < TM; i++) {
-        const bf16x8 fa = TA::frag(sl, (wm * TM + i) * 16, kk, lane);
+      for (int j = 0; j < TN; j++)
 #pragma unroll
-        for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
+        for (int i = 0; i < TM; i++)
+          *(f32x4 *)(o + ((wn * TN + j) * 16 + (lane & 15)) * BM + (wm * TM + i) * 16 + (lane >> 4) * 4) = acc[i][j];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < TN; j++) {
+        const int n = (wn * TN + j) * 16 + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+          f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          if (n < a.N)
+            for (int p = a.stack - 1; p >= 0; p--) v += *(const f32x4 *)(o + (p * a.N + n) * BM + (wm * TM + i) * 16 + (lane >> 4) * 4);
+          acc[i][j] = v;
+        }
       }
     }
   }
 
   // lane: column n = lane % 16 of each tile, rows m = lane / 16 * 4 + 0..3
   const int mw = m0 + wm * TM * 16 + (lane >> 4) * 4, nw = n0 + wn * TN * 16 + (lane & 15);
+  // the wavefront's first row and column, and its part of the LDS for 16-bit results
+  const int m_first = m0 + wm * TM * 16, n_first = n0 + wn * TN * 16;
+  constexpr int kStage = dense_stage_bytes(TM, EPI == DENSE_DGATE ? 8 : 4);
+  static_assert(W * kStage <= NS * kSlot, "the results of 16 columns fit the LDS of the steps");
+  uint8_t *stage = lds + wave * kStage;
+  if constexpr (EPI != DENSE_STATS && EPI != DENSE_GATE_RAW) __syncthreads();
+  if constexpr (EPI == DENSE_STORE || EPI == DENSE_GATE || EPI == DENSE_GATE_RAW) {
+    const float scale = EPI == DENSE_STORE && a.scale ? *a.scale : 1.0f;
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      f32x4 b = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (a.bias && mw + i * 16 < a.M) b = *(const f32x4 *)(a.bias + mw + i * 16);
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[i][j] = (acc[i][j] + b) * scale;
+    }
+  }
   if constexpr (EPI == DENSE_STORE) {
 #pragma unroll
     for (int j = 0; j < TN; j++) {
       const int n = nw + j * 16;
-      if (n >= a.N) continue;
+      if (a.out_mode == 0) {
+        uint16_t q[TM][4];
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) q[i][r] = dense_bf16(acc[i][j][r]);
+        dense_rows<TM, 4>(stage, lane, q, (uint16_t *)a.out + (size_t)(n_first + j * 16) * a.ldo + m_first, a.ldo, a.N - n_first - j * 16, a.M - m_first);
+        continue;
+      }
 #pragma unroll
       for (int i = 0; i < TM; i++) {
         const int m = mw + i * 16;
-        if (m >= a.M) continue;
-        float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
-        if (a.bias) {
-          const float4 b = *(const float4 *)(a.bias + m);
-          v.x += b.x, v.y += b.y, v.z += b.z, v.w += b.w;
-        }
-        const size_t at = (size_t)n * a.ldo + m;
-        if (a.out_mode == 0) {
-          const uint2 u = {dense_bf16(v.x) | (uint32_t)dense_bf16(v.y) << 16, dense_bf16(v.z) | (uint32_t)dense_bf16(v.w) << 16};
-          *(uint2 *)((uint16_t *)a.out + at) = u;
-        } else {
-          float4 *o = (float4 *)((float *)a.out + split * a.split_stride + at);
-          if (a.out_mode == 2) {
-            const float4 b = *o;
-            v.x += b.x, v.y += b.y, v.z += b.z, v.w += b.w;
-          }
-          *o = v;
-        }
+        if (n >= a.N || m >= a.M) continue;
+        f32x4 *o = (f32x4 *)((float *)a.out + split * a.split_stride + (size_t)n * a.ldo + m);
+        *o = a.out_mode == 2 ? acc[i][j] + *o : acc[i][j];
       }
     }
-  } else if constexpr (EPI == DENSE_GATE || EPI == DENSE_GATE_RAW) {
+  } else if constexpr (EPI == DENSE_GATE_RAW) {
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+        if (nw + j * 16 < a.N && mw + i * 16 < a.M) *(f32x4 *)(a.gu + (size_t)(nw + j * 16) * a.M + mw + i * 16) = acc[i][j];
+  } else if constexpr (EPI == DENSE_GATE) {
 #pragma unroll
     for (int j = 0; j < TN; j++) {
-      const int n = nw + j * 16;
-      if (n >= a.N) continue;
+      float h[TM][2];
 #pragma unroll
-      for (int i = 0; i < TM; i++) {
-        const int m = mw + i * 16;
-        if (m >= a.M) continue;
-        float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
-        if (a.bias) {
-          const float4 b = *(const float4 *)(a.bias + m);
-          v.x += b.x, v.y += b.y, v.z += b.z, v.w += b.w;
-        }
-        if constexpr (EPI == DENSE_GATE_RAW) {
-          *(float4 *)(a.gu + (size_t)n * a.M + m) = v;
-        } else {
-          const float h0 = DenseGate(v.x, v.y, a.limit).h(), h1 = DenseGate(v.z, v.w, a.limit).h();
-          uint16_t *o = a.h + (size_t)n * a.ldh + m / 2;
-          if (a.planes == 1) {
-            *(uint32_t *)o = dense_bf16(h0) | (uint32_t)dense_bf16(h1) << 16;
-          } else {
-            uint16_t p0[kPlanes], p1[kPlanes];
-            dense_split(h0, p0);
-            dense_split(h1, p1);
+      for (int i = 0; i < TM; i++)
 #pragma unroll
-            for (int p = 0; p < kPlanes; p++) *(uint32_t *)(o + p * a.h_plane) = p0[p] | (uint32_t)p1[p] << 16;
-          }
-        }
+        for (int r = 0; r < 2; r++) h[i][r] = DenseGate(acc[i][j][2 * r], acc[i][j][2 * r + 1], a.limit).h();
+      for (int p = 0; p < a.planes; p++) {
+        uint16_t q[TM][2];
+#pragma unroll
+        for (int i = 0; i < TM; i++) dense_take(h[i], q[i]);
+        dense_rows<TM, 2>(stage, lane, q, a.h + p * a.h_plane + (size_t)(n_first + j * 16) * a.ldh + m_first / 2, a.ldh,
+                          a.N - n_first - j * 16, (a.M - m_first) / 2);
       }
     }
   } else if constexpr (EPI == DENSE_DGATE) {
+    constexpr int G = TM % 4 == 0 ? 4 : TM % 3 == 0 ? 3 : TM % 2 == 0 ? 2 : 1;  // tiles at a time, for the registers
 #pragma unroll
-    for (int i = 0; i < TM; i++) {
-      const int m = mw + i * 16;
-      float db[8];
+    for (int g0 = 0; g0 < TM; g0 += G) {
+      float db[G][8];
 #pragma unroll
-      for (int r = 0; r < 8; r++) db[r] = 0.0f;
+      for (int i = 0; i < G; i++)
+#pragma unroll
+        for (int r = 0; r < 8; r++) db[i][r] = 0.0f;
 #pragma unroll
       for (int j = 0; j < TN; j++) {
         const int n = nw + j * 16;
-        if (n >= a.N || m >= a.M) continue;
-        const float *row = a.gu + (size_t)n * a.M * 2 + 2 * m;
-        const float4 g01 = *(const float4 *)row, g23 = *(const float4 *)(row + 4);
-        const float gate[4] = {g01.x, g01.z, g23.x, g23.z}, up[4] = {g01.y, g01.w, g23.y, g23.w};
-        float d[8], hv[4];
+        float d[G][8], hv[G][4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const DenseGate g(gate[r], up[r], a.limit);
-          const float dh = acc[i][j][r];
-          hv[r] = g.h();
-          d[2 * r] = gate[r] > a.limit ? 0.0f : dh * (g.U + 1.0f) * (g.s * (1.0f + 1.702f * (g.G * (1.0f - g.s))));
-          d[2 * r + 1] = fabsf(up[r]) > a.limit ? 0.0f : dh * (g.G * g.s);
-        }
-#pragma unroll
-        for (int r = 0; r < 8; r++) db[r] += d[r];
-        for (int p = 0; p < a.planes; p++) {  // each plane takes what the planes before it left
-          uint16_t q[8], e[4];
-#pragma unroll
-          for (int r = 0; r < 8; r++) {
-            q[r] = dense_bf16(d[r]);
-            d[r] = isfinite(bf16_to_f32(q[r])) ? d[r] - bf16_to_f32(q[r]) : 0.0f;
+        for (int i = 0; i < G; i++) {
+          const int m = mw + (g0 + i) * 16;
+          f32x4 g01 = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, g23 = g01;
+          const bool in = n < a.N && m < a.M;
+          if (in) {
+            const f32x4 *row = (const f32x4 *)(a.gu + (size_t)n * a.M * 2 + 2 * m);
+            g01 = row[0];
+            g23 = row[1];
           }
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            e[r] = dense_bf16(hv[r]);
-            hv[r] = isfinite(bf16_to_f32(e[r])) ? hv[r] - bf16_to_f32(e[r]) : 0.0f;
+            const float gate = r < 2 ? g01[2 * r] : g23[2 * r - 4], up = r < 2 ? g01[2 * r + 1] : g23[2 * r - 3];
+            const DenseGate g(gate, up, a.limit);
+            const float dh = acc[g0 + i][j][r];
+            hv[i][r] = g.h();
+            d[i][2 * r] = gate > a.limit ? 0.0f : dh * (g.U + 1.0f) * (g.s * (1.0f + 1.702f * (g.G * (1.0f - g.s))));
+            d[i][2 * r + 1] = fabsf(up) > a.limit ? 0.0f : dh * (g.G * g.s);
           }
-          *(uint4 *)(a.dgu + p * a.dgu_plane + (size_t)n * a.M * 2 + 2 * m) = __builtin_bit_cast(uint4, q);
-          *(uint2 *)(a.h + p * a.h_plane + (size_t)n * a.ldh + m) = __builtin_bit_cast(uint2, e);
+#pragma unroll
+          for (int r = 0; r < 8; r++) db[i][r] += in ? d[i][r] : 0.0f;
+        }
+        const int rows = a.N - n_first - j * 16, m1 = m_first + g0 * 16;
+        for (int p = 0; p < a.planes; p++) {
+          uint16_t q[G][8], e[G][4];
+#pragma unroll
+          for (int i = 0; i < G; i++) {
+            dense_take(d[i], q[i]);
+            dense_take(hv[i], e[i]);
+          }
+          dense_rows<G, 8>(stage, lane, q, a.dgu + p * a.dgu_plane + (size_t)(n_first + j * 16) * a.M * 2 + 2 * m1, (size_t)a.M * 2, rows, 2 * (a.M - m1));
+          dense_rows<G, 4>(stage, lane, e, a.h + p * a.h_plane + (size_t)(n_first + j * 16) * a.ldh + m1, a.ldh, rows, a.M - m1);
         }
       }
       if (a.db_part) {  // over the wavefront's columns: 16 lanes, then a part per wavefront column
 #pragma unroll
-        for (int r = 0; r < 8; r++) {
-          db[r] += __shfl_xor(db[r], 1);
-          db[r] += __shfl_xor(db[r], 2);
-          db[r] += __shfl_xor(db[r], 4);
-          db[r] += __shfl_xor(db[r], 8);
-        }
-        if ((lane & 15) == 0 && m < a.M) {
-          float *o = a.db_part + (size_t)(tile / tiles_m * WN + wn) * a.M * 2 + 2 * m;
-          *(float4 *)o = make_float4(db[0], db[1], db[2], db[3]);
-          *(float4 *)(o + 4) = make_float4(db[4], db[5], db[6], db[7]);
+        for (int i = 0; i < G; i++) {
+#pragma unroll
+          for (int r = 0; r < 8; r++) {
+            float v = db[i][r];
+            v += __shfl_xor(v, 1);
+            v += __shfl_xor(v, 2);
+            v += __shfl_xor(v, 4);
+            v += __shfl_xor(v, 8);
+            db[i][r] = v;
+          }
+          const int m = mw + (g0 + i) * 16;
+          if ((lane & 15) == 0 && m < a.M) {
+            f32x4 *o = (f32x4 *)(a.db_part + (size_t)(tile_n * WN + wn) * a.M * 2 + 2 * m);
+            o[0] = f32x4{db[i][0], db[i][1], db[i][2], db[i][3]};
+            o[1] = f32x4{db[i][4], db[i][5], db[i][6], db[i][7]};
+          }
         }
       }
     }
@@ -350,48 +521,44 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
       if (nan) sum = NAN;
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
-      if (lane < 16 && n < a.N) a.stats[(size_t)(tile % tiles_m * WM + wm) * a.N + n] = make_float2(mx, sum);
+      if (lane < 16 && n < a.N) a.stats[(size_t)(tile_m * WM + wm) * a.N + n] = make_float2(mx, sum);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < TN; j++) {
-      const int n = nw + j * 16;
-      if (n >= a.N) continue;
+      const int n = min(nw + j * 16, a.N - 1);  // (columns past N are not stored)
       const int t = a.targets[n];
-      const float lse = a.lse[n], scale = a.dloss[n];
+      const float lse = a.lse[n], scale = a.dloss[n] / *a.scale;
+      float d[TM][4];
 #pragma unroll
-      for (int i = 0; i < TM; i++) {
-        const int m = mw + i * 16;
-        if ((size_t)m >= a.ld_dl) continue;
-        float d[4];
+      for (int i = 0; i < TM; i++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          d[r] = scale * (dense_exp(acc[i][j][r] - lse) - (a.v0 + m + r == t ? 1.0f : 0.0f));
-          if (t >= a.vocab) d[r] = NAN;
-          if (t < 0 || m + r >= a.M) d[r] = 0.0f;  // ignored token, padding column
+          const int m = mw + i * 16 + r;
+          d[i][r] = scale * (dense_exp(acc[i][j][r] - lse) - (a.v0 + m == t ? 1.0f : 0.0f));
+          if (t >= a.vocab) d[i][r] = NAN;
+          if (t < 0 || m >= a.M) d[i][r] = 0.0f;  // ignored token, padding column
         }
-        for (int p = 0; p < a.planes; p++) {
-          uint16_t q[4];
+      for (int p = 0; p < a.planes; p++) {
+        uint16_t q[TM][4];
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            q[r] = dense_bf16(d[r]);
-            d[r] = isfinite(bf16_to_f32(q[r])) ? d[r] - bf16_to_f32(q[r]) : 0.0f;
-          }
-          *(uint2 *)(a.dl + p * a.dl_plane + (size_t)n * a.ld_dl + m) = __builtin_bit_cast(uint2, q);
-        }
+        for (int i = 0; i < TM; i++) dense_take(d[i], q[i]);
+        dense_rows<TM, 4>(stage, lane, q, a.dl + p * a.dl_plane + (size_t)(n_first + j * 16) * a.ld_dl + m_first, a.ld_dl,
+                          a.N - n_first - j * 16, (int)a.ld_dl - m_first);
       }
     }
   }
 }
 
-template <int BM, int BN, int WM, int WN, bool AT, bool BT, int EPI>
+template <int BM, int BN, int WM, int WN, int NS, bool AT, bool BT, int EPI>
 hipError_t launch_dense_as(const DenseArgs &a, hipStream_t st) {
   static DynLdsOnce once;
-  const size_t bytes = 2 * (BM + BN) * 128;
-  auto kernel = k_dense<BM, BN, WM, WN, AT, BT, EPI>;
+  const size_t bytes = NS * (BM + BN) * 128;
+  auto kernel = k_dense<BM, BN, WM, WN, NS, AT, BT, EPI>;
   hipError_t e = ensure_dyn_lds(once, (const void *)kernel, bytes);
   if (e != hipSuccess) return e;
-  const size_t tiles = (size_t)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
+  const size_t tiles = (size_t)((a.M + BM - 1) / BM) * ((a.N * a.stack + BN - 1) / BN);
+  if (a.stack > 1 && (a.N * a.stack > BN || BN > 64)) return hipErrorInvalidValue;
   if (tiles > 0x7FFFFFFF || a.splits > 65535) return hipErrorInvalidValue;
   kernel<<<dim3((unsigned)tiles, a.splits), 64 * WM * WN, bytes, st>>>(a);
   return hipGetLastError();

@@ -4,28 +4,48 @@
 
 namespace moe {
 
-enum DenseTileShape { TILE_128x16, TILE_128x128 };
+// X(name, rows, columns, wavefronts along each, LDS slots, workgroups of a CU, TFLOP/s of the device full of
+// them). The rates are those of 2880 k values (loss over 201088 rows, 512 tokens and more).
+#define MOE_DENSE_TILES(X)                   \
+  X(288x256, 288, 256, 2, 4, 2, 1, 1115.0)   \
+  X(256x256, 256, 256, 2, 4, 2, 1, 1125.0)   \
+  X(192x256, 192, 256, 2, 4, 2, 1, 1050.0)   \
+  X(128x128, 128, 128, 2, 2, 2, 2, 906.0)    \
+  X(128x64, 128, 64, 2, 2, 3, 2, 660.0)      \
+  X(64x64, 64, 64, 2, 2, 4, 2, 500.0)        \
+  X(32x64, 32, 64, 2, 2, 6, 2, 340.0)        \
+  X(32x32, 32, 32, 2, 2, 8, 2, 240.0)        \
+  X(32x16, 32, 16, 2, 1, 8, 3, 190.0)        \
+  X(128x16, 128, 16, 4, 1, 4, 2, 200.0)
 
-inline DenseTileShape dense_tile(const DenseArgs &a) { return a.N <= 16 ? TILE_128x16 : TILE_128x128; }
+enum DenseTileShape {
+#define X(name, bm, bn, wm, wn, ns, wgs, rate) TILE_##name,
+  MOE_DENSE_TILES(X)
+#undef X
+};
+
+DenseTileShape dense_tile(const DenseShape &s, const DenseArgs &a);
 
 template <bool AT, bool BT, int EPI>
 hipError_t launch_dense_shape(const DenseArgs &a, hipStream_t st) {
-  switch (dense_tile(a)) {
-    case TILE_128x16: return launch_dense_as<128, 16, 4, 1, AT, BT, EPI>(a, st);
-    default: return launch_dense_as<128, 128, 2, 2, AT, BT, EPI>(a, st);
+  switch (dense_tile(DenseShape{AT, BT, (DenseEpi)EPI}, a)) {
+#define X(name, bm, bn, wm, wn, ns, wgs, rate) \
+  case TILE_##name: return launch_dense_as<bm, bn, wm, wn, ns, AT, BT, EPI>(a, st);
+    MOE_DENSE_TILES(X)
+#undef X
   }
+  return hipErrorInvalidValue;
 }
 
-// rows and columns of a tile, and its wavefronts along each
 struct DenseTileDims {
-  int bm, bn, wm, wn;
+  int bm, bn, wm, wn, ns, wgs;
+  double rate;
 };
-inline DenseTileDims dense_tile_dims(DenseTileShape s) {
-  switch (s) {
-    case TILE_128x16: return {128, 16, 4, 1};
-    default: return {128, 128, 2, 2};
-  }
-}
+constexpr DenseTileDims kDenseTiles[] = {
+#define X(name, bm, bn, wm, wn, ns, wgs, rate) {bm, bn, wm, wn, ns, wgs, rate},
+    MOE_DENSE_TILES(X)
+#undef X
+};
 
 hipError_t launch_dense_nt(const DenseShape &s, const DenseArgs &a, hipStream_t st);
 hipError_t launch_dense_tn(const DenseShape &s, const DenseArgs &a, hipStream_t st);

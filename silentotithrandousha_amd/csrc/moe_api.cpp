@@ -1424,7 +1424,7 @@ int ctx_dims(const moe_ctx *c, size_t *H, size_t *I) {
 // Makes the context's device current and describes it.
 int dense_ctx(moe_ctx *c, DenseCtx *d) {
   RETURN_IF(use_dev(c));
-  *d = DenseCtx{c->stream, c->H, c->clamp, c->lm_bf16 ? (const uint16_t *)c->lm_w.p : nullptr, c->lm_vocab, c->n_cu, &c->dense};
+  *d = DenseCtx{c->stream, c->H, c->clamp, c->lm_bf16 ? (const uint16_t *)c->lm_w.p : nullptr, c->lm_vocab, &c->dense};
   return MOE_OK;
 }
 }  // namespace moe

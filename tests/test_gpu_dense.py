@@ -2,6 +2,7 @@
 (tests/dense_ref.py): the loss over the LM head and its gradient, the gated block and its backward pass,
 8-bit checkpoints; their refusals, graphs, streams and workspaces; and a run of them together."""
 import ctypes
+import gc
 
 import numpy as np
 import pytest
@@ -633,6 +634,26 @@ class Step:
             check(lib().moe_memset_device(o.ptr, 0xEE, o.n))
 
 
+class Capture:
+    """Captures the context's stream into a graph. No garbage is collected meanwhile: a buffer freed by the
+    collector (hipFree) would end the capture."""
+
+    def __init__(self, d):
+        self.d, self.graph = d, ctypes.c_void_p()
+
+    def __enter__(self):
+        gc.collect()
+        gc.disable()
+        check(lib().moe_graph_begin(self.d.ctx))
+        return self
+
+    def __exit__(self, *exc):
+        rc = lib().moe_graph_end(self.d.ctx, ctypes.byref(self.graph))
+        gc.enable()
+        if exc[0] is None:
+            check(rc)
+
+
 def same(a, b):
     return all(np.array_equal(a[n], b[n], equal_nan=True) for n in a)
 
@@ -648,23 +669,21 @@ def test_steps_in_graphs(dtype):
     try:
         steps = [Step(d, dtype, 20, H, I, V, 1), Step(d, dtype, 33, H, I, V, 2)]
         refused_first = Step(d, dtype, 20, H, I, V, 1)
-        check(lib().moe_graph_begin(d.ctx))
-        with pytest.raises(MoeError):  # the workspace has no size yet
-            refused_first.enqueue()
-        g = ctypes.c_void_p()
-        if lib().moe_graph_end(d.ctx, ctypes.byref(g)) == 0 and g.value:
-            lib().moe_graph_destroy(g)
+        with pytest.raises(MoeError) as e:  # the workspace has no size yet
+            with Capture(d) as g:
+                refused_first.enqueue()
+        assert "workspace" in str(e.value)
+        if g.graph.value:
+            lib().moe_graph_destroy(g.graph)
         eager = []
         for s in steps:
             s.enqueue()
             d.synchronize()
             eager.append(s.get())
         for s in steps:
-            check(lib().moe_graph_begin(d.ctx))
-            s.enqueue()
-            g = ctypes.c_void_p()
-            check(lib().moe_graph_end(d.ctx, ctypes.byref(g)))
-            graphs.append(g)
+            with Capture(d) as g:
+                s.enqueue()
+            graphs.append(g.graph)
         large = Step(d, dtype, 150, H, I, V, 3)
         for rep in range(3):
             for s, g, want in zip(steps, graphs, eager):
