@@ -3,7 +3,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 
 #include "dense_launch.hpp"
 
@@ -20,18 +19,27 @@ int split_k(const DenseArgs &a) {
 constexpr int kCus = 256;  // of an MI355X: the plan is for the whole device
 
 // Estimated us of a product on one tile shape with its K in `splits` parts. A workgroup's step takes the
-// larger of the time that its products take at the tile's full rate (shared by the workgroups of its CU)
-// and of the time that its loads wait for memory, spread over the steps that its slots hold ahead; each
-// workgroup has a prologue and an epilogue, parts are written and summed in another launch. Against
-// measurements of 9 shapes at 1 to 4096 rows (2880 x 2880 block, 201088 x 2880 head) it picks a tile
-// within 8 % of the fastest.
-double dense_us(const DenseTileDims &d, const DenseArgs &a, int splits) {
-  const double tiles = (double)((a.M + d.bm - 1) / d.bm) * (((long)a.N * a.stack + d.bn - 1) / d.bn) * splits;
+// largest of the time that its products take at the tile's full rate, that its loads of A take where A is
+// read once, from memory (both shared by the workgroups of its CU), and that its loads wait, spread over
+// the steps that its slots hold ahead; each workgroup has a prologue and an epilogue that stores its
+// results (under the steps of the others of its CU, if any); parts are written and summed in another
+// launch. Whole rounds of workgroups and what is left for the last one count apart.
+double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a, int splits) {
+  const long tiles_n = ((long)a.N * a.stack + d.bn - 1) / d.bn, tiles = (long)((a.M + d.bm - 1) / d.bm) * tiles_n * splits;
   const long steps = (((long)a.K + kDenseStep - 1) / kDenseStep * a.n_pass + splits - 1) / splits;
-  const double full = tiles / (kCus * d.wgs), on_cu = std::min<double>(d.wgs, std::max(1.0, tiles / kCus));
-  const double rounds = d.wgs == 1 ? std::ceil(full) : std::max(1.0, full);
-  const double step = std::max(0.45 / (d.ns - 1) + 0.1, on_cu * d.bm * d.bn * 2.0 * kDenseStep * kCus / (d.rate * 1e6));
-  double us = rounds * (steps * step + 2.5);
+  // bytes that a result costs, about
+  const double result = s.epi == DENSE_STATS ? 0.0 : s.epi == DENSE_GATE ? 1.0 : s.epi == DENSE_GATE_RAW ? 4.0 : s.epi == DENSE_DGATE ? 14.0
+                        : s.epi == DENSE_STORE && (a.out_mode || splits > 1) ? 4.0 : 2.0;
+  // a transposed A's rows of k are read in pieces of a tile's rows: below 128 bytes at two thirds of the rate
+  const double memory = s.at && d.bm < 64 ? 15.0 : 23.0;  // GB/s a CU; 5.9 TB/s in all
+  auto round = [&](long on_cu) {
+    double step = std::max(0.45 / (d.ns - 1) + 0.1, on_cu * d.bm * d.bn * 2.0 * kDenseStep * kCus / (d.rate * 1e6));
+    if (tiles_n == 1) step = std::max(step, on_cu * d.bm * 128e-3 / memory);
+    const double stores = on_cu * d.bm * d.bn * result * kCus / 4.5e6;  // us at 4.5 TB/s
+    return steps * step + 2.5 + (d.wgs == 1 ? stores : 0.5 * stores);
+  };
+  const long whole = tiles / (kCus * d.wgs), rest = tiles - whole * kCus * d.wgs;
+  double us = whole * round(d.wgs) + (rest ? round((rest + kCus - 1) / kCus) : 0.0);
   if (splits > 1) us += 3.0 + 8e-6 / 4 * splits * a.M * a.N;
   return us;
 }
@@ -44,7 +52,9 @@ DenseTileShape dense_tile(const DenseShape &s, const DenseArgs &a) {
   for (int t = 0; t < (int)(sizeof(kDenseTiles) / sizeof(kDenseTiles[0])); t++) {
     const DenseTileDims &d = kDenseTiles[t];
     if (a.stack > 1 && (d.bn > 64 || a.N * a.stack > d.bn)) continue;  // stacked planes lie in one tile
-    const double u = dense_us(d, a, dense_split_count(a));
+    // 288 rows: K-contiguous they keep too much in registers (620 TFLOP/s), and their epilogue spills
+    if (d.bm > 256 && (!s.at || a.K < 1024)) continue;
+    const double u = dense_us(s, d, a, dense_split_count(a));
     if (best < 0 || u < us) best = t, us = u;
   }
   return (DenseTileShape)best;
@@ -71,7 +81,7 @@ int dense_splits(const DenseShape &s, const DenseArgs &a0) {
     DenseArgs a = a0;
     a.splits = n;
     a.splits = dense_split_count(a);
-    const double u = dense_us(kDenseTiles[dense_tile(s, a)], a, a.splits);
+    const double u = dense_us(s, kDenseTiles[dense_tile(s, a)], a, a.splits);
     if (n == 1 || u < us) best = a.splits, us = u;
   }
   return best;
@@ -101,34 +111,90 @@ __global__ void k_planes(const float *x, size_t n, uint16_t *out, size_t plane) 
   }
 }
 
+// Sums of parts, in order. Many values: a thread each, 8 parts' loads in flight. Few (bias gradients):
+// a block takes 32 values and 8 spans of the parts, whose sums join in order.
 template <bool BF>
-__global__ void k_sum_parts(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias,
-                            void *out) {
+__device__ __forceinline__ void put(void *out, size_t i, float s) {
+  if constexpr (BF)
+    ((uint16_t *)out)[i] = dense_bf16(s);
+  else
+    ((float *)out)[i] = s;
+}
+__device__ __forceinline__ float sum_span(const float *part, size_t stride, int p0, int p1) {
+  float s = 0.0f;
+  int p = p0;
+  for (; p + 8 <= p1; p += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = part[(size_t)(p + i) * stride];
+#pragma unroll
+    for (int i = 0; i < 8; i++) s += v[i];
+  }
+  for (; p < p1; p++) s += part[(size_t)p * stride];
+  return s;
+}
+template <bool BF>
+__global__ __launch_bounds__(256) void k_sum_parts(const float *part, size_t stride, int parts, size_t n, const float *bias,
+                                                   size_t n_bias, void *out) {
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-    float s = 0.0f;
-    for (int p = 0; p < parts; p++) s += part[p * stride + i];
+    float s = sum_span(part + i, stride, 0, parts);
     if (bias) s += bias[i % n_bias];
-    if constexpr (BF)
-      ((uint16_t *)out)[i] = dense_bf16(s);
-    else
-      ((float *)out)[i] = s;
+    put<BF>(out, i, s);
+  }
+}
+__global__ __launch_bounds__(256) void k_sum_few(const float *part, size_t stride, int parts, size_t n, float *out) {
+  __shared__ float s_sum[8][32];
+  const size_t i = (size_t)blockIdx.x * 32 + threadIdx.x % 32;
+  const int span = threadIdx.x / 32, each = (parts + 7) / 8;
+  if (i < n) s_sum[span][threadIdx.x % 32] = sum_span(part + i, stride, min(span * each, parts), min((span + 1) * each, parts));
+  __syncthreads();
+  if (span == 0 && i < n) {
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) s += s_sum[j][threadIdx.x];
+    out[i] = s;
   }
 }
 
-constexpr int kColRows = 64;  // rows per part
+// A block sums 64 rows of 256 columns: 8 rows at a time by 32 threads of 8 columns.
+constexpr int kColRows = 64;
 template <bool BF>
-__global__ void k_colsum(const void *x, size_t T, size_t H, float *part) {
-  const size_t c = (size_t)blockIdx.x * 256 + threadIdx.x, t0 = (size_t)blockIdx.y * kColRows;
-  if (c >= H) return;
-  const size_t t1 = t0 + kColRows < T ? t0 + kColRows : T;
-  float s = 0.0f;
-  for (size_t t = t0; t < t1; t++) {
-    if constexpr (BF)
-      s += bf16_to_f32(((const uint16_t *)x)[t * H + c]);
-    else
-      s += ((const float *)x)[t * H + c];
+__global__ __launch_bounds__(256) void k_colsum(const void *x, size_t T, size_t H, float *part) {
+  __shared__ float s_sum[8][256];
+  const int in = threadIdx.x % 32, row = threadIdx.x / 32;
+  const size_t c = (size_t)blockIdx.x * 256 + in * 8, t0 = (size_t)blockIdx.y * kColRows;
+  float s[8] = {};
+  if (c < H) {  // (H is a multiple of 32)
+#pragma unroll
+    for (int k = 0; k < kColRows / 8; k++) {
+      const size_t t = t0 + row + k * 8;
+      if (t >= T) break;
+      float v[8];
+      if constexpr (BF) {
+        const uint4 u = *(const uint4 *)((const uint16_t *)x + t * H + c);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+      } else {
+        const f32x4 *p = (const f32x4 *)((const float *)x + t * H + c);
+        const f32x4 a = p[0], b = p[1];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) s[i] += v[i];
+    }
   }
-  part[blockIdx.y * H + c] = s;
+#pragma unroll
+  for (int i = 0; i < 8; i++) s_sum[row][in * 8 + i] = s[i];
+  __syncthreads();
+  const size_t o = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (o < H) {
+    float v = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) v += s_sum[j][threadIdx.x];
+    part[blockIdx.y * H + o] = v;
+  }
 }
 
 // One (maximum, sum of exponentials against it) of two; a sum whose maximum is minus infinity is 0 or NaN.
@@ -189,7 +255,9 @@ hipError_t launch_planes(const float *x, size_t n, uint16_t *out, size_t plane, 
 hipError_t launch_sum_parts(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias,
                             void *out, bool bf16, hipStream_t s) {
   if (!n) return hipSuccess;
-  if (bf16)
+  if (!bf16 && !bias && n <= 65536 && parts > 8)
+    k_sum_few<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(part, stride, parts, n, (float *)out);
+  else if (bf16)
     k_sum_parts<true><<<blocks_for(n), 256, 0, s>>>(part, stride, parts, n, bias, n_bias, out);
   else
     k_sum_parts<false><<<blocks_for(n), 256, 0, s>>>(part, stride, parts, n, bias, n_bias, out);

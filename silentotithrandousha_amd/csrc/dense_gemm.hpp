@@ -40,14 +40,19 @@ __device__ __forceinline__ float dense_exp(float t) {
   return __builtin_amdgcn_exp2f(a) * fmaf(b, 0.6931471805599453f, 1.0f);
 }
 
+// The same within 2^-24 (1 + |t|), for sums whose terms of large |t| vanish and for results that bf16 rounds.
+__device__ __forceinline__ float dense_exp_near(float t) { return __builtin_amdgcn_exp2f(t * 1.4426950408889634f); }
+
 // The gated activation of one pair: G = min(g, limit), U = clamp(u, +-limit), s = sigmoid(1.702 G);
 // h = (U + 1) G s. A NaN stays one.
 struct DenseGate {
   float G, U, s;
-  __device__ __forceinline__ DenseGate(float g, float u, float limit) {
+  template <bool NEAR>
+  __device__ __forceinline__ void set(float g, float u, float limit) {
     G = g > limit ? limit : g;
     U = rclamp(u, -limit, limit);
-    s = __builtin_amdgcn_rcpf(1.0f + dense_exp(-1.702f * G));
+    const float t = -1.702f * G;
+    s = __builtin_amdgcn_rcpf(1.0f + (NEAR ? dense_exp_near(t) : dense_exp(t)));
   }
   __device__ __forceinline__ float h() const { return (U + 1.0f) * (G * s); }
 };
@@ -160,14 +165,30 @@ __device__ __forceinline__ void dense_rows(uint8_t *stage, int lane, const uint1
   __builtin_amdgcn_wave_barrier();
 }
 
-// Takes the bf16 of each value, and leaves what it did not hold.
-template <int N>
+// The same for the f32 results of columns j of the accumulators.
+template <int TM, int TN>
+__device__ __forceinline__ void dense_rows_f32(uint8_t *stage, int lane, const f32x4 (&acc)[TM][TN], int j, float *out, size_t ld, int rows, int cols) {
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  uint16_t q[TM][8];
+#pragma unroll
+  for (int i = 0; i < TM; i++) {
+    const u16x8 v = __builtin_bit_cast(u16x8, acc[i][j]);
+#pragma unroll
+    for (int r = 0; r < 8; r++) q[i][r] = v[r];
+  }
+  dense_rows<TM, 8>(stage, lane, q, (uint16_t *)out, 2 * ld, rows, 2 * cols);
+}
+
+// Takes the bf16 of each value, and leaves what it did not hold (if another is to follow).
+template <bool MORE, int N>
 __device__ __forceinline__ void dense_take(float (&v)[N], uint16_t (&q)[N]) {
 #pragma unroll
   for (int r = 0; r < N; r++) {
     q[r] = dense_bf16(v[r]);
-    const float h = bf16_to_f32(q[r]);
-    v[r] = isfinite(h) ? v[r] - h : 0.0f;
+    if constexpr (MORE) {
+      const float h = bf16_to_f32(q[r]);
+      v[r] = isfinite(h) ? v[r] - h : 0.0f;
+    }
   }
 }
 
@@ -190,6 +211,12 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   const int nk = (k_hi - k_lo + kDenseStep - 1) / kDenseStep, steps = nk * a.n_pass;
 
   const uint32_t lds0 = str_lds(lds), lda = (uint32_t)a.lda * 2, ldb = (uint32_t)a.ldb * 2;
+  // v, for the rare branches of the loop: what they compute from it stays in them (hoisted out of the loop it
+  // would take the registers of the common path)
+  auto apart = [](int v) __attribute__((always_inline)) {
+    asm volatile("" : "+v"(v));
+    return v;
+  };
   TA la;
   TB lb;
   // the step to load: its operands' addresses, k values left in its pass from there
@@ -205,12 +232,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
       pb = a.B + ((a.pb >> 4 * pass) & 15) * a.b_plane + (BT ? (size_t)k_lo * a.ldb + n0 : (size_t)n0 * a.ldb + k_lo);
       left = k_hi - k_lo;
       pass++;
-      la.init(wave, lane, a.M - m0, lda);
-      lb.init(wave, lane, rows_b - n0, ldb);
+      const int l = apart(lane);
+      la.init(wave, l, a.M - m0, lda);
+      lb.init(wave, l, rows_b - n0, ldb);
     }
     if (left < kDenseStep) {
-      la.clamp(wave, lane, lda, left);
-      lb.clamp(wave, lane, ldb, left);
+      const int l = apart(lane);
+      la.clamp(wave, l, lda, left);
+      lb.clamp(wave, l, ldb, left);
     }
   };
   auto load_one = [&](int i, uint32_t slot) __attribute__((always_inline)) {
@@ -283,8 +312,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   int here = k_hi - k_lo;  // k values left in its pass from the next step to be read
   auto zero = [&](uint8_t *sl) __attribute__((always_inline)) {
     if (here < kDenseStep) {
-      TA::zero_tail(sl, here, tid, 64 * W);
-      TB::zero_tail(sl + TA::kBytes, here, tid, 64 * W);
+      const int t = apart(tid);
+      TA::zero_tail(sl, here, t, 64 * W);
+      TB::zero_tail(sl + TA::kBytes, here, t, 64 * W);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
@@ -365,10 +395,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   const int mw = m0 + wm * TM * 16 + (lane >> 4) * 4, nw = n0 + wn * TN * 16 + (lane & 15);
   // the wavefront's first row and column, and its part of the LDS for 16-bit results
   const int m_first = m0 + wm * TM * 16, n_first = n0 + wn * TN * 16;
-  constexpr int kStage = dense_stage_bytes(TM, EPI == DENSE_DGATE ? 8 : 4);
+  constexpr int kStage = dense_stage_bytes(EPI == DENSE_DGATE && TM % 4 == 0 ? 4 : TM, EPI == DENSE_GATE ? 2 : EPI == DENSE_DLOGITS ? 4 : 8);
   static_assert(W * kStage <= NS * kSlot, "the results of 16 columns fit the LDS of the steps");
   uint8_t *stage = lds + wave * kStage;
-  if constexpr (EPI != DENSE_STATS && EPI != DENSE_GATE_RAW) __syncthreads();
+  if constexpr (EPI != DENSE_STATS) __syncthreads();
   if constexpr (EPI == DENSE_STORE || EPI == DENSE_GATE || EPI == DENSE_GATE_RAW) {
     const float scale = EPI == DENSE_STORE && a.scale ? *a.scale : 1.0f;
 #pragma unroll
@@ -392,37 +422,53 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
         dense_rows<TM, 4>(stage, lane, q, (uint16_t *)a.out + (size_t)(n_first + j * 16) * a.ldo + m_first, a.ldo, a.N - n_first - j * 16, a.M - m_first);
         continue;
       }
+if (a.out_mode == 2) {
 #pragma unroll
-      for (int i = 0; i < TM; i++) {
-        const int m = mw + i * 16;
-        if (n >= a.N || m >= a.M) continue;
-        f32x4 *o = (f32x4 *)((float *)a.out + split * a.split_stride + (size_t)n * a.ldo + m);
-        *o = a.out_mode == 2 ? acc[i][j] + *o : acc[i][j];
+        for (int i = 0; i < TM; i++) {
+          const int m = mw + i * 16;
+          if (n >= a.N || m >= a.M) continue;
+          f32x4 *o = (f32x4 *)((float *)a.out + (size_t)n * a.ldo + m);
+          *o = acc[i][j] + *o;
+        }
+        continue;
       }
+      dense_rows_f32(stage, lane, acc, j, (float *)a.out + split * a.split_stride + (size_t)(n_first + j * 16) * a.ldo + m_first, a.ldo,
+                     a.N - n_first - j * 16, a.M - m_first);
     }
   } else if constexpr (EPI == DENSE_GATE_RAW) {
 #pragma unroll
     for (int j = 0; j < TN; j++)
-#pragma unroll
-      for (int i = 0; i < TM; i++)
-        if (nw + j * 16 < a.N && mw + i * 16 < a.M) *(f32x4 *)(a.gu + (size_t)(nw + j * 16) * a.M + mw + i * 16) = acc[i][j];
+      dense_rows_f32(stage, lane, acc, j, a.gu + (size_t)(n_first + j * 16) * a.M + m_first, a.M, a.N - n_first - j * 16, a.M - m_first);
   } else if constexpr (EPI == DENSE_GATE) {
+    auto gate = [&](auto ONE) __attribute__((always_inline)) {  // ONE plane, or kPlanes
+      constexpr bool one = decltype(ONE)::value;
 #pragma unroll
-    for (int j = 0; j < TN; j++) {
-      float h[TM][2];
+      for (int j = 0; j < TN; j++) {
+        float h[TM][2];
 #pragma unroll
-      for (int i = 0; i < TM; i++)
+        for (int i = 0; i < TM; i++)
 #pragma unroll
-        for (int r = 0; r < 2; r++) h[i][r] = DenseGate(acc[i][j][2 * r], acc[i][j][2 * r + 1], a.limit).h();
-      for (int p = 0; p < a.planes; p++) {
-        uint16_t q[TM][2];
+          for (int r = 0; r < 2; r++) {
+            DenseGate g;
+            g.set<one>(acc[i][j][2 * r], acc[i][j][2 * r + 1], a.limit);
+            h[i][r] = g.h();
+          }
+        for (int p = 0; p < (one ? 1 : kPlanes); p++) {
+          uint16_t q[TM][2];
 #pragma unroll
-        for (int i = 0; i < TM; i++) dense_take(h[i], q[i]);
-        dense_rows<TM, 2>(stage, lane, q, a.h + p * a.h_plane + (size_t)(n_first + j * 16) * a.ldh + m_first / 2, a.ldh,
-                          a.N - n_first - j * 16, (a.M - m_first) / 2);
+          for (int i = 0; i < TM; i++) dense_take<!one>(h[i], q[i]);
+          dense_rows<TM, 2>(stage, lane, q, a.h + p * a.h_plane + (size_t)(n_first + j * 16) * a.ldh + m_first / 2, a.ldh,
+                            a.N - n_first - j * 16, (a.M - m_first) / 2);
+        }
       }
-    }
+    };
+    if (a.planes == 1)
+      gate(yes);
+    else
+      gate(no);
   } else if constexpr (EPI == DENSE_DGATE) {
+    auto dgate = [&](auto ONE) __attribute__((always_inline)) {
+    constexpr bool one = decltype(ONE)::value;
     constexpr int G = TM % 4 == 0 ? 4 : TM % 3 == 0 ? 3 : TM % 2 == 0 ? 2 : 1;  // tiles at a time, for the registers
 #pragma unroll
     for (int g0 = 0; g0 < TM; g0 += G) {
@@ -438,17 +484,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
 #pragma unroll
         for (int i = 0; i < G; i++) {
           const int m = mw + (g0 + i) * 16;
-          f32x4 g01 = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, g23 = g01;
           const bool in = n < a.N && m < a.M;
-          if (in) {
-            const f32x4 *row = (const f32x4 *)(a.gu + (size_t)n * a.M * 2 + 2 * m);
-            g01 = row[0];
-            g23 = row[1];
-          }
+          const f32x4 *row = (const f32x4 *)(a.gu + (size_t)min(n, a.N - 1) * a.M * 2 + 2 * min(m, a.M - 4));
+          const f32x4 g01 = row[0], g23 = row[1];
 #pragma unroll
           for (int r = 0; r < 4; r++) {
             const float gate = r < 2 ? g01[2 * r] : g23[2 * r - 4], up = r < 2 ? g01[2 * r + 1] : g23[2 * r - 3];
-            const DenseGate g(gate, up, a.limit);
+            DenseGate g;
+            g.set<one>(gate, up, a.limit);
             const float dh = acc[g0 + i][j][r];
             hv[i][r] = g.h();
             d[i][2 * r] = gate > a.limit ? 0.0f : dh * (g.U + 1.0f) * (g.s * (1.0f + 1.702f * (g.G * (1.0f - g.s))));
@@ -457,13 +500,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
 #pragma unroll
           for (int r = 0; r < 8; r++) db[i][r] += in ? d[i][r] : 0.0f;
         }
+        __builtin_amdgcn_sched_barrier(0);  // (the loads of all columns at once would not fit the registers)
         const int rows = a.N - n_first - j * 16, m1 = m_first + g0 * 16;
-        for (int p = 0; p < a.planes; p++) {
+        for (int p = 0; p < (one ? 1 : kPlanes); p++) {
           uint16_t q[G][8], e[G][4];
 #pragma unroll
           for (int i = 0; i < G; i++) {
-            dense_take(d[i], q[i]);
-            dense_take(hv[i], e[i]);
+            dense_take<!one>(d[i], q[i]);
+            dense_take<!one>(hv[i], e[i]);
           }
           dense_rows<G, 8>(stage, lane, q, a.dgu + p * a.dgu_plane + (size_t)(n_first + j * 16) * a.M * 2 + 2 * m1, (size_t)a.M * 2, rows, 2 * (a.M - m1));
           dense_rows<G, 4>(stage, lane, e, a.h + p * a.h_plane + (size_t)(n_first + j * 16) * a.ldh + m1, a.ldh, rows, a.M - m1);
@@ -490,63 +534,90 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
         }
       }
     }
+    };
+    if (a.planes == 1)
+      dgate(yes);
+    else
+      dgate(no);
   } else if constexpr (EPI == DENSE_STATS) {
-#pragma unroll
-    for (int j = 0; j < TN; j++) {
-      const int n = nw + j * 16;
-      const int want = n < a.N ? a.targets[n] : -1;
-      float mx = -INFINITY;
-      bool nan = false;
-#pragma unroll
-      for (int i = 0; i < TM; i++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int m = mw + i * 16 + r;
-          if (m >= a.M) continue;
-          const float l = acc[i][j][r];
-          mx = fmaxf(mx, l);
-          nan |= l != l;
-          if (a.v0 + m == want) a.picked[n] = l;
-        }
-      mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      // no value above minus infinity: every exponential is 0 against a base of 0
-      const float base = mx == -INFINITY ? 0.0f : mx;
-      float sum = 0.0f;
+    const bool whole = m_first + TM * 16 <= a.M;  // else the rows past the vocabulary count as minus infinity
+    if (!whole) {
 #pragma unroll
       for (int i = 0; i < TM; i++)
 #pragma unroll
         for (int r = 0; r < 4; r++)
-          if (mw + i * 16 + r < a.M) sum += dense_exp(acc[i][j][r] - base);
-      if (nan) sum = NAN;
+          if (mw + i * 16 + r >= a.M) {
+#pragma unroll
+            for (int j = 0; j < TN; j++) acc[i][j][r] = -INFINITY;
+          }
+    }
+#pragma unroll
+    for (int j = 0; j < TN; j++) {
+      const int n = nw + j * 16, t = n < a.N ? a.targets[n] : -1;
+      const int want = t >= a.v0 ? t - a.v0 - mw : -1;  // the target's row from the lane's first
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < TM; i++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) mx = fmaxf(mx, acc[i][j][r]);
+        if (want >> 4 == i && (want & 15) < 4 && t - a.v0 < a.M)
+          a.picked[n] = (want & 2) ? ((want & 1) ? acc[i][j][3] : acc[i][j][2]) : ((want & 1) ? acc[i][j][1] : acc[i][j][0]);
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      // no value above minus infinity: every exponential is 0 against a base of 0
+      const float base = (mx == -INFINITY ? 0.0f : mx) * 1.4426950408889634f;
+      float sum = 0.0f;  // (a NaN among the logits makes it one)
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], 1.4426950408889634f, -base));
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
       if (lane < 16 && n < a.N) a.stats[(size_t)(tile_m * WM + wm) * a.N + n] = make_float2(mx, sum);
     }
   } else {
+    auto dlogits = [&](auto ONE) __attribute__((always_inline)) {
+      constexpr bool one = decltype(ONE)::value;
+      const float unit = *a.scale;
 #pragma unroll
-    for (int j = 0; j < TN; j++) {
-      const int n = min(nw + j * 16, a.N - 1);  // (columns past N are not stored)
-      const int t = a.targets[n];
-      const float lse = a.lse[n], scale = a.dloss[n] / *a.scale;
-      float d[TM][4];
+      for (int j = 0; j < TN; j++) {
+        const int n = min(nw + j * 16, a.N - 1);  // (columns past N are not stored)
+        const int t = a.targets[n];
+        const int want = t >= a.v0 ? t - a.v0 - mw : -1;
+        const float lse = t >= a.vocab ? NAN : a.lse[n], scale = a.dloss[n] / unit;
+        float d[TM][4];
 #pragma unroll
-      for (int i = 0; i < TM; i++)
+        for (int i = 0; i < TM; i++) {
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int m = mw + i * 16 + r;
-          d[i][r] = scale * (dense_exp(acc[i][j][r] - lse) - (a.v0 + m == t ? 1.0f : 0.0f));
-          if (t >= a.vocab) d[i][r] = NAN;
-          if (t < 0 || m >= a.M) d[i][r] = 0.0f;  // ignored token, padding column
+          for (int r = 0; r < 4; r++) {
+            const float x = acc[i][j][r] - lse;
+            d[i][r] = scale * (one ? dense_exp_near(x) : dense_exp(x));
+          }
+          if (want >> 4 == i && (want & 15) < 4) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              const float x = acc[i][j][r] - lse;
+              if ((want & 3) == r) d[i][r] = scale * ((one ? dense_exp_near(x) : dense_exp(x)) - 1.0f);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if (t < 0 || mw + i * 16 + r >= a.M) d[i][r] = 0.0f;  // ignored token, padding column
         }
-      for (int p = 0; p < a.planes; p++) {
-        uint16_t q[TM][4];
+        for (int p = 0; p < (one ? 1 : kPlanes); p++) {
+          uint16_t q[TM][4];
 #pragma unroll
-        for (int i = 0; i < TM; i++) dense_take(d[i], q[i]);
-        dense_rows<TM, 4>(stage, lane, q, a.dl + p * a.dl_plane + (size_t)(n_first + j * 16) * a.ld_dl + m_first, a.ld_dl,
-                          a.N - n_first - j * 16, (int)a.ld_dl - m_first);
+          for (int i = 0; i < TM; i++) dense_take<!one>(d[i], q[i]);
+          dense_rows<TM, 4>(stage, lane, q, a.dl + p * a.dl_plane + (size_t)(n_first + j * 16) * a.ld_dl + m_first, a.ld_dl,
+                            a.N - n_first - j * 16, (int)a.ld_dl - m_first);
+        }
       }
-    }
+    };
+    if (a.planes == 1)
+      dlogits(yes);
+    else
+      dlogits(no);
   }
 }
 

@@ -16,7 +16,9 @@ namespace moe {
   X(32x64, 32, 64, 2, 2, 6, 2, 340.0)        \
   X(32x32, 32, 32, 2, 2, 8, 2, 240.0)        \
   X(32x16, 32, 16, 2, 1, 8, 3, 190.0)        \
-  X(128x16, 128, 16, 4, 1, 4, 2, 200.0)
+  X(128x16, 128, 16, 4, 1, 4, 2, 200.0)      \
+  X(64x16, 64, 16, 4, 1, 8, 2, 190.0)        \
+  X(16x16, 16, 16, 1, 1, 16, 2, 100.0)
 
 enum DenseTileShape {
 #define X(name, bm, bn, wm, wn, ns, wgs, rate) TILE_##name,
@@ -30,7 +32,10 @@ template <bool AT, bool BT, int EPI>
 hipError_t launch_dense_shape(const DenseArgs &a, hipStream_t st) {
   switch (dense_tile(DenseShape{AT, BT, (DenseEpi)EPI}, a)) {
 #define X(name, bm, bn, wm, wn, ns, wgs, rate) \
-  case TILE_##name: return launch_dense_as<bm, bn, wm, wn, ns, AT, BT, EPI>(a, st);
+  case TILE_##name:                 \
+    if constexpr (AT || bm <= 256)  \
+      return launch_dense_as<bm, bn, wm, wn, ns, AT, BT, EPI>(a, st); \
+    break;
     MOE_DENSE_TILES(X)
 #undef X
   }
