@@ -22,8 +22,7 @@ constexpr int kCus = 256;  // of an MI355X: the plan is for the whole device
 // largest of the time that its products take at the tile's full rate, that its loads of A take where A is
 // read once, from memory (both shared by the workgroups of its CU), and that its loads wait, spread over
 // the steps that its slots hold ahead; each workgroup has a prologue and an epilogue that stores its
-// results (under the steps of the others of its CU, if any); parts are written and summed in another
-// launch. Whole rounds of workgroups and what is left for the last one count apart.
+// results; parts are summed in another launch. Whole rounds of workgroups and what is left for the last one count apart.
 double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a, int splits) {
   const long tiles_n = ((long)a.N * a.stack + d.bn - 1) / d.bn, tiles = (long)((a.M + d.bm - 1) / d.bm) * tiles_n * splits;
   const long steps = (((long)a.K + kDenseStep - 1) / kDenseStep * a.n_pass + splits - 1) / splits;
@@ -36,11 +35,11 @@ double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a,
     double step = std::max(0.45 / (d.ns - 1) + 0.1, on_cu * d.bm * d.bn * 2.0 * kDenseStep * kCus / (d.rate * 1e6));
     if (tiles_n == 1) step = std::max(step, on_cu * d.bm * 128e-3 / memory);
     const double stores = on_cu * d.bm * d.bn * result * kCus / 4.5e6;  // us at 4.5 TB/s
-    return steps * step + 2.5 + (d.wgs == 1 ? stores : 0.5 * stores);
+    return steps * step + 2.5 + stores;
   };
   const long whole = tiles / (kCus * d.wgs), rest = tiles - whole * kCus * d.wgs;
   double us = whole * round(d.wgs) + (rest ? round((rest + kCus - 1) / kCus) : 0.0);
-  if (splits > 1) us += 3.0 + 8e-6 / 4 * splits * a.M * a.N;
+  if (splits > 1) us += 3.0 + 4.0 * splits * a.M * a.N / 5e6;
   return us;
 }
 

@@ -66,12 +66,11 @@ struct DenseTile {
   static constexpr int kPairs = R / 16;               // 32-byte pieces of a transposed row
 
   // Transposed: piece of a row that holds the logical piece q in row k. The transposing load's 16 lanes
-  // take rows k = 8g .. 8g + 3 (and + 4): their pieces go to different banks.
+  // take 4 rows k: their pieces go to different banks. (Only within groups of 4 pieces, so that the
+  // fragments of 16 rows lie at 4 addresses and constant distances from them.)
   static __device__ __forceinline__ int piece(int q, int k) {
-    const int f = (k & 3) | ((k >> 1) & 4);
-    const int mask = kPairs >= 8 ? ((q | 7) < kPairs ? 7 : (q | 3) < kPairs ? 3 : 0)
-                                 : kPairs >= 4 ? ((q | 3) < kPairs ? 3 : 0) : kPairs >= 2 ? 1 : 0;
-    return q ^ (f & mask);
+    const int mask = kPairs >= 4 ? ((q | 3) < kPairs ? 3 : 0) : kPairs >= 2 ? 1 : 0;
+    return q ^ (k & mask);
   }
 
   uint32_t off[kLoads];  // byte offset of this lane's 16 bytes from the tile's base
@@ -144,6 +143,13 @@ __device__ __forceinline__ void dense_tile_of(int b, int tiles_m, int tiles_n, i
   tn = n0 + in % width;
 }
 
+// v itself, but what is computed from it stays where it is: hoisted out of the main loop (from its rare
+// branches) or shared by the columns of the epilogue it took registers and was spilled.
+__device__ __forceinline__ int apart(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // Stores 16 rows of 16-bit results of a wavefront: lane l holds the V values q[i] of row l % 16 from column
 // (4 i + l / 16) V on. They pass through LDS (`stage`, the wavefront's own, dense_stage_bytes) so that
 // a row leaves in 16-byte pieces side by side: stored from the accumulators' layout, in pieces of
@@ -153,6 +159,7 @@ template <int TM, int V>
 __device__ __forceinline__ void dense_rows(uint8_t *stage, int lane, const uint16_t (&q)[TM][V], uint16_t *out, size_t ld, int rows, int cols) {
   constexpr int kRow = TM * V * 8, kPieces = kRow / 16;  // bytes and 16-byte pieces of a row
   typedef uint16_t vec __attribute__((ext_vector_type(V)));
+  lane = apart(lane);
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
   for (int i = 0; i < TM; i++) *(vec *)(stage + (lane & 15) * (kRow + 16) + (4 * i + (lane >> 4)) * V * 2) = __builtin_bit_cast(vec, q[i]);
@@ -211,12 +218,6 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   const int nk = (k_hi - k_lo + kDenseStep - 1) / kDenseStep, steps = nk * a.n_pass;
 
   const uint32_t lds0 = str_lds(lds), lda = (uint32_t)a.lda * 2, ldb = (uint32_t)a.ldb * 2;
-  // v, for the rare branches of the loop: what they compute from it stays in them (hoisted out of the loop it
-  // would take the registers of the common path)
-  auto apart = [](int v) __attribute__((always_inline)) {
-    asm volatile("" : "+v"(v));
-    return v;
-  };
   TA la;
   TB lb;
   // the step to load: its operands' addresses, k values left in its pass from there
@@ -395,10 +396,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   const int mw = m0 + wm * TM * 16 + (lane >> 4) * 4, nw = n0 + wn * TN * 16 + (lane & 15);
   // the wavefront's first row and column, and its part of the LDS for 16-bit results
   const int m_first = m0 + wm * TM * 16, n_first = n0 + wn * TN * 16;
-  constexpr int kStage = dense_stage_bytes(EPI == DENSE_DGATE && TM % 4 == 0 ? 4 : TM, EPI == DENSE_GATE ? 2 : EPI == DENSE_DLOGITS ? 4 : 8);
+  constexpr int kStage = dense_stage_bytes(TM, EPI == DENSE_GATE ? 2 : EPI == DENSE_DLOGITS ? 4 : 8);
   static_assert(W * kStage <= NS * kSlot, "the results of 16 columns fit the LDS of the steps");
   uint8_t *stage = lds + wave * kStage;
-  if constexpr (EPI != DENSE_STATS) __syncthreads();
+  if constexpr (EPI != DENSE_STATS && EPI != DENSE_DGATE) __syncthreads();
   if constexpr (EPI == DENSE_STORE || EPI == DENSE_GATE || EPI == DENSE_GATE_RAW) {
     const float scale = EPI == DENSE_STORE && a.scale ? *a.scale : 1.0f;
 #pragma unroll
@@ -467,73 +468,56 @@ if (a.out_mode == 2) {
     else
       gate(no);
   } else if constexpr (EPI == DENSE_DGATE) {
+    // (stored from the accumulators' layout, 64 and 32 bytes of a row at a time: staged as the other results
+    // it kept too much in registers and was no faster, 107 and 116 us of 4096 x 2880 against 108)
     auto dgate = [&](auto ONE) __attribute__((always_inline)) {
-    constexpr bool one = decltype(ONE)::value;
-    constexpr int G = TM % 4 == 0 ? 4 : TM % 3 == 0 ? 3 : TM % 2 == 0 ? 2 : 1;  // tiles at a time, for the registers
+      constexpr bool one = decltype(ONE)::value;
 #pragma unroll
-    for (int g0 = 0; g0 < TM; g0 += G) {
-      float db[G][8];
+      for (int i = 0; i < TM; i++) {
+        const int m = mw + i * 16;
+        float db[8] = {};
 #pragma unroll
-      for (int i = 0; i < G; i++)
-#pragma unroll
-        for (int r = 0; r < 8; r++) db[i][r] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < TN; j++) {
-        const int n = nw + j * 16;
-        float d[G][8], hv[G][4];
-#pragma unroll
-        for (int i = 0; i < G; i++) {
-          const int m = mw + (g0 + i) * 16;
-          const bool in = n < a.N && m < a.M;
-          const f32x4 *row = (const f32x4 *)(a.gu + (size_t)min(n, a.N - 1) * a.M * 2 + 2 * min(m, a.M - 4));
+        for (int j = 0; j < TN; j++) {
+          const int n = nw + j * 16;
+          if (n >= a.N || m >= a.M) continue;
+          const f32x4 *row = (const f32x4 *)(a.gu + (size_t)n * a.M * 2 + 2 * m);
           const f32x4 g01 = row[0], g23 = row[1];
+          float d[8], hv[4];
 #pragma unroll
           for (int r = 0; r < 4; r++) {
             const float gate = r < 2 ? g01[2 * r] : g23[2 * r - 4], up = r < 2 ? g01[2 * r + 1] : g23[2 * r - 3];
             DenseGate g;
             g.set<one>(gate, up, a.limit);
-            const float dh = acc[g0 + i][j][r];
-            hv[i][r] = g.h();
-            d[i][2 * r] = gate > a.limit ? 0.0f : dh * (g.U + 1.0f) * (g.s * (1.0f + 1.702f * (g.G * (1.0f - g.s))));
-            d[i][2 * r + 1] = fabsf(up) > a.limit ? 0.0f : dh * (g.G * g.s);
+            const float dh = acc[i][j][r];
+            hv[r] = g.h();
+            d[2 * r] = gate > a.limit ? 0.0f : dh * (g.U + 1.0f) * (g.s * (1.0f + 1.702f * (g.G * (1.0f - g.s))));
+            d[2 * r + 1] = fabsf(up) > a.limit ? 0.0f : dh * (g.G * g.s);
           }
 #pragma unroll
-          for (int r = 0; r < 8; r++) db[i][r] += in ? d[i][r] : 0.0f;
-        }
-        __builtin_amdgcn_sched_barrier(0);  // (the loads of all columns at once would not fit the registers)
-        const int rows = a.N - n_first - j * 16, m1 = m_first + g0 * 16;
-        for (int p = 0; p < (one ? 1 : kPlanes); p++) {
-          uint16_t q[G][8], e[G][4];
-#pragma unroll
-          for (int i = 0; i < G; i++) {
-            dense_take<!one>(d[i], q[i]);
-            dense_take<!one>(hv[i], e[i]);
+          for (int r = 0; r < 8; r++) db[r] += d[r];
+          for (int p = 0; p < (one ? 1 : kPlanes); p++) {
+            uint16_t q[8], e[4];
+            dense_take<!one>(d, q);
+            dense_take<!one>(hv, e);
+            *(uint4 *)(a.dgu + p * a.dgu_plane + (size_t)n * a.M * 2 + 2 * m) = __builtin_bit_cast(uint4, q);
+            *(uint2 *)(a.h + p * a.h_plane + (size_t)n * a.ldh + m) = __builtin_bit_cast(uint2, e);
           }
-          dense_rows<G, 8>(stage, lane, q, a.dgu + p * a.dgu_plane + (size_t)(n_first + j * 16) * a.M * 2 + 2 * m1, (size_t)a.M * 2, rows, 2 * (a.M - m1));
-          dense_rows<G, 4>(stage, lane, e, a.h + p * a.h_plane + (size_t)(n_first + j * 16) * a.ldh + m1, a.ldh, rows, a.M - m1);
         }
-      }
-      if (a.db_part) {  // over the wavefront's columns: 16 lanes, then a part per wavefront column
-#pragma unroll
-        for (int i = 0; i < G; i++) {
+        if (a.db_part) {  // over the wavefront's columns: 16 lanes, then a part per wavefront column
 #pragma unroll
           for (int r = 0; r < 8; r++) {
-            float v = db[i][r];
-            v += __shfl_xor(v, 1);
-            v += __shfl_xor(v, 2);
-            v += __shfl_xor(v, 4);
-            v += __shfl_xor(v, 8);
-            db[i][r] = v;
+            db[r] += __shfl_xor(db[r], 1);
+            db[r] += __shfl_xor(db[r], 2);
+            db[r] += __shfl_xor(db[r], 4);
+            db[r] += __shfl_xor(db[r], 8);
           }
-          const int m = mw + (g0 + i) * 16;
           if ((lane & 15) == 0 && m < a.M) {
             f32x4 *o = (f32x4 *)(a.db_part + (size_t)(tile_n * WN + wn) * a.M * 2 + 2 * m);
-            o[0] = f32x4{db[i][0], db[i][1], db[i][2], db[i][3]};
-            o[1] = f32x4{db[i][4], db[i][5], db[i][6], db[i][7]};
+            o[0] = f32x4{db[0], db[1], db[2], db[3]};
+            o[1] = f32x4{db[4], db[5], db[6], db[7]};
           }
         }
       }
-    }
     };
     if (a.planes == 1)
       dgate(yes);

@@ -7,18 +7,18 @@ namespace moe {
 // X(name, rows, columns, wavefronts along each, LDS slots, workgroups of a CU, TFLOP/s of the device full of
 // them). The rates are those of 2880 k values (loss over 201088 rows, 512 tokens and more).
 #define MOE_DENSE_TILES(X)                   \
-  X(288x256, 288, 256, 2, 4, 2, 1, 1115.0)   \
-  X(256x256, 256, 256, 2, 4, 2, 1, 1125.0)   \
-  X(192x256, 192, 256, 2, 4, 2, 1, 1050.0)   \
-  X(128x128, 128, 128, 2, 2, 2, 2, 906.0)    \
-  X(128x64, 128, 64, 2, 2, 3, 2, 660.0)      \
-  X(64x64, 64, 64, 2, 2, 4, 2, 500.0)        \
-  X(32x64, 32, 64, 2, 2, 6, 2, 340.0)        \
-  X(32x32, 32, 32, 2, 2, 8, 2, 240.0)        \
-  X(32x16, 32, 16, 2, 1, 8, 3, 190.0)        \
-  X(128x16, 128, 16, 4, 1, 4, 2, 200.0)      \
-  X(64x16, 64, 16, 4, 1, 8, 2, 190.0)        \
-  X(16x16, 16, 16, 1, 1, 16, 2, 100.0)
+  X(288x256, 288, 256, 2, 4, 2, 1, 1180.0)   \
+  X(256x256, 256, 256, 2, 4, 2, 1, 1290.0)   \
+  X(192x256, 192, 256, 2, 4, 2, 1, 1190.0)   \
+  X(128x128, 128, 128, 2, 2, 2, 2, 1000.0)    \
+  X(128x64, 128, 64, 2, 2, 3, 2, 800.0)      \
+  X(64x64, 64, 64, 2, 2, 4, 2, 600.0)        \
+  X(32x64, 32, 64, 2, 2, 6, 2, 430.0)        \
+  X(32x32, 32, 32, 2, 2, 8, 2, 300.0)        \
+  X(32x16, 32, 16, 2, 1, 8, 3, 220.0)        \
+  X(128x16, 128, 16, 4, 1, 4, 2, 220.0)      \
+  X(64x16, 64, 16, 4, 1, 8, 2, 210.0)        \
+  X(16x16, 16, 16, 1, 1, 16, 2, 110.0)
 
 enum DenseTileShape {
 #define X(name, bm, bn, wm, wn, ns, wgs, rate) TILE_##name,

@@ -9,14 +9,8 @@ HALF = 32
 
 
 def piece(q, k, pairs):
-    f = (k & 3) | ((k >> 1) & 4)
-    if pairs >= 8:
-        mask = np.where((q | 7) < pairs, 7, np.where((q | 3) < pairs, 3, 0))
-    elif pairs >= 4:
-        mask = np.where((q | 3) < pairs, 3, 0)
-    else:
-        mask = 1 if pairs >= 2 else 0
-    return q ^ (f & mask)
+    mask = np.where((q | 3) < pairs, 3, 0) if pairs >= 4 else 1 if pairs >= 2 else 0
+    return q ^ (k & mask)
 
 
 def load(mem, base, ld, R, W, transposed, rows, left, clamp=True):
