@@ -27,7 +27,7 @@ double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a,
   const long tiles_n = ((long)a.N * a.stack + d.bn - 1) / d.bn, tiles = (long)((a.M + d.bm - 1) / d.bm) * tiles_n * splits;
   const long steps = (((long)a.K + kDenseStep - 1) / kDenseStep * a.n_pass + splits - 1) / splits;
   // bytes that a result costs, about
-  const double result = s.epi == DENSE_STATS ? 0.0 : s.epi == DENSE_GATE ? 1.0 : s.epi == DENSE_GATE_RAW ? 4.0 : s.epi == DENSE_DGATE ? 14.0
+  const double result = s.epi == DENSE_STATS ? 0.0 : s.epi == DENSE_GATE ? 1.0 : s.epi == DENSE_DGATE ? 14.0
                         : s.epi == DENSE_STORE && (a.out_mode || splits > 1) ? 4.0 : 2.0;
   // a transposed A's rows of k are read in pieces of a tile's rows: below 128 bytes at two thirds of the rate
   const double memory = s.at && d.bm < 64 ? 15.0 : 23.0;  // GB/s a CU; 5.9 TB/s in all
@@ -71,7 +71,12 @@ int dense_split_count(const DenseArgs &a) {
   return (int)((a.K + k - 1) / k);
 }
 
+double dense_estimate(const DenseShape &s, const DenseArgs &a) {
+  return dense_us(s, kDenseTiles[dense_tile(s, a)], a, dense_split_count(a));
+}
+
 int dense_splits(const DenseShape &s, const DenseArgs &a0) {
+  if (dense_few_fits(s, a0)) return 1;
   const long steps = ((long)a0.K + kDenseStep - 1) / kDenseStep;
   int best = 1;
   double us = 0.0;
@@ -80,7 +85,7 @@ int dense_splits(const DenseShape &s, const DenseArgs &a0) {
     DenseArgs a = a0;
     a.splits = n;
     a.splits = dense_split_count(a);
-    const double u = dense_us(s, kDenseTiles[dense_tile(s, a)], a, a.splits);
+    const double u = dense_estimate(s, a);
     if (n == 1 || u < us) best = a.splits, us = u;
   }
   return best;
@@ -95,6 +100,7 @@ hipError_t launch_dense(const DenseShape &s, const DenseArgs &a0, hipStream_t st
   a.k_split = split_k(a0);
   a.splits = dense_split_count(a0);
   if (a.splits > 1 && (s.epi != DENSE_STORE || a.out_mode != 1)) return hipErrorInvalidValue;
+  if (dense_few_fits(s, a)) return launch_dense_few(s, a, st);
   return s.at ? launch_dense_tn(s, a, st) : launch_dense_nt(s, a, st);
 }
 
@@ -196,6 +202,66 @@ __global__ __launch_bounds__(256) void k_colsum(const void *x, size_t T, size_t 
   }
 }
 
+// A block takes 16 rows of 128 inner columns, 2 rows a thread of 4 columns. Bound by its bytes.
+constexpr int kDgateRows = 16;
+template <bool ONE>
+__global__ __launch_bounds__(256) void k_dgate(const DgateArgs a) {
+  __shared__ float s_db[8][256];
+  const int in = threadIdx.x % 32, row = threadIdx.x / 32, i = blockIdx.x * 128 + in * 4;
+  float db[8] = {};
+  if (i < a.I) {  // (I is a multiple of 8)
+#pragma unroll
+    for (int k = 0; k < kDgateRows / 8; k++) {
+      const size_t t = (size_t)blockIdx.y * kDgateRows + k * 8 + row;
+      if (t >= (size_t)a.T) break;
+      float v[8] = {}, dh[4] = {}, d[8], hv[4];
+      for (int p = 0; p < a.gu_parts; p++) {
+        const f32x4 *x = (const f32x4 *)(a.gu + (p * (size_t)a.T + t) * 2 * a.I + 2 * i);
+        const f32x4 lo = x[0], hi = x[1];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] += lo[r], v[4 + r] += hi[r];
+      }
+      for (int p = 0; p < a.dh_parts; p++) {
+        const f32x4 x = *(const f32x4 *)(a.dh + (p * (size_t)a.T + t) * a.I + i);
+#pragma unroll
+        for (int r = 0; r < 4; r++) dh[r] += x[r];
+      }
+      if (a.bias)
+#pragma unroll
+        for (int r = 0; r < 8; r++) v[r] += a.bias[2 * i + r];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        DenseGate g;
+        g.set<ONE>(v[2 * r], v[2 * r + 1], a.limit);
+        hv[r] = g.h();
+        d[2 * r] = g.dg(dh[r], v[2 * r], a.limit);
+        d[2 * r + 1] = g.du(dh[r], v[2 * r + 1], a.limit);
+      }
+#pragma unroll
+      for (int r = 0; r < 8; r++) db[r] += d[r];
+      const size_t plane = (size_t)a.T * a.I;
+      for (int p = 0; p < (ONE ? 1 : kPlanes); p++) {
+        uint16_t q[8], e[4];
+        dense_take<!ONE>(d, q);
+        dense_take<!ONE>(hv, e);
+        *(uint4 *)(a.dgu + p * 2 * plane + t * 2 * a.I + 2 * i) = __builtin_bit_cast(uint4, q);
+        *(uint2 *)(a.h + p * plane + t * a.I + i) = __builtin_bit_cast(uint2, e);
+      }
+    }
+  }
+  if (!a.db_part) return;
+#pragma unroll
+  for (int r = 0; r < 8; r++) s_db[row][in * 8 + r] = db[r];
+  __syncthreads();
+  const int o = blockIdx.x * 256 + threadIdx.x;
+  if (o < 2 * a.I) {
+    float v = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) v += s_db[j][threadIdx.x];
+    a.db_part[(size_t)blockIdx.y * 2 * a.I + o] = v;
+  }
+}
+
 // One (maximum, sum of exponentials against it) of two; a sum whose maximum is minus infinity is 0 or NaN.
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x);
@@ -260,6 +326,17 @@ hipError_t launch_sum_parts(const float *part, size_t stride, int parts, size_t 
     k_sum_parts<true><<<blocks_for(n), 256, 0, s>>>(part, stride, parts, n, bias, n_bias, out);
   else
     k_sum_parts<false><<<blocks_for(n), 256, 0, s>>>(part, stride, parts, n, bias, n_bias, out);
+  return hipGetLastError();
+}
+
+int dense_dgate_parts(int T) { return (T + kDgateRows - 1) / kDgateRows; }
+hipError_t launch_dgate(const DgateArgs &a, hipStream_t s) {
+  const dim3 grid((a.I + 127) / 128, dense_dgate_parts(a.T));
+  if (a.T < 1 || a.I < 8 || a.I % 8 || grid.y > 65535) return hipErrorInvalidValue;
+  if (a.planes == 1)
+    k_dgate<true><<<grid, 256, 0, s>>>(a);
+  else
+    k_dgate<false><<<grid, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 

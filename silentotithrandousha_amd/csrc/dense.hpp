@@ -18,10 +18,9 @@ constexpr int kMaxPass = 6;
 enum DenseEpi {
   DENSE_STORE = 0,   // out (+ bias) as f32 or bf16, or added to f32
   DENSE_GATE = 1,    // rows of D are interleaved gate and up: h = act(gate, up) as bf16 planes
-  DENSE_GATE_RAW = 2,  // the same rows with their bias, as f32 (for the backward pass)
-  DENSE_DGATE = 3,   // D = dh: gate and up from DENSE_GATE_RAW give h, d(gate, up) and bias sums
-  DENSE_STATS = 4,   // D = logits: running maximum and sum of exponentials of each column's tile
-  DENSE_DLOGITS = 5  // D = logits: their gradient as bf16 planes
+  DENSE_DGATE = 2,   // D = dh: with the gate and up of gu they give h, d(gate, up) and bias sums
+  DENSE_STATS = 3,   // D = logits: running maximum and sum of exponentials of each column's tile
+  DENSE_DLOGITS = 4  // D = logits: their gradient as bf16 planes
 };
 
 // D[m][n] = sum over passes and k of A_p[m][k] B_p[n][k], stored as [n][m] (m contiguous).
@@ -48,7 +47,7 @@ struct DenseArgs {
   float limit;
   uint16_t *h;              // [planes][N][ldh] bf16
   size_t h_plane, ldh;
-  float *gu;                // [N][M] (GATE_RAW), [N][2 M] (DGATE)
+  const float *gu;          // [N][2 M]
   uint16_t *dgu;            // [planes][N][2 M]
   size_t dgu_plane;
   float *db_part;           // [parts][2 M] or NULL
@@ -72,7 +71,20 @@ int dense_parts(const DenseShape &s, const DenseArgs &a);  // parts of db_part /
 // K splits worth taking (none of them empty)
 int dense_splits(const DenseShape &s, const DenseArgs &a);
 int dense_split_count(const DenseArgs &a);  // the splits that a launch with a.splits makes (none of them empty)
+double dense_estimate(const DenseShape &s, const DenseArgs &a);  // us of a launch, about
 hipError_t launch_dense(const DenseShape &s, const DenseArgs &a, hipStream_t st);
+
+// DENSE_DGATE's epilogue as a kernel of its own, for gate, up and dh that come in K parts: gu [gu_parts][T][2 I]
+// (+ bias), dh [dh_parts][T][I]; db_part [dense_dgate_parts(T)][2 I] or NULL.
+struct DgateArgs {
+  const float *gu, *bias, *dh;
+  int gu_parts, dh_parts, T, I, planes;
+  float limit;
+  uint16_t *h, *dgu;  // [planes][T][I], [planes][T][2 I]
+  float *db_part;
+};
+int dense_dgate_parts(int T);
+hipError_t launch_dgate(const DgateArgs &a, hipStream_t s);
 
 // x [n] f32 as kPlanes bf16 planes, `plane` elements apart.
 hipError_t launch_planes(const float *x, size_t n, uint16_t *out, size_t plane, hipStream_t s);

@@ -429,19 +429,31 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
   const int P = dtype == MOE_BF16 ? 1 : kPlanes;
   const bool bf = dtype == MOE_BF16;
   const bool inner = out->x || out->gate_up || out->gate_up_bias || out->down;
-  const DenseShape sg{true, false, DENSE_DGATE}, sx{true, false, DENSE_STORE}, sw{true, true, DENSE_STORE};
+  const DenseShape ss{false, false, DENSE_STORE}, sg{true, false, DENSE_DGATE}, sx{true, false, DENSE_STORE}, sw{true, true, DENSE_STORE};
   Carve w;
   Rows r, d, h, dgu;
-  float *gu = nullptr, *db = nullptr, *col = nullptr, *part = nullptr;
-  int nx = 1, ngu = 1, nd = 1, db_parts = 0;
+  float *gu = nullptr, *dh = nullptr, *db = nullptr, *col = nullptr, *part = nullptr;
+  int nx = 1, ngu = 1, nd = 1, db_parts = 0, n_raw = 1, n_dh = 1;
+  bool apart = false;  // d(gate, up) in a kernel of its own, from K parts of gate, up and dh
   for (int placed = 0; placed < 2; placed++) {
     if (inner) {
       r = x_type == MOE_MXFP8 ? Rows{w.take<uint16_t>(T * H), 1, 0} : plane_rows(w, x, dtype, T * H);
       d = plane_rows(w, dy, dtype, T * H);
-      gu = w.take<float>(T * 2 * I);
+      // Few rows leave most of the device idle in products that are not split: then gate, up and dh come in K
+      // parts, which a kernel of its own joins (333 f32 rows, 2048 x 1536: DENSE_DGATE 35 us)
+      DenseArgs raw = product(b->gate_up, H, 0, 1, r.p, H, r.plane, r.planes, 2 * I, T, H);
+      DenseArgs in = product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H);
+      raw.out_mode = in.out_mode = 1;
+      const double one = dense_estimate(ss, raw) + dense_estimate(sg, in);
+      raw.splits = n_raw = dense_splits(ss, raw);
+      in.splits = n_dh = dense_splits(sx, in);
+      apart = dense_estimate(ss, raw) + dense_estimate(sx, in) + 1.0 + 26e-6 / 5 * T * I < one && T <= 65536;
+      if (!apart) n_raw = n_dh = 1;
+      gu = w.take<float>(n_raw * T * 2 * I);
+      dh = apart ? w.take<float>(n_dh * T * I) : nullptr;
       h = Rows{w.take<uint16_t>(P * T * I), P, T * I};
       dgu = Rows{w.take<uint16_t>(P * T * 2 * I), P, T * 2 * I};
-      db_parts = dense_parts(sg, product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H));
+      db_parts = apart ? dense_dgate_parts((int)T) : dense_parts(sg, product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H));
       db = out->gate_up_bias ? w.take<float>((size_t)db_parts * 2 * I) : nullptr;
       nx = dense_splits(sx, product(b->gate_up, H, 0, 1, dgu.p, 2 * I, dgu.plane, P, H, T, 2 * I));
       ngu = dense_splits(sw, product(r.p, H, r.plane, r.planes, dgu.p, 2 * I, dgu.plane, P, H, 2 * I, T, true));
@@ -468,21 +480,35 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
   else
     RETURN_IF(fill_rows(r, x, dtype, T * H, s));
   RETURN_IF(fill_rows(d, dy, dtype, T * H, s));
-  DenseArgs g = product(b->gate_up, H, 0, 1, r.p, H, r.plane, r.planes, 2 * I, T, H);
-  g.bias = b->gate_up_bias;
-  g.gu = gu;
-  HIP_TRY(launch_dense(DenseShape{false, false, DENSE_GATE_RAW}, g, s));
-  g = product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H);
-  g.limit = c.clamp;
-  g.gu = gu;
-  g.h = const_cast<uint16_t *>(h.p);
-  g.h_plane = h.plane;
-  g.ldh = I;
-  g.dgu = const_cast<uint16_t *>(dgu.p);
-  g.dgu_plane = dgu.plane;
-  g.db_part = db;
-  g.planes = P;
-  HIP_TRY(launch_dense(sg, g, s));
+  // gate and up as f32, their K parts side by side
+  auto parts = [&](const DenseShape &shape, DenseArgs g, int splits, const float *bias, float *out) -> int {
+    g.ldo = (size_t)g.M;
+    g.out = out;
+    g.out_mode = 1;
+    g.splits = splits;
+    g.split_stride = (size_t)g.M * g.N;
+    g.bias = bias;
+    HIP_TRY(launch_dense(shape, g, s));
+    return MOE_OK;
+  };
+  RETURN_IF(parts(ss, product(b->gate_up, H, 0, 1, r.p, H, r.plane, r.planes, 2 * I, T, H), n_raw, apart ? nullptr : b->gate_up_bias, gu));
+  DenseArgs g = product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H);
+  if (apart) {
+    RETURN_IF(parts(sx, g, n_dh, nullptr, dh));
+    HIP_TRY(launch_dgate(DgateArgs{gu, b->gate_up_bias, dh, n_raw, n_dh, (int)T, (int)I, P, c.clamp, const_cast<uint16_t *>(h.p),
+                                   const_cast<uint16_t *>(dgu.p), db}, s));
+  } else {
+    g.limit = c.clamp;
+    g.gu = gu;
+    g.h = const_cast<uint16_t *>(h.p);
+    g.h_plane = h.plane;
+    g.ldh = I;
+    g.dgu = const_cast<uint16_t *>(dgu.p);
+    g.dgu_plane = dgu.plane;
+    g.db_part = db;
+    g.planes = P;
+    HIP_TRY(launch_dense(sg, g, s));
+  }
   if (db) HIP_TRY(launch_sum_parts(db, 2 * I, db_parts, 2 * I, nullptr, 1, out->gate_up_bias, false, s));
   if (out->x)
     RETURN_IF(store(product(b->gate_up, H, 0, 1, dgu.p, 2 * I, dgu.plane, P, H, T, 2 * I), true, false, nx, part, nullptr,

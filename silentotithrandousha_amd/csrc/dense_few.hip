@@ -1,0 +1,91 @@
+// The dense products of few rows (up to 16, a row's planes counted): the weights stream once through
+// registers, no LDS.
+//
+// A workgroup takes 16 rows of A; its 8 wavefronts take the K-steps of 64 values in turn, each with the
+// loads of its next 6 steps under way, and their sums join in LDS, in order. Bound by the weights' bytes
+// and the latency of the first of them: one row of 2880 x 2880 weights (33 MB of gate and up, 16.6 MB
+// down) took 10.6 and 8.3 us (with the sum of its K parts) through the LDS rings of dense_gemm.hpp.
+#include "dense_gemm.hpp"
+#include "dense_launch.hpp"
+
+namespace moe {
+namespace {
+
+constexpr int kWaves = 8, kAhead = 6;
+
+template <int EPI>
+__global__ __launch_bounds__(64 * kWaves) void k_dense_few(const DenseArgs a) {
+  __shared__ float s_sum[kWaves][16][17];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m0 = blockIdx.x * 16, rows_b = a.N * a.stack, at = lane >> 4;
+  const uint16_t *A = a.A + (size_t)(m0 + (lane & 15)) * a.lda, *B = a.B + (size_t)min(lane & 15, rows_b - 1) * a.ldb;
+  const int steps = (a.K + kDenseStep - 1) / kDenseStep;
+  f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = wave; s0 < steps; s0 += kWaves * kAhead) {
+    uint4 fa[kAhead][2], fb[kAhead][2];
+#pragma unroll
+    for (int i = 0; i < kAhead; i++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int k = (s0 + i * kWaves) * kDenseStep + h * kDenseHalf + at * 8, c = min(k, a.K - 8);
+        const bool in = k < a.K;  // (K is a multiple of 8)
+        fa[i][h] = *(const uint4 *)(A + c);
+        fb[i][h] = *(const uint4 *)(B + c);
+        if (!in) fa[i][h] = fb[i][h] = uint4{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+    for (int i = 0; i < kAhead; i++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(fa[i][h]), as_bf16x8(fb[i][h]), acc, 0, 0, 0);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; r++) s_sum[wave][lane & 15][at * 4 + r] = acc[r];
+  __syncthreads();
+  // the sum of the wavefronts' parts, and of a row's planes from the lowest terms up
+  auto sum = [&](int n, int m) __attribute__((always_inline)) {
+    float v = 0.0f;
+    for (int p = a.stack - 1; p >= 0; p--)
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) v += s_sum[w][p * a.N + n][m];
+    return v + (a.bias ? a.bias[m0 + m] : 0.0f);
+  };
+  if constexpr (EPI == DENSE_STORE) {
+    const int n = threadIdx.x / 16, m = threadIdx.x % 16;
+    if (n < a.N) {
+      const float v = sum(n, m);
+      const size_t o = (size_t)n * a.ldo + m0 + m;
+      if (a.out_mode == 0)
+        ((uint16_t *)a.out)[o] = dense_bf16(v);
+      else
+        ((float *)a.out)[o] = v;
+    }
+  } else {
+    const int n = threadIdx.x / 8, i = threadIdx.x % 8;
+    if (n < a.N) {
+      DenseGate g;
+      g.set<false>(sum(n, 2 * i), sum(n, 2 * i + 1), a.limit);
+      uint16_t q[kPlanes];
+      dense_split(g.h(), q);
+      for (int p = 0; p < a.planes; p++) a.h[p * a.h_plane + (size_t)n * a.ldh + m0 / 2 + i] = q[p];
+    }
+  }
+}
+
+}  // namespace
+
+// (more rows of A than 4 tiles a CU keep the rings' larger tiles full)
+bool dense_few_fits(const DenseShape &s, const DenseArgs &a) {
+  return !s.at && !s.bt && (s.epi == DENSE_GATE || s.epi == DENSE_STORE) && a.n_pass == 1 && a.N * a.stack <= 16 && a.M % 16 == 0 &&
+         a.K % 8 == 0 && a.M <= 16 * 1024 && a.splits <= 1 && !a.scale && a.out_mode != 2;
+}
+
+hipError_t launch_dense_few(const DenseShape &s, const DenseArgs &a, hipStream_t st) {
+  if (!dense_few_fits(s, a)) return hipErrorInvalidValue;
+  if (s.epi == DENSE_GATE)
+    k_dense_few<DENSE_GATE><<<a.M / 16, 64 * kWaves, 0, st>>>(a);
+  else
+    k_dense_few<DENSE_STORE><<<a.M / 16, 64 * kWaves, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace moe

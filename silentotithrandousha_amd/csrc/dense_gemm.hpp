@@ -55,6 +55,11 @@ struct DenseGate {
     s = __builtin_amdgcn_rcpf(1.0f + (NEAR ? dense_exp_near(t) : dense_exp(t)));
   }
   __device__ __forceinline__ float h() const { return (U + 1.0f) * (G * s); }
+  // d loss / d(g, u) from dh = d loss / d h: nothing passes a clamp
+  __device__ __forceinline__ float dg(float dh, float g, float limit) const {
+    return g > limit ? 0.0f : dh * (U + 1.0f) * (s * (1.0f + 1.702f * (G * (1.0f - s))));
+  }
+  __device__ __forceinline__ float du(float dh, float u, float limit) const { return fabsf(u) > limit ? 0.0f : dh * (G * s); }
 };
 
 // One operand's tile: R rows (of M or N) x 64 k, W wavefronts loading it.
@@ -400,7 +405,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   static_assert(W * kStage <= NS * kSlot, "the results of 16 columns fit the LDS of the steps");
   uint8_t *stage = lds + wave * kStage;
   if constexpr (EPI != DENSE_STATS && EPI != DENSE_DGATE) __syncthreads();
-  if constexpr (EPI == DENSE_STORE || EPI == DENSE_GATE || EPI == DENSE_GATE_RAW) {
+  if constexpr (EPI == DENSE_STORE || EPI == DENSE_GATE) {
     const float scale = EPI == DENSE_STORE && a.scale ? *a.scale : 1.0f;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
@@ -436,10 +441,6 @@ if (a.out_mode == 2) {
       dense_rows_f32(stage, lane, acc, j, (float *)a.out + split * a.split_stride + (size_t)(n_first + j * 16) * a.ldo + m_first, a.ldo,
                      a.N - n_first - j * 16, a.M - m_first);
     }
-  } else if constexpr (EPI == DENSE_GATE_RAW) {
-#pragma unroll
-    for (int j = 0; j < TN; j++)
-      dense_rows_f32(stage, lane, acc, j, a.gu + (size_t)(n_first + j * 16) * a.M + m_first, a.M, a.N - n_first - j * 16, a.M - m_first);
   } else if constexpr (EPI == DENSE_GATE) {
     auto gate = [&](auto ONE) __attribute__((always_inline)) {  // ONE plane, or kPlanes
       constexpr bool one = decltype(ONE)::value;
@@ -490,8 +491,8 @@ if (a.out_mode == 2) {
             g.set<one>(gate, up, a.limit);
             const float dh = acc[i][j][r];
             hv[r] = g.h();
-            d[2 * r] = gate > a.limit ? 0.0f : dh * (g.U + 1.0f) * (g.s * (1.0f + 1.702f * (g.G * (1.0f - g.s))));
-            d[2 * r + 1] = fabsf(up) > a.limit ? 0.0f : dh * (g.G * g.s);
+            d[2 * r] = g.dg(dh, gate, a.limit);
+            d[2 * r + 1] = g.du(dh, up, a.limit);
           }
 #pragma unroll
           for (int r = 0; r < 8; r++) db[r] += d[r];

@@ -52,6 +52,8 @@ constexpr DenseTileDims kDenseTiles[] = {
 #undef X
 };
 
+bool dense_few_fits(const DenseShape &s, const DenseArgs &a);
+hipError_t launch_dense_few(const DenseShape &s, const DenseArgs &a, hipStream_t st);
 hipError_t launch_dense_nt(const DenseShape &s, const DenseArgs &a, hipStream_t st);
 hipError_t launch_dense_tn(const DenseShape &s, const DenseArgs &a, hipStream_t st);
 
