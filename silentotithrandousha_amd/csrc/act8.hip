@@ -15,8 +15,8 @@ namespace moe {
 namespace {
 
 __device__ __forceinline__ void load8(const float *x, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = x[i];
+  const float4 a = *(const float4 *)x, b = *(const float4 *)(x + 4);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 __device__ __forceinline__ void load8(const uint16_t *x, float (&v)[8]) {
   const uint4 u = *(const uint4 *)x;
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void k_act8_pack(const S *x, size_t blocks, ui
 }
 
 template <class D>
-__global__ __launch_bounds__(256) void k_act8_unpack(const uint8_t *codes, const uint8_t *scales, size_t blocks, D *out) {
+__global__ __launch_bounds__(256) void k_act8_unpack(const uint8_t *codes, const uint8_t *scales, size_t blocks, D *out, int copies) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, b = i / 4;
   if (b >= blocks) return;
   const uint2 u = *(const uint2 *)(codes + i * 8);
@@ -79,14 +79,17 @@ __global__ __launch_bounds__(256) void k_act8_unpack(const uint8_t *codes, const
 #pragma unroll
   for (int j = 0; j < 8; j++)
     if (sc == 255) v[j] = NAN;
-  if constexpr (sizeof(D) == 4) {
+  for (int c = 0; c < copies; c++, out += blocks * 32) {
+    if constexpr (sizeof(D) == 4) {
+      float4 *o = (float4 *)(out + i * 8);
+      o[0] = make_float4(v[0], v[1], v[2], v[3]);
+      o[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint16_t q[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) out[i * 8 + j] = v[j];
-  } else {
-    uint16_t q[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) q[j] = __builtin_bit_cast(uint16_t, (__bf16)v[j]);
-    *(uint4 *)(out + i * 8) = __builtin_bit_cast(uint4, q);
+      for (int j = 0; j < 8; j++) q[j] = __builtin_bit_cast(uint16_t, (__bf16)v[j]);
+      *(uint4 *)(out + i * 8) = __builtin_bit_cast(uint4, q);
+    }
   }
 }
 
@@ -105,16 +108,16 @@ hipError_t launch_act8_pack(const void *x, bool bf16, size_t n, size_t cols, uin
   return hipGetLastError();
 }
 
-hipError_t launch_act8_unpack(const uint8_t *packed, size_t n, size_t cols, void *out, bool bf16, hipStream_t s) {
+hipError_t launch_act8_unpack(const uint8_t *packed, size_t n, size_t cols, void *out, bool bf16, int copies, hipStream_t s) {
   const size_t blocks = n * cols / 32;
   if (!blocks) return hipSuccess;
   const size_t grid = (blocks * 4 + 255) / 256;
   if (cols % 32 || grid > 0x7FFFFFFF) return hipErrorInvalidValue;
   const uint8_t *scales = packed + n * cols;
   if (bf16)
-    k_act8_unpack<<<(unsigned)grid, 256, 0, s>>>(packed, scales, blocks, (uint16_t *)out);
+    k_act8_unpack<<<(unsigned)grid, 256, 0, s>>>(packed, scales, blocks, (uint16_t *)out, copies);
   else
-    k_act8_unpack<<<(unsigned)grid, 256, 0, s>>>(packed, scales, blocks, (float *)out);
+    k_act8_unpack<<<(unsigned)grid, 256, 0, s>>>(packed, scales, blocks, (float *)out, copies);
   return hipGetLastError();
 }
 

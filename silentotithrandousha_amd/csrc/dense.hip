@@ -29,8 +29,8 @@ double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a,
   // bytes that a result costs, about
   const double result = s.epi == DENSE_STATS ? 0.0 : s.epi == DENSE_GATE ? 1.0 : s.epi == DENSE_DGATE ? 14.0
                         : s.epi == DENSE_STORE && (a.out_mode || splits > 1) ? 4.0 : 2.0;
-  // a transposed A's rows of k are read in pieces of a tile's rows: below 128 bytes at two thirds of the rate
-  const double memory = s.at && d.bm < 64 ? 15.0 : 23.0;  // GB/s a CU; 5.9 TB/s in all
+  // a transposed A's rows of k are read in pieces of a tile's rows: below 128 bytes the slower for it
+  const double memory = s.at && d.bm < 64 ? 23.0 * d.bm / 64 : 23.0;  // GB/s a CU; 5.9 TB/s in all
   auto round = [&](long on_cu) {
     double step = std::max(0.45 / (d.ns - 1) + 0.1, on_cu * d.bm * d.bn * 2.0 * kDenseStep * kCus / (d.rate * 1e6));
     if (tiles_n == 1) step = std::max(step, on_cu * d.bm * 128e-3 / memory);
@@ -39,7 +39,7 @@ double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a,
   };
   const long whole = tiles / (kCus * d.wgs), rest = tiles - whole * kCus * d.wgs;
   double us = whole * round(d.wgs) + (rest ? round((rest + kCus - 1) / kCus) : 0.0);
-  if (splits > 1) us += 3.0 + 4.0 * splits * a.M * a.N / 5e6;
+  if (splits > 1) us += 4.5 + 4.0 * splits * a.M * a.N / 5e6;
   return us;
 }
 
@@ -106,13 +106,22 @@ hipError_t launch_dense(const DenseShape &s, const DenseArgs &a0, hipStream_t st
 
 namespace {
 
-// One value per thread and step; bound by its 4 bytes read and 6 written.
-__global__ void k_planes(const float *x, size_t n, uint16_t *out, size_t plane) {
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-    uint16_t p[kPlanes];
-    dense_split(x[i], p);
+// Two arrays in one launch (the rows and their gradients, of one length). Bound by its 4 bytes read and 6
+// written a value, of few by the launch.
+__global__ void k_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n) {
+  const float *x = blockIdx.y ? x1 : x0;
+  uint16_t *out = blockIdx.y ? out1 : out0;
+  const uint32_t where = blockIdx.y ? where1 : where0;
+  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (size_t)gridDim.x * 1024) {  // (n is a multiple of 32)
+    const f32x4 v = *(const f32x4 *)(x + i);
+    uint16_t p[4][kPlanes];
 #pragma unroll
-    for (int j = 0; j < kPlanes; j++) out[j * plane + i] = p[j];
+    for (int j = 0; j < 4; j++) dense_split(v[j], p[j]);
+#pragma unroll
+    for (int k = 0; k < kPlanes; k++) {
+      const uint2 q = {p[0][k] | (uint32_t)p[1][k] << 16, p[2][k] | (uint32_t)p[3][k] << 16};
+      dense_slots(where, k, [&](size_t at) { *(uint2 *)(out + at * n + i) = q; });
+    }
   }
 }
 
@@ -244,8 +253,8 @@ __global__ __launch_bounds__(256) void k_dgate(const DgateArgs a) {
         uint16_t q[8], e[4];
         dense_take<!ONE>(d, q);
         dense_take<!ONE>(hv, e);
-        *(uint4 *)(a.dgu + p * 2 * plane + t * 2 * a.I + 2 * i) = __builtin_bit_cast(uint4, q);
-        *(uint2 *)(a.h + p * plane + t * a.I + i) = __builtin_bit_cast(uint2, e);
+        dense_slots(a.dgu_where, p, [&](size_t at) { *(uint4 *)(a.dgu + at * 2 * plane + t * 2 * a.I + 2 * i) = __builtin_bit_cast(uint4, q); });
+        dense_slots(a.h_where, p, [&](size_t at) { *(uint2 *)(a.h + at * plane + t * a.I + i) = __builtin_bit_cast(uint2, e); });
       }
     }
   }
@@ -311,9 +320,11 @@ unsigned blocks_for(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 25
 
 }  // namespace
 
-hipError_t launch_planes(const float *x, size_t n, uint16_t *out, size_t plane, hipStream_t s) {
+hipError_t launch_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n,
+                         hipStream_t s) {
   if (!n) return hipSuccess;
-  k_planes<<<blocks_for(n), 256, 0, s>>>(x, n, out, plane);
+  if (n % 4) return hipErrorInvalidValue;
+  k_planes<<<dim3(blocks_for(n / 4), x1 ? 2 : 1), 256, 0, s>>>(x0, out0, where0, x1, out1, where1, n);
   return hipGetLastError();
 }
 

@@ -10,9 +10,16 @@
 namespace moe {
 
 // f32 values enter the bf16 MFMA as the sum of kPlanes bf16 values (8 significant bits each: the 24
-// of an f32 exactly, short of the subnormal range); bf16 values as one.
+// of an f32 exactly, short of the subnormal range); bf16 values as one. A matrix of such values lies in
+// the workspace as slots [slot][rows][cols], each a plane: `where` holds in byte p the slots of plane p.
+// The product of two such matrices over their rows (a weight gradient) leaves out the planes' products
+// below 2^-24 of the largest and takes the other six as one product over 6 times the rows: its left
+// operand's slots hold the planes 0 1 2 0 1 0, its right one's 2 1 0 1 0 0. (As six passes over K, each with
+// a K tail of its own, the gradient of the LM head for 19 rows took 54 us.)
 constexpr int kPlanes = 3;
-constexpr int kMaxPass = 6;
+constexpr int kPairs6 = 6;
+constexpr uint32_t kWhereOne = 0x01, kWhereThree = 0x040201, kWhereLeft = 0x041229, kWhereRight = 0x010A34;
+constexpr int kMaxPass = 3;
 
 // Epilogues.
 enum DenseEpi {
@@ -29,12 +36,12 @@ enum DenseEpi {
 // rounded up to 8.
 struct DenseArgs {
   const uint16_t *A, *B;
-  size_t a_plane, b_plane;  // elements between planes
+  size_t b_slot;            // elements between slots of B
   size_t lda, ldb;          // elements between rows of the stored matrix
   int M, N, K;
-  int stack;                // planes of B that one pass takes as rows [plane][N] (N * stack <= 64), else 1
+  int stack;                // slots of B that one pass takes as rows [slot][N] (N * stack <= 64), else 1
   int n_pass;
-  uint32_t pa, pb;          // planes of A and B of each pass, 4 bits each
+  uint32_t pb;              // the slot of B of each pass, 4 bits each
   int splits;               // K split (DENSE_STORE with f32 only): out + split * split_stride
   int k_split;              // K per split, a multiple of the step
   // DENSE_STORE
@@ -45,11 +52,13 @@ struct DenseArgs {
   const float *scale;       // factor of the result (one value) or NULL; of the loss: what dloss is divided by
   // gated block
   float limit;
-  uint16_t *h;              // [planes][N][ldh] bf16
-  size_t h_plane, ldh;
+  uint16_t *h;              // [slots][N][ldh] bf16
+  size_t h_slot, ldh;
+  uint32_t h_where;
   const float *gu;          // [N][2 M]
-  uint16_t *dgu;            // [planes][N][2 M]
-  size_t dgu_plane;
+  uint16_t *dgu;            // [slots][N][2 M]
+  size_t dgu_slot;
+  uint32_t dgu_where;
   float *db_part;           // [parts][2 M] or NULL
   int planes;
   // loss
@@ -59,8 +68,9 @@ struct DenseArgs {
   float *picked;            // [N] target logits
   const float *lse, *dloss; // [N]
   int vocab;                // rows of the whole vocabulary: targets at or above it are invalid
-  uint16_t *dl;             // [planes][N][ld_dl]
-  size_t dl_plane, ld_dl;
+  uint16_t *dl;             // [slots][N][ld_dl]
+  size_t dl_slot, ld_dl;
+  uint32_t dl_where;
 };
 
 struct DenseShape {
@@ -80,14 +90,16 @@ struct DgateArgs {
   const float *gu, *bias, *dh;
   int gu_parts, dh_parts, T, I, planes;
   float limit;
-  uint16_t *h, *dgu;  // [planes][T][I], [planes][T][2 I]
+  uint16_t *h, *dgu;  // [slots][T][I], [slots][T][2 I]
+  uint32_t h_where, dgu_where;
   float *db_part;
 };
 int dense_dgate_parts(int T);
 hipError_t launch_dgate(const DgateArgs &a, hipStream_t s);
 
-// x [n] f32 as kPlanes bf16 planes, `plane` elements apart.
-hipError_t launch_planes(const float *x, size_t n, uint16_t *out, size_t plane, hipStream_t s);
+// x0 [n] f32 as kPlanes bf16 planes in the slots (n elements each) of `where0`; x1 (or NULL) likewise.
+hipError_t launch_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n,
+                         hipStream_t s);
 // out[i] = sum over parts of part[p * stride + i] (+ bias[i % n_bias]) for i < n, in order; bf16 or f32.
 hipError_t launch_sum_parts(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias,
                             void *out, bool bf16, hipStream_t s);
@@ -103,7 +115,8 @@ hipError_t launch_dloss_scale(const float *dloss, size_t T, float *scale, hipStr
 
 // MXFP8 activation checkpoints (act8.hip): codes [n][cols], then scales [n][cols / 32].
 hipError_t launch_act8_pack(const void *x, bool bf16, size_t n, size_t cols, uint8_t *packed, hipStream_t s);
-hipError_t launch_act8_unpack(const uint8_t *packed, size_t n, size_t cols, void *out, bool bf16, hipStream_t s);
+// (copies: of the values, one behind the other)
+hipError_t launch_act8_unpack(const uint8_t *packed, size_t n, size_t cols, void *out, bool bf16, int copies, hipStream_t s);
 
 // Device workspace of the dense operators: grows at need; a buffer that a captured graph may hold is
 // kept until the context goes.

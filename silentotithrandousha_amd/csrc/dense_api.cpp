@@ -112,56 +112,71 @@ int check_distinct(std::initializer_list<const void *> outs, std::initializer_li
   return MOE_OK;
 }
 
-// Rows [n][cols] as the products take them: bf16 planes.
+// Rows [n][cols] as the products take them: their values, or their planes in slots.
 struct Rows {
   const uint16_t *p = nullptr;
-  int planes = 1;
-  size_t plane = 0;  // elements between planes
+  size_t n = 0, cols = 0, ld = 0;
+  int slots = 1;
+  uint32_t where = kWhereOne;
+  uint16_t *out() const { return const_cast<uint16_t *>(p); }
+  size_t slot() const { return n * ld; }
+  size_t size() const { return slots * slot(); }
 };
-
-// Products of the planes of A and B, smallest terms first; terms below 2^-24 of the result are left out.
-void set_passes(DenseArgs &a, int na, int nb) {
-  a.n_pass = 0;
-  a.pa = a.pb = 0;
-  for (int sum = kPlanes - 1; sum >= 0; sum--)
-    for (int i = 0; i <= sum; i++)
-      if (i < na && sum - i < nb) {
-        a.pa |= (uint32_t)i << 4 * a.n_pass;
-        a.pb |= (uint32_t)(sum - i) << 4 * a.n_pass;
-        a.n_pass++;
-      }
+Rows rows_of(int dtype, uint32_t where, size_t n, size_t cols, size_t ld) {
+  if (dtype == MOE_BF16) return Rows{nullptr, n, cols, ld};
+  return Rows{nullptr, n, cols, ld, where == kWhereThree ? kPlanes : kPairs6, where};
+}
+// rows in the workspace; of a caller's matrix only if it is f32
+Rows place(Carve &w, Rows r) {
+  r.p = w.take<uint16_t>(r.size());
+  return r;
+}
+Rows place(Carve &w, Rows r, const void *x, int dtype) {
+  if (dtype != MOE_BF16) return place(w, r);
+  r.p = (const uint16_t *)x;
+  return r;
+}
+int fill(const Rows &r, const void *x, int dtype, hipStream_t s) {
+  if (dtype == MOE_F32) HIP_TRY(launch_planes((const float *)x, r.out(), r.where, nullptr, nullptr, 0, r.slot(), s));
+  return MOE_OK;
 }
 
-DenseArgs product(const uint16_t *A, size_t lda, size_t a_plane, int na, const uint16_t *B, size_t ldb, size_t b_plane, int nb,
-                  size_t M, size_t N, size_t K, bool bt = false) {
+// Weights times rows: D[m][n] = sum W[m][k] rows[n][k] (W [M][K], or [K][M] for a launch with A transposed),
+// the rows' lower planes first; of few rows, all planes in one pass.
+DenseArgs product(const uint16_t *W, size_t ldw, const Rows &b, size_t M) {
   DenseArgs a{};
-  a.A = A;
-  a.lda = lda;
-  a.a_plane = a_plane;
-  a.B = B;
-  a.ldb = ldb;
-  a.b_plane = b_plane;
+  a.A = W;
+  a.lda = ldw;
+  a.B = b.p;
+  a.ldb = b.ld;
+  a.b_slot = b.slot();
   a.M = (int)M;
-  a.N = (int)N;
-  a.K = (int)K;
-  a.splits = 1;
-  a.stack = 1;
-  if (!bt && na == 1 && nb > 1 && N * nb <= 64 && b_plane == N * ldb) {  // few rows: the planes of B as its rows
-    a.stack = nb;
-    nb = 1;
+  a.N = (int)b.n;
+  a.K = (int)b.cols;
+  a.splits = a.stack = a.n_pass = 1;
+  if (b.where != kWhereOne) {
+    if (b.n * kPlanes <= 64) {
+      a.stack = kPlanes;  // the first three slots, one of each plane
+    } else {
+      a.n_pass = kPlanes;
+      for (int i = 0; i < kPlanes; i++) a.pb |= (uint32_t)__builtin_ctz(b.where >> 8 * (kPlanes - 1 - i)) << 4 * i;
+    }
   }
-  set_passes(a, na, nb);
   return a;
 }
-
-// f32 rows: their planes in the workspace. bf16 rows: as they are.
-Rows plane_rows(Carve &w, const void *x, int dtype, size_t n) {
-  if (dtype == MOE_BF16) return Rows{(const uint16_t *)x, 1, 0};
-  return Rows{w.take<uint16_t>(kPlanes * n), kPlanes, n};
-}
-int fill_rows(const Rows &r, const void *x, int dtype, size_t n, hipStream_t s) {
-  if (dtype == MOE_F32) HIP_TRY(launch_planes((const float *)x, n, const_cast<uint16_t *>(r.p), r.plane, s));
-  return MOE_OK;
+// Rows times rows over their rows: D[m][n] = sum_t a[t][m] b[t][n]; of a's values (or copies of them) and
+// b's planes, or of both's planes in pairs.
+DenseArgs gradient(const Rows &x, const Rows &y) {
+  DenseArgs a{};
+  a.A = x.p;
+  a.lda = x.ld;
+  a.B = y.p;
+  a.ldb = y.ld;
+  a.M = (int)x.cols;
+  a.N = (int)y.cols;
+  a.K = (int)(std::min(x.slots, y.slots) * x.n);
+  a.splits = a.stack = a.n_pass = 1;
+  return a;
 }
 
 // out [N][M] (+ bias) of a product, K split where that fills the device; part: [splits][N][M] f32 then.
@@ -238,12 +253,14 @@ int moe_lm_head_loss_device(moe_ctx *ctx, const void *x, int dtype, const int32_
   float2 *stats = nullptr;
   float *picked = nullptr;
   for (int placed = 0; placed < 2; placed++) {
-    r = plane_rows(w, x, dtype, T * H);
+    r = rows_of(dtype, kWhereThree, Tc, H, H);
     size_t most = 0;  // (the last piece of tokens may take another tile)
     for (size_t t0 = 0; t0 < T; t0 += Tc) {
-      const size_t n = std::min(Tc, T - t0);
-      most = std::max(most, n * (size_t)dense_parts(shape, product(c.lm_w, H, 0, 1, r.p, H, r.plane, r.planes, vocab, n, H)));
+      r.n = std::min(Tc, T - t0);
+      most = std::max(most, r.n * (size_t)dense_parts(shape, product(c.lm_w, H, r, vocab)));
     }
+    r.n = Tc;
+    r = place(w, r, x, dtype);
     stats = w.take<float2>(most);
     picked = w.take<float>(Tc);
     if (!placed) {
@@ -251,10 +268,13 @@ int moe_lm_head_loss_device(moe_ctx *ctx, const void *x, int dtype, const int32_
       w = Carve{(char *)c.work->p};
     }
   }
-  RETURN_IF(fill_rows(r, x, dtype, T * H, s));
   for (size_t t0 = 0; t0 < T; t0 += Tc) {
     const size_t n = std::min(Tc, T - t0);
-    DenseArgs a = product(c.lm_w, H, 0, 1, r.p + t0 * H, H, r.plane, r.planes, vocab, n, H);
+    Rows piece = r;
+    piece.n = n;
+    if (dtype == MOE_BF16) piece.p += t0 * H;
+    RETURN_IF(fill(piece, (const char *)x + t0 * H * elem(dtype), dtype, s));
+    DenseArgs a = product(c.lm_w, H, piece, vocab);
     a.targets = targets + t0;
     a.stats = stats;
     a.picked = picked;
@@ -280,20 +300,19 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
   const bool bf = dtype == MOE_BF16;
   // pieces of tokens and of the vocabulary whose gradient of the logits is held at once
   const size_t Tc = std::min(T, kGradTokens), nt = (T + Tc - 1) / Tc;
-  const size_t most = std::max<size_t>(256, kGradBytes / (2 * P * Tc) / 256 * 256), nv = (vocab + most - 1) / most;
+  const size_t most = std::max<size_t>(256, kGradBytes / (2 * (bf ? 1 : kPairs6) * Tc) / 256 * 256), nv = (vocab + most - 1) / most;
   const size_t Vc = std::min(vocab, ((vocab + nv - 1) / nv + 255) / 256 * 256), ld = (Vc + 7) / 8 * 8;
   const DenseShape sx{true, false, DENSE_STORE}, sw{true, true, DENSE_STORE};
   // few tokens: dx from K splits of every piece of the vocabulary, summed at the end; many: added up
-  const int splits = dense_splits(sx, product(c.lm_w, H, 0, 1, nullptr, ld, 0, P, H, Tc, Vc));
+  const int splits = dense_splits(sx, product(c.lm_w, H, rows_of(dtype, kWhereRight, Tc, Vc, ld), H));
   const bool parts = dx && splits > 1 && nt == 1;
   Carve w;
-  Rows r;
-  uint16_t *dl = nullptr;
+  Rows r, dl;
   float *dx_acc = nullptr, *dw_acc = nullptr, *scale = nullptr;
   for (int placed = 0; placed < 2; placed++) {
-    r = plane_rows(w, x, dtype, T * H);
+    r = place(w, rows_of(dtype, kWhereLeft, T, H, H), x, dtype);  // (f32: the slots of each piece of tokens together)
     scale = w.take<float>(1);
-    dl = w.take<uint16_t>(P * Tc * ld);
+    dl = place(w, rows_of(dtype, kWhereRight, Tc, Vc, ld));
     if (parts)
       dx_acc = w.take<float>(nv * splits * T * H);
     else if (dx)
@@ -304,7 +323,16 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
       w = Carve{(char *)c.work->p};
     }
   }
-  RETURN_IF(fill_rows(r, x, dtype, T * H, s));
+  auto piece = [&](size_t t0, size_t n) {
+    Rows q = r;
+    q.p += r.slots * t0 * H;
+    q.n = n;
+    return q;
+  };
+  for (size_t t0 = 0; t0 < T && !bf; t0 += Tc) {
+    const size_t n = std::min(Tc, T - t0);
+    RETURN_IF(fill(piece(t0, n), (const float *)x + t0 * H, dtype, s));
+  }
   // The gradient of the logits is held over the largest |dloss| and the results multiplied by it: for the
   // mean's constant dloss the entries of the targets, which weigh most, then lie next to -1 and are rounded
   // by their p alone, where bf16(1 / n) would put one error into all of them.
@@ -315,20 +343,25 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
     const uint16_t *wv = c.lm_w + v0 * H;
     for (size_t t0 = 0; t0 < T; t0 += Tc) {
       const size_t n = std::min(Tc, T - t0);
-      DenseArgs a = product(wv, H, 0, 1, r.p + t0 * H, H, r.plane, r.planes, nvoc, n, H);
+      const Rows rows = piece(t0, n);
+      Rows d = dl;
+      d.n = n;
+      d.cols = nvoc;
+      DenseArgs a = product(wv, H, rows, nvoc);
       a.targets = targets + t0;
       a.lse = lse + t0;
       a.dloss = dloss + t0;
       a.scale = scale;
       a.v0 = (int)v0;
       a.vocab = (int)vocab;
-      a.dl = dl;
-      a.dl_plane = Tc * ld;
+      a.dl = d.out();
+      a.dl_slot = d.slot();
+      a.dl_where = d.where;
       a.ld_dl = ld;
       a.planes = P;
       HIP_TRY(launch_dense(DenseShape{false, false, DENSE_DLOGITS}, a, s));
       if (dx) {
-        DenseArgs g = product(wv, H, 0, 1, dl, ld, Tc * ld, P, H, n, nvoc);
+        DenseArgs g = product(wv, H, d, H);
         g.ldo = H;
         g.scale = scale;
         if (parts) {
@@ -346,7 +379,7 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
         HIP_TRY(launch_dense(sx, g, s));
       }
       if (dw) {
-        DenseArgs g = product(r.p + t0 * H, H, r.plane, r.planes, dl, ld, Tc * ld, P, H, nvoc, n, true);
+        DenseArgs g = gradient(rows, d);
         g.ldo = H;
         g.scale = scale;
         if (!bf || dw_acc) {
@@ -384,9 +417,9 @@ int moe_ffn_forward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int dt
   float *part = nullptr;
   int splits = 1;
   for (int placed = 0; placed < 2; placed++) {
-    r = plane_rows(w, x, dtype, T * H);
-    h = Rows{w.take<uint16_t>(P * T * I), P, T * I};
-    splits = dense_splits(DenseShape{false, false, DENSE_STORE}, product(b->down, I, 0, 1, h.p, I, h.plane, P, H, T, I));
+    r = place(w, rows_of(dtype, kWhereThree, T, H, H), x, dtype);
+    h = place(w, rows_of(dtype, kWhereThree, T, I, I));
+    splits = dense_splits(DenseShape{false, false, DENSE_STORE}, product(b->down, I, h, H));
     part = splits > 1 ? w.take<float>(splits * T * H) : nullptr;
     if (!placed) {
       RETURN_IF(ensure(c, w.off, s));
@@ -394,16 +427,17 @@ int moe_ffn_forward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int dt
     }
   }
   if (x8) HIP_TRY(launch_act8_pack(x, dtype == MOE_BF16, T, H, x8, s));
-  RETURN_IF(fill_rows(r, x, dtype, T * H, s));
-  DenseArgs g = product(b->gate_up, H, 0, 1, r.p, H, r.plane, r.planes, 2 * I, T, H);
+  RETURN_IF(fill(r, x, dtype, s));
+  DenseArgs g = product(b->gate_up, H, r, 2 * I);
   g.bias = b->gate_up_bias;
   g.limit = c.clamp;
-  g.h = const_cast<uint16_t *>(h.p);
-  g.h_plane = h.plane;
+  g.h = h.out();
+  g.h_slot = h.slot();
+  g.h_where = h.where;
   g.ldh = I;
   g.planes = P;
   HIP_TRY(launch_dense(DenseShape{false, false, DENSE_GATE}, g, s));
-  return store(product(b->down, I, 0, 1, h.p, I, h.plane, P, H, T, I), false, false, splits, part, b->down_bias, y, dtype, s);
+  return store(product(b->down, I, h, H), false, false, splits, part, b->down_bias, y, dtype, s);
 }
 
 int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x_type, const void *dy, int dtype, size_t T,
@@ -437,12 +471,17 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
   bool apart = false;  // d(gate, up) in a kernel of its own, from K parts of gate, up and dh
   for (int placed = 0; placed < 2; placed++) {
     if (inner) {
-      r = x_type == MOE_MXFP8 ? Rows{w.take<uint16_t>(T * H), 1, 0} : plane_rows(w, x, dtype, T * H);
-      d = plane_rows(w, dy, dtype, T * H);
+      if (x_type == MOE_MXFP8) {  // exact in bf16: one plane, a copy of it for each of the planes it meets
+        r = Rows{nullptr, T, H, H, bf ? 1 : kPlanes};
+        r = place(w, r);
+      } else {
+        r = place(w, rows_of(dtype, kWhereLeft, T, H, H), x, dtype);
+      }
+      d = place(w, rows_of(dtype, kWhereRight, T, H, H), dy, dtype);
       // Few rows leave most of the device idle in products that are not split: then gate, up and dh come in K
       // parts, which a kernel of its own joins (333 f32 rows, 2048 x 1536: DENSE_DGATE 35 us)
-      DenseArgs raw = product(b->gate_up, H, 0, 1, r.p, H, r.plane, r.planes, 2 * I, T, H);
-      DenseArgs in = product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H);
+      DenseArgs raw = product(b->gate_up, H, r, 2 * I);
+      DenseArgs in = product(b->down, I, d, I);
       raw.out_mode = in.out_mode = 1;
       const double one = dense_estimate(ss, raw) + dense_estimate(sg, in);
       raw.splits = n_raw = dense_splits(ss, raw);
@@ -451,20 +490,21 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
       if (!apart) n_raw = n_dh = 1;
       gu = w.take<float>(n_raw * T * 2 * I);
       dh = apart ? w.take<float>(n_dh * T * I) : nullptr;
-      h = Rows{w.take<uint16_t>(P * T * I), P, T * I};
-      dgu = Rows{w.take<uint16_t>(P * T * 2 * I), P, T * 2 * I};
-      db_parts = apart ? dense_dgate_parts((int)T) : dense_parts(sg, product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H));
-      db = out->gate_up_bias ? w.take<float>((size_t)db_parts * 2 * I) : nullptr;
-      nx = dense_splits(sx, product(b->gate_up, H, 0, 1, dgu.p, 2 * I, dgu.plane, P, H, T, 2 * I));
-      ngu = dense_splits(sw, product(r.p, H, r.plane, r.planes, dgu.p, 2 * I, dgu.plane, P, H, 2 * I, T, true));
-      nd = dense_splits(sw, product(h.p, I, h.plane, P, d.p, H, d.plane, P, I, H, T, true));
+      h = place(w, rows_of(dtype, kWhereLeft, T, I, I));
+      dgu = place(w, rows_of(dtype, kWhereRight, T, 2 * I, 2 * I));
+      db_parts = apart ? dense_dgate_parts((int)T) : dense_parts(sg, product(b->down, I, d, I));
+      // (one part is the result)
+      db = !out->gate_up_bias ? nullptr : db_parts > 1 ? w.take<float>((size_t)db_parts * 2 * I) : out->gate_up_bias;
+      nx = dense_splits(sx, product(b->gate_up, H, dgu, H));
+      ngu = dense_splits(sw, gradient(r, dgu));
+      nd = dense_splits(sw, gradient(h, d));
       size_t most = 0;  // one after the other, so they share it
       if (out->x && nx > 1) most = std::max(most, nx * T * H);
       if (out->gate_up && ngu > 1) most = std::max(most, ngu * 2 * I * H);
       if (out->down && nd > 1) most = std::max(most, nd * I * H);
       part = w.take<float>(most);
     }
-    col = out->down_bias ? w.take<float>(dense_colsum_parts(T) * H) : nullptr;
+    col = !out->down_bias ? nullptr : dense_colsum_parts(T) > 1 ? w.take<float>(dense_colsum_parts(T) * H) : out->down_bias;
     if (!placed) {
       RETURN_IF(ensure(c, w.off, s));
       w = Carve{(char *)c.work->p};
@@ -472,14 +512,12 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
   }
   if (out->down_bias) {
     HIP_TRY(launch_colsum(dy, bf, T, H, col, s));
-    HIP_TRY(launch_sum_parts(col, H, dense_colsum_parts(T), H, nullptr, 1, out->down_bias, false, s));
+    if (dense_colsum_parts(T) > 1) HIP_TRY(launch_sum_parts(col, H, dense_colsum_parts(T), H, nullptr, 1, out->down_bias, false, s));
   }
   if (!inner) return MOE_OK;
-  if (x_type == MOE_MXFP8)
-    HIP_TRY(launch_act8_unpack((const uint8_t *)x, T, H, const_cast<uint16_t *>(r.p), true, s));
-  else
-    RETURN_IF(fill_rows(r, x, dtype, T * H, s));
-  RETURN_IF(fill_rows(d, dy, dtype, T * H, s));
+  if (x_type == MOE_MXFP8) HIP_TRY(launch_act8_unpack((const uint8_t *)x, T, H, r.out(), true, r.slots, s));
+  if (dtype == MOE_F32)
+    HIP_TRY(launch_planes((const float *)dy, d.out(), d.where, x_type == MOE_F32 ? (const float *)x : nullptr, r.out(), r.where, T * H, s));
   // gate and up as f32, their K parts side by side
   auto parts = [&](const DenseShape &shape, DenseArgs g, int splits, const float *bias, float *out) -> int {
     g.ldo = (size_t)g.M;
@@ -491,33 +529,34 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
     HIP_TRY(launch_dense(shape, g, s));
     return MOE_OK;
   };
-  RETURN_IF(parts(ss, product(b->gate_up, H, 0, 1, r.p, H, r.plane, r.planes, 2 * I, T, H), n_raw, apart ? nullptr : b->gate_up_bias, gu));
-  DenseArgs g = product(b->down, I, 0, 1, d.p, H, d.plane, P, I, T, H);
+  RETURN_IF(parts(ss, product(b->gate_up, H, r, 2 * I), n_raw, apart ? nullptr : b->gate_up_bias, gu));
+  DenseArgs g = product(b->down, I, d, I);
   if (apart) {
     RETURN_IF(parts(sx, g, n_dh, nullptr, dh));
-    HIP_TRY(launch_dgate(DgateArgs{gu, b->gate_up_bias, dh, n_raw, n_dh, (int)T, (int)I, P, c.clamp, const_cast<uint16_t *>(h.p),
-                                   const_cast<uint16_t *>(dgu.p), db}, s));
+    HIP_TRY(launch_dgate(DgateArgs{gu, b->gate_up_bias, dh, n_raw, n_dh, (int)T, (int)I, P, c.clamp, h.out(), dgu.out(), h.where, dgu.where, db}, s));
   } else {
     g.limit = c.clamp;
     g.gu = gu;
-    g.h = const_cast<uint16_t *>(h.p);
-    g.h_plane = h.plane;
+    g.h = h.out();
+    g.h_slot = h.slot();
+    g.h_where = h.where;
     g.ldh = I;
-    g.dgu = const_cast<uint16_t *>(dgu.p);
-    g.dgu_plane = dgu.plane;
+    g.dgu = dgu.out();
+    g.dgu_slot = dgu.slot();
+    g.dgu_where = dgu.where;
     g.db_part = db;
     g.planes = P;
     HIP_TRY(launch_dense(sg, g, s));
   }
-  if (db) HIP_TRY(launch_sum_parts(db, 2 * I, db_parts, 2 * I, nullptr, 1, out->gate_up_bias, false, s));
+  if (db && db_parts > 1) HIP_TRY(launch_sum_parts(db, 2 * I, db_parts, 2 * I, nullptr, 1, out->gate_up_bias, false, s));
   if (out->x)
-    RETURN_IF(store(product(b->gate_up, H, 0, 1, dgu.p, 2 * I, dgu.plane, P, H, T, 2 * I), true, false, nx, part, nullptr,
+    RETURN_IF(store(product(b->gate_up, H, dgu, H), true, false, nx, part, nullptr,
                     out->x, dtype, s));
   if (out->gate_up)
-    RETURN_IF(store(product(r.p, H, r.plane, r.planes, dgu.p, 2 * I, dgu.plane, P, H, 2 * I, T, true), true, true, ngu, part, nullptr,
+    RETURN_IF(store(gradient(r, dgu), true, true, ngu, part, nullptr,
                     out->gate_up, dtype, s));
   if (out->down)
-    RETURN_IF(store(product(h.p, I, h.plane, P, d.p, H, d.plane, P, I, H, T, true), true, true, nd, part, nullptr, out->down, dtype, s));
+    RETURN_IF(store(gradient(h, d), true, true, nd, part, nullptr, out->down, dtype, s));
   return MOE_OK;
 }
 
@@ -544,7 +583,7 @@ int moe_act8_unpack_device(moe_ctx *ctx, const uint8_t *packed, size_t n, size_t
   DenseCtx c;
   RETURN_IF(dense_ctx(ctx, &c));
   RETURN_IF(check_act8(packed, out, dtype, n, cols));
-  HIP_TRY(launch_act8_unpack(packed, n, cols, out, dtype == MOE_BF16, stream ? (hipStream_t)stream : c.stream));
+  HIP_TRY(launch_act8_unpack(packed, n, cols, out, dtype == MOE_BF16, 1, stream ? (hipStream_t)stream : c.stream));
   return MOE_OK;
 }
 

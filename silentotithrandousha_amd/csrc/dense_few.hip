@@ -1,4 +1,4 @@
-// The dense products of few rows (up to 16, a row's planes counted): the weights stream once through
+// The dense products of few rows (up to 8, a row's planes counted): the weights stream once through
 // registers, no LDS.
 //
 // A workgroup takes 16 rows of A; its 8 wavefronts take the K-steps of 64 values in turn, each with the
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_dense_few(const DenseArgs a) {
 #pragma unroll
   for (int r = 0; r < 4; r++) s_sum[wave][lane & 15][at * 4 + r] = acc[r];
   __syncthreads();
-  // the sum of the wavefronts' parts, and of a row's planes from the lowest terms up
+  // the sum of the wavefronts' parts, and of a row's planes
   auto sum = [&](int n, int m) __attribute__((always_inline)) {
     float v = 0.0f;
     for (int p = a.stack - 1; p >= 0; p--)
@@ -66,16 +66,18 @@ __global__ __launch_bounds__(64 * kWaves) void k_dense_few(const DenseArgs a) {
       g.set<false>(sum(n, 2 * i), sum(n, 2 * i + 1), a.limit);
       uint16_t q[kPlanes];
       dense_split(g.h(), q);
-      for (int p = 0; p < a.planes; p++) a.h[p * a.h_plane + (size_t)n * a.ldh + m0 / 2 + i] = q[p];
+      for (int p = 0; p < a.planes; p++)
+        dense_slots(a.h_where, p, [&](size_t at) { a.h[at * a.h_slot + (size_t)n * a.ldh + m0 / 2 + i] = q[p]; });
     }
   }
 }
 
 }  // namespace
 
-// (more rows of A than 4 tiles a CU keep the rings' larger tiles full)
+// (more rows of A than 4 tiles a CU keep the rings' larger tiles full, and 16 rows of B took 21.6 us in the
+// 2880 x 2880 block against 20.9 through the rings)
 bool dense_few_fits(const DenseShape &s, const DenseArgs &a) {
-  return !s.at && !s.bt && (s.epi == DENSE_GATE || s.epi == DENSE_STORE) && a.n_pass == 1 && a.N * a.stack <= 16 && a.M % 16 == 0 &&
+  return !s.at && !s.bt && (s.epi == DENSE_GATE || s.epi == DENSE_STORE) && a.n_pass == 1 && a.N * a.stack <= 8 && a.M % 16 == 0 &&
          a.K % 8 == 0 && a.M <= 16 * 1024 && a.splits <= 1 && !a.scale && a.out_mode != 2;
 }
 

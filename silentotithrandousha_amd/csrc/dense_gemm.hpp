@@ -191,6 +191,12 @@ __device__ __forceinline__ void dense_rows_f32(uint8_t *stage, int lane, const f
   dense_rows<TM, 8>(stage, lane, q, (uint16_t *)out, 2 * ld, rows, 2 * cols);
 }
 
+// f(slot) for the slots of plane p.
+template <class F>
+__device__ __forceinline__ void dense_slots(uint32_t where, int p, F &&f) {
+  for (uint32_t m = (where >> 8 * p) & 255; m; m &= m - 1) f((size_t)__builtin_ctz(m));
+}
+
 // Takes the bf16 of each value, and leaves what it did not hold (if another is to follow).
 template <bool MORE, int N>
 __device__ __forceinline__ void dense_take(float (&v)[N], uint16_t (&q)[N]) {
@@ -234,8 +240,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
     pa += step_a;
     pb += step_b;
     if (left <= 0) {
-      pa = a.A + ((a.pa >> 4 * pass) & 15) * a.a_plane + (AT ? (size_t)k_lo * a.lda + m0 : (size_t)m0 * a.lda + k_lo);
-      pb = a.B + ((a.pb >> 4 * pass) & 15) * a.b_plane + (BT ? (size_t)k_lo * a.ldb + n0 : (size_t)n0 * a.ldb + k_lo);
+      pa = a.A + (AT ? (size_t)k_lo * a.lda + m0 : (size_t)m0 * a.lda + k_lo);
+      pb = a.B + ((a.pb >> 4 * pass) & 15) * a.b_slot + (BT ? (size_t)k_lo * a.ldb + n0 : (size_t)n0 * a.ldb + k_lo);
       left = k_hi - k_lo;
       pass++;
       const int l = apart(lane);
@@ -373,7 +379,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
 
   if constexpr (BM * BN * 4 <= NS * kSlot && BN <= 64) {
     // B's planes were stacked as rows of one pass (so that A, which few rows wait for, streams once): a
-    // column's result is the sum of its planes' columns, from the lowest terms up
+    // column's result is the sum of its planes' columns
     if (a.stack > 1) {
       __syncthreads();
       float *o = (float *)lds;
@@ -459,8 +465,10 @@ if (a.out_mode == 2) {
           uint16_t q[TM][2];
 #pragma unroll
           for (int i = 0; i < TM; i++) dense_take<!one>(h[i], q[i]);
-          dense_rows<TM, 2>(stage, lane, q, a.h + p * a.h_plane + (size_t)(n_first + j * 16) * a.ldh + m_first / 2, a.ldh,
-                            a.N - n_first - j * 16, (a.M - m_first) / 2);
+          dense_slots(a.h_where, p, [&](size_t at) {
+            dense_rows<TM, 2>(stage, lane, q, a.h + at * a.h_slot + (size_t)(n_first + j * 16) * a.ldh + m_first / 2, a.ldh,
+                              a.N - n_first - j * 16, (a.M - m_first) / 2);
+          });
         }
       }
     };
@@ -500,8 +508,8 @@ if (a.out_mode == 2) {
             uint16_t q[8], e[4];
             dense_take<!one>(d, q);
             dense_take<!one>(hv, e);
-            *(uint4 *)(a.dgu + p * a.dgu_plane + (size_t)n * a.M * 2 + 2 * m) = __builtin_bit_cast(uint4, q);
-            *(uint2 *)(a.h + p * a.h_plane + (size_t)n * a.ldh + m) = __builtin_bit_cast(uint2, e);
+            dense_slots(a.dgu_where, p, [&](size_t at) { *(uint4 *)(a.dgu + at * a.dgu_slot + (size_t)n * a.M * 2 + 2 * m) = __builtin_bit_cast(uint4, q); });
+            dense_slots(a.h_where, p, [&](size_t at) { *(uint2 *)(a.h + at * a.h_slot + (size_t)n * a.ldh + m) = __builtin_bit_cast(uint2, e); });
           }
         }
         if (a.db_part) {  // over the wavefront's columns: 16 lanes, then a part per wavefront column
@@ -594,8 +602,10 @@ if (a.out_mode == 2) {
           uint16_t q[TM][4];
 #pragma unroll
           for (int i = 0; i < TM; i++) dense_take<!one>(d[i], q[i]);
-          dense_rows<TM, 4>(stage, lane, q, a.dl + p * a.dl_plane + (size_t)(n_first + j * 16) * a.ld_dl + m_first, a.ld_dl,
-                            a.N - n_first - j * 16, (int)a.ld_dl - m_first);
+          dense_slots(a.dl_where, p, [&](size_t at) {
+            dense_rows<TM, 4>(stage, lane, q, a.dl + at * a.dl_slot + (size_t)(n_first + j * 16) * a.ld_dl + m_first, a.ld_dl,
+                              a.N - n_first - j * 16, (int)a.ld_dl - m_first);
+          });
         }
       }
     };
