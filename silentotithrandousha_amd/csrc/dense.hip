@@ -32,7 +32,7 @@ double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a,
   // a transposed A's rows of k are read in pieces of a tile's rows: below 128 bytes the slower for it
   const double memory = s.at && d.bm < 64 ? 23.0 * d.bm / 64 : 23.0;  // GB/s a CU; 5.9 TB/s in all
   auto round = [&](long on_cu) {
-    double step = std::max(0.45 / (d.ns - 1) + 0.1, on_cu * d.bm * d.bn * 2.0 * kDenseStep * kCus / (d.rate * 1e6));
+    double step = std::max(0.52 / (d.ns - 1) + 0.12, on_cu * d.bm * d.bn * 2.0 * kDenseStep * kCus / (d.rate * 1e6));
     if (tiles_n == 1) step = std::max(step, on_cu * d.bm * 128e-3 / memory);
     const double stores = on_cu * d.bm * d.bn * result * kCus / 4.5e6;  // us at 4.5 TB/s
     return steps * step + 2.5 + stores;
