@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "dense_launch.hpp"
 
@@ -31,14 +32,15 @@ double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a,
                         : s.epi == DENSE_STORE && (a.out_mode || splits > 1) ? 4.0 : 2.0;
   // a transposed A's rows of k are read in pieces of a tile's rows: below 128 bytes the slower for it
   const double memory = s.at && d.bm < 64 ? 23.0 * d.bm / 64 : 23.0;  // GB/s a CU; 5.9 TB/s in all
-  auto round = [&](long on_cu) {
+  auto round = [&](double on_cu) {
     double step = std::max(0.52 / (d.ns - 1) + 0.12, on_cu * d.bm * d.bn * 2.0 * kDenseStep * kCus / (d.rate * 1e6));
     if (tiles_n == 1) step = std::max(step, on_cu * d.bm * 128e-3 / memory);
     const double stores = on_cu * d.bm * d.bn * result * kCus / 4.5e6;  // us at 4.5 TB/s
     return steps * step + 2.5 + stores;
   };
   const long whole = tiles / (kCus * d.wgs), rest = tiles - whole * kCus * d.wgs;
-  double us = whole * round(d.wgs) + (rest ? round((rest + kCus - 1) / kCus) : 0.0);
+  const double on = (double)rest / kCus;  // of the last round: between the busiest CU's and the mean
+  double us = whole * round(d.wgs) + (rest ? round(std::max(1.0, 0.5 * (on + std::ceil(on)))) : 0.0);
   if (splits > 1) us += 4.5 + 4.0 * splits * a.M * a.N / 5e6;
   return us;
 }
@@ -287,8 +289,17 @@ __global__ __launch_bounds__(1024) void k_loss(const float2 *stats, int parts, c
   const int in = threadIdx.x & ((1 << lt) - 1), rows = 1024 >> lt;
   const size_t t = ((size_t)blockIdx.x << lt) + in;
   float2 v = make_float2(-INFINITY, 0.0f);
-  if (t < T)
-    for (int p = threadIdx.x >> lt; p < parts; p += rows) v = join(v, stats[p * T + t]);
+  if (t < T) {
+    int p = threadIdx.x >> lt;
+    for (; p + 3 * rows < parts; p += 4 * rows) {  // 4 loads under way
+      float2 q[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) q[i] = stats[(p + i * rows) * T + t];
+#pragma unroll
+      for (int i = 0; i < 4; i++) v = join(v, q[i]);
+    }
+    for (; p < parts; p += rows) v = join(v, stats[p * T + t]);
+  }
   s_part[threadIdx.x] = v;
   for (int h = 512; h >= 1 << lt; h >>= 1) {
     __syncthreads();

@@ -158,9 +158,10 @@ __device__ __forceinline__ int apart(int v) {
 // Stores 16 rows of 16-bit results of a wavefront: lane l holds the V values q[i] of row l % 16 from column
 // (4 i + l / 16) V on. They pass through LDS (`stage`, the wavefront's own, dense_stage_bytes) so that
 // a row leaves in 16-byte pieces side by side: stored from the accumulators' layout, in pieces of
-// 8 bytes over 16 rows, the gradient of the LM head ran at 2.3 TB/s.
+// 8 bytes over 16 rows, the gradient of the LM head ran at 2.3 TB/s. ONCE: results that no later launch of
+// the call reads go past the caches (that gradient for 16 rows of x 320 -> 260 us).
 constexpr int dense_stage_bytes(int tm, int v) { return 16 * (tm * v * 8 + 16); }
-template <int TM, int V>
+template <int TM, int V, bool ONCE = false>
 __device__ __forceinline__ void dense_rows(uint8_t *stage, int lane, const uint16_t (&q)[TM][V], uint16_t *out, size_t ld, int rows, int cols) {
   constexpr int kRow = TM * V * 8, kPieces = kRow / 16;  // bytes and 16-byte pieces of a row
   typedef uint16_t vec __attribute__((ext_vector_type(V)));
@@ -172,13 +173,20 @@ __device__ __forceinline__ void dense_rows(uint8_t *stage, int lane, const uint1
 #pragma unroll
   for (int c = 0; c < 16 * kPieces; c += 64) {
     const int at = c + lane, row = at / kPieces, piece = at % kPieces;
-    if (row < min(rows, 16) && piece * 8 < cols) *(uint4 *)(out + row * ld + piece * 8) = *(const uint4 *)(stage + row * (kRow + 16) + piece * 16);
+    if (row < min(rows, 16) && piece * 8 < cols) {
+      const u32x4 v = *(const u32x4 *)(stage + row * (kRow + 16) + piece * 16);
+      u32x4 *o = (u32x4 *)(out + row * ld + piece * 8);
+      if constexpr (ONCE)
+        __builtin_nontemporal_store(v, o);
+      else
+        *o = v;
+    }
   }
   __builtin_amdgcn_wave_barrier();
 }
 
 // The same for the f32 results of columns j of the accumulators.
-template <int TM, int TN>
+template <bool ONCE, int TM, int TN>
 __device__ __forceinline__ void dense_rows_f32(uint8_t *stage, int lane, const f32x4 (&acc)[TM][TN], int j, float *out, size_t ld, int rows, int cols) {
   typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
   uint16_t q[TM][8];
@@ -188,7 +196,7 @@ __device__ __forceinline__ void dense_rows_f32(uint8_t *stage, int lane, const f
 #pragma unroll
     for (int r = 0; r < 8; r++) q[i][r] = v[r];
   }
-  dense_rows<TM, 8>(stage, lane, q, (uint16_t *)out, 2 * ld, rows, 2 * cols);
+  dense_rows<TM, 8, ONCE>(stage, lane, q, (uint16_t *)out, 2 * ld, rows, 2 * cols);
 }
 
 // f(slot) for the slots of plane p.
@@ -271,6 +279,26 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   for (int i = 0; i < TM; i++)
 #pragma unroll
     for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  // what the loss's epilogues need of a lane's columns: before the steps where the registers hold it (the
+  // wait for it after 45 steps of a 32 x 16 tile was a sixth of the launch)
+  constexpr bool kLoss = EPI == DENSE_STATS || EPI == DENSE_DLOGITS, kEarly = kLoss && TN <= 2;
+  struct Column {
+    int target;
+    float lse, scale;
+  } columns[kLoss ? TN : 1];
+  auto column = [&](int j) __attribute__((always_inline)) {
+    const int n = min(n0 + (wn * TN + j) * 16 + (lane & 15), a.N - 1);  // (columns past N are not stored)
+    Column c{a.targets[n], 0.0f, 0.0f};
+    if constexpr (EPI == DENSE_DLOGITS) {
+      c.lse = a.lse[n];
+      c.scale = a.dloss[n] / *a.scale;
+    }
+    return c;
+  };
+  if constexpr (kEarly) {
+#pragma unroll
+    for (int j = 0; j < TN; j++) columns[j] = column(j);
+  }
   // two sets of A fragments where the registers hold them, else one, whose rows take the next half as soon
   // as their products are done
   constexpr bool kTwoA = 4 * (TM * TN + 2 * (TM + TN)) <= 224;
@@ -431,7 +459,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
         for (int i = 0; i < TM; i++)
 #pragma unroll
           for (int r = 0; r < 4; r++) q[i][r] = dense_bf16(acc[i][j][r]);
-        dense_rows<TM, 4>(stage, lane, q, (uint16_t *)a.out + (size_t)(n_first + j * 16) * a.ldo + m_first, a.ldo, a.N - n_first - j * 16, a.M - m_first);
+        dense_rows<TM, 4, BT>(stage, lane, q, (uint16_t *)a.out + (size_t)(n_first + j * 16) * a.ldo + m_first, a.ldo, a.N - n_first - j * 16, a.M - m_first);
         continue;
       }
 if (a.out_mode == 2) {
@@ -444,7 +472,7 @@ if (a.out_mode == 2) {
         }
         continue;
       }
-      dense_rows_f32(stage, lane, acc, j, (float *)a.out + split * a.split_stride + (size_t)(n_first + j * 16) * a.ldo + m_first, a.ldo,
+      dense_rows_f32<BT>(stage, lane, acc, j, (float *)a.out + split * a.split_stride + (size_t)(n_first + j * 16) * a.ldo + m_first, a.ldo,
                      a.N - n_first - j * 16, a.M - m_first);
     }
   } else if constexpr (EPI == DENSE_GATE) {
@@ -546,7 +574,8 @@ if (a.out_mode == 2) {
     }
 #pragma unroll
     for (int j = 0; j < TN; j++) {
-      const int n = nw + j * 16, t = n < a.N ? a.targets[n] : -1;
+      if constexpr (!kEarly) columns[j] = column(j);
+      const int n = nw + j * 16, t = n < a.N ? columns[j].target : -1;
       const int want = t >= a.v0 ? t - a.v0 - mw : -1;  // the target's row from the lane's first
       float mx = -INFINITY;
 #pragma unroll
@@ -572,13 +601,12 @@ if (a.out_mode == 2) {
   } else {
     auto dlogits = [&](auto ONE) __attribute__((always_inline)) {
       constexpr bool one = decltype(ONE)::value;
-      const float unit = *a.scale;
 #pragma unroll
       for (int j = 0; j < TN; j++) {
-        const int n = min(nw + j * 16, a.N - 1);  // (columns past N are not stored)
-        const int t = a.targets[n];
+        if constexpr (!kEarly) columns[j] = column(j);
+        const int t = columns[j].target;
         const int want = t >= a.v0 ? t - a.v0 - mw : -1;
-        const float lse = t >= a.vocab ? NAN : a.lse[n], scale = a.dloss[n] / unit;
+        const float lse = t >= a.vocab ? NAN : columns[j].lse, scale = columns[j].scale;
         float d[TM][4];
 #pragma unroll
         for (int i = 0; i < TM; i++) {
