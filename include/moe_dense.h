@@ -13,7 +13,7 @@
  * context take and return, or MOE_BF16. Weights are bf16, biases f32. Products accumulate in f32:
  * bf16 values enter as they are, f32 values as three bf16 terms (their 24 bits). The logits' gradient,
  * the activation h and the gradients of gate and up enter the products after them in `dtype`'s
- * precision: one bf16 rounding (2^-9 relative) for MOE_BF16, none that f32 would not make for MOE_F32.
+ * precision: one bf16 rounding (2^-8 relative) for MOE_BF16, none that f32 would not make for MOE_F32.
  * Results do not depend on anything but the arguments' values and the shapes: no atomics.
  *
  * Workspace: the context's, which grows at need (the old one is kept if a captured graph may hold it).
@@ -47,6 +47,8 @@ int moe_lm_head_loss_device(moe_ctx *ctx, const void *x, int dtype, const int32_
 /* Its gradient: with p = exp(x . W - lse), d = dloss (p - [v = target]) (0 for ignored tokens):
  *   dx [n_tokens, H] = d W, dw [vocab, H] = d^T x, both of type `dtype`, either may be NULL.
  * lse as moe_lm_head_loss_device returned it; dloss [n_tokens] f32, the gradient of each token's loss.
+ * (dloss at tokens with a gradient has one scale: terms of d below 2^-126 of its largest magnitude may
+ * count as 0; at the others it may hold anything.)
  * n_tokens 0 zeroes dw. The head's rows are read, not changed: after an update of the weights call
  * moe_init_lm_head_bf16_device again. */
 int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, const int32_t *targets,

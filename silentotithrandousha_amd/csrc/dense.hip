@@ -53,8 +53,8 @@ DenseTileShape dense_tile(const DenseShape &s, const DenseArgs &a) {
   for (int t = 0; t < (int)(sizeof(kDenseTiles) / sizeof(kDenseTiles[0])); t++) {
     const DenseTileDims &d = kDenseTiles[t];
     if (a.stack > 1 && (d.bn > 64 || a.N * a.stack > d.bn)) continue;  // stacked planes lie in one tile
-    // 288 rows: K-contiguous they keep too much in registers (620 TFLOP/s), and their epilogue spills
-    if (d.bm > 256 && (!s.at || a.K < 1024)) continue;
+    // 288 rows: K-contiguous they keep too much in registers (620 TFLOP/s)
+    if (d.bm > 256 && (!s.at || s.epi != DENSE_STORE || a.K < 1024)) continue;
     const double u = dense_us(s, d, a, dense_split_count(a));
     if (best < 0 || u < us) best = t, us = u;
   }
@@ -313,10 +313,11 @@ __global__ __launch_bounds__(1024) void k_loss(const float2 *stats, int parts, c
   }
 }
 
-__global__ __launch_bounds__(1024) void k_dloss_scale(const float *dloss, size_t T, float *scale) {
+__global__ __launch_bounds__(1024) void k_dloss_scale(const float *dloss, const int32_t *targets, size_t T, int vocab, float *scale) {
   __shared__ float part[16];
   float m = 0.0f;
-  for (size_t t = threadIdx.x; t < T; t += 1024) m = fmaxf(m, fabsf(dloss[t]));
+  for (size_t t = threadIdx.x; t < T; t += 1024)
+    if ((unsigned)targets[t] < (unsigned)vocab) m = fmaxf(m, fabsf(dloss[t]));
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
   if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = m;
@@ -362,8 +363,8 @@ hipError_t launch_dgate(const DgateArgs &a, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_dloss_scale(const float *dloss, size_t T, float *scale, hipStream_t s) {
-  k_dloss_scale<<<1, 1024, 0, s>>>(dloss, T, scale);
+hipError_t launch_dloss_scale(const float *dloss, const int32_t *targets, size_t T, int vocab, float *scale, hipStream_t s) {
+  k_dloss_scale<<<1, 1024, 0, s>>>(dloss, targets, T, vocab, scale);
   return hipGetLastError();
 }
 

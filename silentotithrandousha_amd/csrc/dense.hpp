@@ -110,8 +110,9 @@ hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *pa
 hipError_t launch_loss(const float2 *stats, int parts, const float *picked, const int32_t *targets, size_t T,
                        int vocab, float *loss, float *lse, hipStream_t s);
 
-// The largest magnitude of dloss [T], 1 where that is 0 or not finite.
-hipError_t launch_dloss_scale(const float *dloss, size_t T, float *scale, hipStream_t s);
+// The largest magnitude of dloss [T] at tokens whose target lies in the vocabulary (the others' may be
+// anything), 1 where that is 0 or not finite.
+hipError_t launch_dloss_scale(const float *dloss, const int32_t *targets, size_t T, int vocab, float *scale, hipStream_t s);
 
 // MXFP8 activation checkpoints (act8.hip): codes [n][cols], then scales [n][cols / 32].
 hipError_t launch_act8_pack(const void *x, bool bf16, size_t n, size_t cols, uint8_t *packed, hipStream_t s);

@@ -292,9 +292,9 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
   RETURN_IF(check_aligned({dx, dw}));
   const hipStream_t s = stream ? (hipStream_t)stream : c.stream;
   const size_t H = c.H;
+  RETURN_IF(check_distinct({dx, dw}, {x, targets, lse, dloss, c.lm_w}));
   if (!T) return zero(dw, vocab * H * elem(dtype), s);
   if (!lse || !dloss) return fail(MOE_ERR_INVALID, "null lse or dloss");
-  RETURN_IF(check_distinct({dx, dw}, {x, targets, lse, dloss, c.lm_w}));
   if (!dx && !dw) return MOE_OK;
   const int P = dtype == MOE_BF16 ? 1 : kPlanes;
   const bool bf = dtype == MOE_BF16;
@@ -336,7 +336,7 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
   // The gradient of the logits is held over the largest |dloss| and the results multiplied by it: for the
   // mean's constant dloss the entries of the targets, which weigh most, then lie next to -1 and are rounded
   // by their p alone, where bf16(1 / n) would put one error into all of them.
-  HIP_TRY(launch_dloss_scale(dloss, T, scale, s));
+  HIP_TRY(launch_dloss_scale(dloss, targets, T, (int)vocab, scale, s));
   int written = 0;  // parts of dx
   for (size_t v0 = 0; v0 < vocab; v0 += Vc) {
     const size_t nvoc = std::min(Vc, vocab - v0);

@@ -462,7 +462,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
         dense_rows<TM, 4, BT>(stage, lane, q, (uint16_t *)a.out + (size_t)(n_first + j * 16) * a.ldo + m_first, a.ldo, a.N - n_first - j * 16, a.M - m_first);
         continue;
       }
-if (a.out_mode == 2) {
+      if (a.out_mode == 2) {
 #pragma unroll
         for (int i = 0; i < TM; i++) {
           const int m = mw + i * 16;

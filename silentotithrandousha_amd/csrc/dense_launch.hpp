@@ -33,7 +33,7 @@ hipError_t launch_dense_shape(const DenseArgs &a, hipStream_t st) {
   switch (dense_tile(DenseShape{AT, BT, (DenseEpi)EPI}, a)) {
 #define X(name, bm, bn, wm, wn, ns, wgs, rate) \
   case TILE_##name:                 \
-    if constexpr (AT || bm <= 256)  \
+    if constexpr ((AT && EPI == DENSE_STORE) || bm <= 256)  \
       return launch_dense_as<bm, bn, wm, wn, ns, AT, BT, EPI>(a, st); \
     break;
     MOE_DENSE_TILES(X)

@@ -165,6 +165,47 @@ def test_loss_targets(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_loss_gradient_of_tokens_that_do_not_count(dtype):
+    """dloss of an ignored token may be anything: it moves nothing. Small dloss beside it keep their bits."""
+    T, H, V = 30, 64, 200
+    x, xv, w, wv, targets, dloss = loss_case(dtype, T, H, V, seed=11)
+    dloss *= np.float32(2.0 ** -20)
+    targets[[3, 8, 20, 29]] = -1
+    want = ref.Loss(xv, wv, targets, np.where(targets < 0, 0.0, dloss.astype(np.float64)), dtype)
+    dloss[[3, 8, 20, 29]] = 3e38, np.inf, np.nan, -np.inf
+    d = context(H, w)
+    try:
+        xd, td, loss, lse = run_loss(d, x, dtype, targets, V)
+        dx, dw = run_loss_backward(d, xd, dtype, td, lse, dloss, T, H, V)
+        ref.assert_close(dx.get(), want.dx, want.dx_tol, "dx")
+        ref.assert_close(dw.get(), want.dw, want.dw_tol, "dw")
+    finally:
+        d.close()
+
+
+# Sizes at which each tile shape of the plan is taken by each of its products (the large ones in both
+# types), with more than two steps and a tail of one
+TILES_LOSS = [(1, 736, 4320, MOE_BF16), (33, 160, 2772, MOE_F32), (15, 224, 124, MOE_F32), (6, 224, 21505, MOE_F32),
+              (2, 160, 38963, MOE_BF16), (6, 160, 34985, MOE_F32), (18, 160, 12710, MOE_BF16), (51, 160, 4593, MOE_F32),
+              (1, 160, 21750, MOE_BF16), (22, 160, 16463, MOE_F32), (28, 160, 36238, MOE_F32), (37, 1472, 2076, MOE_F32),
+              (163, 160, 37761, MOE_BF16), (22, 416, 26172, MOE_F32), (646, 160, 11029, MOE_F32), (257, 160, 30609, MOE_BF16),
+              (257, 160, 30609, MOE_F32), (146, 416, 22646, MOE_BF16), (148, 160, 24214, MOE_F32), (7064, 1216, 136, MOE_BF16),
+              (7064, 1216, 136, MOE_F32), (8021, 1600, 131, MOE_BF16), (8021, 1600, 131, MOE_F32), (171, 1056, 14315, MOE_F32),
+              (1448, 1952, 3505, MOE_F32), (1058, 1440, 10839, MOE_BF16)]
+TILES_BLOCK = [(27, 224, 296, MOE_F32), (6, 160, 80, MOE_F32), (3, 224, 4360, MOE_F32), (11, 160, 3224, MOE_F32),
+               (26, 160, 6496, MOE_F32), (39, 160, 5176, MOE_BF16), (69, 160, 3800, MOE_F32), (36, 1280, 200, MOE_F32),
+               (8587, 224, 112, MOE_BF16), (946, 32, 1064, MOE_F32), (347, 160, 5368, MOE_BF16), (619, 160, 808, MOE_BF16),
+               (150, 288, 5648, MOE_BF16), (978, 160, 4368, MOE_F32), (6266, 160, 264, MOE_F32), (6596, 160, 616, MOE_BF16),
+               (6451, 544, 72, MOE_BF16), (810, 224, 7048, MOE_BF16), (810, 224, 7048, MOE_F32), (7227, 2080, 528, MOE_BF16),
+               (5000, 160, 2056, MOE_BF16), (1155, 160, 6904, MOE_F32), (11279, 160, 1168, MOE_BF16), (11819, 160, 1048, MOE_F32)]
+
+
+@pytest.mark.parametrize("T,H,V,dtype", TILES_LOSS)
+def test_loss_tiles(T, H, V, dtype):
+    test_loss_and_gradient(dtype, T, H, V)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_loss_smaller_vocabulary_and_far_logits(dtype):
     """The first rows of a larger head; logits of hundreds, of one sign and the other."""
     T, H, V = 9, 64, 100
@@ -301,6 +342,11 @@ def test_block(dtype, T, H, I):  # noqa: E741
         check_grads(grads, want)
     finally:
         d.close()
+
+
+@pytest.mark.parametrize("T,H,I,dtype", TILES_BLOCK)
+def test_block_tiles(T, H, I, dtype):  # noqa: E741
+    test_block(dtype, T, H, I)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -535,6 +581,7 @@ def test_refusals():
         refused(inv, backward, dx=dw)
         refused(inv, backward, dx=dx.ptr + 8)
         forward(n_tokens=0, x=None, targets=None)
+        refused(inv, backward, n_tokens=0, x=None, targets=None, dw=dx)
 
         c = block_case(MOE_F32, T, H, I)
         b = BlockOnDevice(c)
