@@ -26,14 +26,16 @@ constexpr int kCus = 256;  // of an MI355X: the plan is for the whole device
 // results; parts are summed in another launch. Whole rounds of workgroups and what is left for the last one count apart.
 double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a, int splits) {
   const long tiles_n = ((long)a.N * a.stack + d.bn - 1) / d.bn, tiles = (long)((a.M + d.bm - 1) / d.bm) * tiles_n * splits;
-  const long steps = (((long)a.K + kDenseStep - 1) / kDenseStep * a.n_pass + splits - 1) / splits;
-  // bytes that a result costs, about
-  const double result = s.epi == DENSE_STATS ? 0.0 : s.epi == DENSE_GATE ? 1.0 : s.epi == DENSE_DGATE ? 14.0
-                        : s.epi == DENSE_STORE && (a.out_mode || splits > 1) ? 4.0 : 2.0;
+  const long steps = (((long)a.K + kDenseStep - 1) / kDenseStep + splits - 1) / splits;
+  // bytes that a result costs, about: of rows in planes, results in planes (GATE 3 slots, the gradients 6)
+  const bool planes = a.b_planes > 1 || a.stack > 1;
+  const double result = s.epi == DENSE_STATS ? 0.0 : s.epi == DENSE_GATE ? (planes ? 3.0 : 1.0)
+                        : s.epi == DENSE_DGATE ? (planes ? 44.0 : 14.0) : s.epi == DENSE_DLOGITS ? (planes ? 12.0 : 2.0)
+                        : a.out_mode || splits > 1 ? 4.0 : 2.0;
   // a transposed A's rows of k are read in pieces of a tile's rows: below 128 bytes the slower for it
   const double memory = s.at && d.bm < 64 ? 23.0 * d.bm / 64 : 23.0;  // GB/s a CU; 5.9 TB/s in all
   auto round = [&](double on_cu) {
-    double step = std::max(0.52 / (d.ns - 1) + 0.12, on_cu * d.bm * d.bn * 2.0 * kDenseStep * kCus / (d.rate * 1e6));
+    double step = std::max(0.52 / (d.ns - 1) + 0.12, on_cu * d.bm * d.bn * 2.0 * kDenseStep * d.planes * kCus / (d.rate * 1e6));
     if (tiles_n == 1) step = std::max(step, on_cu * d.bm * 128e-3 / memory);
     const double stores = on_cu * d.bm * d.bn * result * kCus / 4.5e6;  // us at 4.5 TB/s
     return steps * step + 2.5 + stores;
@@ -47,18 +49,19 @@ double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a,
 
 }  // namespace
 
-DenseTileShape dense_tile(const DenseShape &s, const DenseArgs &a) {
+int dense_tile(const DenseShape &s, const DenseArgs &a) {
   int best = -1;
   double us = 0.0;
-  for (int t = 0; t < (int)(sizeof(kDenseTiles) / sizeof(kDenseTiles[0])); t++) {
+  for (int t = 0; t < kDenseTileCount; t++) {
     const DenseTileDims &d = kDenseTiles[t];
+    if (d.planes != a.b_planes) continue;
     if (a.stack > 1 && (d.bn > 64 || a.N * a.stack > d.bn)) continue;  // stacked planes lie in one tile
     // 288 rows: K-contiguous they keep too much in registers (620 TFLOP/s)
     if (d.bm > 256 && (!s.at || s.epi != DENSE_STORE || a.K < 1024)) continue;
     const double u = dense_us(s, d, a, dense_split_count(a));
     if (best < 0 || u < us) best = t, us = u;
   }
-  return (DenseTileShape)best;
+  return best;
 }
 
 int dense_parts(const DenseShape &s, const DenseArgs &a) {
@@ -95,7 +98,7 @@ int dense_splits(const DenseShape &s, const DenseArgs &a0) {
 
 hipError_t launch_dense(const DenseShape &s, const DenseArgs &a0, hipStream_t st) {
   DenseArgs a = a0;
-  if (a.M <= 0 || a.N <= 0 || a.K <= 0 || a.n_pass < 1 || a.n_pass > kMaxPass || a.stack < 1 || a.lda % 8 || a.ldb % 8)
+  if (a.M <= 0 || a.N <= 0 || a.K <= 0 || (a.b_planes != 1 && a.b_planes != kPlanes) || a.stack < 1 || a.lda % 8 || a.ldb % 8)
     return hipErrorInvalidValue;
   // (stores of 4 rows)
   if (a.M % 4 && s.epi != DENSE_STATS && s.epi != DENSE_DLOGITS) return hipErrorInvalidValue;

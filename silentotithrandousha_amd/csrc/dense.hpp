@@ -19,7 +19,6 @@ namespace moe {
 constexpr int kPlanes = 3;
 constexpr int kPairs6 = 6;
 constexpr uint32_t kWhereOne = 0x01, kWhereThree = 0x040201, kWhereLeft = 0x041229, kWhereRight = 0x010A34;
-constexpr int kMaxPass = 3;
 
 // Epilogues.
 enum DenseEpi {
@@ -30,7 +29,7 @@ enum DenseEpi {
   DENSE_DLOGITS = 4  // D = logits: their gradient as bf16 planes
 };
 
-// D[m][n] = sum over passes and k of A_p[m][k] B_p[n][k], stored as [n][m] (m contiguous).
+// D[m][n] = sum over B's planes and k of A[m][k] B_p[n][k], stored as [n][m] (m contiguous).
 // Layouts of an operand: K-contiguous ([rows][k], the fast case) or transposed ([k][rows]).
 // A K-contiguous operand is readable up to K rounded up to 8; a transposed one's rows up to M (N)
 // rounded up to 8.
@@ -39,9 +38,9 @@ struct DenseArgs {
   size_t b_slot;            // elements between slots of B
   size_t lda, ldb;          // elements between rows of the stored matrix
   int M, N, K;
-  int stack;                // slots of B that one pass takes as rows [slot][N] (N * stack <= 64), else 1
-  int n_pass;
-  uint32_t pb;              // the slot of B of each pass, 4 bits each
+  int stack;                // slots of B that are taken as rows [slot][N] (N * stack <= 64), else 1
+  int b_planes;             // slots of B that meet A's values in turn: 1, or kPlanes
+  uint32_t pb;              // those slots, 4 bits each, in the order of their products
   int splits;               // K split (DENSE_STORE with f32 only): out + split * split_stride
   int k_split;              // K per split, a multiple of the step
   // DENSE_STORE

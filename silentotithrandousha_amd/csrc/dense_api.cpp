@@ -142,7 +142,7 @@ int fill(const Rows &r, const void *x, int dtype, hipStream_t s) {
 }
 
 // Weights times rows: D[m][n] = sum W[m][k] rows[n][k] (W [M][K], or [K][M] for a launch with A transposed),
-// the rows' lower planes first; of few rows, all planes in one pass.
+// the rows' lower planes first; of few rows, all planes as rows.
 DenseArgs product(const uint16_t *W, size_t ldw, const Rows &b, size_t M) {
   DenseArgs a{};
   a.A = W;
@@ -153,12 +153,12 @@ DenseArgs product(const uint16_t *W, size_t ldw, const Rows &b, size_t M) {
   a.M = (int)M;
   a.N = (int)b.n;
   a.K = (int)b.cols;
-  a.splits = a.stack = a.n_pass = 1;
+  a.splits = a.stack = a.b_planes = 1;
   if (b.where != kWhereOne) {
     if (b.n * kPlanes <= 64) {
       a.stack = kPlanes;  // the first three slots, one of each plane
     } else {
-      a.n_pass = kPlanes;
+      a.b_planes = kPlanes;
       for (int i = 0; i < kPlanes; i++) a.pb |= (uint32_t)__builtin_ctz(b.where >> 8 * (kPlanes - 1 - i)) << 4 * i;
     }
   }
@@ -175,7 +175,7 @@ DenseArgs gradient(const Rows &x, const Rows &y) {
   a.M = (int)x.cols;
   a.N = (int)y.cols;
   a.K = (int)(std::min(x.slots, y.slots) * x.n);
-  a.splits = a.stack = a.n_pass = 1;
+  a.splits = a.stack = a.b_planes = 1;
   return a;
 }
 
@@ -486,7 +486,8 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
       const double one = dense_estimate(ss, raw) + dense_estimate(sg, in);
       raw.splits = n_raw = dense_splits(ss, raw);
       in.splits = n_dh = dense_splits(sx, in);
-      apart = dense_estimate(ss, raw) + dense_estimate(sx, in) + 1.0 + 26e-6 / 5 * T * I < one && T <= 65536;
+      const double bytes = (8.0 * n_raw + 4.0 * n_dh + 6.0 * (bf ? 1 : kPairs6)) * T * I;  // of that kernel, at 5 TB/s
+      apart = dense_estimate(ss, raw) + dense_estimate(sx, in) + 1.0 + bytes / 5e6 < one && T <= 65536;
       if (!apart) n_raw = n_dh = 1;
       gu = w.take<float>(n_raw * T * 2 * I);
       dh = apart ? w.take<float>(n_dh * T * I) : nullptr;

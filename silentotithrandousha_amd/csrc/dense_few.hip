@@ -77,7 +77,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_dense_few(const DenseArgs a) {
 // (more rows of A than 4 tiles a CU keep the rings' larger tiles full, and 16 rows of B took 21.6 us in the
 // 2880 x 2880 block against 20.9 through the rings)
 bool dense_few_fits(const DenseShape &s, const DenseArgs &a) {
-  return !s.at && !s.bt && (s.epi == DENSE_GATE || s.epi == DENSE_STORE) && a.n_pass == 1 && a.N * a.stack <= 8 && a.M % 16 == 0 &&
+  return !s.at && !s.bt && (s.epi == DENSE_GATE || s.epi == DENSE_STORE) && a.b_planes == 1 && a.N * a.stack <= 8 && a.M % 16 == 0 &&
          a.K % 8 == 0 && a.M <= 16 * 1024 && a.splits <= 1 && !a.scale && a.out_mode != 2;
 }
 

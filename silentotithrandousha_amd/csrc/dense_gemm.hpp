@@ -7,6 +7,9 @@
 // small ones, which wait for memory). Fragments are read one half ahead of the MFMAs, the first half of
 // the next step included: the step's one barrier stands between its halves, where this step's reads are
 // done (its slot takes the step NS ahead) and the next step's loads have landed.
+// f32 rows are three bf16 planes: a step then holds a tile of A and PL = 3 tiles of B, and A's fragments meet
+// each of them, the lowest plane first. As three passes over K, each loading A again, the 64 x 64 tile's wave
+// read 4 fragments for 4 MFMAs instead of 8 for 12 (loss of 333 rows over 50257 x 2048: 242 -> 200 us).
 // A K-contiguous operand lies in LDS as rows of 128 bytes (a line each, so that no line is asked for
 // twice) whose 16-byte chunks are permuted by the row (chunk ^ row % 8), so that 8 lanes reading one chunk
 // of 8 rows touch different banks. A transposed one lies as its 64 rows of k, and the fragments are read
@@ -218,13 +221,13 @@ __device__ __forceinline__ void dense_take(float (&v)[N], uint16_t (&q)[N]) {
   }
 }
 
-template <int BM, int BN, int WM, int WN, int NS, bool AT, bool BT, int EPI>
+template <int BM, int BN, int WM, int WN, int NS, int PL, bool AT, bool BT, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   using TA = DenseTile<BM, W, AT>;
   using TB = DenseTile<BN, W, BT>;
   extern __shared__ __align__(16) uint8_t lds[];
-  constexpr int kSlot = TA::kBytes + TB::kBytes, kLoads = TA::kLoads + TB::kLoads;
+  constexpr int kSlot = TA::kBytes + PL * TB::kBytes, kLoads = TA::kLoads + PL * TB::kLoads;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM;
   const int rows_b = a.N * a.stack;
@@ -234,44 +237,46 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   const int m0 = tile_m * BM, n0 = tile_n * BN;
   const int split = blockIdx.y;
   const int k_lo = split * a.k_split, k_hi = min(a.K, k_lo + a.k_split);
-  const int nk = (k_hi - k_lo + kDenseStep - 1) / kDenseStep, steps = nk * a.n_pass;
+  const int steps = (k_hi - k_lo + kDenseStep - 1) / kDenseStep;
 
   const uint32_t lds0 = str_lds(lds), lda = (uint32_t)a.lda * 2, ldb = (uint32_t)a.ldb * 2;
   TA la;
   TB lb;
-  // the step to load: its operands' addresses, k values left in its pass from there
-  int pass = 0, left = 0;
-  const uint16_t *pa = nullptr, *pb = nullptr;
-  const size_t step_a = AT ? a.lda * kDenseStep : kDenseStep, step_b = BT ? a.ldb * kDenseStep : kDenseStep;
-  auto next_load = [&]() __attribute__((always_inline)) {
-    left -= kDenseStep;
-    pa += step_a;
-    pb += step_b;
-    if (left <= 0) {
-      pa = a.A + (AT ? (size_t)k_lo * a.lda + m0 : (size_t)m0 * a.lda + k_lo);
-      pb = a.B + ((a.pb >> 4 * pass) & 15) * a.b_slot + (BT ? (size_t)k_lo * a.ldb + n0 : (size_t)n0 * a.ldb + k_lo);
-      left = k_hi - k_lo;
-      pass++;
-      const int l = apart(lane);
-      la.init(wave, l, a.M - m0, lda);
-      lb.init(wave, l, rows_b - n0, ldb);
-    }
-    if (left < kDenseStep) {
+  la.init(wave, lane, a.M - m0, lda);
+  lb.init(wave, lane, rows_b - n0, ldb);
+  // the step to load: its operands' addresses, k values left from there
+  int left = k_hi - k_lo;
+  const uint16_t *pa = a.A + (AT ? (size_t)k_lo * a.lda + m0 : (size_t)m0 * a.lda + k_lo), *pb[PL];
+#pragma unroll
+  for (int p = 0; p < PL; p++)
+    pb[p] = a.B + ((a.pb >> 4 * p) & 15) * a.b_slot + (BT ? (size_t)k_lo * a.ldb + n0 : (size_t)n0 * a.ldb + k_lo);
+  auto tail = [&]() __attribute__((always_inline)) {
+    if (left > 0 && left < kDenseStep) {
       const int l = apart(lane);
       la.clamp(wave, l, lda, left);
       lb.clamp(wave, l, ldb, left);
     }
   };
+  tail();
+  auto loaded = [&]() __attribute__((always_inline)) {
+    left -= kDenseStep;
+    pa += AT ? a.lda * kDenseStep : kDenseStep;
+#pragma unroll
+    for (int p = 0; p < PL; p++) pb[p] += BT ? a.ldb * kDenseStep : kDenseStep;
+    tail();
+  };
   auto load_one = [&](int i, uint32_t slot) __attribute__((always_inline)) {
-    if (i < TA::kLoads)
+    if (i < TA::kLoads) {
       la.load(i, pa, slot, wave);
-    else
-      lb.load(i - TA::kLoads, pb, slot + TA::kBytes, wave);
+    } else {
+      const int p = (i - TA::kLoads) / TB::kLoads;
+      lb.load((i - TA::kLoads) % TB::kLoads, pb[p], slot + TA::kBytes + p * TB::kBytes, wave);
+    }
   };
   auto load = [&](uint32_t slot) __attribute__((always_inline)) {
-    next_load();
 #pragma unroll
     for (int i = 0; i < kLoads; i++) load_one(i, slot);
+    loaded();
   };
 
   f32x4 acc[TM][TN];
@@ -304,14 +309,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   constexpr bool kTwoA = 4 * (TM * TN + 2 * (TM + TN)) <= 224;
   constexpr bool kPinned = !AT || kTwoA;  // (the transposing loads' addresses take registers: 288 x 256 spilled)
   bf16x8 fa0[TM], fa1[kTwoA ? TM : 1], fb0[TN], fb1[TN];
-  auto read_b = [&](const uint8_t *sl, int half, int j) __attribute__((always_inline)) { return TB::frag(sl + TA::kBytes, (wn * TN + j) * 16, half, lane); };
+  auto read_b = [&](const uint8_t *sl, int half, int p, int j) __attribute__((always_inline)) { return TB::frag(sl + TA::kBytes + p * TB::kBytes, (wn * TN + j) * 16, half, lane); };
   auto read_a = [&](const uint8_t *sl, int half, int i) __attribute__((always_inline)) { return TA::frag(sl, (wm * TM + i) * 16, half, lane); };
-  // The products of a half (fa, fb), row by row, and between the rows the reads of the half after it (`half`
-  // of sl, into na and nb, if READ) and the LDS-DMAs of the step after the next (into slot `to`, if DMA): issued in
-  // one go they held the MFMAs up, as the LDS serves 8 wavefronts' 12 reads in 768 cycles (256 x 256: 958
-  // against 1130 TFLOP/s). The reads come in the first three quarters of the rows.
-  auto multiply = [&](auto DMA, auto READ, auto &fa, const bf16x8(&fb)[TN], auto &na, bf16x8(&nb)[TN], const uint8_t *sl, int half, uint32_t to) __attribute__((always_inline)) {
-    constexpr int kReads = kTwoA ? TN + TM : TN, kOver = (3 * TM + 3) / 4, kEach = (kReads + kOver - 1) / kOver;
+  // The products of a half with one of B's planes (fa, fb), row by row, and between the rows the reads for
+  // the products after them (half `half` and plane `p` of sl, into nb and, if READ is 2, na) and the LDS-DMAs
+  // of the step NS ahead (into slot `to`, if DMA): issued in one go they held the MFMAs up, as the LDS serves 8
+  // wavefronts' 12 reads in 768 cycles (256 x 256: 958 against 1130 TFLOP/s). The reads come in the first three
+  // quarters of the rows.
+  auto multiply = [&](auto DMA, auto READ, auto &fa, const bf16x8(&fb)[TN], auto &na, bf16x8(&nb)[TN], const uint8_t *sl, int half, int p, uint32_t to) __attribute__((always_inline)) {
+    constexpr int kRead = decltype(READ)::value, kReads = kTwoA && kRead == 2 ? TN + TM : TN, kOver = (3 * TM + 3) / 4, kEach = (kReads + kOver - 1) / kOver;
     constexpr int kDma = kPinned ? (kLoads + TM - 1) / TM : kLoads;
     if constexpr (kPinned) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -320,18 +326,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
 #pragma unroll
         for (int l = i * kDma; l < (i + 1) * kDma && l < kLoads; l++) load_one(l, to);
       }
-      if constexpr (decltype(READ)::value) {
+      if constexpr (kRead != 0) {
 #pragma unroll
         for (int r = i * kEach; r < (i + 1) * kEach && r < kReads; r++) {
           if (r < TN)
-            nb[r] = read_b(sl, half, r);
+            nb[r] = read_b(sl, half, p, r);
           else
             na[r - TN] = read_a(sl, half, r - TN);
         }
       }
 #pragma unroll
       for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
-      if constexpr (!kTwoA && decltype(READ)::value) fa[i] = read_a(sl, half, i);
+      if constexpr (!kTwoA && kRead == 2) fa[i] = read_a(sl, half, i);
       if constexpr (decltype(DMA)::value && kPinned) {
 #pragma unroll
         for (int l = i * kDma; l < (i + 1) * kDma && l < kLoads; l++) load_one(l, to);
@@ -341,6 +347,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   };
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
+  constexpr std::integral_constant<int, 0> none{};
+  constexpr std::integral_constant<int, 1> only_b{};
+  constexpr std::integral_constant<int, 2> both{};
   // this wavefront's loads have landed, up to those of the `NS - 2` steps after it if MORE are on their way,
   // and its reads are done, and every other's
   auto meet = [&](auto MORE) __attribute__((always_inline)) {
@@ -349,18 +358,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  int here = k_hi - k_lo;  // k values left in its pass from the next step to be read
+  int here = k_hi - k_lo;  // k values left from the next step to be read
   auto zero = [&](uint8_t *sl) __attribute__((always_inline)) {
     if (here < kDenseStep) {
       const int t = apart(tid);
       TA::zero_tail(sl, here, t, 64 * W);
-      TB::zero_tail(sl + TA::kBytes, here, t, 64 * W);
+#pragma unroll
+      for (int p = 0; p < PL; p++) TB::zero_tail(sl + TA::kBytes + p * TB::kBytes, here, t, 64 * W);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     }
     here -= kDenseStep;
-    if (here <= 0) here = k_hi - k_lo;
   };
   auto landed = [&](auto MORE, uint8_t *sl) __attribute__((always_inline)) {
     meet(MORE);
@@ -375,7 +384,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   asm volatile("" ::: "memory");
   zero(lds);
 #pragma unroll
-  for (int j = 0; j < TN; j++) fb0[j] = read_b(lds, 0, j);
+  for (int j = 0; j < TN; j++) fb0[j] = read_b(lds, 0, 0, j);
 #pragma unroll
   for (int i = 0; i < TM; i++) fa0[i] = read_a(lds, 0, i);
   uint32_t cur = 0;
@@ -386,26 +395,35 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
     const uint32_t n = slot + kSlot;
     return n == NS * kSlot ? 0u : n;
   };
+  // A step: the products of its two halves with each of B's planes. Its last ones run while the next step's
+  // first fragments are read (if MORE) and its slot takes the step NS ahead (if DMA).
+  auto step = [&](auto MORE, auto DMA) __attribute__((always_inline)) {
+    const uint32_t next = after(cur);
+    uint8_t *sl = lds + cur;
+    if constexpr (PL == 1) {
+      multiply(no, both, fa0, fb0, fa_odd, fb1, sl, 1, 0, 0);
+    } else {
+      multiply(no, only_b, fa0, fb0, fa_odd, fb1, sl, 0, 1, 0);
+      multiply(no, only_b, fa0, fb1, fa_odd, fb0, sl, 0, 2, 0);
+      multiply(no, both, fa0, fb0, fa_odd, fb1, sl, 1, 0, 0);
+      multiply(no, only_b, fa_odd, fb1, fa0, fb0, sl, 1, 1, 0);
+      multiply(no, only_b, fa_odd, fb0, fa0, fb1, sl, 1, 2, 0);
+    }
+    if constexpr (decltype(MORE)::value) {
+      landed(DMA, lds + next);
+      multiply(DMA, both, fa_odd, fb1, fa0, fb0, lds + next, 0, 0, lds0 + cur);
+      if constexpr (decltype(DMA)::value) loaded();
+    } else {
+      multiply(no, none, fa_odd, fb1, fa0, fb0, sl, 0, 0, 0);
+    }
+    cur = next;
+  };
   int s = 0;
-  for (; s + NS < steps; s++) {
-    const uint32_t next = after(cur);
-    multiply(no, yes, fa0, fb0, fa_odd, fb1, lds + cur, 1, 0);
-    landed(yes, lds + next);
-    next_load();
-    multiply(yes, yes, fa_odd, fb1, fa0, fb0, lds + next, 0, lds0 + cur);
-    cur = next;
-  }
-  for (; s + 1 < steps; s++) {
-    const uint32_t next = after(cur);
-    multiply(no, yes, fa0, fb0, fa_odd, fb1, lds + cur, 1, 0);
-    landed(no, lds + next);
-    multiply(no, yes, fa_odd, fb1, fa0, fb0, lds + next, 0, 0);
-    cur = next;
-  }
-  multiply(no, yes, fa0, fb0, fa_odd, fb1, lds + cur, 1, 0);
-  multiply(no, no, fa_odd, fb1, fa0, fb0, lds, 0, 0);
+  for (; s + NS < steps; s++) step(yes, yes);
+  for (; s + 1 < steps; s++) step(yes, no);
+  step(no, no);
 
-  if constexpr (BM * BN * 4 <= NS * kSlot && BN <= 64) {
+  if constexpr (PL == 1 && BM * BN * 4 <= NS * kSlot && BN <= 64) {
     // B's planes were stacked as rows of one pass (so that A, which few rows wait for, streams once): a
     // column's result is the sum of its planes' columns
     if (a.stack > 1) {
@@ -439,6 +457,17 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
   static_assert(W * kStage <= NS * kSlot, "the results of 16 columns fit the LDS of the steps");
   uint8_t *stage = lds + wave * kStage;
   if constexpr (EPI != DENSE_STATS && EPI != DENSE_DGATE) __syncthreads();
+  // results in planes come of rows in planes, which only the small tiles take beside single ones
+  auto by_planes = [&](auto &&f) __attribute__((always_inline)) {
+    if constexpr (PL > 1)
+      f(no);
+    else if constexpr (BN > 64)
+      f(yes);
+    else if (a.planes == 1)
+      f(yes);
+    else
+      f(no);
+  };
   if constexpr (EPI == DENSE_STORE || EPI == DENSE_GATE) {
     const float scale = EPI == DENSE_STORE && a.scale ? *a.scale : 1.0f;
 #pragma unroll
@@ -500,10 +529,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
         }
       }
     };
-    if (a.planes == 1)
-      gate(yes);
-    else
-      gate(no);
+    by_planes(gate);
   } else if constexpr (EPI == DENSE_DGATE) {
     // (stored from the accumulators' layout, 64 and 32 bytes of a row at a time: staged as the other results
     // it kept too much in registers and was no faster, 107 and 116 us of 4096 x 2880 against 108)
@@ -556,10 +582,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
         }
       }
     };
-    if (a.planes == 1)
-      dgate(yes);
-    else
-      dgate(no);
+    by_planes(dgate);
   } else if constexpr (EPI == DENSE_STATS) {
     const bool whole = m_first + TM * 16 <= a.M;  // else the rows past the vocabulary count as minus infinity
     if (!whole) {
@@ -637,22 +660,20 @@ __global__ __launch_bounds__(64 * WM * WN) void k_dense(const DenseArgs a) {
         }
       }
     };
-    if (a.planes == 1)
-      dlogits(yes);
-    else
-      dlogits(no);
+    by_planes(dlogits);
   }
 }
 
-template <int BM, int BN, int WM, int WN, int NS, bool AT, bool BT, int EPI>
+template <int BM, int BN, int WM, int WN, int NS, int PL, bool AT, bool BT, int EPI>
 hipError_t launch_dense_as(const DenseArgs &a, hipStream_t st) {
   static DynLdsOnce once;
-  const size_t bytes = NS * (BM + BN) * 128;
-  auto kernel = k_dense<BM, BN, WM, WN, NS, AT, BT, EPI>;
+  const size_t bytes = NS * (BM + PL * BN) * 128;
+  auto kernel = k_dense<BM, BN, WM, WN, NS, PL, AT, BT, EPI>;
   hipError_t e = ensure_dyn_lds(once, (const void *)kernel, bytes);
   if (e != hipSuccess) return e;
   const size_t tiles = (size_t)((a.M + BM - 1) / BM) * ((a.N * a.stack + BN - 1) / BN);
-  if (a.stack > 1 && (a.N * a.stack > BN || BN > 64)) return hipErrorInvalidValue;
+  if (a.b_planes != PL || (a.stack > 1 && (PL > 1 || a.N * a.stack > BN || BN > 64))) return hipErrorInvalidValue;
+  if ((EPI == DENSE_GATE || EPI == DENSE_DGATE || EPI == DENSE_DLOGITS) && (PL > 1 ? a.planes == 1 : BN > 64 && a.planes > 1)) return hipErrorInvalidValue;
   if (tiles > 0x7FFFFFFF || a.splits > 65535) return hipErrorInvalidValue;
   kernel<<<dim3((unsigned)tiles, a.splits), 64 * WM * WN, bytes, st>>>(a);
   return hipGetLastError();
