@@ -113,7 +113,7 @@ namespace {
 
 // Two arrays in one launch (the rows and their gradients, of one length). Bound by its 4 bytes read and 6
 // written a value, of few by the launch.
-__global__ void k_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n) {
+__global__ __launch_bounds__(256) void k_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n) {
   const float *x = blockIdx.y ? x1 : x0;
   uint16_t *out = blockIdx.y ? out1 : out0;
   const uint32_t where = blockIdx.y ? where1 : where0;
@@ -130,8 +130,9 @@ __global__ void k_planes(const float *x0, uint16_t *out0, uint32_t where0, const
   }
 }
 
-// Sums of parts, in order. Many values: a thread each, 8 parts' loads in flight. Few (bias gradients):
-// a block takes 32 values and 8 spans of the parts, whose sums join in order.
+// Sums of parts, in order, of several results in one launch (each of its own cost 2 to 3 us, mostly the
+// launch). Many values: a thread each, 8 parts' loads in flight. Few of many parts (bias gradients): a
+// block takes 32 values and 8 spans of the parts, whose sums join in order.
 template <bool BF>
 __device__ __forceinline__ void put(void *out, size_t i, float s) {
   if constexpr (BF)
@@ -153,41 +154,44 @@ __device__ __forceinline__ float sum_span(const float *part, size_t stride, int 
   return s;
 }
 template <bool BF>
-__global__ __launch_bounds__(256) void k_sum_parts(const float *part, size_t stride, int parts, size_t n, const float *bias,
-                                                   size_t n_bias, void *out) {
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-    float s = sum_span(part + i, stride, 0, parts);
-    if (bias) s += bias[i % n_bias];
-    put<BF>(out, i, s);
+__device__ __forceinline__ void sum_many(const DenseSum &d, unsigned block) {
+  for (size_t i = (size_t)block * 256 + threadIdx.x; i < d.n; i += (size_t)d.blocks * 256) {
+    float s = sum_span(d.part + i, d.stride, 0, d.parts);
+    if (d.bias) s += d.bias[i % d.n_bias];
+    put<BF>(d.out, i, s);
   }
 }
-__global__ __launch_bounds__(256) void k_sum_few(const float *part, size_t stride, int parts, size_t n, float *out) {
+__global__ __launch_bounds__(256) void k_sums(const DenseSums a) {
   __shared__ float s_sum[8][32];
-  const size_t i = (size_t)blockIdx.x * 32 + threadIdx.x % 32;
-  const int span = threadIdx.x / 32, each = (parts + 7) / 8;
-  if (i < n) s_sum[span][threadIdx.x % 32] = sum_span(part + i, stride, min(span * each, parts), min((span + 1) * each, parts));
+  unsigned block = blockIdx.x;
+  int j = 0;
+  while (block >= a.d[j].blocks) block -= a.d[j++].blocks;
+  const DenseSum &d = a.d[j];
+  if (d.bf16) return sum_many<true>(d, block);
+  if (!d.few) return sum_many<false>(d, block);
+  const size_t i = (size_t)block * 32 + threadIdx.x % 32;
+  const int span = threadIdx.x / 32, each = (d.parts + 7) / 8;
+  if (i < d.n) s_sum[span][threadIdx.x % 32] = sum_span(d.part + i, d.stride, min(span * each, d.parts), min((span + 1) * each, d.parts));
   __syncthreads();
-  if (span == 0 && i < n) {
+  if (span == 0 && i < d.n) {
     float s = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) s += s_sum[j][threadIdx.x];
-    out[i] = s;
+    for (int k = 0; k < 8; k++) s += s_sum[k][threadIdx.x];
+    ((float *)d.out)[i] = s;
   }
 }
 
-// A block sums 64 rows of 256 columns: 8 rows at a time by 32 threads of 8 columns.
-constexpr int kColRows = 64;
+// A block sums its rows (512, or up to 1024 if they are all) of 64 columns: 128 rows at a time by 8 threads
+// of 8 columns. Bound by its bytes; few rows stay without parts, whose sum would be another launch.
 template <bool BF>
-__global__ __launch_bounds__(256) void k_colsum(const void *x, size_t T, size_t H, float *part) {
-  __shared__ float s_sum[8][256];
-  const int in = threadIdx.x % 32, row = threadIdx.x / 32;
-  const size_t c = (size_t)blockIdx.x * 256 + in * 8, t0 = (size_t)blockIdx.y * kColRows;
+__global__ __launch_bounds__(1024) void k_colsum(const void *x, size_t T, size_t H, size_t rows, float *part) {
+  __shared__ float s_sum[16][64];
+  const int in = threadIdx.x % 8, row = threadIdx.x / 8;
+  const size_t c = (size_t)blockIdx.x * 64 + in * 8, t0 = (size_t)blockIdx.y * rows, t1 = min(T, t0 + rows);
   float s[8] = {};
   if (c < H) {  // (H is a multiple of 32)
-#pragma unroll
-    for (int k = 0; k < kColRows / 8; k++) {
-      const size_t t = t0 + row + k * 8;
-      if (t >= T) break;
+#pragma unroll 4
+    for (size_t t = t0 + row; t < t1; t += 128) {
       float v[8];
       if constexpr (BF) {
         const uint4 u = *(const uint4 *)((const uint16_t *)x + t * H + c);
@@ -204,14 +208,20 @@ __global__ __launch_bounds__(256) void k_colsum(const void *x, size_t T, size_t 
       for (int i = 0; i < 8; i++) s[i] += v[i];
     }
   }
+  // over the 8 rows of a wavefront, then over the wavefronts in order
 #pragma unroll
-  for (int i = 0; i < 8; i++) s_sum[row][in * 8 + i] = s[i];
+  for (int i = 0; i < 8; i++) {
+    s[i] += __shfl_xor(s[i], 8);
+    s[i] += __shfl_xor(s[i], 16);
+    s[i] += __shfl_xor(s[i], 32);
+    if (threadIdx.x % 64 < 8) s_sum[threadIdx.x / 64][in * 8 + i] = s[i];
+  }
   __syncthreads();
-  const size_t o = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (o < H) {
+  const size_t o = (size_t)blockIdx.x * 64 + threadIdx.x;
+  if (threadIdx.x < 64 && o < H) {
     float v = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) v += s_sum[j][threadIdx.x];
+    for (int j = 0; j < 16; j++) v += s_sum[j][threadIdx.x];
     part[blockIdx.y * H + o] = v;
   }
 }
@@ -343,15 +353,14 @@ hipError_t launch_planes(const float *x0, uint16_t *out0, uint32_t where0, const
   return hipGetLastError();
 }
 
-hipError_t launch_sum_parts(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias,
-                            void *out, bool bf16, hipStream_t s) {
-  if (!n) return hipSuccess;
-  if (!bf16 && !bias && n <= 65536 && parts > 8)
-    k_sum_few<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(part, stride, parts, n, (float *)out);
-  else if (bf16)
-    k_sum_parts<true><<<blocks_for(n), 256, 0, s>>>(part, stride, parts, n, bias, n_bias, out);
-  else
-    k_sum_parts<false><<<blocks_for(n), 256, 0, s>>>(part, stride, parts, n, bias, n_bias, out);
+void DenseSums::add(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias, void *out, bool bf16) {
+  const bool few = !bf16 && !bias && n <= 65536 && parts > 8;
+  d[count++] = DenseSum{part, stride, n, n_bias, bias, out, parts, few ? (unsigned)((n + 31) / 32) : blocks_for(n), bf16, few};
+}
+hipError_t launch_sums(const DenseSums &a, hipStream_t s) {
+  unsigned blocks = 0;
+  for (int i = 0; i < a.count; i++) blocks += a.d[i].blocks;
+  if (blocks) k_sums<<<blocks, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -371,14 +380,15 @@ hipError_t launch_dloss_scale(const float *dloss, const int32_t *targets, size_t
   return hipGetLastError();
 }
 
-int dense_colsum_parts(size_t T) { return (int)((T + kColRows - 1) / kColRows); }
+static size_t colsum_rows(size_t T) { return T <= 1024 ? 1024 : 512; }
+int dense_colsum_parts(size_t T) { return (int)((T + colsum_rows(T) - 1) / colsum_rows(T)); }
 hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *part, hipStream_t s) {
-  const dim3 grid((unsigned)((H + 255) / 256), (unsigned)dense_colsum_parts(T));
+  const dim3 grid((unsigned)((H + 63) / 64), (unsigned)dense_colsum_parts(T));
   if (!T || !H) return hipSuccess;
   if (bf16)
-    k_colsum<true><<<grid, 256, 0, s>>>(x, T, H, part);
+    k_colsum<true><<<grid, 1024, 0, s>>>(x, T, H, colsum_rows(T), part);
   else
-    k_colsum<false><<<grid, 256, 0, s>>>(x, T, H, part);
+    k_colsum<false><<<grid, 1024, 0, s>>>(x, T, H, colsum_rows(T), part);
   return hipGetLastError();
 }
 

@@ -100,8 +100,22 @@ hipError_t launch_dgate(const DgateArgs &a, hipStream_t s);
 hipError_t launch_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n,
                          hipStream_t s);
 // out[i] = sum over parts of part[p * stride + i] (+ bias[i % n_bias]) for i < n, in order; bf16 or f32.
-hipError_t launch_sum_parts(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias,
-                            void *out, bool bf16, hipStream_t s);
+struct DenseSum {
+  const float *part;
+  size_t stride, n, n_bias;
+  const float *bias;
+  void *out;
+  int parts;
+  unsigned blocks;
+  bool bf16, few;
+};
+// Up to 5 of them in one launch (those that a backward pass of the gated block can need).
+struct DenseSums {
+  DenseSum d[5];
+  int count = 0;
+  void add(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias, void *out, bool bf16);
+};
+hipError_t launch_sums(const DenseSums &a, hipStream_t s);
 // Column sums of x [T][H] (f32 or bf16) into parts [dense_colsum_parts(T)][H].
 int dense_colsum_parts(size_t T);
 hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *part, hipStream_t s);

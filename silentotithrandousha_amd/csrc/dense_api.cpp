@@ -179,8 +179,9 @@ DenseArgs gradient(const Rows &x, const Rows &y) {
   return a;
 }
 
-// out [N][M] (+ bias) of a product, K split where that fills the device; part: [splits][N][M] f32 then.
-int store(DenseArgs a, bool at, bool bt, int splits, float *part, const float *bias, void *out, int dtype, hipStream_t s) {
+// out [N][M] (+ bias) of a product, K split where that fills the device; part: [splits][N][M] f32 then, whose
+// sum is left to `sums`.
+int store(DenseArgs a, bool at, bool bt, int splits, float *part, const float *bias, void *out, int dtype, DenseSums &sums, hipStream_t s) {
   const DenseShape shape{at, bt, DENSE_STORE};
   a.ldo = (size_t)a.M;
   if (splits > 1) {
@@ -189,7 +190,7 @@ int store(DenseArgs a, bool at, bool bt, int splits, float *part, const float *b
     a.out = part;
     a.out_mode = 1;
     HIP_TRY(launch_dense(shape, a, s));
-    HIP_TRY(launch_sum_parts(part, a.split_stride, splits, a.split_stride, bias, (size_t)a.M, out, dtype == MOE_BF16, s));
+    sums.add(part, a.split_stride, dense_split_count(a), a.split_stride, bias, (size_t)a.M, out, dtype == MOE_BF16);
     return MOE_OK;
   }
   a.out = out;
@@ -391,12 +392,18 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
         HIP_TRY(launch_dense(sw, g, s));
       }
     }
-    if (dw && dw_acc) HIP_TRY(launch_sum_parts(dw_acc, 0, 1, nvoc * H, nullptr, 1, (uint16_t *)dw + v0 * H, true, s));
+    if (dw && dw_acc) {
+      DenseSums sums;
+      sums.add(dw_acc, 0, 1, nvoc * H, nullptr, 1, (uint16_t *)dw + v0 * H, true);
+      HIP_TRY(launch_sums(sums, s));
+    }
   }
+  DenseSums sums;
   if (parts)
-    HIP_TRY(launch_sum_parts(dx_acc, T * H, written, T * H, nullptr, 1, dx, bf, s));
+    sums.add(dx_acc, T * H, written, T * H, nullptr, 1, dx, bf);
   else if (dx && dx_acc && bf)
-    HIP_TRY(launch_sum_parts(dx_acc, 0, 1, T * H, nullptr, 1, dx, true, s));
+    sums.add(dx_acc, 0, 1, T * H, nullptr, 1, dx, true);
+  HIP_TRY(launch_sums(sums, s));
   return MOE_OK;
 }
 
@@ -437,7 +444,10 @@ int moe_ffn_forward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int dt
   g.ldh = I;
   g.planes = P;
   HIP_TRY(launch_dense(DenseShape{false, false, DENSE_GATE}, g, s));
-  return store(product(b->down, I, h, H), false, false, splits, part, b->down_bias, y, dtype, s);
+  DenseSums sums;
+  RETURN_IF(store(product(b->down, I, h, H), false, false, splits, part, b->down_bias, y, dtype, sums, s));
+  HIP_TRY(launch_sums(sums, s));
+  return MOE_OK;
 }
 
 int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x_type, const void *dy, int dtype, size_t T,
@@ -466,7 +476,7 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
   const DenseShape ss{false, false, DENSE_STORE}, sg{true, false, DENSE_DGATE}, sx{true, false, DENSE_STORE}, sw{true, true, DENSE_STORE};
   Carve w;
   Rows r, d, h, dgu;
-  float *gu = nullptr, *dh = nullptr, *db = nullptr, *col = nullptr, *part = nullptr;
+  float *gu = nullptr, *dh = nullptr, *db = nullptr, *col = nullptr, *px = nullptr, *pgu = nullptr, *pd = nullptr;
   int nx = 1, ngu = 1, nd = 1, db_parts = 0, n_raw = 1, n_dh = 1;
   bool apart = false;  // d(gate, up) in a kernel of its own, from K parts of gate, up and dh
   for (int placed = 0; placed < 2; placed++) {
@@ -499,11 +509,9 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
       nx = dense_splits(sx, product(b->gate_up, H, dgu, H));
       ngu = dense_splits(sw, gradient(r, dgu));
       nd = dense_splits(sw, gradient(h, d));
-      size_t most = 0;  // one after the other, so they share it
-      if (out->x && nx > 1) most = std::max(most, nx * T * H);
-      if (out->gate_up && ngu > 1) most = std::max(most, ngu * 2 * I * H);
-      if (out->down && nd > 1) most = std::max(most, nd * I * H);
-      part = w.take<float>(most);
+      px = out->x && nx > 1 ? w.take<float>(nx * T * H) : nullptr;
+      pgu = out->gate_up && ngu > 1 ? w.take<float>(ngu * 2 * I * H) : nullptr;
+      pd = out->down && nd > 1 ? w.take<float>(nd * I * H) : nullptr;
     }
     col = !out->down_bias ? nullptr : dense_colsum_parts(T) > 1 ? w.take<float>(dense_colsum_parts(T) * H) : out->down_bias;
     if (!placed) {
@@ -511,11 +519,15 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
       w = Carve{(char *)c.work->p};
     }
   }
+  DenseSums sums;  // in one launch at the end
   if (out->down_bias) {
     HIP_TRY(launch_colsum(dy, bf, T, H, col, s));
-    if (dense_colsum_parts(T) > 1) HIP_TRY(launch_sum_parts(col, H, dense_colsum_parts(T), H, nullptr, 1, out->down_bias, false, s));
+    if (col != out->down_bias) sums.add(col, H, dense_colsum_parts(T), H, nullptr, 1, out->down_bias, false);
   }
-  if (!inner) return MOE_OK;
+  if (!inner) {
+    HIP_TRY(launch_sums(sums, s));
+    return MOE_OK;
+  }
   if (x_type == MOE_MXFP8) HIP_TRY(launch_act8_unpack((const uint8_t *)x, T, H, r.out(), true, r.slots, s));
   if (dtype == MOE_F32)
     HIP_TRY(launch_planes((const float *)dy, d.out(), d.where, x_type == MOE_F32 ? (const float *)x : nullptr, r.out(), r.where, T * H, s));
@@ -549,15 +561,11 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
     g.planes = P;
     HIP_TRY(launch_dense(sg, g, s));
   }
-  if (db && db_parts > 1) HIP_TRY(launch_sum_parts(db, 2 * I, db_parts, 2 * I, nullptr, 1, out->gate_up_bias, false, s));
-  if (out->x)
-    RETURN_IF(store(product(b->gate_up, H, dgu, H), true, false, nx, part, nullptr,
-                    out->x, dtype, s));
-  if (out->gate_up)
-    RETURN_IF(store(gradient(r, dgu), true, true, ngu, part, nullptr,
-                    out->gate_up, dtype, s));
-  if (out->down)
-    RETURN_IF(store(gradient(h, d), true, true, nd, part, nullptr, out->down, dtype, s));
+  if (db && db_parts > 1) sums.add(db, 2 * I, db_parts, 2 * I, nullptr, 1, out->gate_up_bias, false);
+  if (out->x) RETURN_IF(store(product(b->gate_up, H, dgu, H), true, false, nx, px, nullptr, out->x, dtype, sums, s));
+  if (out->gate_up) RETURN_IF(store(gradient(r, dgu), true, true, ngu, pgu, nullptr, out->gate_up, dtype, sums, s));
+  if (out->down) RETURN_IF(store(gradient(h, d), true, true, nd, pd, nullptr, out->down, dtype, sums, s));
+  HIP_TRY(launch_sums(sums, s));
   return MOE_OK;
 }
 
