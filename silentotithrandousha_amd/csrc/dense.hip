@@ -43,7 +43,7 @@ double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a,
   const long whole = tiles / (kCus * d.wgs), rest = tiles - whole * kCus * d.wgs;
   const double on = (double)rest / kCus;  // of the last round: between the busiest CU's and the mean
   double us = whole * round(d.wgs) + (rest ? round(std::max(1.0, 0.5 * (on + std::ceil(on)))) : 0.0);
-  if (splits > 1) us += 4.5 + 4.0 * splits * a.M * a.N / 5e6;
+  if (splits > 1) us += (a.joined ? 0.5 : 4.5) + 4.0 * splits * a.M * a.N / 5e6;
   return us;
 }
 

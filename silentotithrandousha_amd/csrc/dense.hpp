@@ -43,6 +43,7 @@ struct DenseArgs {
   uint32_t pb;              // those slots, 4 bits each, in the order of their products
   int splits;               // K split (DENSE_STORE with f32 only): out + split * split_stride
   int k_split;              // K per split, a multiple of the step
+  bool joined;              // for the plan: a launch that comes anyway sums the splits
   // DENSE_STORE
   void *out;
   size_t ldo, split_stride;

@@ -494,9 +494,11 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
       DenseArgs in = product(b->down, I, d, I);
       raw.out_mode = in.out_mode = 1;
       const double one = dense_estimate(ss, raw) + dense_estimate(sg, in);
+      raw.joined = in.joined = true;
       raw.splits = n_raw = dense_splits(ss, raw);
       in.splits = n_dh = dense_splits(sx, in);
-      const double bytes = (8.0 * n_raw + 4.0 * n_dh + 6.0 * (bf ? 1 : kPairs6)) * T * I;  // of that kernel, at 5 TB/s
+      // (that kernel's bytes at 5 TB/s; what its parts cost is in the estimates)
+      const double bytes = ((n_raw > 1 ? 0.0 : 8.0) + (n_dh > 1 ? 0.0 : 4.0) + 6.0 * (bf ? 1 : kPairs6)) * T * I;
       apart = dense_estimate(ss, raw) + dense_estimate(sx, in) + 1.0 + bytes / 5e6 < one && T <= 65536;
       if (!apart) n_raw = n_dh = 1;
       gu = w.take<float>(n_raw * T * 2 * I);
@@ -506,9 +508,13 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
       db_parts = apart ? dense_dgate_parts((int)T) : dense_parts(sg, product(b->down, I, d, I));
       // (one part is the result)
       db = !out->gate_up_bias ? nullptr : db_parts > 1 ? w.take<float>((size_t)db_parts * 2 * I) : out->gate_up_bias;
-      nx = dense_splits(sx, product(b->gate_up, H, dgu, H));
-      ngu = dense_splits(sw, gradient(r, dgu));
-      nd = dense_splits(sw, gradient(h, d));
+      auto splits = [&](const DenseShape &shape, DenseArgs a) {
+        a.joined = db_parts > 1 && out->gate_up_bias;
+        return dense_splits(shape, a);
+      };
+      nx = splits(sx, product(b->gate_up, H, dgu, H));
+      ngu = splits(sw, gradient(r, dgu));
+      nd = splits(sw, gradient(h, d));
       px = out->x && nx > 1 ? w.take<float>(nx * T * H) : nullptr;
       pgu = out->gate_up && ngu > 1 ? w.take<float>(ngu * 2 * I * H) : nullptr;
       pd = out->down && nd > 1 ? w.take<float>(nd * I * H) : nullptr;
