@@ -197,7 +197,8 @@ TILES_BLOCK = [(27, 224, 296, MOE_F32), (6, 160, 80, MOE_F32), (3, 224, 4360, MO
                (8587, 224, 112, MOE_BF16), (946, 32, 1064, MOE_F32), (347, 160, 5368, MOE_BF16), (619, 160, 808, MOE_BF16),
                (150, 288, 5648, MOE_BF16), (978, 160, 4368, MOE_F32), (6266, 160, 264, MOE_F32), (6596, 160, 616, MOE_BF16),
                (6451, 544, 72, MOE_BF16), (810, 224, 7048, MOE_BF16), (810, 224, 7048, MOE_F32), (7227, 2080, 528, MOE_BF16),
-               (5000, 160, 2056, MOE_BF16), (1155, 160, 6904, MOE_F32), (11279, 160, 1168, MOE_BF16), (11819, 160, 1048, MOE_F32)]
+               (5000, 160, 2056, MOE_BF16), (1155, 160, 6904, MOE_F32), (11279, 160, 1168, MOE_BF16), (11819, 160, 1048, MOE_F32),
+               (1, 224, 2056, MOE_BF16), (8, 160, 2568, MOE_BF16), (2, 96, 2056, MOE_F32)]
 
 
 @pytest.mark.parametrize("T,H,V,dtype", TILES_LOSS)
