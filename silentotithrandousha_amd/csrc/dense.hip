@@ -23,9 +23,9 @@ constexpr int kCus = 256;  // of an MI355X: the plan is for the whole device
 // largest of the time that its products take at the tile's full rate, that its loads of A take where A is
 // read once, from memory (both shared by the workgroups of its CU), and that its loads wait, spread over
 // the steps that its slots hold ahead; each workgroup has a prologue and an epilogue that stores its
-// results; parts are summed in another launch. Whole rounds of workgroups and what is left for the last one count apart.
-double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a, int splits) {
-  const long tiles_n = ((long)a.N * a.stack + d.bn - 1) / d.bn, tiles = (long)((a.M + d.bm - 1) / d.bm) * tiles_n * splits;
+// results; parts are summed in another launch. `others`: tiles of the same shape in the launch, as many as do the same steps. Whole rounds of workgroups and what is left for the last one count apart.
+double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a, int splits, long others = 0) {
+  const long tiles_n = ((long)a.N * a.stack + d.bn - 1) / d.bn, tiles = (long)((a.M + d.bm - 1) / d.bm) * tiles_n * splits + others;
   const long steps = (((long)a.K + kDenseStep - 1) / kDenseStep + splits - 1) / splits;
   // bytes that a result costs, about: of rows in planes, results in planes (GATE 3 slots, the gradients 6)
   const bool planes = a.b_planes > 1 || a.stack > 1;
@@ -47,6 +47,26 @@ double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a,
   return us;
 }
 
+bool tile_fits(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a) {
+  if (d.planes != a.b_planes) return false;
+  if (a.stack > 1 && (d.bn > 64 || a.N * a.stack > d.bn)) return false;  // stacked planes lie in one tile
+  // 288 rows: K-contiguous they keep too much in registers (620 TFLOP/s)
+  return d.bm <= 256 || (s.at && s.epi == DENSE_STORE && a.K >= 1024);
+}
+
+constexpr DenseShape kGradient{true, true, DENSE_STORE};
+int pair_tile(const DenseArgs &a, const DenseArgs &b, double &us) {
+  int best = -1;
+  for (int t = 0; t < kDenseTileCount; t++) {
+    const DenseTileDims &d = kDenseTiles[t];
+    if (!tile_fits(kGradient, d, a)) continue;
+    const double tiles = (double)((b.M + d.bm - 1) / d.bm) * ((b.N + d.bn - 1) / d.bn);
+    const double u = dense_us(kGradient, d, a, 1, (long)std::ceil(tiles * b.K / a.K));
+    if (best < 0 || u < us) best = t, us = u;
+  }
+  return best;
+}
+
 }  // namespace
 
 int dense_tile(const DenseShape &s, const DenseArgs &a) {
@@ -54,10 +74,7 @@ int dense_tile(const DenseShape &s, const DenseArgs &a) {
   double us = 0.0;
   for (int t = 0; t < kDenseTileCount; t++) {
     const DenseTileDims &d = kDenseTiles[t];
-    if (d.planes != a.b_planes) continue;
-    if (a.stack > 1 && (d.bn > 64 || a.N * a.stack > d.bn)) continue;  // stacked planes lie in one tile
-    // 288 rows: K-contiguous they keep too much in registers (620 TFLOP/s)
-    if (d.bm > 256 && (!s.at || s.epi != DENSE_STORE || a.K < 1024)) continue;
+    if (!tile_fits(s, d, a)) continue;
     const double u = dense_us(s, d, a, dense_split_count(a));
     if (best < 0 || u < us) best = t, us = u;
   }
@@ -94,6 +111,24 @@ int dense_splits(const DenseShape &s, const DenseArgs &a0) {
     if (n == 1 || u < us) best = a.splits, us = u;
   }
   return best;
+}
+
+bool dense_pair_pays(const DenseArgs &a, const DenseArgs &b) {
+  if (a.splits > 1 || b.splits > 1 || a.K < b.K) return false;
+  double us = 0.0;
+  pair_tile(a, b, us);
+  return us < dense_estimate(kGradient, a) + dense_estimate(kGradient, b);
+}
+
+hipError_t launch_dense_pair(const DenseArgs &a0, const DenseArgs &b0, hipStream_t st) {
+  DenseArgs x[2] = {a0, b0};
+  for (DenseArgs &a : x) {
+    if (a.M <= 0 || a.N <= 0 || a.K <= 0 || a.b_planes != 1 || a.stack != 1 || a.lda % 8 || a.ldb % 8 || a.M % 4 || a.splits > 1 || a.K > a0.K)
+      return hipErrorInvalidValue;
+    a.k_split = split_k(a);
+  }
+  double us = 0.0;
+  return launch_dense_tt_pair(pair_tile(x[0], x[1], us), x[0], x[1], st);
 }
 
 hipError_t launch_dense(const DenseShape &s, const DenseArgs &a0, hipStream_t st) {

@@ -83,6 +83,10 @@ int dense_splits(const DenseShape &s, const DenseArgs &a);
 int dense_split_count(const DenseArgs &a);  // the splits that a launch with a.splits makes (none of them empty)
 double dense_estimate(const DenseShape &s, const DenseArgs &a);  // us of a launch, about
 hipError_t launch_dense(const DenseShape &s, const DenseArgs &a, hipStream_t st);
+// Two weight gradients (both operands transposed, DENSE_STORE) in one launch, the one with more rows first;
+// whether the plan takes that for faster than two.
+hipError_t launch_dense_pair(const DenseArgs &a, const DenseArgs &b, hipStream_t st);
+bool dense_pair_pays(const DenseArgs &a, const DenseArgs &b);
 
 // DENSE_DGATE's epilogue as a kernel of its own, for gate, up and dh that come in K parts: gu [gu_parts][T][2 I]
 // (+ bias), dh [dh_parts][T][I]; db_part [dense_dgate_parts(T)][2 I] or NULL.

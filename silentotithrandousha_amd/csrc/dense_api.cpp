@@ -569,8 +569,18 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
   }
   if (db && db_parts > 1) sums.add(db, 2 * I, db_parts, 2 * I, nullptr, 1, out->gate_up_bias, false);
   if (out->x) RETURN_IF(store(product(b->gate_up, H, dgu, H), true, false, nx, px, nullptr, out->x, dtype, sums, s));
-  if (out->gate_up) RETURN_IF(store(gradient(r, dgu), true, true, ngu, pgu, nullptr, out->gate_up, dtype, sums, s));
-  if (out->down) RETURN_IF(store(gradient(h, d), true, true, nd, pd, nullptr, out->down, dtype, sums, s));
+  DenseArgs wd = gradient(h, d), wgu = gradient(r, dgu);  // (of a checkpoint's x, wgu has the fewer rows)
+  wd.out_mode = wgu.out_mode = bf ? 0 : 1;
+  if (out->gate_up && out->down && ngu == 1 && nd == 1 && dense_pair_pays(wd, wgu)) {
+    wd.ldo = I;
+    wd.out = out->down;
+    wgu.ldo = H;
+    wgu.out = out->gate_up;
+    HIP_TRY(launch_dense_pair(wd, wgu, s));
+  } else {
+    if (out->gate_up) RETURN_IF(store(wgu, true, true, ngu, pgu, nullptr, out->gate_up, dtype, sums, s));
+    if (out->down) RETURN_IF(store(wd, true, true, nd, pd, nullptr, out->down, dtype, sums, s));
+  }
   HIP_TRY(launch_sums(sums, s));
   return MOE_OK;
 }

@@ -54,6 +54,17 @@ hipError_t launch_dense_shape(const DenseArgs &a, hipStream_t st) {
   return launch_dense_tile<0, AT, BT, EPI>(dense_tile(DenseShape{AT, BT, (DenseEpi)EPI}, a), a, st);
 }
 
+template <int I>
+hipError_t launch_dense_pair_tile(int tile, const DenseArgs &a, const DenseArgs &b, hipStream_t st) {
+  if constexpr (I < kDenseTileCount) {
+    constexpr DenseTileDims d = kDenseTiles[I];
+    if constexpr (d.planes == 1)
+      if (tile == I) return launch_dense_pair_as<d.bm, d.bn, d.wm, d.wn, d.ns>(a, b, st);
+    return launch_dense_pair_tile<I + 1>(tile, a, b, st);
+  }
+  return hipErrorInvalidValue;
+}
+hipError_t launch_dense_tt_pair(int tile, const DenseArgs &a, const DenseArgs &b, hipStream_t st);
 bool dense_few_fits(const DenseShape &s, const DenseArgs &a);
 hipError_t launch_dense_few(const DenseShape &s, const DenseArgs &a, hipStream_t st);
 hipError_t launch_dense_nt(const DenseShape &s, const DenseArgs &a, hipStream_t st);

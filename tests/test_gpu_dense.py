@@ -351,7 +351,7 @@ def test_block_tiles(T, H, I, dtype):  # noqa: E741
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T,H,I", [(1, 64, 40), (50, 96, 72), (300, 128, 320)])
+@pytest.mark.parametrize("T,H,I", [(1, 64, 40), (50, 96, 72), (300, 128, 320), (257, 416, 1000), (1, 224, 2056)])
 def test_block_from_checkpoint(dtype, T, H, I):  # noqa: E741
     """The forward pass keeps x in 8 bits, the backward pass reads that: the gradients are those at the
     values kept, to the operators' own tolerance."""
