@@ -146,9 +146,33 @@ hipError_t launch_dense(const DenseShape &s, const DenseArgs &a0, hipStream_t st
 
 namespace {
 
-// Two arrays in one launch (the rows and their gradients, of one length). Bound by its 4 bytes read and 6
-// written a value, of few by the launch.
-__global__ __launch_bounds__(256) void k_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n) {
+// by one block
+__device__ __forceinline__ void dloss_scale(const DlossScale &d) {
+  __shared__ float part[16];
+  const int threads = blockDim.x;
+  float m = 0.0f;
+  for (size_t t = threadIdx.x; t < d.T; t += threads)
+    if ((unsigned)d.targets[t] < (unsigned)d.vocab) m = fmaxf(m, fabsf(d.dloss[t]));
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
+  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < threads / 64; i++) m = fmaxf(m, part[i]);
+    *d.scale = m > 0.0f && isfinite(m) ? m : 1.0f;
+  }
+}
+__global__ __launch_bounds__(1024) void k_dloss_scale(const DlossScale d) { dloss_scale(d); }
+
+// Two arrays in one launch (the rows and their gradients, of one length), or one and the scale of dloss, whose
+// launch of its own cost 3 us of the 99 of 19 rows' loss and gradient. Bound by its 4 bytes read and 6 written
+// a value, of few by the launch.
+__global__ __launch_bounds__(256) void k_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n,
+                                                const DlossScale d) {
+  if (blockIdx.y && !x1) {
+    if (blockIdx.x == 0) dloss_scale(d);
+    return;
+  }
   const float *x = blockIdx.y ? x1 : x0;
   uint16_t *out = blockIdx.y ? out1 : out0;
   const uint32_t where = blockIdx.y ? where1 : where0;
@@ -361,30 +385,14 @@ __global__ __launch_bounds__(1024) void k_loss(const float2 *stats, int parts, c
   }
 }
 
-__global__ __launch_bounds__(1024) void k_dloss_scale(const float *dloss, const int32_t *targets, size_t T, int vocab, float *scale) {
-  __shared__ float part[16];
-  float m = 0.0f;
-  for (size_t t = threadIdx.x; t < T; t += 1024)
-    if ((unsigned)targets[t] < (unsigned)vocab) m = fmaxf(m, fabsf(dloss[t]));
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
-  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; i++) m = fmaxf(m, part[i]);
-    *scale = m > 0.0f && isfinite(m) ? m : 1.0f;
-  }
-}
-
 unsigned blocks_for(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, 65536); }
 
 }  // namespace
 
 hipError_t launch_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n,
-                         hipStream_t s) {
-  if (!n) return hipSuccess;
-  if (n % 4) return hipErrorInvalidValue;
-  k_planes<<<dim3(blocks_for(n / 4), x1 ? 2 : 1), 256, 0, s>>>(x0, out0, where0, x1, out1, where1, n);
+                         const DlossScale *d, hipStream_t s) {
+  if (n % 4 || !n || (x1 && d)) return n ? hipErrorInvalidValue : hipSuccess;
+  k_planes<<<dim3(blocks_for(n / 4), x1 || d ? 2 : 1), 256, 0, s>>>(x0, out0, where0, x1, out1, where1, n, d ? *d : DlossScale{});
   return hipGetLastError();
 }
 
@@ -410,8 +418,8 @@ hipError_t launch_dgate(const DgateArgs &a, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_dloss_scale(const float *dloss, const int32_t *targets, size_t T, int vocab, float *scale, hipStream_t s) {
-  k_dloss_scale<<<1, 1024, 0, s>>>(dloss, targets, T, vocab, scale);
+hipError_t launch_dloss_scale(const DlossScale &d, hipStream_t s) {
+  k_dloss_scale<<<1, 1024, 0, s>>>(d);
   return hipGetLastError();
 }
 

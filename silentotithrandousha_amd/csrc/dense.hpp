@@ -101,9 +101,21 @@ struct DgateArgs {
 int dense_dgate_parts(int T);
 hipError_t launch_dgate(const DgateArgs &a, hipStream_t s);
 
-// x0 [n] f32 as kPlanes bf16 planes in the slots (n elements each) of `where0`; x1 (or NULL) likewise.
+// scale: the largest magnitude of dloss [T] at tokens whose target lies in the vocabulary (the others' may
+// be anything), 1 where that is 0 or not finite.
+struct DlossScale {
+  const float *dloss;
+  const int32_t *targets;
+  size_t T;
+  int vocab;
+  float *scale;
+};
+hipError_t launch_dloss_scale(const DlossScale &d, hipStream_t s);
+
+// x0 [n] f32 as kPlanes bf16 planes in the slots (n elements each) of `where0`; x1 (or NULL) likewise; or
+// beside x0 the scale d (or NULL), for few tokens.
 hipError_t launch_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n,
-                         hipStream_t s);
+                         const DlossScale *d, hipStream_t s);
 // out[i] = sum over parts of part[p * stride + i] (+ bias[i % n_bias]) for i < n, in order; bf16 or f32.
 struct DenseSum {
   const float *part;
@@ -127,10 +139,6 @@ hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *pa
 // loss and log-sum-exp of each token from the parts of DENSE_STATS.
 hipError_t launch_loss(const float2 *stats, int parts, const float *picked, const int32_t *targets, size_t T,
                        int vocab, float *loss, float *lse, hipStream_t s);
-
-// The largest magnitude of dloss [T] at tokens whose target lies in the vocabulary (the others' may be
-// anything), 1 where that is 0 or not finite.
-hipError_t launch_dloss_scale(const float *dloss, const int32_t *targets, size_t T, int vocab, float *scale, hipStream_t s);
 
 // MXFP8 activation checkpoints (act8.hip): codes [n][cols], then scales [n][cols / 32].
 hipError_t launch_act8_pack(const void *x, bool bf16, size_t n, size_t cols, uint8_t *packed, hipStream_t s);

@@ -136,8 +136,8 @@ Rows place(Carve &w, Rows r, const void *x, int dtype) {
   r.p = (const uint16_t *)x;
   return r;
 }
-int fill(const Rows &r, const void *x, int dtype, hipStream_t s) {
-  if (dtype == MOE_F32) HIP_TRY(launch_planes((const float *)x, r.out(), r.where, nullptr, nullptr, 0, r.slot(), s));
+int fill(const Rows &r, const void *x, int dtype, hipStream_t s, const DlossScale *d = nullptr) {
+  if (dtype == MOE_F32) HIP_TRY(launch_planes((const float *)x, r.out(), r.where, nullptr, nullptr, 0, r.slot(), d, s));
   return MOE_OK;
 }
 
@@ -330,14 +330,16 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
     q.n = n;
     return q;
   };
-  for (size_t t0 = 0; t0 < T && !bf; t0 += Tc) {
-    const size_t n = std::min(Tc, T - t0);
-    RETURN_IF(fill(piece(t0, n), (const float *)x + t0 * H, dtype, s));
-  }
   // The gradient of the logits is held over the largest |dloss| and the results multiplied by it: for the
   // mean's constant dloss the entries of the targets, which weigh most, then lie next to -1 and are rounded
   // by their p alone, where bf16(1 / n) would put one error into all of them.
-  HIP_TRY(launch_dloss_scale(dloss, targets, T, (int)vocab, scale, s));
+  const DlossScale largest{dloss, targets, T, (int)vocab, scale};
+  const bool beside = !bf && T <= 1024;  // in the launch of the rows' planes
+  if (!beside) HIP_TRY(launch_dloss_scale(largest, s));
+  for (size_t t0 = 0; t0 < T && !bf; t0 += Tc) {
+    const size_t n = std::min(Tc, T - t0);
+    RETURN_IF(fill(piece(t0, n), (const float *)x + t0 * H, dtype, s, beside ? &largest : nullptr));
+  }
   int written = 0;  // parts of dx
   for (size_t v0 = 0; v0 < vocab; v0 += Vc) {
     const size_t nvoc = std::min(Vc, vocab - v0);
@@ -536,7 +538,7 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
   }
   if (x_type == MOE_MXFP8) HIP_TRY(launch_act8_unpack((const uint8_t *)x, T, H, r.out(), true, r.slots, s));
   if (dtype == MOE_F32)
-    HIP_TRY(launch_planes((const float *)dy, d.out(), d.where, x_type == MOE_F32 ? (const float *)x : nullptr, r.out(), r.where, T * H, s));
+    HIP_TRY(launch_planes((const float *)dy, d.out(), d.where, x_type == MOE_F32 ? (const float *)x : nullptr, r.out(), r.where, T * H, nullptr, s));
   // gate and up as f32, their K parts side by side
   auto parts = [&](const DenseShape &shape, DenseArgs g, int splits, const float *bias, float *out) -> int {
     g.ldo = (size_t)g.M;
