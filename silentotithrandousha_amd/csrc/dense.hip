@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "act8.hpp"
 #include "dense_launch.hpp"
 
 namespace moe {
@@ -146,6 +147,35 @@ hipError_t launch_dense(const DenseShape &s, const DenseArgs &a0, hipStream_t st
 
 namespace {
 
+// The job of this block of a launch of several: the first whose blocks end behind it. (The ends lie side by
+// side, one scalar load.)
+template <int N>
+__device__ __forceinline__ int job_of(const unsigned (&end)[N]) {
+  int j = 0;
+#pragma unroll
+  for (int i = 0; i < N - 1; i++) j += blockIdx.x >= end[i];
+  return j;
+}
+
+// What a call does with its rows before its products, in one launch (each of its own cost 2 to 3 us): the
+// planes of f32 rows, a checkpoint written or read, the column sums of up to kColRows rows, the scale of dloss.
+// Bound by their bytes, of few rows by the launch.
+__device__ __forceinline__ void rows_planes(const DenseRows &d, unsigned block) {
+  const float *x = (const float *)d.x;
+  uint16_t *out = (uint16_t *)d.out;
+  for (size_t i = ((size_t)block * 256 + threadIdx.x) * 4; i < d.n; i += (size_t)d.blocks * 1024) {  // (n is a multiple of 32)
+    const f32x4 v = *(const f32x4 *)(x + i);
+    uint16_t p[4][kPlanes];
+#pragma unroll
+    for (int j = 0; j < 4; j++) dense_split(v[j], p[j]);
+#pragma unroll
+    for (int k = 0; k < kPlanes; k++) {
+      const uint2 q = {p[0][k] | (uint32_t)p[1][k] << 16, p[2][k] | (uint32_t)p[3][k] << 16};
+      dense_slots(d.where, k, [&](size_t at) { *(uint2 *)(out + at * d.n + i) = q; });
+    }
+  }
+}
+
 // by one block
 __device__ __forceinline__ void dloss_scale(const DlossScale &d) {
   __shared__ float part[16];
@@ -164,28 +194,67 @@ __device__ __forceinline__ void dloss_scale(const DlossScale &d) {
 }
 __global__ __launch_bounds__(1024) void k_dloss_scale(const DlossScale d) { dloss_scale(d); }
 
-// Two arrays in one launch (the rows and their gradients, of one length), or one and the scale of dloss, whose
-// launch of its own cost 3 us of the 99 of 19 rows' loss and gradient. Bound by its 4 bytes read and 6 written
-// a value, of few by the launch.
-__global__ __launch_bounds__(256) void k_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n,
-                                                const DlossScale d) {
-  if (blockIdx.y && !x1) {
-    if (blockIdx.x == 0) dloss_scale(d);
-    return;
-  }
-  const float *x = blockIdx.y ? x1 : x0;
-  uint16_t *out = blockIdx.y ? out1 : out0;
-  const uint32_t where = blockIdx.y ? where1 : where0;
-  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (size_t)gridDim.x * 1024) {  // (n is a multiple of 32)
-    const f32x4 v = *(const f32x4 *)(x + i);
-    uint16_t p[4][kPlanes];
+// The column sums of rows t0 to t1: a block of THREADS takes 64 columns, 8 threads of 8 columns a row.
+template <int THREADS, class S>
+__device__ __forceinline__ void column_sums(const S *x, size_t t0, size_t t1, size_t H, unsigned block, float *out) {
+  __shared__ float s_sum[THREADS / 64][64];
+  const int in = threadIdx.x % 8, row = threadIdx.x / 8;
+  const size_t c = (size_t)block * 64 + in * 8;
+  float s[8] = {};
+  if (c < H) {  // (H is a multiple of 32)
+#pragma unroll 4
+    for (size_t t = t0 + row; t < t1; t += THREADS / 8) {
+      float v[8];
+      act8_load(x + t * H + c, v);
 #pragma unroll
-    for (int j = 0; j < 4; j++) dense_split(v[j], p[j]);
-#pragma unroll
-    for (int k = 0; k < kPlanes; k++) {
-      const uint2 q = {p[0][k] | (uint32_t)p[1][k] << 16, p[2][k] | (uint32_t)p[3][k] << 16};
-      dense_slots(where, k, [&](size_t at) { *(uint2 *)(out + at * n + i) = q; });
+      for (int i = 0; i < 8; i++) s[i] += v[i];
     }
+  }
+  // over the 8 rows of a wavefront, then over the wavefronts in order
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    s[i] += __shfl_xor(s[i], 8);
+    s[i] += __shfl_xor(s[i], 16);
+    s[i] += __shfl_xor(s[i], 32);
+    if (threadIdx.x % 64 < 8) s_sum[threadIdx.x / 64][in * 8 + i] = s[i];
+  }
+  __syncthreads();
+  const size_t o = (size_t)block * 64 + threadIdx.x;
+  if (threadIdx.x < 64 && o < H) {
+    float v = 0.0f;
+#pragma unroll
+    for (int j = 0; j < THREADS / 64; j++) v += s_sum[j][threadIdx.x];
+    out[o] = v;
+  }
+}
+constexpr size_t kColRows = 512;  // of a block
+template <class S>
+__global__ __launch_bounds__(1024) void k_colsum(const S *x, size_t T, size_t H, float *part) {
+  const size_t t0 = (size_t)blockIdx.y * kColRows;
+  column_sums<1024>(x, t0, min(T, t0 + kColRows), H, blockIdx.x, part + blockIdx.y * H);
+}
+
+// (planes alone, without the choice among jobs: 0.5 to 1 us less)
+__global__ __launch_bounds__(256) void k_planes(const DenseRows d) { rows_planes(d, blockIdx.x); }
+__global__ __launch_bounds__(256) void k_rows(const DenseRowJobs a) {
+  const int j = job_of(a.end);
+  const unsigned block = blockIdx.x - (j ? a.end[j - 1] : 0);
+  const DenseRows &d = a.d[j];
+  const size_t i = (size_t)block * 256 + threadIdx.x;  // of 8 values
+  if (d.what == ROWS_PLANES) {
+    rows_planes(d, block);
+  } else if (d.what == ROWS_PACK8) {
+    uint8_t *codes = (uint8_t *)d.out;
+    if (i * 8 < d.n) act8_pack8((const float *)d.x, i, codes, codes + d.n);
+  } else if (d.what == ROWS_UNPACK8) {
+    const uint8_t *codes = (const uint8_t *)d.x;
+    if (i * 8 < d.n) act8_unpack8(codes, codes + d.n, i, d.n / 32, (uint16_t *)d.out, d.copies);
+  } else if (d.what == ROWS_SUM_BF16) {
+    column_sums<256>((const uint16_t *)d.x, 0, d.n, d.cols, block, (float *)d.out);
+  } else if (d.what == ROWS_SUM_F32) {
+    column_sums<256>((const float *)d.x, 0, d.n, d.cols, block, (float *)d.out);
+  } else {
+    dloss_scale(a.scale);
   }
 }
 
@@ -222,9 +291,8 @@ __device__ __forceinline__ void sum_many(const DenseSum &d, unsigned block) {
 }
 __global__ __launch_bounds__(256) void k_sums(const DenseSums a) {
   __shared__ float s_sum[8][32];
-  unsigned block = blockIdx.x;
-  int j = 0;
-  while (block >= a.d[j].blocks) block -= a.d[j++].blocks;
+  const int j = job_of(a.end);
+  const unsigned block = blockIdx.x - (j ? a.end[j - 1] : 0);
   const DenseSum &d = a.d[j];
   if (d.bf16) return sum_many<true>(d, block);
   if (!d.few) return sum_many<false>(d, block);
@@ -237,51 +305,6 @@ __global__ __launch_bounds__(256) void k_sums(const DenseSums a) {
 #pragma unroll
     for (int k = 0; k < 8; k++) s += s_sum[k][threadIdx.x];
     ((float *)d.out)[i] = s;
-  }
-}
-
-// A block sums its rows (512, or up to 1024 if they are all) of 64 columns: 128 rows at a time by 8 threads
-// of 8 columns. Bound by its bytes; few rows stay without parts, whose sum would be another launch.
-template <bool BF>
-__global__ __launch_bounds__(1024) void k_colsum(const void *x, size_t T, size_t H, size_t rows, float *part) {
-  __shared__ float s_sum[16][64];
-  const int in = threadIdx.x % 8, row = threadIdx.x / 8;
-  const size_t c = (size_t)blockIdx.x * 64 + in * 8, t0 = (size_t)blockIdx.y * rows, t1 = min(T, t0 + rows);
-  float s[8] = {};
-  if (c < H) {  // (H is a multiple of 32)
-#pragma unroll 4
-    for (size_t t = t0 + row; t < t1; t += 128) {
-      float v[8];
-      if constexpr (BF) {
-        const uint4 u = *(const uint4 *)((const uint16_t *)x + t * H + c);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
-      } else {
-        const f32x4 *p = (const f32x4 *)((const float *)x + t * H + c);
-        const f32x4 a = p[0], b = p[1];
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 8; i++) s[i] += v[i];
-    }
-  }
-  // over the 8 rows of a wavefront, then over the wavefronts in order
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    s[i] += __shfl_xor(s[i], 8);
-    s[i] += __shfl_xor(s[i], 16);
-    s[i] += __shfl_xor(s[i], 32);
-    if (threadIdx.x % 64 < 8) s_sum[threadIdx.x / 64][in * 8 + i] = s[i];
-  }
-  __syncthreads();
-  const size_t o = (size_t)blockIdx.x * 64 + threadIdx.x;
-  if (threadIdx.x < 64 && o < H) {
-    float v = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 16; j++) v += s_sum[j][threadIdx.x];
-    part[blockIdx.y * H + o] = v;
   }
 }
 
@@ -389,10 +412,42 @@ unsigned blocks_for(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 25
 
 }  // namespace
 
-hipError_t launch_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n,
-                         const DlossScale *d, hipStream_t s) {
-  if (n % 4 || !n || (x1 && d)) return n ? hipErrorInvalidValue : hipSuccess;
-  k_planes<<<dim3(blocks_for(n / 4), x1 || d ? 2 : 1), 256, 0, s>>>(x0, out0, where0, x1, out1, where1, n, d ? *d : DlossScale{});
+namespace {
+// where the blocks of each job end; their number
+template <class J>
+size_t dense_ends(J &a) {
+  size_t blocks = 0;
+  for (int i = 0; i < (int)(sizeof(a.d) / sizeof(a.d[0])); i++) {
+    if (i < a.count) blocks += a.d[i].blocks;
+    a.end[i] = (unsigned)blocks;
+  }
+  return blocks;
+}
+}  // namespace
+
+void DenseRowJobs::planes(const float *x, uint16_t *out, uint32_t where, size_t n) {
+  if (n) d[count++] = DenseRows{ROWS_PLANES, x, out, n, 0, where, 0, blocks_for(n / 4)};
+}
+void DenseRowJobs::pack8(const float *x, size_t n, uint8_t *packed) {
+  if (n) d[count++] = DenseRows{ROWS_PACK8, x, packed, n, 0, 0, 0, (unsigned)((n / 8 + 255) / 256)};
+}
+void DenseRowJobs::unpack8(const uint8_t *packed, size_t n, uint16_t *out, int copies) {
+  if (n) d[count++] = DenseRows{ROWS_UNPACK8, packed, out, n, 0, 0, copies, (unsigned)((n / 8 + 255) / 256)};
+}
+void DenseRowJobs::column_sums(const void *x, bool bf16, size_t T, size_t H, float *out) {
+  d[count++] = DenseRows{bf16 ? ROWS_SUM_BF16 : ROWS_SUM_F32, x, out, T, H, 0, 0, (unsigned)((H + 63) / 64)};
+}
+void DenseRowJobs::dloss_scale(const DlossScale &s) {
+  scale = s;
+  d[count++] = DenseRows{ROWS_DLOSS_SCALE, nullptr, nullptr, 0, 0, 0, 0, 1};
+}
+hipError_t launch_rows(DenseRowJobs a, hipStream_t s) {
+  const size_t blocks = dense_ends(a);
+  if (blocks > 0xFFFFFF) return hipErrorInvalidValue;  // (2^32 threads)
+  if (a.count == 1 && a.d[0].what == ROWS_PLANES)
+    k_planes<<<(unsigned)blocks, 256, 0, s>>>(a.d[0]);
+  else if (blocks)
+    k_rows<<<(unsigned)blocks, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -400,10 +455,9 @@ void DenseSums::add(const float *part, size_t stride, int parts, size_t n, const
   const bool few = !bf16 && !bias && n <= 65536 && parts > 8;
   d[count++] = DenseSum{part, stride, n, n_bias, bias, out, parts, few ? (unsigned)((n + 31) / 32) : blocks_for(n), bf16, few};
 }
-hipError_t launch_sums(const DenseSums &a, hipStream_t s) {
-  unsigned blocks = 0;
-  for (int i = 0; i < a.count; i++) blocks += a.d[i].blocks;
-  if (blocks) k_sums<<<blocks, 256, 0, s>>>(a);
+hipError_t launch_sums(DenseSums a, hipStream_t s) {
+  const size_t blocks = dense_ends(a);
+  if (blocks) k_sums<<<(unsigned)blocks, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -423,15 +477,14 @@ hipError_t launch_dloss_scale(const DlossScale &d, hipStream_t s) {
   return hipGetLastError();
 }
 
-static size_t colsum_rows(size_t T) { return T <= 1024 ? 1024 : 512; }
-int dense_colsum_parts(size_t T) { return (int)((T + colsum_rows(T) - 1) / colsum_rows(T)); }
+int dense_colsum_parts(size_t T) { return (int)((T + kColRows - 1) / kColRows); }
 hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *part, hipStream_t s) {
   const dim3 grid((unsigned)((H + 63) / 64), (unsigned)dense_colsum_parts(T));
   if (!T || !H) return hipSuccess;
   if (bf16)
-    k_colsum<true><<<grid, 1024, 0, s>>>(x, T, H, colsum_rows(T), part);
+    k_colsum<<<grid, 1024, 0, s>>>((const uint16_t *)x, T, H, part);
   else
-    k_colsum<false><<<grid, 1024, 0, s>>>(x, T, H, colsum_rows(T), part);
+    k_colsum<<<grid, 1024, 0, s>>>((const float *)x, T, H, part);
   return hipGetLastError();
 }
 

@@ -112,10 +112,32 @@ struct DlossScale {
 };
 hipError_t launch_dloss_scale(const DlossScale &d, hipStream_t s);
 
-// x0 [n] f32 as kPlanes bf16 planes in the slots (n elements each) of `where0`; x1 (or NULL) likewise; or
-// beside x0 the scale d (or NULL), for few tokens.
-hipError_t launch_planes(const float *x0, uint16_t *out0, uint32_t where0, const float *x1, uint16_t *out1, uint32_t where1, size_t n,
-                         const DlossScale *d, hipStream_t s);
+// Work on rows in one launch.
+enum DenseRowsWhat { ROWS_PLANES, ROWS_PACK8, ROWS_UNPACK8, ROWS_SUM_BF16, ROWS_SUM_F32, ROWS_DLOSS_SCALE };
+struct DenseRows {
+  DenseRowsWhat what;
+  const void *x;
+  void *out;
+  size_t n, cols;
+  uint32_t where;
+  int copies;
+  unsigned blocks;
+};
+struct DenseRowJobs {
+  unsigned end[4];  // set by the launch
+  DenseRows d[4];
+  DlossScale scale{};
+  int count = 0;
+  // x [n] f32 as kPlanes bf16 planes in the slots (n elements each) of `where`
+  void planes(const float *x, uint16_t *out, uint32_t where, size_t n);
+  // f32 values as a checkpoint; one as bf16 values, `copies` of them one behind the other (act8.hip's forms)
+  void pack8(const float *x, size_t n, uint8_t *packed);
+  void unpack8(const uint8_t *packed, size_t n, uint16_t *out, int copies);
+  void column_sums(const void *x, bool bf16, size_t T, size_t H, float *out);  // dense_colsum_parts(T) == 1
+  void dloss_scale(const DlossScale &s);  // few tokens
+};
+hipError_t launch_rows(DenseRowJobs a, hipStream_t s);
+
 // out[i] = sum over parts of part[p * stride + i] (+ bias[i % n_bias]) for i < n, in order; bf16 or f32.
 struct DenseSum {
   const float *part;
@@ -128,11 +150,12 @@ struct DenseSum {
 };
 // Up to 5 of them in one launch (those that a backward pass of the gated block can need).
 struct DenseSums {
+  unsigned end[5];  // set by the launch
   DenseSum d[5];
   int count = 0;
   void add(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias, void *out, bool bf16);
 };
-hipError_t launch_sums(const DenseSums &a, hipStream_t s);
+hipError_t launch_sums(DenseSums a, hipStream_t s);
 // Column sums of x [T][H] (f32 or bf16) into parts [dense_colsum_parts(T)][H].
 int dense_colsum_parts(size_t T);
 hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *part, hipStream_t s);
@@ -142,8 +165,7 @@ hipError_t launch_loss(const float2 *stats, int parts, const float *picked, cons
 
 // MXFP8 activation checkpoints (act8.hip): codes [n][cols], then scales [n][cols / 32].
 hipError_t launch_act8_pack(const void *x, bool bf16, size_t n, size_t cols, uint8_t *packed, hipStream_t s);
-// (copies: of the values, one behind the other)
-hipError_t launch_act8_unpack(const uint8_t *packed, size_t n, size_t cols, void *out, bool bf16, int copies, hipStream_t s);
+hipError_t launch_act8_unpack(const uint8_t *packed, size_t n, size_t cols, void *out, bool bf16, hipStream_t s);
 
 // Device workspace of the dense operators: grows at need; a buffer that a captured graph may hold is
 // kept until the context goes.

@@ -136,9 +136,8 @@ Rows place(Carve &w, Rows r, const void *x, int dtype) {
   r.p = (const uint16_t *)x;
   return r;
 }
-int fill(const Rows &r, const void *x, int dtype, hipStream_t s, const DlossScale *d = nullptr) {
-  if (dtype == MOE_F32) HIP_TRY(launch_planes((const float *)x, r.out(), r.where, nullptr, nullptr, 0, r.slot(), d, s));
-  return MOE_OK;
+void fill(DenseRowJobs &jobs, const Rows &r, const void *x, int dtype) {
+  if (dtype == MOE_F32) jobs.planes((const float *)x, r.out(), r.where, r.slot());
 }
 
 // Weights times rows: D[m][n] = sum W[m][k] rows[n][k] (W [M][K], or [K][M] for a launch with A transposed),
@@ -274,7 +273,9 @@ int moe_lm_head_loss_device(moe_ctx *ctx, const void *x, int dtype, const int32_
     Rows piece = r;
     piece.n = n;
     if (dtype == MOE_BF16) piece.p += t0 * H;
-    RETURN_IF(fill(piece, (const char *)x + t0 * H * elem(dtype), dtype, s));
+    DenseRowJobs jobs;
+    fill(jobs, piece, (const char *)x + t0 * H * elem(dtype), dtype);
+    HIP_TRY(launch_rows(jobs, s));
     DenseArgs a = product(c.lm_w, H, piece, vocab);
     a.targets = targets + t0;
     a.stats = stats;
@@ -338,7 +339,10 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
   if (!beside) HIP_TRY(launch_dloss_scale(largest, s));
   for (size_t t0 = 0; t0 < T && !bf; t0 += Tc) {
     const size_t n = std::min(Tc, T - t0);
-    RETURN_IF(fill(piece(t0, n), (const float *)x + t0 * H, dtype, s, beside ? &largest : nullptr));
+    DenseRowJobs jobs;
+    fill(jobs, piece(t0, n), (const float *)x + t0 * H, dtype);
+    if (beside) jobs.dloss_scale(largest);
+    HIP_TRY(launch_rows(jobs, s));
   }
   int written = 0;  // parts of dx
   for (size_t v0 = 0; v0 < vocab; v0 += Vc) {
@@ -435,8 +439,11 @@ int moe_ffn_forward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int dt
       w = Carve{(char *)c.work->p};
     }
   }
-  if (x8) HIP_TRY(launch_act8_pack(x, dtype == MOE_BF16, T, H, x8, s));
-  RETURN_IF(fill(r, x, dtype, s));
+  DenseRowJobs jobs;
+  fill(jobs, r, x, dtype);
+  if (x8 && dtype == MOE_F32) jobs.pack8((const float *)x, T * H, x8);
+  if (x8 && dtype == MOE_BF16) HIP_TRY(launch_act8_pack(x, true, T, H, x8, s));
+  HIP_TRY(launch_rows(jobs, s));
   DenseArgs g = product(b->gate_up, H, r, 2 * I);
   g.bias = b->gate_up_bias;
   g.limit = c.clamp;
@@ -528,17 +535,23 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
     }
   }
   DenseSums sums;  // in one launch at the end
-  if (out->down_bias) {
+  DenseRowJobs jobs;
+  if (out->down_bias && col == out->down_bias) {
+    jobs.column_sums(dy, bf, T, H, col);
+  } else if (out->down_bias) {
     HIP_TRY(launch_colsum(dy, bf, T, H, col, s));
-    if (col != out->down_bias) sums.add(col, H, dense_colsum_parts(T), H, nullptr, 1, out->down_bias, false);
+    sums.add(col, H, dense_colsum_parts(T), H, nullptr, 1, out->down_bias, false);
   }
+  if (inner) {
+    if (x_type == MOE_MXFP8) jobs.unpack8((const uint8_t *)x, T * H, r.out(), r.slots);
+    if (dtype == MOE_F32) jobs.planes((const float *)dy, d.out(), d.where, T * H);
+    if (x_type == MOE_F32) jobs.planes((const float *)x, r.out(), r.where, T * H);
+  }
+  HIP_TRY(launch_rows(jobs, s));
   if (!inner) {
     HIP_TRY(launch_sums(sums, s));
     return MOE_OK;
   }
-  if (x_type == MOE_MXFP8) HIP_TRY(launch_act8_unpack((const uint8_t *)x, T, H, r.out(), true, r.slots, s));
-  if (dtype == MOE_F32)
-    HIP_TRY(launch_planes((const float *)dy, d.out(), d.where, x_type == MOE_F32 ? (const float *)x : nullptr, r.out(), r.where, T * H, nullptr, s));
   // gate and up as f32, their K parts side by side
   auto parts = [&](const DenseShape &shape, DenseArgs g, int splits, const float *bias, float *out) -> int {
     g.ldo = (size_t)g.M;
@@ -610,7 +623,7 @@ int moe_act8_unpack_device(moe_ctx *ctx, const uint8_t *packed, size_t n, size_t
   DenseCtx c;
   RETURN_IF(dense_ctx(ctx, &c));
   RETURN_IF(check_act8(packed, out, dtype, n, cols));
-  HIP_TRY(launch_act8_unpack(packed, n, cols, out, dtype == MOE_BF16, 1, stream ? (hipStream_t)stream : c.stream));
+  HIP_TRY(launch_act8_unpack(packed, n, cols, out, dtype == MOE_BF16, stream ? (hipStream_t)stream : c.stream));
   return MOE_OK;
 }
 
