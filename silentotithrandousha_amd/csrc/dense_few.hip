@@ -4,7 +4,8 @@
 // A workgroup takes 16 or 24 rows of A; its 8 wavefronts take the K-steps of 64 values in turn, each with the
 // loads of its next 6 steps under way, and their sums join in LDS, in order. Bound by the weights' bytes
 // and the latency of the first of them: one row of 2880 x 2880 weights (33 MB of gate and up, 16.6 MB
-// down) took 10.6 and 8.3 us (with the sum of its K parts) through the LDS rings of dense_gemm.hpp.
+// down) takes 9.4 and 5.5 us, both 14.5 with the launches (10.1 and 5.3 with 16 rows a workgroup for gate and up;
+// 10.6 and 8.3, with the sum of its K parts, through the LDS rings of dense_gemm.hpp).
 #include "dense_gemm.hpp"
 #include "dense_launch.hpp"
 

@@ -5,7 +5,8 @@
 namespace moe {
 
 // X(rows, columns, wavefronts along each, LDS slots, B's planes, workgroups of a CU, TFLOP/s of the device
-// full of them, planes counted). The rates are those of 2880 k values (loss over 201088 rows, 512 tokens and more).
+// full of them, planes counted). The rates are those of 2880 k values (loss over 201088 rows, 512 tokens and
+// more), with planes those of 2048 (loss of 100 and 333 rows over 50257).
 #define MOE_DENSE_TILES(X)            \
   X(288, 256, 2, 4, 2, 1, 1, 1180.0)  \
   X(256, 256, 2, 4, 2, 1, 1, 1290.0)  \

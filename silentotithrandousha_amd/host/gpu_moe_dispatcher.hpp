@@ -1,5 +1,5 @@
 // C++ host mirror of the reference's GpuMoeDispatcher (src/gpu/moe_dispatch.rs:36-684) over
-// the C ABI of libmxfp4moe.so (include/mxfp4_moe.h). Header-only; link -lmxfp4moe.
+// the C ABI of libmxfp4moe.so (include/mxfp4_moe.h, moe_dense.h). Header-only; link -lmxfp4moe.
 //
 // Same method names, argument meaning and error behaviour as the Rust type:
 //   * the constructor is the only fallible call and returns Result<GpuMoeDispatcher>
@@ -20,6 +20,7 @@
 #include <utility>
 #include <vector>
 
+#include "../../include/moe_dense.h"
 #include "../../include/mxfp4_moe.h"
 
 namespace silentot {
@@ -233,6 +234,28 @@ class GpuMoeDispatcher {
     std::vector<float> y(x.size());
     moe_check(moe_layer_forward(ctx_, layer, x.data(), x.size() / hidden_size_, top_k, y.data()));
     return y;
+  }
+
+  // The dense operators (include/moe_dense.h), on device pointers; stream nullptr = the context's.
+  void init_lm_head_bf16_device(const uint16_t *weights, size_t vocab_size, void *stream = nullptr) {
+    moe_check(moe_init_lm_head_bf16_device(ctx_, weights, vocab_size, stream));
+  }
+  void lm_head_loss_device(const void *x, moe_dtype dtype, const int32_t *targets, size_t T, size_t vocab, float *loss,
+                           float *lse, void *stream = nullptr) const {
+    moe_check(moe_lm_head_loss_device(ctx_, x, dtype, targets, T, vocab, loss, lse, stream));
+  }
+  void lm_head_loss_backward_device(const void *x, moe_dtype dtype, const int32_t *targets, const float *lse,
+                                    const float *dloss, size_t T, size_t vocab, void *dx, void *dw,
+                                    void *stream = nullptr) const {
+    moe_check(moe_lm_head_loss_backward_device(ctx_, x, dtype, targets, lse, dloss, T, vocab, dx, dw, stream));
+  }
+  void ffn_forward_device(const moe_ffn &block, const void *x, moe_dtype dtype, size_t T, void *y, uint8_t *x8 = nullptr,
+                          void *stream = nullptr) const {
+    moe_check(moe_ffn_forward_device(ctx_, &block, x, dtype, T, y, x8, stream));
+  }
+  void ffn_backward_device(const moe_ffn &block, const void *x, moe_dtype x_type, const void *dy, moe_dtype dtype, size_t T,
+                           const moe_ffn_grads &grads, void *stream = nullptr) const {
+    moe_check(moe_ffn_backward_device(ctx_, &block, x, x_type, dy, dtype, T, &grads, stream));
   }
 
  private:
