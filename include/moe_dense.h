@@ -11,7 +11,8 @@
  *
  * Types of activations and of their gradients (`dtype`): MOE_F32, the rows that the other calls of a
  * context take and return, or MOE_BF16. Weights are bf16, biases f32. Products accumulate in f32:
- * bf16 values enter as they are, f32 values as three bf16 terms (their 24 bits). The logits' gradient,
+ * bf16 values enter as they are, f32 values as three bf16 terms (their 24 bits; a finite value that rounds to bf16's infinity, above
+ * 3.39e38, as an infinity). The logits' gradient,
  * the activation h and the gradients of gate and up enter the products after them in `dtype`'s
  * precision: one bf16 rounding (2^-8 relative) for MOE_BF16, none that f32 would not make for MOE_F32.
  * Results do not depend on anything but the arguments' values and the shapes: no atomics.
@@ -45,7 +46,8 @@ enum moe_dtype {
 int moe_lm_head_loss_device(moe_ctx *ctx, const void *x, int dtype, const int32_t *targets, size_t n_tokens,
                             size_t vocab, float *loss, float *lse, void *stream);
 /* Its gradient: with p = exp(x . W - lse), d = dloss (p - [v = target]) (0 for ignored tokens):
- *   dx [n_tokens, H] = d W, dw [vocab, H] = d^T x, both of type `dtype`, either may be NULL.
+ *   dx [n_tokens, H] = d W, dw [vocab, H] = d^T x, both of type `dtype`, either may be NULL. The rows of
+ * ignored tokens may hold anything.
  * lse as moe_lm_head_loss_device returned it; dloss [n_tokens] f32, the gradient of each token's loss.
  * (dloss at tokens with a gradient has one scale: terms of d below 2^-126 of its largest magnitude may
  * count as 0; at the others it may hold anything.)

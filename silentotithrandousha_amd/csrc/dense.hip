@@ -160,11 +160,21 @@ __device__ __forceinline__ int job_of(const unsigned (&end)[N]) {
 // What a call does with its rows before its products, in one launch (each of its own cost 2 to 3 us): the
 // planes of f32 rows, a checkpoint written or read, the column sums of up to kColRows rows, the scale of dloss.
 // Bound by their bytes, of few rows by the launch.
+// Rows of ignored tokens enter the loss's products as zeros: 0 times what they hold would make a NaN of dw.
+__device__ __forceinline__ bool rows_ignored(const DenseRows &d, size_t i) {  // of value i
+  if (!d.targets) return false;
+  return d.targets[i >> 32 ? i / d.cols : (size_t)((uint32_t)i / (uint32_t)d.cols)] < 0;
+}
+__device__ __forceinline__ void rows_copy(const DenseRows &d, unsigned block) {
+  for (size_t i = ((size_t)block * 256 + threadIdx.x) * 8; i < d.n; i += (size_t)d.blocks * 2048)
+    *(uint4 *)((uint16_t *)d.out + i) = rows_ignored(d, i) ? uint4{0u, 0u, 0u, 0u} : *(const uint4 *)((const uint16_t *)d.x + i);
+}
 __device__ __forceinline__ void rows_planes(const DenseRows &d, unsigned block) {
   const float *x = (const float *)d.x;
   uint16_t *out = (uint16_t *)d.out;
   for (size_t i = ((size_t)block * 256 + threadIdx.x) * 4; i < d.n; i += (size_t)d.blocks * 1024) {  // (n is a multiple of 32)
-    const f32x4 v = *(const f32x4 *)(x + i);
+    f32x4 v = *(const f32x4 *)(x + i);
+    if (rows_ignored(d, i)) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     uint16_t p[4][kPlanes];
 #pragma unroll
     for (int j = 0; j < 4; j++) dense_split(v[j], p[j]);
@@ -243,6 +253,8 @@ __global__ __launch_bounds__(256) void k_rows(const DenseRowJobs a) {
   const size_t i = (size_t)block * 256 + threadIdx.x;  // of 8 values
   if (d.what == ROWS_PLANES) {
     rows_planes(d, block);
+  } else if (d.what == ROWS_COPY) {
+    rows_copy(d, block);
   } else if (d.what == ROWS_PACK8) {
     uint8_t *codes = (uint8_t *)d.out;
     if (i * 8 < d.n) act8_pack8((const float *)d.x, i, codes, codes + d.n);
@@ -427,21 +439,24 @@ size_t dense_ends(J &a) {
 }
 }  // namespace
 
-void DenseRowJobs::planes(const float *x, uint16_t *out, uint32_t where, size_t n) {
-  if (n) d[count++] = DenseRows{ROWS_PLANES, x, out, n, 0, where, 0, blocks_for(n / 4)};
+void DenseRowJobs::planes(const float *x, uint16_t *out, uint32_t where, size_t n, const int32_t *targets, size_t cols) {
+  if (n) d[count++] = DenseRows{ROWS_PLANES, x, out, n, cols, where, 0, blocks_for(n / 4), targets};
+}
+void DenseRowJobs::copy(const uint16_t *x, uint16_t *out, size_t n, const int32_t *targets, size_t cols) {
+  if (n) d[count++] = DenseRows{ROWS_COPY, x, out, n, cols, 0, 0, blocks_for(n / 8), targets};
 }
 void DenseRowJobs::pack8(const float *x, size_t n, uint8_t *packed) {
-  if (n) d[count++] = DenseRows{ROWS_PACK8, x, packed, n, 0, 0, 0, (unsigned)((n / 8 + 255) / 256)};
+  if (n) d[count++] = DenseRows{ROWS_PACK8, x, packed, n, 0, 0, 0, (unsigned)((n / 8 + 255) / 256), nullptr};
 }
 void DenseRowJobs::unpack8(const uint8_t *packed, size_t n, uint16_t *out, int copies) {
-  if (n) d[count++] = DenseRows{ROWS_UNPACK8, packed, out, n, 0, 0, copies, (unsigned)((n / 8 + 255) / 256)};
+  if (n) d[count++] = DenseRows{ROWS_UNPACK8, packed, out, n, 0, 0, copies, (unsigned)((n / 8 + 255) / 256), nullptr};
 }
 void DenseRowJobs::column_sums(const void *x, bool bf16, size_t T, size_t H, float *out) {
-  d[count++] = DenseRows{bf16 ? ROWS_SUM_BF16 : ROWS_SUM_F32, x, out, T, H, 0, 0, (unsigned)((H + 63) / 64)};
+  d[count++] = DenseRows{bf16 ? ROWS_SUM_BF16 : ROWS_SUM_F32, x, out, T, H, 0, 0, (unsigned)((H + 63) / 64), nullptr};
 }
 void DenseRowJobs::dloss_scale(const DlossScale &s) {
   scale = s;
-  d[count++] = DenseRows{ROWS_DLOSS_SCALE, nullptr, nullptr, 0, 0, 0, 0, 1};
+  d[count++] = DenseRows{ROWS_DLOSS_SCALE, nullptr, nullptr, 0, 0, 0, 0, 1, nullptr};
 }
 hipError_t launch_rows(DenseRowJobs a, hipStream_t s) {
   const size_t blocks = dense_ends(a);

@@ -113,7 +113,7 @@ struct DlossScale {
 hipError_t launch_dloss_scale(const DlossScale &d, hipStream_t s);
 
 // Work on rows in one launch.
-enum DenseRowsWhat { ROWS_PLANES, ROWS_PACK8, ROWS_UNPACK8, ROWS_SUM_BF16, ROWS_SUM_F32, ROWS_DLOSS_SCALE };
+enum DenseRowsWhat { ROWS_PLANES, ROWS_COPY, ROWS_PACK8, ROWS_UNPACK8, ROWS_SUM_BF16, ROWS_SUM_F32, ROWS_DLOSS_SCALE };
 struct DenseRows {
   DenseRowsWhat what;
   const void *x;
@@ -122,6 +122,7 @@ struct DenseRows {
   uint32_t where;
   int copies;
   unsigned blocks;
+  const int32_t *targets;  // of rows of `cols`, or NULL: rows of negative ones as zeros
 };
 struct DenseRowJobs {
   unsigned end[4];  // set by the launch
@@ -129,7 +130,9 @@ struct DenseRowJobs {
   DlossScale scale{};
   int count = 0;
   // x [n] f32 as kPlanes bf16 planes in the slots (n elements each) of `where`
-  void planes(const float *x, uint16_t *out, uint32_t where, size_t n);
+  void planes(const float *x, uint16_t *out, uint32_t where, size_t n, const int32_t *targets = nullptr, size_t cols = 0);
+  // bf16 values
+  void copy(const uint16_t *x, uint16_t *out, size_t n, const int32_t *targets, size_t cols);
   // f32 values as a checkpoint; one as bf16 values, `copies` of them one behind the other (act8.hip's forms)
   void pack8(const float *x, size_t n, uint8_t *packed);
   void unpack8(const uint8_t *packed, size_t n, uint16_t *out, int copies);

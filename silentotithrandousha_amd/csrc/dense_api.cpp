@@ -66,6 +66,11 @@ int ensure(const DenseCtx &c, size_t bytes, hipStream_t s) {
   HIP_TRY(hipStreamIsCapturing(s, &cap));
   const bool capturing = cap != hipStreamCaptureStatusNone;
   if (bytes > w.cap) {
+    try {  // (room to keep the old one, before there is anything to undo)
+      w.kept.reserve(w.kept.size() + 1);
+    } catch (...) {
+      return fail(MOE_ERR_OOM, "out of host memory");
+    }
     if (capturing)
       return fail(MOE_ERR_STATE, "workspace too small for this call during graph capture; run it once uncaptured first");
     void *q = nullptr;
@@ -308,11 +313,13 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
   // few tokens: dx from K splits of every piece of the vocabulary, summed at the end; many: added up
   const int splits = dense_splits(sx, product(c.lm_w, H, rows_of(dtype, kWhereRight, Tc, Vc, ld), H));
   const bool parts = dx && splits > 1 && nt == 1;
+  const bool masked = !bf || dw;  // the rows in the workspace, those of ignored tokens as zeros
   Carve w;
   Rows r, dl;
   float *dx_acc = nullptr, *dw_acc = nullptr, *scale = nullptr;
   for (int placed = 0; placed < 2; placed++) {
-    r = place(w, rows_of(dtype, kWhereLeft, T, H, H), x, dtype);  // (f32: the slots of each piece of tokens together)
+    r = rows_of(dtype, kWhereLeft, T, H, H);
+    r = masked ? place(w, r) : place(w, r, x, dtype);  // (f32: the slots of each piece of tokens together)
     scale = w.take<float>(1);
     dl = place(w, rows_of(dtype, kWhereRight, Tc, Vc, ld));
     if (parts)
@@ -335,12 +342,16 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
   // mean's constant dloss the entries of the targets, which weigh most, then lie next to -1 and are rounded
   // by their p alone, where bf16(1 / n) would put one error into all of them.
   const DlossScale largest{dloss, targets, T, (int)vocab, scale};
-  const bool beside = !bf && T <= 1024;  // in the launch of the rows' planes
+  const bool beside = masked && T <= 1024;  // in the launch that prepares the rows
   if (!beside) HIP_TRY(launch_dloss_scale(largest, s));
-  for (size_t t0 = 0; t0 < T && !bf; t0 += Tc) {
+  for (size_t t0 = 0; t0 < T && masked; t0 += Tc) {
     const size_t n = std::min(Tc, T - t0);
+    const Rows p = piece(t0, n);
     DenseRowJobs jobs;
-    fill(jobs, piece(t0, n), (const float *)x + t0 * H, dtype);
+    if (bf)
+      jobs.copy((const uint16_t *)x + t0 * H, p.out(), n * H, targets + t0, H);
+    else
+      jobs.planes((const float *)x + t0 * H, p.out(), p.where, n * H, targets + t0, H);
     if (beside) jobs.dloss_scale(largest);
     HIP_TRY(launch_rows(jobs, s));
   }

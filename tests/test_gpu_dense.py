@@ -241,11 +241,14 @@ def test_loss_not_finite(dtype):
         assert np.isnan(got[[3, 8]]).all()
         rest = np.delete(np.arange(T), [3, 8])
         ref.assert_close(got[rest], clean.loss[rest], clean.loss_tol[rest], "loss")
-        targets[[3, 8]] = -1  # ignored, the same rows add nothing to dx; dw takes 0 * NaN from x
+        targets[[3, 8]] = -1  # ignored, the same rows add nothing
+        clean = ref.Loss(xv, wv, targets, dloss.astype(np.float64), dtype)
         xd, td, loss, lse = run_loss(d, x, dtype, targets, V)
-        dx, _ = run_loss_backward(d, xd, dtype, td, lse, dloss, T, H, V, dw=False)
-        assert (loss.get()[[3, 8]] == 0).all() and (dx.get()[[3, 8]] == 0).all()
-        ref.assert_close(dx.get()[rest], clean.dx[rest], clean.dx_tol[rest], "dx")
+        for with_dw in (False, True):
+            dx, dw = run_loss_backward(d, xd, dtype, td, lse, dloss, T, H, V, dw=with_dw)
+            assert (loss.get()[[3, 8]] == 0).all() and (dx.get()[[3, 8]] == 0).all()
+            ref.assert_close(dx.get()[rest], clean.dx[rest], clean.dx_tol[rest], "dx")
+        ref.assert_close(dw.get(), clean.dw, clean.dw_tol, "dw")
     finally:
         d.close()
 
@@ -525,6 +528,87 @@ def test_act8_not_finite(dtype):
         d.synchronize()
         assert np.array_equal(packed.download(np.uint8, (4 * 96 + 12,))[4 * 96:].reshape(4, 3), scales)
         assert np.array_equal(out.get(), values, equal_nan=True) and np.isnan(values).sum() == 96
+    finally:
+        d.close()
+
+
+# ------------------------------------------------------------------ the largest sizes
+
+
+def tail(buf, dtype, rows, cols, count):
+    """The last `count` rows of a device matrix: (bits, values in 64 bits)."""
+    el = 4 if dtype == MOE_F32 else 2
+    out = np.empty((count, cols), np.float32 if dtype == MOE_F32 else np.uint16)
+    check(lib().moe_memcpy_d2h(out.ctypes.data, buf.ptr + (rows - count) * cols * el, out.nbytes))
+    return out, out.astype(np.float64) if dtype == MOE_F32 else ref.from_bf16(out).astype(np.float64)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_past_32_bits(dtype):
+    """2^20 tokens of 2080 values: offsets past 2^32 bytes and 2^31 values. Loss, block and their dx in the last rows."""
+    T, H, V, I, n = 2**20, 2080, 24, 8, 70  # noqa: E741
+    el = 4 if dtype == MOE_F32 else 2
+    rng = np.random.default_rng(12)
+    w, wv = ref.rows(rng, (V, H), MOE_BF16, 2 / np.sqrt(H))
+    c = block_case(dtype, 1, H, I, seed=13)
+    targets = rng.integers(-1, V, T).astype(np.int32)
+    dloss = rng.uniform(-1, 1, T).astype(np.float32)
+    d = context(H, w)
+    try:
+        x, out = DeviceBuffer(T * H * el), DeviceBuffer(T * H * el)
+        check(lib().moe_synth_fill_device(x.ptr, T * H, 2 if dtype == MOE_F32 else 1, 1, 1.0, 0.0, None))
+        check(lib().moe_synchronize(d.ctx))
+        td, gd, loss, lse = dev(targets), dev(dloss), Out((T,), MOE_F32), Out((T,), MOE_F32)
+        xv = tail(x, dtype, T, H, n)[1]
+        want = ref.Loss(xv, wv, targets[-n:], dloss[-n:].astype(np.float64), dtype)
+        d.lm_head_loss_device(x, dtype, td, T, V, loss, lse)
+        d.lm_head_loss_backward_device(x, dtype, td, lse, gd, T, V, out, None)
+        d.synchronize()
+        ref.assert_close(lse.get()[-n:], want.lse, want.lse_tol, "lse")
+        ref.assert_close(loss.get()[-n:], want.loss, want.loss_tol, "loss")
+        ref.assert_close(tail(out, dtype, T, H, n)[1], want.dx, want.dx_tol, "dx")
+        b = BlockOnDevice(c)
+        c = dict(c, x=(None, xv), dy=(None, xv))
+        want = block_ref(c, dtype)
+        d.ffn_forward_device(b.block, x, dtype, T, out)
+        d.synchronize()
+        ref.assert_close(tail(out, dtype, T, H, n)[1], want.y, want.y_tol, "y")
+        d.ffn_backward_device(b.block, x, dtype, x.ptr, dtype, T, GatedFfnGrads(out.ptr))
+        d.synchronize()
+        ref.assert_close(tail(out, dtype, T, H, n)[1], want.dx, want.dx_tol, "dx")
+    finally:
+        d.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_most_tokens(dtype):
+    """Every gradient over 2^20 tokens, ten of which have one: the others' dloss and dy are zero, so that the sums
+    are those of ten."""
+    T, H, V, I = 2**20, 32, 5, 8  # noqa: E741
+    at = np.array([0, 1, 8191, 8192, 16384, 65535, 65536, 500000, T - 2, T - 1])
+    x, xv, w, wv, targets, dloss = loss_case(dtype, T, H, V, seed=14)
+    targets = np.abs(targets)
+    dloss[np.isin(np.arange(T), at, invert=True)] = 0.0
+    c = block_case(dtype, T, H, I, seed=15)
+    dy = np.zeros((T, H), c["dy"][0].dtype)
+    dy[at] = c["dy"][0][at]
+    c["dy"] = (dy, None)
+    d = context(H, w)
+    try:
+        xd, td, loss, lse = run_loss(d, x, dtype, targets, V)
+        dx, dw = run_loss_backward(d, xd, dtype, td, lse, dloss, T, H, V)
+        want = ref.Loss(xv[at], wv, targets[at], dloss[at].astype(np.float64), dtype)
+        ref.assert_close(loss.get()[at], want.loss, want.loss_tol, "loss")
+        ref.assert_close(dx.get()[at], want.dx, want.dx_tol, "dx")
+        ref.assert_close(dw.get(), want.dw, want.dw_tol, "dw")
+        b = BlockOnDevice(c)
+        g = b.backward(d, dtype)
+        d.synchronize()
+        few = dict(c, x=(None, c["x"][1][at]), dy=(None, dy[at].astype(np.float64) if dtype == MOE_F32 else ref.from_bf16(dy[at]).astype(np.float64)))
+        want = block_ref(few, dtype)
+        ref.assert_close(g["x"].get()[at], want.dx, want.dx_tol, "dx")
+        g.pop("x")
+        check_grads(g, want)
     finally:
         d.close()
 
