@@ -39,6 +39,9 @@ double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a,
     double step = std::max(0.52 / (d.ns - 1) + 0.12, on_cu * d.bm * d.bn * 2.0 * kDenseStep * d.planes * kCus / (d.rate * 1e6));
     if (tiles_n == 1) step = std::max(step, on_cu * d.bm * 128e-3 / memory);
     const double stores = on_cu * d.bm * d.bn * result * kCus / 4.5e6;  // us at 4.5 TB/s
+    // f32 weight gradients of few rows, bound by their stores: of two workgroups a CU one stores while the other
+    // starts (19 rows, 32003 x 1024: 128 x 128 31.7 us, 256 x 256 34.3; bf16 rows of such tiles, 256 bytes, went slower)
+    if (s.bt && a.out_mode && d.bn == 128 && on_cu == d.wgs && stores > 2.0 * steps * step) return std::max(steps * step + 2.5, stores);
     return steps * step + 2.5 + stores;
   };
   const long whole = tiles / (kCus * d.wgs), rest = tiles - whole * kCus * d.wgs;
