@@ -1,11 +1,11 @@
 // The dense products of few rows (up to 8, a row's planes counted): the weights stream once through
 // registers, no LDS.
 //
-// A workgroup takes 16 or 24 rows of A; its 8 wavefronts take the K-steps of 64 values in turn, each with the
+// A workgroup takes 8 to 24 rows of A; its 8 wavefronts take the K-steps of 64 values in turn, each with the
 // loads of its next 6 steps under way, and their sums join in LDS, in order. Bound by the weights' bytes
 // and the latency of the first of them: one row of 2880 x 2880 weights (33 MB of gate and up, 16.6 MB
-// down) takes 9.4 and 5.5 us, both 14.5 with the launches (10.1 and 5.3 with 16 rows a workgroup for gate and up;
-// 10.6 and 8.3, with the sum of its K parts, through the LDS rings of dense_gemm.hpp).
+// down) takes 9.0 and 4.9 us, both 13.3 with the launches (10.1 and 5.5, 15.0, with 16 rows a workgroup; 10.6 and
+// 8.3, with the sum of its K parts, through the LDS rings of dense_gemm.hpp).
 #include "dense_gemm.hpp"
 #include "dense_launch.hpp"
 
@@ -22,8 +22,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_dense_few(const DenseArgs a) {
   const int m0 = blockIdx.x * ROWS, rows_b = a.N * a.stack, at = lane >> 4;
   const uint16_t *A[kTiles], *B = a.B + (size_t)min(lane & 15, rows_b - 1) * a.ldb;
 #pragma unroll
-  for (int t = 0; t < kTiles; t++)  // (of a half tile the lanes' second half reads the first's rows)
-    A[t] = a.A + (size_t)min(m0 + t * 16 + (lane & (ROWS - t * 16 < 16 ? 7 : 15)), a.M - 1) * a.lda;
+  for (int t = 0; t < kTiles; t++)  // (of a part of a tile the lanes past it read its last row)
+    A[t] = a.A + (size_t)min(m0 + min(t * 16 + (lane & 15), ROWS - 1), a.M - 1) * a.lda;
   const int steps = (a.K + kDenseStep - 1) / kDenseStep;
   f32x4 acc[kTiles];
 #pragma unroll
@@ -108,11 +108,17 @@ bool dense_few_fits(const DenseShape &s, const DenseArgs &a) {
 
 hipError_t launch_dense_few(const DenseShape &s, const DenseArgs &a, hipStream_t st) {
   if (!dense_few_fits(s, a)) return hipErrorInvalidValue;
-  // 24 rows where those fit the CUs once and 16 do not: the CUs that took two workgroups of 16 were waited for
-  if (a.M > 16 * 256 && a.M <= 24 * 256)
-    launch_few<24>(s, a, st);
-  else
+  // the fewest rows that fit the CUs once: where some CUs take two workgroups they are waited for (5760 rows of
+  // weights by 16: 10.1 us, by 24: 9.4), and where many take none the others have the more to read
+  const int rows = (a.M + 255) / 256;
+  if (rows <= 8)
+    launch_few<8>(s, a, st);
+  else if (rows <= 12)
+    launch_few<12>(s, a, st);
+  else if (rows <= 16 || rows > 24)
     launch_few<16>(s, a, st);
+  else
+    launch_few<24>(s, a, st);
   return hipGetLastError();
 }
 

@@ -791,16 +791,16 @@ def same(a, b):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_steps_in_graphs(dtype):
+@pytest.mark.parametrize("H,I,V,tokens", [(64, 72, 300, (20, 33, 150)), (160, 520, 1500, (130, 3, 600))])
+def test_steps_in_graphs(dtype, H, I, V, tokens):  # noqa: E741
     """Two captured steps of different sizes on one context, replayed in turn with eager work between them
     and with the workspace grown after their capture: every replay gives the eager bits."""
-    H, I, V = 64, 72, 300  # noqa: E741
     w = loss_case(dtype, 1, H, V)[2]
     d = context(H, w)
     graphs = []
     try:
-        steps = [Step(d, dtype, 20, H, I, V, 1), Step(d, dtype, 33, H, I, V, 2)]
-        refused_first = Step(d, dtype, 20, H, I, V, 1)
+        steps = [Step(d, dtype, tokens[0], H, I, V, 1), Step(d, dtype, tokens[1], H, I, V, 2)]
+        refused_first = Step(d, dtype, tokens[0], H, I, V, 1)
         with pytest.raises(MoeError) as e:  # the workspace has no size yet
             with Capture(d) as g:
                 refused_first.enqueue()
@@ -816,7 +816,7 @@ def test_steps_in_graphs(dtype):
             with Capture(d) as g:
                 s.enqueue()
             graphs.append(g.graph)
-        large = Step(d, dtype, 150, H, I, V, 3)
+        large = Step(d, dtype, tokens[2], H, I, V, 3)
         for rep in range(3):
             for s, g, want in zip(steps, graphs, eager):
                 s.clear()
