@@ -403,6 +403,34 @@ def test_block_clamps(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_block_far_below_the_clamp(dtype):
+    """Gates of -3e38 close: that token's h and gradients are 0, and the others' results are theirs alone."""
+    T, H, I = 3, 32, 16  # noqa: E741
+    c = block_case(dtype, T, H, I, seed=8, bias=False)
+    wgu = np.zeros((2 * I, H), np.float32)
+    for i in range(I):
+        wgu[2 * i, i], wgu[2 * i + 1, 16 + i] = 1.0, 1.0
+    c["wgu"] = ref.store(wgu, MOE_BF16)
+    x = c["x"][1].astype(np.float32)
+    x[1, :16] = -3e38
+    c["x"] = ref.store(x, dtype)
+    rest = [0, 2]
+    want = block_ref(dict(c, x=(None, c["x"][1][rest]), dy=(None, c["dy"][1][rest])), dtype)
+    want.dbd, want.dbd_tol = c["dy"][1].sum(0), (T + 1) * 2.0 ** -24 * np.abs(c["dy"][1]).sum(0)
+    d = context(H)
+    try:
+        b = BlockOnDevice(c, bias=False)
+        y, g = b.forward(d, dtype), b.backward(d, dtype)
+        d.synchronize()
+        assert (y.get()[1] == 0).all() and (g["x"].get()[1] == 0).all()
+        ref.assert_close(y.get()[rest], want.y, want.y_tol, "y")
+        ref.assert_close(g.pop("x").get()[rest], want.dx, want.dx_tol, "dx")
+        check_grads(g, want)
+    finally:
+        d.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("skip", [("x",), ("gate_up", "gate_up_bias"), ("x", "gate_up", "gate_up_bias", "down"),
                                   ("x", "down", "down_bias"), ("x", "gate_up", "gate_up_bias", "down", "down_bias")])
 def test_block_some_gradients(dtype, skip):
