@@ -41,10 +41,12 @@ __device__ __forceinline__ void dense_split(float v, uint16_t (&p)[kPlanes]) {
   p[2] = dense_bf16(r - bf16_to_f32(p[1]));
 }
 
-// exp(t) as 2^(t log2 e), the product in two parts so that a large |t| costs no bits.
+// exp(t) as 2^(t log2 e), the product in two parts so that a large |t| costs no bits. The second part is far
+// below 1 wherever the result is neither 0 nor infinite; past that it is bounded, as 2^a alone is the result there
+// (above 2.36e38 the first part overflows and the second is infinite, for an infinite t it is NaN).
 __device__ __forceinline__ float dense_exp(float t) {
   const float a = t * 1.4426950408889634f;
-  const float b = fmaxf(fmaf(t, 1.4426950408889634f, -a) + t * 1.925963e-8f, -1.0f);  // (NaN for an infinite t)
+  const float b = fminf(fmaxf(fmaf(t, 1.4426950408889634f, -a) + t * 1.925963e-8f, -1.0f), 1.0f);
   return __builtin_amdgcn_exp2f(a) * fmaf(b, 0.6931471805599453f, 1.0f);
 }
 
@@ -615,13 +617,14 @@ __device__ __forceinline__ void dense_tile_product(const DenseArgs &a, int block
       }
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      // no value above minus infinity: every exponential is 0 against a base of 0
-      const float base = (mx == -INFINITY ? 0.0f : mx) * 1.4426950408889634f;
+      // no value above minus infinity: every exponential is 0 against a base of 0. (The difference before the
+      // factor log2 e: a maximum above 2.36e38 would overflow with it.)
+      const float base = mx == -INFINITY ? 0.0f : mx;
       float sum = 0.0f;  // (a NaN among the logits makes it one)
 #pragma unroll
       for (int i = 0; i < TM; i++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], 1.4426950408889634f, -base));
+        for (int r = 0; r < 4; r++) sum += dense_exp_near(acc[i][j][r] - base);
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
       if (lane < 16 && n < a.N) a.stats[(size_t)(tile_m * WM + wm) * a.N + n] = make_float2(mx, sum);
