@@ -67,7 +67,7 @@ struct DenseGate {
   __device__ __forceinline__ float h() const { return (U + 1.0f) * (G * s); }
   // d loss / d(g, u) from dh = d loss / d h: nothing passes a clamp
   __device__ __forceinline__ float dg(float dh, float g, float limit) const {
-    return g > limit ? 0.0f : dh * (U + 1.0f) * (s + 1.702f * (G * s) * (1.0f - s));  // (G s is 0 where G (1 - s) overflows)
+    return g > limit ? 0.0f : dh * (U + 1.0f) * (s + 1.702f * ((G * s) * (1.0f - s)));  // (G s is 0 where G (1 - s) overflows, 1 - s where 1.702 G s does)
   }
   __device__ __forceinline__ float du(float dh, float u, float limit) const { return fabsf(u) > limit ? 0.0f : dh * (G * s); }
 };

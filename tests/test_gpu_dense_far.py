@@ -1,10 +1,11 @@
-"""The dense operators at the far ends of f32's range: logits whose exponents overflow a factor log2 e, against 64-bit results (tests/dense_ref.py)."""
+"""The dense operators at the far ends of f32's range: logits, gates and clamps whose exponents overflow a
+factor log2 e, against 64-bit results (tests/dense_ref.py)."""
 import numpy as np
 import pytest
 
-from silentotithrandousha_amd import MOE_BF16, MOE_F32
+from silentotithrandousha_amd import MOE_BF16, MOE_F32, GpuMoeDispatcher
 from tests import dense_ref as ref
-from tests.test_gpu_dense import context, run_loss, run_loss_backward
+from tests.test_gpu_dense import BlockOnDevice, block_case, block_ref, check_grads, context, run_loss, run_loss_backward
 
 pytestmark = pytest.mark.gpu
 
@@ -79,5 +80,40 @@ def test_loss_far_above(dtype, T, V, first):
         assert lse.get()[t] == FAR and loss.get()[t] == FAR  # (log 400 and the target's logit are below its half step)
         dx, dw = run_loss_backward(d, xd, dtype, td, lse, dloss, T, H, V)
         assert np.isfinite(dx.get()).all() and np.isfinite(dw.get()).all()
+    finally:
+        d.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1, 5, 40, 300])
+def test_block_far_clamp(dtype, T, monkeypatch):
+    """A clamp of 3e38 and gates of +-2.6e38 below it (ups of -1/2, so that h stays in range): h is (U + 1) G there and 0
+    for the negative ones, the gate's gradient dh (U + 1) and 0."""
+    H, I = 32, 16  # noqa: E741
+    monkeypatch.setattr(ref, "CLAMP", 3e38)
+    c = block_case(dtype, T, H, I, seed=3, bias=False)
+    wgu = np.zeros((2 * I, H), np.float32)
+    for i in range(I):
+        wgu[2 * i, i], wgu[2 * i + 1, 16 + i] = 1.0, 1.0
+    c["wgu"] = ref.store(wgu, MOE_BF16)
+    c["wd"] = ref.store((ref.from_bf16(c["wd"][0]) * 2.0 ** -30).astype(np.float32), MOE_BF16)
+    c["dy"] = ref.store((c["dy"][1] * 2.0 ** -30).astype(np.float32), dtype)
+    x = np.array(c["x"][1], np.float32)
+    x[:, 16:] = -0.5
+    x[T // 2, :16] = np.where(np.arange(16) % 2, FAR, -FAR)
+    c["x"] = ref.store(x, dtype)
+    with np.errstate(over="ignore"):  # exp of 1.702 times the far negative gates
+        want = block_ref(c, dtype)
+    d = GpuMoeDispatcher(H, 32, 3e38)
+    try:
+        b = BlockOnDevice(c, bias=False)
+        y, g = b.forward(d, dtype), b.backward(d, dtype)
+        d.synchronize()
+        ref.assert_close(y.get(), want.y, want.y_tol, "y")
+        # an up's gradient times the far x is past f32's range (dh of 2^-60 times 2^254): those entries are not compared
+        inside, got = np.abs(want.dwgu) < 2.0 ** 127, g.pop("gate_up").get()
+        assert not inside.all() and inside.mean() > 0.5
+        ref.assert_close(got[inside], want.dwgu[inside], want.dwgu_tol[inside], "gate_up")
+        check_grads(g, want)
     finally:
         d.close()
