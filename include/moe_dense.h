@@ -11,9 +11,9 @@
  *
  * Types of activations and of their gradients (`dtype`): MOE_F32, the rows that the other calls of a
  * context take and return, or MOE_BF16. Weights are bf16, biases f32. Products accumulate in f32:
- * bf16 values enter as they are, f32 values as three bf16 terms (their 24 bits; a finite value that rounds to bf16's infinity, above
- * 3.39e38, as an infinity). The logits' gradient,
- * the activation h and the gradients of gate and up enter the products after them in `dtype`'s
+ * bf16 values enter as they are, f32 values as three bf16 terms (their 24 bits, as far as those lie above 2^-126; a finite value
+ * that rounds to bf16's infinity, above 3.39e38, as an infinity). An infinity or NaN among the rows makes of the results what it does in
+ * f32; an infinite weight makes NaN of the results of f32 rows that it enters. The logits' gradient, the activation h and the gradients of gate and up enter the products after them in `dtype`'s
  * precision: one bf16 rounding (2^-8 relative) for MOE_BF16, none that f32 would not make for MOE_F32.
  * Results do not depend on anything but the arguments' values and the shapes: no atomics.
  *

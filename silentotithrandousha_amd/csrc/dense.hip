@@ -183,8 +183,8 @@ __device__ __forceinline__ void rows_planes(const DenseRows &d, unsigned block) 
     for (int j = 0; j < 4; j++) dense_split(v[j], p[j]);
 #pragma unroll
     for (int k = 0; k < kPlanes; k++) {
-      const uint2 q = {p[0][k] | (uint32_t)p[1][k] << 16, p[2][k] | (uint32_t)p[3][k] << 16};
-      dense_slots(d.where, k, [&](size_t at) { *(uint2 *)(out + at * d.n + i) = q; });
+      uint16_t q[4] = {p[0][k], p[1][k], p[2][k], p[3][k]};
+      dense_slots<false>(d.where, k, q, [&](size_t at, const auto &q) { *(uint2 *)(out + at * d.n + i) = __builtin_bit_cast(uint2, q); });
     }
   }
 }
@@ -366,8 +366,8 @@ __global__ __launch_bounds__(256) void k_dgate(const DgateArgs a) {
         uint16_t q[8], e[4];
         dense_take<!ONE>(d, q);
         dense_take<!ONE>(hv, e);
-        dense_slots(a.dgu_where, p, [&](size_t at) { *(uint4 *)(a.dgu + at * 2 * plane + t * 2 * a.I + 2 * i) = __builtin_bit_cast(uint4, q); });
-        dense_slots(a.h_where, p, [&](size_t at) { *(uint2 *)(a.h + at * plane + t * a.I + i) = __builtin_bit_cast(uint2, e); });
+        dense_slots<ONE>(a.dgu_where, p, q, [&](size_t at, const auto &q) { *(uint4 *)(a.dgu + at * 2 * plane + t * 2 * a.I + 2 * i) = __builtin_bit_cast(uint4, q); });
+        dense_slots<ONE>(a.h_where, p, e, [&](size_t at, const auto &e) { *(uint2 *)(a.h + at * plane + t * a.I + i) = __builtin_bit_cast(uint2, e); });
       }
     }
   }

@@ -14,11 +14,16 @@ namespace moe {
 // the workspace as slots [slot][rows][cols], each a plane: `where` holds in byte p the slots of plane p.
 // The product of two such matrices over their rows (a weight gradient) leaves out the planes' products
 // below 2^-24 of the largest and takes the other six as one product over 6 times the rows: its left
-// operand's slots hold the planes 0 1 2 0 1 0, its right one's 2 1 0 1 0 0. (As six passes over K, each with
+// operand's slots hold the planes 0 0 1 1 2 0, its right one's 1 2 0 1 0 0. (As six passes over K, each with
 // a K tail of its own, the gradient of the LM head for 19 rows took 54 us.)
+// A value that is not finite (or is not as bf16) is plane 0 alone, and in the last slot of that plane alone, 0 in
+// the others: met with the other operand's lower planes, which may be 0 or of the other sign, an infinity would
+// become NaN. So the last slots of plane 0 meet each other, and the products that read one slot of each plane
+// take the last ones: 5 3 4 (left) and 5 3 1 (right), of three slots 2 1 0.
 constexpr int kPlanes = 3;
 constexpr int kPairs6 = 6;
-constexpr uint32_t kWhereOne = 0x01, kWhereThree = 0x040201, kWhereLeft = 0x041229, kWhereRight = 0x010A34;
+constexpr uint32_t kWhereOne = 0x01, kWhereThree = 0x010204, kWhereLeft = 0x100C23, kWhereRight = 0x020934;
+constexpr int dense_last_slot(uint32_t where, int plane) { return 31 - __builtin_clz(where >> 8 * plane & 255); }
 
 // Epilogues.
 enum DenseEpi {
@@ -39,6 +44,7 @@ struct DenseArgs {
   size_t lda, ldb;          // elements between rows of the stored matrix
   int M, N, K;
   int stack;                // slots of B that are taken as rows [slot][N] (N * stack <= 64), else 1
+  int stack_step;           // from one of these slots to the next: 1 or 2
   int b_planes;             // slots of B that meet A's values in turn: 1, or kPlanes
   uint32_t pb;              // those slots, 4 bits each, in the order of their products
   int splits;               // K split (DENSE_STORE with f32 only): out + split * split_stride

@@ -146,7 +146,7 @@ void fill(DenseRowJobs &jobs, const Rows &r, const void *x, int dtype) {
 }
 
 // Weights times rows: D[m][n] = sum W[m][k] rows[n][k] (W [M][K], or [K][M] for a launch with A transposed),
-// the rows' lower planes first; of few rows, all planes as rows.
+// the rows' lower planes first; of few rows, all planes as rows. (Before the rows have a place, for the plan alone.)
 DenseArgs product(const uint16_t *W, size_t ldw, const Rows &b, size_t M) {
   DenseArgs a{};
   a.A = W;
@@ -157,19 +157,21 @@ DenseArgs product(const uint16_t *W, size_t ldw, const Rows &b, size_t M) {
   a.M = (int)M;
   a.N = (int)b.n;
   a.K = (int)b.cols;
-  a.splits = a.stack = a.b_planes = 1;
+  a.splits = a.stack = a.stack_step = a.b_planes = 1;
   if (b.where != kWhereOne) {
     if (b.n * kPlanes <= 64) {
-      a.stack = kPlanes;  // the first three slots, one of each plane
+      a.stack = kPlanes;  // the last slots of the planes: three in a row, of a right operand every other one
+      a.stack_step = b.where == kWhereRight ? 2 : 1;
+      if (a.B) a.B += (dense_last_slot(b.where, 0) - (kPlanes - 1) * a.stack_step) * a.b_slot;
     } else {
       a.b_planes = kPlanes;
-      for (int i = 0; i < kPlanes; i++) a.pb |= (uint32_t)__builtin_ctz(b.where >> 8 * (kPlanes - 1 - i)) << 4 * i;
+      for (int i = 0; i < kPlanes; i++) a.pb |= (uint32_t)dense_last_slot(b.where, kPlanes - 1 - i) << 4 * i;
     }
   }
   return a;
 }
-// Rows times rows over their rows: D[m][n] = sum_t a[t][m] b[t][n]; of a's values (or copies of them) and
-// b's planes, or of both's planes in pairs.
+// Rows times rows over their rows: D[m][n] = sum_t a[t][m] b[t][n]; of copies of a's values and b's three planes,
+// or of both's planes in pairs.
 DenseArgs gradient(const Rows &x, const Rows &y) {
   DenseArgs a{};
   a.A = x.p;
@@ -179,7 +181,7 @@ DenseArgs gradient(const Rows &x, const Rows &y) {
   a.M = (int)x.cols;
   a.N = (int)y.cols;
   a.K = (int)(std::min(x.slots, y.slots) * x.n);
-  a.splits = a.stack = a.b_planes = 1;
+  a.splits = a.stack = a.stack_step = a.b_planes = 1;
   return a;
 }
 
@@ -494,6 +496,7 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
   const bool bf = dtype == MOE_BF16;
   const bool inner = out->x || out->gate_up || out->gate_up_bias || out->down;
   const DenseShape ss{false, false, DENSE_STORE}, sg{true, false, DENSE_DGATE}, sx{true, false, DENSE_STORE}, sw{true, true, DENSE_STORE};
+  const uint32_t to_x = x_type == MOE_MXFP8 ? kWhereThree : kWhereRight;  // d(gate, up): a checkpoint's copies meet its planes one by one
   Carve w;
   Rows r, d, h, dgu;
   float *gu = nullptr, *dh = nullptr, *db = nullptr, *col = nullptr, *px = nullptr, *pgu = nullptr, *pd = nullptr;
@@ -519,13 +522,14 @@ int moe_ffn_backward_device(moe_ctx *ctx, const moe_ffn *b, const void *x, int x
       raw.splits = n_raw = dense_splits(ss, raw);
       in.splits = n_dh = dense_splits(sx, in);
       // (that kernel's bytes at 5 TB/s; what its parts cost is in the estimates)
-      const double bytes = ((n_raw > 1 ? 0.0 : 8.0) + (n_dh > 1 ? 0.0 : 4.0) + 6.0 * (bf ? 1 : kPairs6)) * T * I;
+      const double bytes = ((n_raw > 1 ? 0.0 : 8.0) + (n_dh > 1 ? 0.0 : 4.0) + 2.0 * rows_of(dtype, kWhereLeft, T, I, I).slots +
+                            4.0 * rows_of(dtype, to_x, T, I, I).slots) * T * I;
       apart = dense_estimate(ss, raw) + dense_estimate(sx, in) + 1.0 + bytes / 5e6 < one && T <= 65536;
       if (!apart) n_raw = n_dh = 1;
       gu = w.take<float>(n_raw * T * 2 * I);
       dh = apart ? w.take<float>(n_dh * T * I) : nullptr;
       h = place(w, rows_of(dtype, kWhereLeft, T, I, I));
-      dgu = place(w, rows_of(dtype, kWhereRight, T, 2 * I, 2 * I));
+      dgu = place(w, rows_of(dtype, to_x, T, 2 * I, 2 * I));
       db_parts = apart ? dense_dgate_parts((int)T) : dense_parts(sg, product(b->down, I, d, I));
       // (one part is the result)
       db = !out->gate_up_bias ? nullptr : db_parts > 1 ? w.take<float>((size_t)db_parts * 2 * I) : out->gate_up_bias;

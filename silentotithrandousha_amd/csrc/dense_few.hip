@@ -20,7 +20,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_dense_few(const DenseArgs a) {
   __shared__ float s_sum[kWaves][16][16 * kTiles + 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m0 = blockIdx.x * ROWS, rows_b = a.N * a.stack, at = lane >> 4;
-  const uint16_t *A[kTiles], *B = a.B + (size_t)min(lane & 15, rows_b - 1) * a.ldb;
+  const int row_b = min(lane & 15, rows_b - 1);  // of the stacked planes, which may lie in every other slot
+  const uint16_t *A[kTiles], *B = a.B + (size_t)(row_b + row_b / a.N * a.N * (a.stack_step - 1)) * a.ldb;
 #pragma unroll
   for (int t = 0; t < kTiles; t++)  // (of a part of a tile the lanes past it read its last row)
     A[t] = a.A + (size_t)min(m0 + min(t * 16 + (lane & 15), ROWS - 1), a.M - 1) * a.lda;
@@ -60,7 +61,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_dense_few(const DenseArgs a) {
   // the sum of the wavefronts' parts, and of a row's planes
   auto sum = [&](int n, int m) __attribute__((always_inline)) {
     float v = 0.0f;
-    for (int p = a.stack - 1; p >= 0; p--)
+    for (int p = 0; p < a.stack; p++)
 #pragma unroll
       for (int w = 0; w < kWaves; w++) v += s_sum[w][p * a.N + n][m];
     return v + (a.bias ? a.bias[m0 + m] : 0.0f);
@@ -83,7 +84,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_dense_few(const DenseArgs a) {
       uint16_t q[kPlanes];
       dense_split(g.h(), q);
       for (int p = 0; p < a.planes; p++)
-        dense_slots(a.h_where, p, [&](size_t at) { a.h[at * a.h_slot + (size_t)n * a.ldh + m0 / 2 + i] = q[p]; });
+        dense_slots<false>(a.h_where, p, q[p], [&](size_t at, uint16_t v) { a.h[at * a.h_slot + (size_t)n * a.ldh + m0 / 2 + i] = v; });
     }
   }
 }

@@ -96,13 +96,16 @@ struct DenseTile {
   }
   // chunk c of the tile: the first k of its values if K-contiguous, its row's k if transposed
   static __device__ __forceinline__ int k_of(int c) { return TR ? c / (R / 8) : ((c & 7) ^ ((c >> 3) & 7)) * 8; }
-  // rows: valid rows from the tile's first; ld: bytes between stored rows
-  __device__ __forceinline__ void init(int wave, int lane, int rows, uint32_t ld) {
+  // rows: valid rows from the tile's first; ld: bytes between stored rows; after every `skip_every` rows (of planes
+  // stacked from every other slot) as many are left out, none if it is 0
+  __device__ __forceinline__ void init(int wave, int lane, int rows, uint32_t ld, int skip_every = 0) {
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
       const int c = dma(i, wave) * 64 + lane, k = k_of(c);
       if constexpr (!TR) {
-        off[i] = (uint32_t)min(c >> 3, rows - 1) * ld + k * 2;
+        int row = min(c >> 3, rows - 1);
+        if (skip_every) row += row / skip_every * skip_every;
+        off[i] = (uint32_t)row * ld + k * 2;
       } else {
         const int pos = c % (R / 8);
         int col = piece(pos >> 1, k) * 16 + (pos & 1) * 8;  // the permutation is its own inverse
@@ -209,10 +212,29 @@ __device__ __forceinline__ void dense_rows_f32(uint8_t *stage, int lane, const f
   dense_rows<TM, 8, ONCE>(stage, lane, q, (uint16_t *)out, 2 * ld, rows, 2 * cols);
 }
 
-// f(slot) for the slots of plane p.
-template <class F>
-__device__ __forceinline__ void dense_slots(uint32_t where, int p, F &&f) {
-  for (uint32_t m = (where >> 8 * p) & 255; m; m &= m - 1) f((size_t)__builtin_ctz(m));
+// f(slot, values) for the slots of plane p, the last of them with the values q as they are, the others with 0 for
+// those that are not finite (which are in plane 0). ONE: rows of one plane, slot 0.
+__device__ __forceinline__ void dense_finite(uint16_t &q) {
+  if ((q & 0x7F80) == 0x7F80) q = 0;
+}
+template <class Q, int N>
+__device__ __forceinline__ void dense_finite(Q (&q)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) dense_finite(q[i]);
+}
+template <bool ONE, class Q, class F>
+__device__ __forceinline__ void dense_slots(uint32_t where, int p, Q &q, F &&f) {
+  if constexpr (ONE) {
+    f((size_t)0, q);
+  } else {
+    uint32_t m = (where >> 8 * p) & 255;
+    const int last = dense_last_slot(where, p);
+    f((size_t)last, q);
+    m ^= 1u << last;
+    if (!m) return;
+    if (p == 0) dense_finite(q);
+    for (; m; m &= m - 1) f((size_t)__builtin_ctz(m), q);
+  }
 }
 
 // Takes the bf16 of each value, and leaves what it did not hold (if another is to follow).
@@ -250,7 +272,7 @@ __device__ __forceinline__ void dense_tile_product(const DenseArgs &a, int block
   TA la;
   TB lb;
   la.init(wave, lane, a.M - m0, lda);
-  lb.init(wave, lane, rows_b - n0, ldb);
+  lb.init(wave, lane, rows_b - n0, ldb, PL == 1 && BN <= 64 && !BT && a.stack_step > 1 ? a.N : 0);
   // the step to load: its operands' addresses, k values left from there
   int left = k_hi - k_lo;
   const uint16_t *pa = a.A + (AT ? (size_t)k_lo * a.lda + m0 : (size_t)m0 * a.lda + k_lo), *pb[PL];
@@ -432,7 +454,7 @@ __device__ __forceinline__ void dense_tile_product(const DenseArgs &a, int block
 
   if constexpr (PL == 1 && BM * BN * 4 <= NS * kSlot && BN <= 64) {
     // B's planes were stacked as rows of one pass (so that A, which few rows wait for, streams once): a
-    // column's result is the sum of its planes' columns
+    // column's result is the sum of its planes' columns, the first plane's last
     if (a.stack > 1) {
       __syncthreads();
       float *o = (float *)lds;
@@ -449,7 +471,7 @@ __device__ __forceinline__ void dense_tile_product(const DenseArgs &a, int block
         for (int i = 0; i < TM; i++) {
           f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
           if (n < a.N)
-            for (int p = a.stack - 1; p >= 0; p--) v += *(const f32x4 *)(o + (p * a.N + n) * BM + (wm * TM + i) * 16 + (lane >> 4) * 4);
+            for (int p = 0; p < a.stack; p++) v += *(const f32x4 *)(o + (p * a.N + n) * BM + (wm * TM + i) * 16 + (lane >> 4) * 4);
           acc[i][j] = v;
         }
       }
@@ -529,7 +551,7 @@ __device__ __forceinline__ void dense_tile_product(const DenseArgs &a, int block
           uint16_t q[TM][2];
 #pragma unroll
           for (int i = 0; i < TM; i++) dense_take<!one>(h[i], q[i]);
-          dense_slots(a.h_where, p, [&](size_t at) {
+          dense_slots<one>(a.h_where, p, q, [&](size_t at, const auto &q) {
             dense_rows<TM, 2>(stage, lane, q, a.h + at * a.h_slot + (size_t)(n_first + j * 16) * a.ldh + m_first / 2, a.ldh,
                               a.N - n_first - j * 16, (a.M - m_first) / 2);
           });
@@ -569,8 +591,8 @@ __device__ __forceinline__ void dense_tile_product(const DenseArgs &a, int block
             uint16_t q[8], e[4];
             dense_take<!one>(d, q);
             dense_take<!one>(hv, e);
-            dense_slots(a.dgu_where, p, [&](size_t at) { *(uint4 *)(a.dgu + at * a.dgu_slot + (size_t)n * a.M * 2 + 2 * m) = __builtin_bit_cast(uint4, q); });
-            dense_slots(a.h_where, p, [&](size_t at) { *(uint2 *)(a.h + at * a.h_slot + (size_t)n * a.ldh + m) = __builtin_bit_cast(uint2, e); });
+            dense_slots<one>(a.dgu_where, p, q, [&](size_t at, const auto &q) { *(uint4 *)(a.dgu + at * a.dgu_slot + (size_t)n * a.M * 2 + 2 * m) = __builtin_bit_cast(uint4, q); });
+            dense_slots<one>(a.h_where, p, e, [&](size_t at, const auto &e) { *(uint2 *)(a.h + at * a.h_slot + (size_t)n * a.ldh + m) = __builtin_bit_cast(uint2, e); });
           }
         }
         if (a.db_part) {  // over the wavefront's columns: 16 lanes, then a part per wavefront column
@@ -661,7 +683,7 @@ __device__ __forceinline__ void dense_tile_product(const DenseArgs &a, int block
           uint16_t q[TM][4];
 #pragma unroll
           for (int i = 0; i < TM; i++) dense_take<!one>(d[i], q[i]);
-          dense_slots(a.dl_where, p, [&](size_t at) {
+          dense_slots<one>(a.dl_where, p, q, [&](size_t at, const auto &q) {
             dense_rows<TM, 4>(stage, lane, q, a.dl + at * a.dl_slot + (size_t)(n_first + j * 16) * a.ld_dl + m_first, a.ld_dl,
                               a.N - n_first - j * 16, (int)a.ld_dl - m_first);
           });
