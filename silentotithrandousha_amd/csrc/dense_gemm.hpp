@@ -639,14 +639,19 @@ __device__ __forceinline__ void dense_tile_product(const DenseArgs &a, int block
       }
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      // no value above minus infinity: every exponential is 0 against a base of 0. (The difference before the
-      // factor log2 e: a maximum above 2.36e38 would overflow with it.)
-      const float base = mx == -INFINITY ? 0.0f : mx;
+      // no value above minus infinity: every exponential is 0 against a base of 0
+      float base = mx == -INFINITY ? 0.0f : mx;
+      if (__any(fabsf(base) > 2e38f)) {  // its product with log2 e may overflow: the difference first
+#pragma unroll
+        for (int i = 0; i < TM; i++) acc[i][j] -= f32x4{base, base, base, base};
+        base = 0.0f;
+      }
+      base *= 1.4426950408889634f;
       float sum = 0.0f;  // (a NaN among the logits makes it one)
 #pragma unroll
       for (int i = 0; i < TM; i++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) sum += dense_exp_near(acc[i][j][r] - base);
+        for (int r = 0; r < 4; r++) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], 1.4426950408889634f, -base));
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
       if (lane < 16 && n < a.N) a.stats[(size_t)(tile_m * WM + wm) * a.N + n] = make_float2(mx, sum);
