@@ -253,9 +253,11 @@ int fail(int code, const char *fmt, ...) {
 #define BV_HIP(call)                                                                          \
   do {                                                                                        \
     hipError_t e_ = (call);                                                                   \
-    if (e_ != hipSuccess)                                                                     \
+    if (e_ != hipSuccess) {                                                                   \
+      (void)hipGetLastError(); /* not left for the next launch */                             \
       return fail(e_ == hipErrorOutOfMemory ? MOE_ERR_OOM : MOE_ERR_HIP, "%s: %s", #call,     \
                   hipGetErrorString(e_));                                                     \
+    }                                                                                         \
   } while (0)
 
 }  // namespace

@@ -28,12 +28,15 @@ int fail(int code, const char *fmt, ...) {
   return api_fail(code, buf);
 }
 
+// (a reported error is not left for the next launch, which would report it again as its own)
 #define HIP_TRY(call)                                                                          \
   do {                                                                                         \
     hipError_t e_ = (call);                                                                    \
-    if (e_ != hipSuccess)                                                                      \
+    if (e_ != hipSuccess) {                                                                    \
+      (void)hipGetLastError();                                                                 \
       return fail(e_ == hipErrorOutOfMemory ? MOE_ERR_OOM : MOE_ERR_HIP, "%s: %s (%s:%d)",     \
                   #call, hipGetErrorString(e_), __FILE__, __LINE__);                           \
+    }                                                                                          \
   } while (0)
 
 #define RETURN_IF(rc)  \
@@ -75,7 +78,10 @@ int ensure(const DenseCtx &c, size_t bytes, hipStream_t s) {
       return fail(MOE_ERR_STATE, "workspace too small for this call during graph capture; run it once uncaptured first");
     void *q = nullptr;
     const hipError_t e = hipMalloc(&q, bytes);
-    if (e != hipSuccess) return fail(MOE_ERR_OOM, "hipMalloc(%zu): %s", bytes, hipGetErrorString(e));
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(MOE_ERR_OOM, "hipMalloc(%zu): %s", bytes, hipGetErrorString(e));
+    }
     if (w.p && w.captured)
       w.kept.push_back(w.p);
     else if (w.p)

@@ -31,12 +31,15 @@ int fail(int code, const char *fmt, ...) {
   return code;
 }
 
+// (a reported error is not left for the next launch, which would report it again as its own)
 #define HIP_TRY(call)                                                                      \
   do {                                                                                     \
     hipError_t e_ = (call);                                                                \
-    if (e_ != hipSuccess)                                                                  \
+    if (e_ != hipSuccess) {                                                                \
+      (void)hipGetLastError();                                                             \
       return fail(e_ == hipErrorOutOfMemory ? MOE_ERR_OOM : MOE_ERR_HIP, "%s: %s (%s:%d)", \
                   #call, hipGetErrorString(e_), __FILE__, __LINE__);                       \
+    }                                                                                      \
   } while (0)
 
 #define RETURN_IF(rc) \
@@ -55,7 +58,10 @@ struct DevBuf {
     const size_t want = std::max(bytes, (size_t)4096);
     void *q = nullptr;
     hipError_t e = hipMalloc(&q, want);
-    if (e != hipSuccess) return fail(MOE_ERR_OOM, "hipMalloc(%zu): %s", want, hipGetErrorString(e));
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(MOE_ERR_OOM, "hipMalloc(%zu): %s", want, hipGetErrorString(e));
+    }
     if (p) (void)hipFree(p);
     p = q;
     cap = want;
@@ -76,7 +82,10 @@ struct HostBuf {
     if (bytes <= cap) return MOE_OK;
     void *q = nullptr;
     hipError_t e = hipHostMalloc(&q, bytes, hipHostMallocDefault);
-    if (e != hipSuccess) return fail(MOE_ERR_OOM, "hipHostMalloc(%zu): %s", bytes, hipGetErrorString(e));
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(MOE_ERR_OOM, "hipHostMalloc(%zu): %s", bytes, hipGetErrorString(e));
+    }
     release();
     p = q;
     cap = bytes;
