@@ -10,141 +10,19 @@
 
 namespace moe {
 
-namespace {
-
-// k values of each split, a multiple of the step
-int split_k(const DenseArgs &a) {
-  const long steps = ((long)a.K + kDenseStep - 1) / kDenseStep, n = a.splits < 1 ? 1 : a.splits;
-  return (int)((steps + n - 1) / n * kDenseStep);
-}
-
-constexpr int kCus = 256;  // of an MI355X: the plan is for the whole device
-
-// Estimated us of a product on one tile shape with its K in `splits` parts. A workgroup's step takes the
-// largest of the time that its products take at the tile's full rate, that its loads of A take where A is
-// read once, from memory (both shared by the workgroups of its CU), and that its loads wait, spread over
-// the steps that its slots hold ahead; each workgroup has a prologue and an epilogue that stores its
-// results; parts are summed in another launch. `others`: tiles of the same shape in the launch, as many as do the same steps. Whole rounds of workgroups and what is left for the last one count apart.
-double dense_us(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a, int splits, long others = 0) {
-  const long tiles_n = ((long)a.N * a.stack + d.bn - 1) / d.bn, tiles = (long)((a.M + d.bm - 1) / d.bm) * tiles_n * splits + others;
-  const long steps = (((long)a.K + kDenseStep - 1) / kDenseStep + splits - 1) / splits;
-  // bytes that a result costs, about: of rows in planes, results in planes (GATE 3 slots, the gradients 6)
-  const bool planes = a.b_planes > 1 || a.stack > 1;
-  const double result = s.epi == DENSE_STATS ? 0.0 : s.epi == DENSE_GATE ? (planes ? 3.0 : 1.0)
-                        : s.epi == DENSE_DGATE ? (planes ? 44.0 : 14.0) : s.epi == DENSE_DLOGITS ? (planes ? 12.0 : 2.0)
-                        : a.out_mode || splits > 1 ? 4.0 : 2.0;
-  // a transposed A's rows of k are read in pieces of a tile's rows: below 128 bytes the slower for it
-  const double memory = s.at && d.bm < 64 ? 23.0 * d.bm / 64 : 23.0;  // GB/s a CU; 5.9 TB/s in all
-  auto round = [&](double on_cu) {
-    double step = std::max(0.52 / (d.ns - 1) + 0.12, on_cu * d.bm * d.bn * 2.0 * kDenseStep * d.planes * kCus / (d.rate * 1e6));
-    if (tiles_n == 1) step = std::max(step, on_cu * d.bm * 128e-3 / memory);
-    const double stores = on_cu * d.bm * d.bn * result * kCus / 4.5e6;  // us at 4.5 TB/s
-    // f32 weight gradients of few rows, bound by their stores: of two workgroups a CU one stores while the other
-    // starts (19 rows, 32003 x 1024: 128 x 128 31.7 us, 256 x 256 34.3; bf16 rows of such tiles, 256 bytes, went slower)
-    if (s.bt && a.out_mode && d.bn == 128 && on_cu == d.wgs && stores > 2.0 * steps * step) return std::max(steps * step + 2.5, stores);
-    return steps * step + 2.5 + stores;
-  };
-  const long whole = tiles / (kCus * d.wgs), rest = tiles - whole * kCus * d.wgs;
-  const double on = (double)rest / kCus;  // of the last round: between the busiest CU's and the mean
-  double us = whole * round(d.wgs) + (rest ? round(std::max(1.0, 0.5 * (on + std::ceil(on)))) : 0.0);
-  if (splits > 1) us += (a.joined ? 0.5 : 4.5) + 4.0 * splits * a.M * a.N / 5e6;
-  return us;
-}
-
-bool tile_fits(const DenseShape &s, const DenseTileDims &d, const DenseArgs &a) {
-  if (d.planes != a.b_planes) return false;
-  if (a.stack > 1 && (d.bn > 64 || a.N * a.stack > d.bn)) return false;  // stacked planes lie in one tile
-  // 288 rows: K-contiguous they keep too much in registers (620 TFLOP/s)
-  return d.bm <= 256 || (s.at && s.epi == DENSE_STORE && a.K >= 1024);
-}
-
-constexpr DenseShape kGradient{true, true, DENSE_STORE};
-int pair_tile(const DenseArgs &a, const DenseArgs &b, double &us) {
-  int best = -1;
-  for (int t = 0; t < kDenseTileCount; t++) {
-    const DenseTileDims &d = kDenseTiles[t];
-    if (!tile_fits(kGradient, d, a)) continue;
-    const double tiles = (double)((b.M + d.bm - 1) / d.bm) * ((b.N + d.bn - 1) / d.bn);
-    const double u = dense_us(kGradient, d, a, 1, (long)std::ceil(tiles * b.K / a.K));
-    if (best < 0 || u < us) best = t, us = u;
-  }
-  return best;
-}
-
-}  // namespace
-
-int dense_tile(const DenseShape &s, const DenseArgs &a) {
-  int best = -1;
-  double us = 0.0;
-  for (int t = 0; t < kDenseTileCount; t++) {
-    const DenseTileDims &d = kDenseTiles[t];
-    if (!tile_fits(s, d, a)) continue;
-    const double u = dense_us(s, d, a, dense_split_count(a));
-    if (best < 0 || u < us) best = t, us = u;
-  }
-  return best;
-}
-
-int dense_parts(const DenseShape &s, const DenseArgs &a) {
-  const DenseTileDims &d = kDenseTiles[dense_tile(s, a)];
-  if (s.epi == DENSE_STATS) return (a.M + d.bm - 1) / d.bm * d.wm;
-  if (s.epi == DENSE_DGATE) return (a.N * a.stack + d.bn - 1) / d.bn * d.wn;
-  return 0;
-}
-
-int dense_split_count(const DenseArgs &a) {
-  const long k = split_k(a);
-  return (int)((a.K + k - 1) / k);
-}
-
-double dense_estimate(const DenseShape &s, const DenseArgs &a) {
-  return dense_us(s, kDenseTiles[dense_tile(s, a)], a, dense_split_count(a));
-}
-
-int dense_splits(const DenseShape &s, const DenseArgs &a0) {
-  if (dense_few_fits(s, a0)) return 1;
-  const long steps = ((long)a0.K + kDenseStep - 1) / kDenseStep;
-  int best = 1;
-  double us = 0.0;
-  for (int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-    if (n > 1 && steps / n < 4) break;
-    DenseArgs a = a0;
-    a.splits = n;
-    a.splits = dense_split_count(a);
-    const double u = dense_estimate(s, a);
-    if (n == 1 || u < us) best = a.splits, us = u;
-  }
-  return best;
-}
-
-bool dense_pair_pays(const DenseArgs &a, const DenseArgs &b) {
-  if (a.splits > 1 || b.splits > 1 || a.K < b.K) return false;
-  double us = 0.0;
-  pair_tile(a, b, us);
-  return us < dense_estimate(kGradient, a) + dense_estimate(kGradient, b);
-}
-
 hipError_t launch_dense_pair(const DenseArgs &a0, const DenseArgs &b0, hipStream_t st) {
-  DenseArgs x[2] = {a0, b0};
-  for (DenseArgs &a : x) {
-    if (a.M <= 0 || a.N <= 0 || a.K <= 0 || a.b_planes != 1 || a.stack != 1 || a.lda % 8 || a.ldb % 8 || a.M % 4 || a.splits > 1 || a.K > a0.K)
-      return hipErrorInvalidValue;
-    a.k_split = split_k(a);
-  }
+  DenseArgs a = a0, b = b0;
+  const hipError_t e = dense_prepare_pair(a, b);
+  if (e != hipSuccess) return e;
   double us = 0.0;
-  return launch_dense_tt_pair(pair_tile(x[0], x[1], us), x[0], x[1], st);
+  return launch_dense_tt_pair(dense_pair_tile(a, b, us), a, b, st);
 }
 
 hipError_t launch_dense(const DenseShape &s, const DenseArgs &a0, hipStream_t st) {
   DenseArgs a = a0;
-  if (a.M <= 0 || a.N <= 0 || a.K <= 0 || (a.b_planes != 1 && a.b_planes != kPlanes) || a.stack < 1 || a.lda % 8 || a.ldb % 8)
-    return hipErrorInvalidValue;
-  // (stores of 4 rows)
-  if (a.M % 4 && s.epi != DENSE_STATS && s.epi != DENSE_DLOGITS) return hipErrorInvalidValue;
-  a.k_split = split_k(a0);
-  a.splits = dense_split_count(a0);
-  if (a.splits > 1 && (s.epi != DENSE_STORE || a.out_mode != 1)) return hipErrorInvalidValue;
-  if (dense_few_fits(s, a)) return launch_dense_few(s, a, st);
+  const hipError_t e = dense_prepare(s, a);
+  if (e != hipSuccess) return e;
+  if (dense_few_rows(s, a)) return launch_dense_few(s, a, st);
   return s.at ? launch_dense_tn(s, a, st) : launch_dense_nt(s, a, st);
 }
 
@@ -240,7 +118,6 @@ __device__ __forceinline__ void column_sums(const S *x, size_t t0, size_t t1, si
     out[o] = v;
   }
 }
-constexpr size_t kColRows = 512;  // of a block
 template <class S>
 __global__ __launch_bounds__(1024) void k_colsum(const S *x, size_t T, size_t H, float *part) {
   const size_t t0 = (size_t)blockIdx.y * kColRows;
@@ -325,7 +202,6 @@ __global__ __launch_bounds__(256) void k_sums(const DenseSums a) {
 
 // A block takes 16 rows of 128 inner columns, 2 rows a thread of 4 columns. Bound by its bytes (333 f32 rows of
 // 1536, gate and up and dh in three parts each: 55 MB in 10 us, most of it from the caches).
-constexpr int kDgateRows = 16;
 template <bool ONE>
 __global__ __launch_bounds__(256) void k_dgate(const DgateArgs a) {
   __shared__ float s_db[8][256];
@@ -425,44 +301,10 @@ __global__ __launch_bounds__(1024) void k_loss(const float2 *stats, int parts, c
   }
 }
 
-unsigned blocks_for(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, 65536); }
-
 }  // namespace
 
-namespace {
-// where the blocks of each job end; their number
-template <class J>
-size_t dense_ends(J &a) {
-  size_t blocks = 0;
-  for (int i = 0; i < (int)(sizeof(a.d) / sizeof(a.d[0])); i++) {
-    if (i < a.count) blocks += a.d[i].blocks;
-    a.end[i] = (unsigned)blocks;
-  }
-  return blocks;
-}
-}  // namespace
-
-void DenseRowJobs::planes(const float *x, uint16_t *out, uint32_t where, size_t n, const int32_t *targets, size_t cols) {
-  if (n) d[count++] = DenseRows{ROWS_PLANES, x, out, n, cols, where, 0, blocks_for(n / 4), targets};
-}
-void DenseRowJobs::copy(const uint16_t *x, uint16_t *out, size_t n, const int32_t *targets, size_t cols) {
-  if (n) d[count++] = DenseRows{ROWS_COPY, x, out, n, cols, 0, 0, blocks_for(n / 8), targets};
-}
-void DenseRowJobs::pack8(const float *x, size_t n, uint8_t *packed) {
-  if (n) d[count++] = DenseRows{ROWS_PACK8, x, packed, n, 0, 0, 0, (unsigned)((n / 8 + 255) / 256), nullptr};
-}
-void DenseRowJobs::unpack8(const uint8_t *packed, size_t n, uint16_t *out, int copies) {
-  if (n) d[count++] = DenseRows{ROWS_UNPACK8, packed, out, n, 0, 0, copies, (unsigned)((n / 8 + 255) / 256), nullptr};
-}
-void DenseRowJobs::column_sums(const void *x, bool bf16, size_t T, size_t H, float *out) {
-  d[count++] = DenseRows{bf16 ? ROWS_SUM_BF16 : ROWS_SUM_F32, x, out, T, H, 0, 0, (unsigned)((H + 63) / 64), nullptr};
-}
-void DenseRowJobs::dloss_scale(const DlossScale &s) {
-  scale = s;
-  d[count++] = DenseRows{ROWS_DLOSS_SCALE, nullptr, nullptr, 0, 0, 0, 0, 1, nullptr};
-}
 hipError_t launch_rows(DenseRowJobs a, hipStream_t s) {
-  const size_t blocks = dense_ends(a);
+  const size_t blocks = a.ends();
   if (blocks > 0xFFFFFF) return hipErrorInvalidValue;  // (2^32 threads)
   if (a.count == 1 && a.d[0].what == ROWS_PLANES)
     k_planes<<<(unsigned)blocks, 256, 0, s>>>(a.d[0]);
@@ -471,17 +313,12 @@ hipError_t launch_rows(DenseRowJobs a, hipStream_t s) {
   return hipGetLastError();
 }
 
-void DenseSums::add(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias, void *out, bool bf16) {
-  const bool few = !bf16 && !bias && n <= 65536 && parts > 8;
-  d[count++] = DenseSum{part, stride, n, n_bias, bias, out, parts, few ? (unsigned)((n + 31) / 32) : blocks_for(n), bf16, few};
-}
 hipError_t launch_sums(DenseSums a, hipStream_t s) {
-  const size_t blocks = dense_ends(a);
+  const size_t blocks = a.ends();
   if (blocks) k_sums<<<(unsigned)blocks, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
-int dense_dgate_parts(int T) { return (T + kDgateRows - 1) / kDgateRows; }
 hipError_t launch_dgate(const DgateArgs &a, hipStream_t s) {
   const dim3 grid((a.I + 127) / 128, dense_dgate_parts(a.T));
   if (a.T < 1 || a.I < 8 || a.I % 8 || grid.y > 65535) return hipErrorInvalidValue;
@@ -497,7 +334,6 @@ hipError_t launch_dloss_scale(const DlossScale &d, hipStream_t s) {
   return hipGetLastError();
 }
 
-int dense_colsum_parts(size_t T) { return (int)((T + kColRows - 1) / kColRows); }
 hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *part, hipStream_t s) {
   const dim3 grid((unsigned)((H + 63) / 64), (unsigned)dense_colsum_parts(T));
   if (!T || !H) return hipSuccess;

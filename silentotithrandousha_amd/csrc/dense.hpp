@@ -104,6 +104,7 @@ struct DgateArgs {
   uint32_t h_where, dgu_where;
   float *db_part;
 };
+constexpr int kDgateRows = 16;  // rows of a part
 int dense_dgate_parts(int T);
 hipError_t launch_dgate(const DgateArgs &a, hipStream_t s);
 
@@ -144,6 +145,7 @@ struct DenseRowJobs {
   void unpack8(const uint8_t *packed, size_t n, uint16_t *out, int copies);
   void column_sums(const void *x, bool bf16, size_t T, size_t H, float *out);  // dense_colsum_parts(T) == 1
   void dloss_scale(const DlossScale &s);  // few tokens
+  size_t ends();  // sets `end`; the blocks of all
 };
 hipError_t launch_rows(DenseRowJobs a, hipStream_t s);
 
@@ -163,9 +165,11 @@ struct DenseSums {
   DenseSum d[5];
   int count = 0;
   void add(const float *part, size_t stride, int parts, size_t n, const float *bias, size_t n_bias, void *out, bool bf16);
+  size_t ends();
 };
 hipError_t launch_sums(DenseSums a, hipStream_t s);
 // Column sums of x [T][H] (f32 or bf16) into parts [dense_colsum_parts(T)][H].
+constexpr size_t kColRows = 512;  // of a part
 int dense_colsum_parts(size_t T);
 hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *part, hipStream_t s);
 // loss and log-sum-exp of each token from the parts of DENSE_STATS.

@@ -100,26 +100,14 @@ void launch_few(const DenseShape &s, const DenseArgs &a, hipStream_t st) {
 
 }  // namespace
 
-// (more rows of A than 4 tiles a CU keep the rings' larger tiles full, and 16 rows of B took 21.6 us in the
-// 2880 x 2880 block against 20.9 through the rings)
-bool dense_few_fits(const DenseShape &s, const DenseArgs &a) {
-  return !s.at && !s.bt && (s.epi == DENSE_GATE || s.epi == DENSE_STORE) && a.b_planes == 1 && a.N * a.stack <= 8 && a.M % 16 == 0 &&
-         a.K % 8 == 0 && a.M <= 16 * 1024 && a.splits <= 1 && !a.scale && a.out_mode != 2;
-}
-
 hipError_t launch_dense_few(const DenseShape &s, const DenseArgs &a, hipStream_t st) {
-  if (!dense_few_fits(s, a)) return hipErrorInvalidValue;
-  // the fewest rows that fit the CUs once: where some CUs take two workgroups they are waited for (5760 rows of
-  // weights by 16: 10.1 us, by 24: 9.4), and where many take none the others have the more to read
-  const int rows = (a.M + 255) / 256;
-  if (rows <= 8)
-    launch_few<8>(s, a, st);
-  else if (rows <= 12)
-    launch_few<12>(s, a, st);
-  else if (rows <= 16 || rows > 24)
-    launch_few<16>(s, a, st);
-  else
-    launch_few<24>(s, a, st);
+  switch (dense_few_rows(s, a)) {
+    case 8: launch_few<8>(s, a, st); break;
+    case 12: launch_few<12>(s, a, st); break;
+    case 16: launch_few<16>(s, a, st); break;
+    case 24: launch_few<24>(s, a, st); break;
+    default: return hipErrorInvalidValue;
+  }
   return hipGetLastError();
 }
 

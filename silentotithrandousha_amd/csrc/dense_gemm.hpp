@@ -21,12 +21,11 @@
 // 1.46; of 333 f32 rows (50257 x 2048, three planes) 200 to 230 us, 0.89 to 1.03 PFLOP/s. Those of few rows by
 // the weights: one f32 row, 1.16 GB in 184 us, 6.3 TB/s. In between by the tiles that 256 CUs do not share evenly.
 #pragma once
-#include "dense.hpp"
+#include "dense_index.hpp"
+#include "dense_plan.hpp"
 #include "stream.hpp"
 
 namespace moe {
-constexpr int kDenseStep = 64;  // k values per step
-constexpr int kDenseHalf = 32;  // and per half, an MFMA's
 
 __device__ __forceinline__ uint16_t dense_bf16(float v) {
   return __builtin_bit_cast(uint16_t, (__bf16)v);  // round to nearest even
@@ -72,94 +71,42 @@ struct DenseGate {
   __device__ __forceinline__ float du(float dh, float u, float limit) const { return fabsf(u) > limit ? 0.0f : dh * (G * s); }
 };
 
-// One operand's tile: R rows (of M or N) x 64 k, W wavefronts loading it.
+// One operand's tile (dense_index.hpp) as a wavefront loads and reads it.
 template <int R, int W, bool TR>
-struct DenseTile {
-  static constexpr int kBytes = R * 128;
-  static constexpr int kDmas = R / 8;                 // LDS-DMAs of 1 KB
-  static constexpr int kLoads = (kDmas + W - 1) / W;  // per wavefront; past the last one again (the same bytes)
-  static constexpr int kPairs = R / 16;               // 32-byte pieces of a transposed row
+struct DenseTile : DenseIndex<R, W, TR> {
+  using At = DenseIndex<R, W, TR>;
+  uint32_t off[At::kLoads];  // byte offset of this lane's 16 bytes from the tile's base
 
-  // Transposed: piece of a row that holds the logical piece q in row k. The transposing load's 16 lanes
-  // take 4 rows k: their pieces go to different banks. (Only within groups of 4 pieces, so that the
-  // fragments of 16 rows lie at 4 addresses and constant distances from them.)
-  static __device__ __forceinline__ int piece(int q, int k) {
-    const int mask = kPairs >= 4 ? ((q | 3) < kPairs ? 3 : 0) : kPairs >= 2 ? 1 : 0;
-    return q ^ (k & mask);
-  }
-
-  uint32_t off[kLoads];  // byte offset of this lane's 16 bytes from the tile's base
-
-  static __device__ __forceinline__ int dma(int i, int wave) {
-    const int d = i * W + wave;
-    return kDmas % W == 0 ? d : d % kDmas;
-  }
-  // chunk c of the tile: the first k of its values if K-contiguous, its row's k if transposed
-  static __device__ __forceinline__ int k_of(int c) { return TR ? c / (R / 8) : ((c & 7) ^ ((c >> 3) & 7)) * 8; }
-  // rows: valid rows from the tile's first; ld: bytes between stored rows; after every `skip_every` rows (of planes
-  // stacked from every other slot) as many are left out, none if it is 0
   __device__ __forceinline__ void init(int wave, int lane, int rows, uint32_t ld, int skip_every = 0) {
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) {
-      const int c = dma(i, wave) * 64 + lane, k = k_of(c);
-      if constexpr (!TR) {
-        int row = min(c >> 3, rows - 1);
-        if (skip_every) row += row / skip_every * skip_every;
-        off[i] = (uint32_t)row * ld + k * 2;
-      } else {
-        const int pos = c % (R / 8);
-        int col = piece(pos >> 1, k) * 16 + (pos & 1) * 8;  // the permutation is its own inverse
-        if (col >= rows) col = 0;
-        off[i] = (uint32_t)k * ld + col * 2;
-      }
-    }
+    for (int i = 0; i < At::kLoads; i++) off[i] = At::offset(i, wave, lane, rows, ld, skip_every);
   }
   // the wavefront's load i of the step whose first k is at `base`
   __device__ __forceinline__ void load(int i, const uint16_t *base, uint32_t lds, int wave) const {
-    str_dma16(off[i], base, lds + dma(i, wave) * 1024);
+    str_dma16(off[i], base, lds + At::dma(i, wave) * 1024);
   }
-  // for a step with fewer k values left than its 64: past them a valid place instead (zero_tail clears it)
   __device__ __forceinline__ void clamp(int wave, int lane, uint32_t ld, int left) {
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) {
-      const int k = k_of(dma(i, wave) * 64 + lane);
-      if (k >= left) off[i] -= TR ? (uint32_t)(k - (left - 1)) * ld : (uint32_t)k * 2;
-    }
+    for (int i = 0; i < At::kLoads; i++) off[i] -= At::behind(i, wave, lane, ld, left);
   }
   // zeroes the k values of the step past `left` (the last step of a K that is no multiple of 64)
   __device__ __forceinline__ static void zero_tail(uint8_t *lds, int left, int tid, int threads) {
     for (int c = tid; c < R * 8; c += threads)
-      if (k_of(c) >= left) *(uint4 *)(lds + c * 16) = uint4{0u, 0u, 0u, 0u};
+      if (At::k_of(c) >= left) *(uint4 *)(lds + c * 16) = uint4{0u, 0u, 0u, 0u};
   }
   // MFMA operand of 16 rows from row0 (tile-relative), half h of the step at lds
   static __device__ __forceinline__ bf16x8 frag(const uint8_t *lds, int row0, int h, int lane) {
     if constexpr (!TR) {
-      const int row = row0 + (lane & 15), ch = h * 4 + (lane >> 4);
-      return *(const bf16x8 *)(lds + row * 128 + ((ch ^ (row & 7)) << 4));
+      return *(const bf16x8 *)At::frag_at(lds, row0, h, lane, 0);
     } else {
       typedef short s16x4 __attribute__((ext_vector_type(4)));
-      const int i = lane & 15, k = (lane >> 4) * 8 + (i >> 2);
-      const int q = row0 >> 4;
-      auto at = [&](int k) {
-        return (__attribute__((address_space(3))) s16x4 *)(lds + (h * kDenseHalf + k) * (R * 2) + piece(q, k) * 32 + (i & 3) * 8);
-      };
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(k));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(k + 4));
+      auto at = [&](int part) { return (__attribute__((address_space(3))) s16x4 *)At::frag_at(lds, row0, h, lane, part); };
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(0));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(1));
       return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
 };
-
-// The tile of workgroup b: 8 XCDs take the workgroups in turn, so each gets a contiguous share of the
-// order; in it, 8 tiles along n, then along m, so that the 32 workgroups of an XCD share the rows of
-// about 4 x 8 tiles in its L2.
-__device__ __forceinline__ void dense_tile_of(int b, int tiles_m, int tiles_n, int &tm, int &tn) {
-  const int total = tiles_m * tiles_n, x = b & 7, q = total >> 3, r = total & 7;
-  const int t = x * q + min(x, r) + (b >> 3);
-  const int group = t / (tiles_m * 8), n0 = group * 8, width = min(8, tiles_n - n0), in = t - group * tiles_m * 8;
-  tm = in / width;
-  tn = n0 + in % width;
-}
 
 // v itself, but what is computed from it stays where it is: hoisted out of the main loop (from its rare
 // branches) or shared by the columns of the epilogue it took registers and was spilled.

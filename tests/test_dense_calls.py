@@ -1,0 +1,73 @@
+"""The dense operators' host code and index arithmetic, replayed without a GPU by two programs that compile the sources
+themselves: tests/cpp/dense_calls_test.cpp (every call's launches, workspace and planes) and tests/cpp/dense_tiles_test.cpp
+(where a tile's values lie in memory and LDS)."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "silentotithrandousha_amd", "csrc")
+
+
+def build(folder, name, *sources):
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not available")
+    out = str(folder / name)
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                    os.path.join(ROOT, "tests", "cpp", name + ".cpp"), *(os.path.join(CSRC, s) for s in sources), "-o", out], check=True)
+    return out
+
+
+@pytest.fixture(scope="module")
+def calls(tmp_path_factory):
+    return build(tmp_path_factory.mktemp("calls"), "dense_calls_test", "dense_api.cpp", "dense_plan.cpp")
+
+
+@pytest.fixture(scope="module")
+def tiles(tmp_path_factory):
+    return build(tmp_path_factory.mktemp("tiles"), "dense_tiles_test")
+
+
+def replay(exe, lines, *mode):
+    """(exit code, {call: its forms}, the last line) of lines as dense_calls_test.cpp describes them."""
+    r = subprocess.run([exe, *(mode or ("calls",))], input="\n".join(lines), capture_output=True, text=True, timeout=100)
+    out = r.stdout.splitlines()
+    return r.returncode, dict(line.split(" : ") if " : " in line else (line, "") for line in out if " :" in line), out[-1]
+
+
+# every kind of call, of one token, few, many, more than one piece; padded and odd sizes
+CALLS = [f"{op} {T} {H} {X} {dtype}{tail}" for dtype in (0, 1) for T, H, X in ((1, 32, 8), (5, 96, 504), (21, 64, 1000), (22, 64, 1000),
+         (333, 2048, 1536), (4096, 2880, 2880), (8197, 64, 4096), (20000, 160, 2056))
+         for op, tail in (("loss", ""), ("lossgrad", " 1 1"), ("lossgrad", " 1 0"), ("lossgrad", " 0 1"), ("ffn", " 0"), ("ffn", " 1"),
+                          *(("ffngrad", f" {kept} {mask}") for kept in (0, 1) for mask in (31, 1, 2, 4, 8, 16, 14, 27)))]
+CALLS += [f"loss{g} {T} {H} {V} {dtype}{' 1 1' * bool(g)}" for g in ("", "grad") for dtype in (0, 1)
+          for T, H, V in ((1, 2880, 201088), (16389, 32, 4097), (8200, 32, 33000), (8193, 64, 11001), (3, 32, 1), (2048, 2880, 201088))]
+
+
+def test_calls_stay_in_their_buffers(calls):
+    rc, got, last = replay(calls, CALLS)
+    assert rc == 0 and last == "faults 0" and len(got) == len(set(CALLS))
+
+
+def test_drawn_calls_stay_in_their_buffers(calls):
+    r = subprocess.run([calls, "draw", "30000", "5"], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.splitlines()[-1] == "faults 0"
+
+
+@pytest.mark.parametrize("mistake", ["slot", "behind", "short"])
+def test_a_planted_mistake_in_a_call_is_found(calls, mistake):
+    """Planes read from other slots, rows longer than they are, an allocation 4 KB short."""
+    rc, _, last = replay(calls, CALLS, "plant", mistake)
+    assert rc == 3 and last != "faults 0"
+
+
+def test_tiles(tiles):
+    r = subprocess.run([tiles], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0, r.stdout.splitlines()[-1]
+
+
+@pytest.mark.parametrize("mistake,code", [("clamp", 3), ("pieces", 4)])
+def test_a_planted_mistake_in_the_tiles_is_found(tiles, mistake, code):
+    assert subprocess.run([tiles, mistake], capture_output=True, timeout=100).returncode == code
