@@ -25,7 +25,6 @@ constexpr int kDenseHalf = 32;  // and per half, an MFMA's
   X(64, 16, 4, 1, 8, 1, 2, 210.0)     \
   X(16, 16, 1, 1, 16, 1, 2, 110.0)    \
   X(256, 128, 4, 2, 2, 3, 1, 1280.0)  \
-  X(128, 128, 2, 4, 2, 3, 1, 1150.0)  \
   X(128, 64, 2, 2, 2, 3, 2, 1200.0)   \
   X(64, 64, 2, 2, 2, 3, 2, 980.0)     \
   X(64, 32, 2, 2, 4, 3, 2, 780.0)     \

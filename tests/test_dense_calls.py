@@ -2,6 +2,7 @@
 themselves: tests/cpp/dense_calls_test.cpp (every call's launches, workspace and planes) and tests/cpp/dense_tiles_test.cpp
 (where a tile's values lie in memory and LDS)."""
 import os
+import re
 import shutil
 import subprocess
 
@@ -71,3 +72,28 @@ def test_tiles(tiles):
 @pytest.mark.parametrize("mistake,code", [("clamp", 3), ("pieces", 4)])
 def test_a_planted_mistake_in_the_tiles_is_found(tiles, mistake, code):
     assert subprocess.run([tiles, mistake], capture_output=True, timeout=100).returncode == code
+
+
+def plan_tiles():
+    """(rows, columns, planes) of every tile shape of the plan."""
+    text = open(os.path.join(CSRC, "dense_plan.hpp")).read()
+    rows = [[int(float(v)) for v in m.split(",")] for m in re.findall(r"^  X\(([^)]*)\)", text, re.M)]
+    return {(r[0], r[1], r[5]) for r in rows}
+
+
+@pytest.fixture(scope="module")
+def drawn(calls):
+    """The forms that 200000 calls of 1 to 16384 tokens take."""
+    r = subprocess.run([calls, "draw", "200000", "2"], capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0
+    return {line.split(" : ")[0].strip() for line in r.stdout.splitlines() if " : " in line}
+
+
+def test_every_tile_is_taken(drawn):
+    """Each shape of the plan is some call's."""
+    taken = set()
+    for f in drawn:
+        m = re.match(r"(?:store|gate|dgate|stats|dlogits)\.\w\w\.(\d+)x(\d+)(.*)", f)
+        if m:
+            taken.add((int(m[1]), int(m[2]), 3 if ".planes" in m[3] else 1))
+    assert plan_tiles() == taken
