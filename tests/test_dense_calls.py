@@ -97,3 +97,40 @@ def test_every_tile_is_taken(drawn):
         if m:
             taken.add((int(m[1]), int(m[2]), 3 if ".planes" in m[3] else 1))
     assert plan_tiles() == taken
+
+
+def parameters(test):
+    """The parameter sets of a test, as dicts."""
+    sets = [{}]
+    for m in test.pytestmark:
+        if m.name == "parametrize":
+            names = [n.strip() for n in m.args[0].split(",")]
+            sets = [dict(s, **dict(zip(names, v if len(names) > 1 else (v,)))) for s in sets for v in m.args[1]]
+    return sets
+
+
+def lines_of(kind, T, H, X, dtype):
+    """The calls that the GPU tests of a size make."""
+    return {"loss": [f"loss {T} {H} {X} {dtype}", f"lossgrad {T} {H} {X} {dtype} 1 1"],
+            "dx": [f"lossgrad {T} {H} {X} {dtype} 1 0"],
+            "block": [f"ffn {T} {H} {X} {dtype} 0", f"ffngrad {T} {H} {X} {dtype} 0 31"],
+            "kept": [f"ffn {T} {H} {X} {dtype} 1", f"ffngrad {T} {H} {X} {dtype} 1 31"]}[kind]
+
+
+def tested_sizes():
+    from tests import dense_sizes as more
+    from tests import test_gpu_dense as gpu
+    kinds = [("loss", gpu.test_loss_and_gradient, "V"), ("loss", gpu.test_loss_tiles, "V"), ("block", gpu.test_block, "I"),
+             ("block", gpu.test_block_tiles, "I"), ("kept", gpu.test_block_from_checkpoint, "I")]
+    sizes = [(kind, p["T"], p["H"], p[x], p["dtype"]) for kind, test, x in kinds for p in parameters(test)]
+    sizes += [("loss", p["T"], 32, p["V"], p["dtype"]) for p in parameters(gpu.test_loss_gradient_in_pieces)]
+    for kind, sized in (("loss", more.LOSS), ("dx", more.LOSS_DX), ("block", more.BLOCK), ("kept", more.KEPT)):
+        sizes += [(kind, *s) for s in sized]
+    return sizes
+
+
+def test_every_form_is_tested(calls, drawn):
+    """The GPU tests run every form of launch that drawn calls take, against 64 bits."""
+    rc, got, _ = replay(calls, [line for s in tested_sizes() for line in lines_of(*s)])
+    assert rc == 0
+    assert drawn - set(" ".join(got.values()).split()) == set()
