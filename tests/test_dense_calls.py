@@ -117,7 +117,7 @@ def lines_of(kind, T, H, X, dtype):
             "kept": [f"ffn {T} {H} {X} {dtype} 1", f"ffngrad {T} {H} {X} {dtype} 1 31"]}[kind]
 
 
-def tested_sizes():
+def sizes_run():
     from tests import dense_sizes as more
     from tests import test_gpu_dense as gpu
     kinds = [("loss", gpu.test_loss_and_gradient, "V"), ("loss", gpu.test_loss_tiles, "V"), ("block", gpu.test_block, "I"),
@@ -131,6 +131,6 @@ def tested_sizes():
 
 def test_every_form_is_tested(calls, drawn):
     """The GPU tests run every form of launch that drawn calls take, against 64 bits."""
-    rc, got, _ = replay(calls, [line for s in tested_sizes() for line in lines_of(*s)])
+    rc, got, _ = replay(calls, [line for s in sizes_run() for line in lines_of(*s)])
     assert rc == 0
     assert drawn - set(" ".join(got.values()).split()) == set()
