@@ -134,11 +134,25 @@ int dense_few_rows(const DenseShape &s, const DenseArgs &a) {
   return rows <= 8 ? 8 : rows <= 12 ? 12 : rows <= 16 || rows > 24 ? 16 : 24;
 }
 
+namespace {
+// Results leave in pieces of 16 bytes (dense_rows; d(gate, up) 4 rows at a time): whole ones, in rows that lie so.
+bool stores_fit(DenseEpi epi, const DenseArgs &a) {
+  const size_t M = (size_t)a.M;
+  switch (epi) {
+    case DENSE_STORE: return a.out_mode == 0 ? M % 8 == 0 && a.ldo % 8 == 0 && a.ldo >= M : M % 4 == 0 && a.ldo % 4 == 0 && a.ldo >= M;
+    case DENSE_GATE: return M % 16 == 0 && a.ldh % 8 == 0 && a.ldh >= M / 2;
+    case DENSE_DGATE: return M % 4 == 0 && a.ldh % 4 == 0 && a.ldh >= M;
+    case DENSE_DLOGITS: return a.ld_dl % 8 == 0 && a.ld_dl >= M;
+    case DENSE_STATS: return true;
+  }
+  return false;
+}
+}  // namespace
+
 hipError_t dense_prepare(const DenseShape &s, DenseArgs &a) {
   if (a.M <= 0 || a.N <= 0 || a.K <= 0 || (a.b_planes != 1 && a.b_planes != kPlanes) || a.stack < 1 || a.lda % 8 || a.ldb % 8)
     return hipErrorInvalidValue;
-  // (stores of 4 rows)
-  if (a.M % 4 && s.epi != DENSE_STATS && s.epi != DENSE_DLOGITS) return hipErrorInvalidValue;
+  if (!stores_fit(s.epi, a)) return hipErrorInvalidValue;
   a.k_split = split_k(a);
   a.splits = dense_split_count(a);
   if (a.splits > 1 && (s.epi != DENSE_STORE || a.out_mode != 1)) return hipErrorInvalidValue;
@@ -147,7 +161,8 @@ hipError_t dense_prepare(const DenseShape &s, DenseArgs &a) {
 
 hipError_t dense_prepare_pair(DenseArgs &a, DenseArgs &b) {
   for (DenseArgs *x : {&a, &b}) {
-    if (x->M <= 0 || x->N <= 0 || x->K <= 0 || x->b_planes != 1 || x->stack != 1 || x->lda % 8 || x->ldb % 8 || x->M % 4 || x->splits > 1 || x->K > a.K)
+    if (x->M <= 0 || x->N <= 0 || x->K <= 0 || x->b_planes != 1 || x->stack != 1 || x->lda % 8 || x->ldb % 8 || x->splits > 1 || x->K > a.K ||
+        !stores_fit(DENSE_STORE, *x))
       return hipErrorInvalidValue;
     x->k_split = split_k(*x);
   }

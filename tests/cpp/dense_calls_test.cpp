@@ -8,6 +8,7 @@
 //   dense_calls_test calls < lines      a line a call: its forms
 //   dense_calls_test draw N SEED        the forms of N drawn calls, each with the cheapest call that takes it
 //   dense_calls_test plant WHAT < lines the same as `calls` with a mistake: must find it
+//   dense_calls_test checks             products that the kernels could not store in their pieces: each must be refused
 // Lines: "loss T H V dtype", "lossgrad T H V dtype dx dw", "ffn T H I dtype x8", "ffngrad T H I dtype kept mask" (mask: bits
 // of the gradients of x, gate_up, gate_up_bias, down, down_bias).
 #include <algorithm>
@@ -472,6 +473,58 @@ int main(int argc, char **argv) {
     }
     printf("faults %ld\n", g_faults);
     return g_faults ? 3 : fine ? 0 : 4;
+  }
+  if (what == "checks") {
+    // a product that is taken, and what makes it one that is not
+    auto product = [](DenseEpi epi, size_t M) {
+      DenseArgs a{};
+      a.M = (int)M, a.N = 40, a.K = 64, a.lda = up8(M) + 64, a.ldb = 64;
+      a.splits = a.stack = a.stack_step = a.b_planes = a.planes = 1;
+      a.ldo = a.ldh = a.ld_dl = up8(M);
+      if (epi == DENSE_GATE) a.ldh = up8(M / 2);
+      return a;
+    };
+    int wrong = 0, n = 0;
+    auto expect = [&](const char *what, DenseEpi epi, DenseArgs a, bool taken) {
+      n++;
+      if ((dense_prepare(DenseShape{false, false, epi}, a) == hipSuccess) != taken) wrong++, printf("%s: %s\n", what, taken ? "refused" : "taken");
+    };
+    for (size_t M : {4, 8, 12, 16, 20, 24, 32, 36, 60, 64}) {
+      DenseArgs a = product(DENSE_STORE, M);
+      expect("bf16 results in pieces of 8", DENSE_STORE, a, M % 8 == 0);
+      a.ldo = M + 4;
+      expect("bf16 rows that are not 16 bytes apart", DENSE_STORE, a, M % 8 == 0 && a.ldo % 8 == 0);
+      for (int mode : {1, 2}) {
+        a = product(DENSE_STORE, M);
+        a.out_mode = mode;
+        expect("f32 results in pieces of 4", DENSE_STORE, a, true);
+        a.M += 2;
+        expect("f32 results of 2 more", DENSE_STORE, a, false);
+        a.M -= 2, a.ldo += 2;
+        expect("f32 rows that are not 16 bytes apart", DENSE_STORE, a, false);
+      }
+      expect("h in pieces of 8", DENSE_GATE, product(DENSE_GATE, M), M % 16 == 0);
+      a = product(DENSE_GATE, 32);
+      a.ldh += 4;
+      expect("rows of h that are not 16 bytes apart", DENSE_GATE, a, false);
+      expect("d(gate, up) in pieces of 4", DENSE_DGATE, product(DENSE_DGATE, M), true);
+      expect("d(gate, up) of 1 more", DENSE_DGATE, product(DENSE_DGATE, M + 1), false);
+      expect("dlogits", DENSE_DLOGITS, product(DENSE_DLOGITS, M + 1), true);
+      a = product(DENSE_DLOGITS, M);
+      a.ld_dl += 4;
+      expect("rows of dlogits that are not 16 bytes apart", DENSE_DLOGITS, a, false);
+      a = product(DENSE_DLOGITS, M);
+      a.ld_dl -= 8;
+      expect("rows of dlogits without room for the padding", DENSE_DLOGITS, a, false);
+      expect("logits", DENSE_STATS, product(DENSE_STATS, M + 1), true);
+      DenseArgs x = product(DENSE_STORE, M), y = product(DENSE_STORE, 64);
+      n++;
+      if ((dense_prepare_pair(x, y) == hipSuccess) != (M % 8 == 0)) wrong++, printf("a pair of %zu rows\n", M);
+      x = product(DENSE_STORE, 64), y = product(DENSE_STORE, M);
+      if ((dense_prepare_pair(x, y) == hipSuccess) != (M % 8 == 0)) wrong++, printf("a pair of %zu rows\n", M);
+    }
+    printf("checks %d wrong %d\n", n, wrong);
+    return wrong ? 3 : 0;
   }
   if (what == "draw") {
     std::mt19937_64 rng(strtoull(argv[3], nullptr, 10));

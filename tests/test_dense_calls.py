@@ -64,6 +64,12 @@ def test_a_planted_mistake_in_a_call_is_found(calls, mistake):
     assert rc == 3 and last != "faults 0"
 
 
+def test_products_that_do_not_fit_are_refused(calls):
+    """Results leave in pieces of 16 bytes: rows of another length would be written behind."""
+    r = subprocess.run([calls, "checks"], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0, r.stdout
+
+
 def test_tiles(tiles):
     r = subprocess.run([tiles], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0, r.stdout.splitlines()[-1]
