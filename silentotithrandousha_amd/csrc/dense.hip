@@ -130,17 +130,17 @@ __global__ __launch_bounds__(256) void k_rows(const DenseRowJobs a) {
   const int j = job_of(a.end);
   const unsigned block = blockIdx.x - (j ? a.end[j - 1] : 0);
   const DenseRows &d = a.d[j];
-  const size_t i = (size_t)block * 256 + threadIdx.x;  // of 8 values
+  const size_t i0 = (size_t)block * 256 + threadIdx.x, step = (size_t)d.blocks * 256;  // of 8 values
   if (d.what == ROWS_PLANES) {
     rows_planes(d, block);
   } else if (d.what == ROWS_COPY) {
     rows_copy(d, block);
   } else if (d.what == ROWS_PACK8) {
     uint8_t *codes = (uint8_t *)d.out;
-    if (i * 8 < d.n) act8_pack8((const float *)d.x, i, codes, codes + d.n);
+    for (size_t i = i0; i * 8 < d.n; i += step) act8_pack8((const float *)d.x, i, codes, codes + d.n);
   } else if (d.what == ROWS_UNPACK8) {
     const uint8_t *codes = (const uint8_t *)d.x;
-    if (i * 8 < d.n) act8_unpack8(codes, codes + d.n, i, d.n / 32, (uint16_t *)d.out, d.copies);
+    for (size_t i = i0; i * 8 < d.n; i += step) act8_unpack8(codes, codes + d.n, i, d.n / 32, (uint16_t *)d.out, d.copies);
   } else if (d.what == ROWS_SUM_BF16) {
     column_sums<256>((const uint16_t *)d.x, 0, d.n, d.cols, block, (float *)d.out);
   } else if (d.what == ROWS_SUM_F32) {
@@ -305,7 +305,6 @@ __global__ __launch_bounds__(1024) void k_loss(const float2 *stats, int parts, c
 
 hipError_t launch_rows(DenseRowJobs a, hipStream_t s) {
   const size_t blocks = a.ends();
-  if (blocks > 0xFFFFFF) return hipErrorInvalidValue;  // (2^32 threads)
   if (a.count == 1 && a.d[0].what == ROWS_PLANES)
     k_planes<<<(unsigned)blocks, 256, 0, s>>>(a.d[0]);
   else if (blocks)

@@ -47,6 +47,7 @@ int fail(int code, const char *fmt, ...) {
 
 constexpr size_t kMaxTokens = (size_t)1 << 20;  // tokens per call, as the path-level calls
 constexpr size_t kMaxInter = (size_t)1 << 20;
+constexpr size_t kMaxVocab = (size_t)1 << 28;
 
 size_t al(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -225,13 +226,19 @@ int check_loss(const DenseCtx &c, const void *x, int dtype, const int32_t *targe
   if (!c.lm_w) return fail(MOE_ERR_STATE, "the loss reads the bf16 LM head; the context holds the f32 one");
   if (!vocab || vocab > c.lm_vocab)
     return fail(MOE_ERR_INVALID, "vocab %zu outside [1, %zu]", vocab, c.lm_vocab);
-  if (vocab > 0x7FFFFF00) return fail(MOE_ERR_INVALID, "vocab %zu too large", vocab);
+  if (vocab > kMaxVocab) return fail(MOE_ERR_INVALID, "vocab %zu above %zu", vocab, kMaxVocab);
   RETURN_IF(check_tokens(T));
   if (T && (!x || !targets)) return fail(MOE_ERR_INVALID, "null x or targets");
   return check_aligned({x});
 }
 
-constexpr size_t kLossTokens = 16384;                 // tokens whose statistics are kept at once
+// tokens whose statistics are kept at once: up to 16384, and of wide heads (2^18 rows and more) so many that their
+// statistics, a maximum and a sum per 64 to 128 rows, stay below 512 MB and a launch's threads below 2^32, 256 at least
+size_t loss_tokens(size_t vocab) {
+  size_t n = 16384;
+  while (n > 256 && n * (vocab / 64) * 8 > (size_t)512 << 20) n /= 2;
+  return n;
+}
 constexpr size_t kGradTokens = 8192;                  // tokens and bytes of the logits' gradient at once
 constexpr size_t kGradBytes = (size_t)512 << 20;
 
@@ -259,7 +266,7 @@ int moe_lm_head_loss_device(moe_ctx *ctx, const void *x, int dtype, const int32_
   if (!loss || !lse) return fail(MOE_ERR_INVALID, "null loss or lse");
   RETURN_IF(check_distinct({loss, lse}, {x, targets, c.lm_w}));
   const hipStream_t s = stream ? (hipStream_t)stream : c.stream;
-  const size_t H = c.H, Tc = std::min(T, kLossTokens);
+  const size_t H = c.H, Tc = std::min(T, loss_tokens(vocab));
   const DenseShape shape{false, false, DENSE_STATS};
   Carve w;
   Rows r;

@@ -195,10 +195,10 @@ void DenseRowJobs::copy(const uint16_t *x, uint16_t *out, size_t n, const int32_
   if (n) d[count++] = DenseRows{ROWS_COPY, x, out, n, cols, 0, 0, blocks_for(n / 8), targets};
 }
 void DenseRowJobs::pack8(const float *x, size_t n, uint8_t *packed) {
-  if (n) d[count++] = DenseRows{ROWS_PACK8, x, packed, n, 0, 0, 0, (unsigned)((n / 8 + 255) / 256), nullptr};
+  if (n) d[count++] = DenseRows{ROWS_PACK8, x, packed, n, 0, 0, 0, blocks_for(n / 8), nullptr};
 }
 void DenseRowJobs::unpack8(const uint8_t *packed, size_t n, uint16_t *out, int copies) {
-  if (n) d[count++] = DenseRows{ROWS_UNPACK8, packed, out, n, 0, 0, copies, (unsigned)((n / 8 + 255) / 256), nullptr};
+  if (n) d[count++] = DenseRows{ROWS_UNPACK8, packed, out, n, 0, 0, copies, blocks_for(n / 8), nullptr};
 }
 void DenseRowJobs::column_sums(const void *x, bool bf16, size_t T, size_t H, float *out) {
   d[count++] = DenseRows{bf16 ? ROWS_SUM_BF16 : ROWS_SUM_F32, x, out, T, H, 0, 0, (unsigned)((H + 63) / 64), nullptr};

@@ -5,7 +5,7 @@
 //   * the slots of f32 rows hold the planes that the product takes them for, with infinities where they may be.
 // The form of every launch (tile, layout, planes, K parts, ...) is printed, so that a test can tell which of them its
 // sizes take.
-//   dense_calls_test calls < lines      a line a call: its forms
+//   dense_calls_test calls [BYTES] < lines   a line a call: its forms; no workspace may be above BYTES
 //   dense_calls_test draw N SEED        the forms of N drawn calls, each with the cheapest call that takes it
 //   dense_calls_test plant WHAT < lines the same as `calls` with a mistake: must find it
 //   dense_calls_test checks             products that the kernels could not store in their pieces: each must be refused
@@ -130,6 +130,11 @@ void write_slots(void *out, uint32_t where, int planes, size_t bytes) {
 const Slot *slot_at(const void *p, size_t bytes) {
   auto it = g_slots.find((uintptr_t)p);
   return it != g_slots.end() && it->second.bytes >= bytes ? &it->second : nullptr;
+}
+
+// a launch counts its threads in 32 bits
+void grid(size_t tiles, const DenseTileDims &d) {
+  if (tiles * 64 * d.wm * d.wn >> 32) fault("a grid of more threads than a launch has");
 }
 
 // ---- forms
@@ -267,6 +272,7 @@ hipError_t launch_dense(const DenseShape &s, const DenseArgs &a0, hipStream_t) {
     o << "few" << few << "." << epi_name(s.epi) << out << rows;
   } else {
     const DenseTileDims &d = kDenseTiles[dense_tile(s, a)];
+    grid((size_t)((a.M + d.bm - 1) / d.bm) * (((size_t)a.N * a.stack + d.bn - 1) / d.bn), d);
     o << epi_name(s.epi) << (s.at ? (s.bt ? ".tt" : ".tn") : ".nt") << "." << d.bm << "x" << d.bn << out << rows << (a.splits > 1 ? ".parts" : "");
   }
   form(o.str());
@@ -282,6 +288,9 @@ hipError_t launch_dense_pair(const DenseArgs &a0, const DenseArgs &b0, hipStream
   note(s, b);
   double us;
   const DenseTileDims &d = kDenseTiles[dense_pair_tile(a, b, us)];
+  size_t tiles = 0;
+  for (const DenseArgs *x : {&a, &b}) tiles += (size_t)((x->M + d.bm - 1) / d.bm) * ((x->N + d.bn - 1) / d.bn);
+  grid(tiles, d);
   form("pair." + std::to_string(d.bm) + "x" + std::to_string(d.bn) + (a.out_mode ? ".f32" : ".bf16"));
   launched();
   return hipSuccess;
@@ -368,13 +377,14 @@ hipError_t launch_zero(void *p, size_t bytes, hipStream_t) {
 }  // namespace moe
 
 static bool g_capturing;
-static size_t g_allocations;
+static size_t g_allocations, g_most = ~(size_t)0;
 extern "C" {
 hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus *s) {
   *s = g_capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone;
   return hipSuccess;
 }
 hipError_t hipMalloc(void **p, size_t bytes) {
+  if (bytes > g_most) fault("a workspace above the bound");
   *p = (void *)buffer(g_plant == "short" ? bytes - 4096 : bytes, true);
   g_allocations++;
   return hipSuccess;
@@ -458,6 +468,7 @@ bool parse(const std::string &line, Call &c) {
 int main(int argc, char **argv) {
   const std::string what = argc > 1 ? argv[1] : "";
   if (what == "calls" || what == "plant") {
+    if (what == "calls" && argc > 2) g_most = strtoull(argv[2], nullptr, 10);
     if (what == "plant") g_plant = argv[2];
     std::string line;
     Call c;

@@ -52,6 +52,17 @@ def test_calls_stay_in_their_buffers(calls):
     assert rc == 0 and last == "faults 0" and len(got) == len(set(CALLS))
 
 
+# the largest vocabularies that the head of a card holds
+WIDE = [f"loss {T} {H} {V} {dtype}" for dtype in (0, 1) for T in (1, 3, 16, 40, 300, 16384, 40000) for H, V in ((32, 2**25), (64, 2**28))]
+WIDE += [f"lossgrad {T} {H} {V} 1 {dx} {dw}" for T in (1, 16, 40) for H, V in ((32, 2**28), (64, 2**28), (2880, 10**6)) for dx, dw in ((1, 1), (1, 0), (0, 1))]
+
+
+def test_wide_heads(calls):
+    """Grids of less than 2^32 threads, statistics of a bounded size (8.6 GB: 256 tokens of 2^28 rows)."""
+    rc, got, last = replay(calls, WIDE, "calls", str(9 * 10**9))
+    assert rc == 0 and last == "faults 0" and len(got) == len(WIDE)
+
+
 def test_drawn_calls_stay_in_their_buffers(calls):
     r = subprocess.run([calls, "draw", "30000", "5"], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and r.stdout.splitlines()[-1] == "faults 0"
