@@ -41,7 +41,7 @@ enum moe_dtype {
 /* Softmax cross entropy over the LM head's first `vocab` rows (moe_init_lm_head_bf16(_device); not the
  * f32 head), at most 2^28, in pieces of the vocabulary: no logits are kept. For each of n_tokens rows x [H]:
  *   lse = log sum_v exp(x . W_v), loss = lse - x . W_target.
- * targets [n_tokens] (4-byte aligned, as are loss and lse): a negative target is ignored (loss 0, no
+ * targets [n_tokens] (4-byte aligned, as are loss, lse and dloss): a negative target is ignored (loss 0, no
  * gradient); one of vocab or more gives NaN. n_tokens 0 does nothing; at most 2^20. */
 int moe_lm_head_loss_device(moe_ctx *ctx, const void *x, int dtype, const int32_t *targets, size_t n_tokens,
                             size_t vocab, float *loss, float *lse, void *stream);

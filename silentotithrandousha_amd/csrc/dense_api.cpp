@@ -102,10 +102,10 @@ int check_dtype(int dtype) {
   if (dtype != MOE_F32 && dtype != MOE_BF16) return fail(MOE_ERR_INVALID, "dtype %d is neither MOE_F32 nor MOE_BF16", dtype);
   return MOE_OK;
 }
-// Pointers that matrix loads and stores of 16 bytes go through.
-int check_aligned(std::initializer_list<const void *> ps) {
+// Pointers that matrix loads and stores of 16 bytes go through, or values one by one (4 bytes).
+int check_aligned(std::initializer_list<const void *> ps, size_t bytes = 16) {
   for (const void *p : ps)
-    if (!aligned(p, 16)) return fail(MOE_ERR_INVALID, "device pointer %p is not 16-byte aligned", p);
+    if (!aligned(p, bytes)) return fail(MOE_ERR_INVALID, "device pointer %p is not %zu-byte aligned", p, bytes);
   return MOE_OK;
 }
 int check_tokens(size_t T) {
@@ -229,6 +229,7 @@ int check_loss(const DenseCtx &c, const void *x, int dtype, const int32_t *targe
   if (vocab > kMaxVocab) return fail(MOE_ERR_INVALID, "vocab %zu above %zu", vocab, kMaxVocab);
   RETURN_IF(check_tokens(T));
   if (T && (!x || !targets)) return fail(MOE_ERR_INVALID, "null x or targets");
+  RETURN_IF(check_aligned({targets}, 4));
   return check_aligned({x});
 }
 
@@ -264,6 +265,7 @@ int moe_lm_head_loss_device(moe_ctx *ctx, const void *x, int dtype, const int32_
   RETURN_IF(check_loss(c, x, dtype, targets, T, vocab));
   if (!T) return MOE_OK;
   if (!loss || !lse) return fail(MOE_ERR_INVALID, "null loss or lse");
+  RETURN_IF(check_aligned({loss, lse}, 4));
   RETURN_IF(check_distinct({loss, lse}, {x, targets, c.lm_w}));
   const hipStream_t s = stream ? (hipStream_t)stream : c.stream;
   const size_t H = c.H, Tc = std::min(T, loss_tokens(vocab));
@@ -317,6 +319,7 @@ int moe_lm_head_loss_backward_device(moe_ctx *ctx, const void *x, int dtype, con
   RETURN_IF(check_distinct({dx, dw}, {x, targets, lse, dloss, c.lm_w}));
   if (!T) return zero(dw, vocab * H * elem(dtype), s);
   if (!lse || !dloss) return fail(MOE_ERR_INVALID, "null lse or dloss");
+  RETURN_IF(check_aligned({lse, dloss}, 4));
   if (!dx && !dw) return MOE_OK;
   const int P = dtype == MOE_BF16 ? 1 : kPlanes;
   const bool bf = dtype == MOE_BF16;

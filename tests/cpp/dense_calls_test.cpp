@@ -6,6 +6,7 @@
 // The form of every launch (tile, layout, planes, K parts, ...) is printed, so that a test can tell which of them its
 // sizes take.
 //   dense_calls_test calls [BYTES] < lines   a line a call: its forms; no workspace may be above BYTES
+//   dense_calls_test refusals           calls that must be refused before anything is launched
 //   dense_calls_test draw N SEED        the forms of N drawn calls, each with the cheapest call that takes it
 //   dense_calls_test plant WHAT < lines the same as `calls` with a mistake: must find it
 //   dense_calls_test checks             products that the kernels could not store in their pieces: each must be refused
@@ -95,7 +96,10 @@ void write(const void *p, size_t bytes) {
 size_t extent(size_t n, size_t cols, size_t ld, size_t el) { return ((n - 1) * ld + cols) * el; }
 size_t up8(size_t v) { return (v + 7) / 8 * 8; }
 
+long g_launches;
+
 void launched() {
+  g_launches++;
   for (const Range &w : g_writes) {
     for (const Range &r : g_reads)
       if (w.at < r.at + r.bytes && r.at < w.at + w.bytes) fault("a launch writes what it reads");
@@ -536,6 +540,62 @@ int main(int argc, char **argv) {
     }
     printf("checks %d wrong %d\n", n, wrong);
     return wrong ? 3 : 0;
+  }
+  if (what == "refusals") {
+    DenseWork work;
+    moe_ctx ctx{};
+    const size_t T = 4, H = 64, V = 40, I = 24;
+    ctx.d = DenseCtx{nullptr, H, 7.0f, (const uint16_t *)buffer(V * H * 2), V, &work};
+    char *x = (char *)buffer(4096), *y = (char *)buffer(4096), *t = (char *)buffer(64), *a = (char *)buffer(64), *b = (char *)buffer(64),
+         *dw = (char *)buffer(V * H * 4), *w = (char *)buffer(1 << 16);
+    int wrong = 0, n = 0;
+    auto expect = [&](const char *what, int rc, int code = MOE_ERR_INVALID) {
+      n++;
+      if (rc != code || g_launches) wrong++, printf("%s: %d, %ld launches\n", what, rc, g_launches);
+      g_launches = 0;
+    };
+    auto loss = [&](void *x, void *t, void *a, void *b, size_t V = 40) {
+      return moe_lm_head_loss_device(&ctx, x, MOE_F32, (const int32_t *)t, T, V, (float *)a, (float *)b, nullptr);
+    };
+    auto grad = [&](void *x, void *t, void *lse, void *dloss, void *dx, void *dw, size_t V = 40) {
+      return moe_lm_head_loss_backward_device(&ctx, x, MOE_F32, (const int32_t *)t, (const float *)lse, (const float *)dloss, T, V, dx, dw, nullptr);
+    };
+    for (int off : {1, 2, 3}) {
+      expect("targets off", loss(x, t + off, a, b));
+      expect("loss off", loss(x, t, a + off, b));
+      expect("lse off", loss(x, t, a, b + off));
+      expect("targets off", grad(x, t + off, a, b, y, dw));
+      expect("lse off", grad(x, t, a + off, b, y, dw));
+      expect("dloss off", grad(x, t, a, b + off, y, dw));
+    }
+    for (int off : {2, 4, 8}) {
+      expect("x off", loss(x + off, t, a, b));
+      expect("x off", grad(x + off, t, a, b, y, dw));
+      expect("dx off", grad(x, t, a, b, y + off, dw));
+      expect("dw off", grad(x, t, a, b, y, dw + off));
+    }
+    ctx.d.lm_vocab = (size_t)1 << 29;
+    expect("a head of 2^28 rows and one", loss(x, t, a, b, ((size_t)1 << 28) + 1));
+    expect("a head of 2^28 rows and one", grad(x, t, a, b, y, dw, ((size_t)1 << 28) + 1));
+    ctx.d.lm_vocab = V;
+    expect("twice an output", loss(x, t, a, a));
+    expect("an output that is an input", grad(x, t, a, b, x, dw));
+    moe_ffn block{I, (uint16_t *)w, nullptr, (uint16_t *)(w + 8192), nullptr};
+    moe_ffn_grads g{};
+    for (int off : {2, 4, 8}) {
+      moe_ffn off_block = block;
+      off_block.down += off / 2;
+      expect("down off", moe_ffn_forward_device(&ctx, &off_block, x, MOE_F32, T, y, nullptr, nullptr));
+      expect("y off", moe_ffn_forward_device(&ctx, &block, x, MOE_F32, T, y + off, nullptr, nullptr));
+      g.gate_up_bias = (float *)(dw + off);
+      expect("bias gradient off", moe_ffn_backward_device(&ctx, &block, x, MOE_F32, y, MOE_F32, T, &g, nullptr));
+    }
+    // under capture the workspace cannot grow, and is as it was
+    g_capturing = true;
+    expect("a workspace that capture needs", loss(x, t, a, b), MOE_ERR_STATE);
+    if (work.p || work.captured) wrong++, printf("a refused call changed the workspace\n");
+    printf("refusals %d wrong %d\n", n, wrong);
+    return wrong || g_faults ? 3 : 0;
   }
   if (what == "draw") {
     std::mt19937_64 rng(strtoull(argv[3], nullptr, 10));

@@ -81,6 +81,11 @@ def test_products_that_do_not_fit_are_refused(calls):
     assert r.returncode == 0, r.stdout
 
 
+def test_refusals(calls):
+    r = subprocess.run([calls, "refusals"], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0, r.stdout
+
+
 def test_tiles(tiles):
     r = subprocess.run([tiles], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0, r.stdout.splitlines()[-1]
