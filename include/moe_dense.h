@@ -10,16 +10,24 @@
  * output may overlap an input or another output.
  *
  * Types of activations and of their gradients (`dtype`): MOE_F32, the rows that the other calls of a
- * context take and return, or MOE_BF16. Weights are bf16, biases f32. Products accumulate in f32:
- * bf16 values enter as they are, f32 values as three bf16 terms (their 24 bits, as far as those lie above 2^-126; a finite value
- * that rounds to bf16's infinity, above 3.39e38, as an infinity). An infinity or NaN among the rows makes of the results what it does in
- * f32; an infinite weight makes NaN of the results of f32 rows that it enters. The logits' gradient, the activation h and the gradients of gate and up enter the products after them in `dtype`'s
- * precision: one bf16 rounding (2^-8 relative) for MOE_BF16, none that f32 would not make for MOE_F32.
- * Results do not depend on anything but the arguments' values and the shapes: no atomics.
+ * context take and return, or MOE_BF16. Weights are bf16, biases f32. Products accumulate in f32: bf16
+ * values enter as they are, f32 values as three bf16 terms (their 24 bits, as far as those lie above
+ * 2^-126; a finite value that rounds to bf16's infinity, above 3.39e38, as an infinity). An infinity or NaN
+ * among the rows makes of the results what it does in f32; an infinite weight makes NaN of the results of
+ * f32 rows that it enters. The logits' gradient, the activation h and the gradients of gate and up enter
+ * the products after them in `dtype`'s precision: one bf16 rounding (2^-8 relative) for MOE_BF16, none that
+ * f32 would not make for MOE_F32. Results depend on the arguments' values, the shapes and which gradients
+ * are asked for, and on nothing else: no atomics.
  *
- * Workspace: the context's, which grows at need (the old one is kept if a captured graph may hold it).
- * During stream capture it cannot grow (MOE_ERR_STATE): run the same call once before. As for every
- * call of a context, calls that share one, replays of graphs that hold one included, must not overlap.
+ * Workspace: the context's, which grows at need (the old one is kept if a captured graph may hold it). A
+ * call that grows it allocates and waits for the device; lengths that rise little by little do so now and
+ * then, as it grows with room. Bytes a token, about: the loss 6 H for MOE_F32 (of up to 16384 tokens at
+ * once) and up to 512 MB; its gradient 2 H (MOE_BF16) or 12 H (MOE_F32), 4 H for dx of MOE_BF16, and up to
+ * 2 GB; the block forward 2 I or 6 (H + I), backward 14 I or 24 H + 44 I, all tokens at once, and K parts
+ * (65536 tokens of 2880 x 2880 backward: 2.7 or 14.2 GB). MOE_ERR_OOM where there is no memory for it.
+ * During stream capture it cannot grow (MOE_ERR_STATE): run the same call once before. As for every call of
+ * a context, calls that share one, replays of graphs that hold one included, must not overlap. A graph also
+ * holds the LM head: capture it again after a moe_init_lm_head_bf16(_device) with more rows.
  */
 #ifndef MOE_DENSE_H
 #define MOE_DENSE_H
@@ -38,8 +46,8 @@ enum moe_dtype {
 
 /* ------------------------------------------------------------------ loss over the LM head */
 
-/* Softmax cross entropy over the LM head's first `vocab` rows (moe_init_lm_head_bf16(_device); not the
- * f32 head), at most 2^28, in pieces of the vocabulary: no logits are kept. For each of n_tokens rows x [H]:
+/* Softmax cross entropy over the LM head's first `vocab` rows (moe_init_lm_head_bf16(_device), with the
+ * hidden sizes that it takes; not the f32 head), at most 2^28, in pieces of the vocabulary: no logits are kept. For each of n_tokens rows x [H]:
  *   lse = log sum_v exp(x . W_v), loss = lse - x . W_target.
  * targets [n_tokens] (4-byte aligned, as are loss, lse and dloss): a negative target is ignored (loss 0, no
  * gradient); one of vocab or more gives NaN. n_tokens 0 does nothing; at most 2^20. */

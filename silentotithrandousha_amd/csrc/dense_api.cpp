@@ -63,7 +63,9 @@ struct Carve {
   }
 };
 
-// Grows the context's workspace to `bytes`. A call under capture marks it: a graph may hold it.
+// Grows the context's workspace to `bytes`, a second time and later with room above them (a quarter, at most 256 MB): the
+// old one's release waits for the device, which lengths that rise by one would make every call do. A call under capture
+// marks it: a graph may hold it.
 int ensure(const DenseCtx &c, size_t bytes, hipStream_t s) {
   DenseWork &w = *c.work;
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
@@ -78,7 +80,12 @@ int ensure(const DenseCtx &c, size_t bytes, hipStream_t s) {
     if (capturing)
       return fail(MOE_ERR_STATE, "workspace too small for this call during graph capture; run it once uncaptured first");
     void *q = nullptr;
-    const hipError_t e = hipMalloc(&q, bytes);
+    size_t want = bytes + (w.p ? std::min(bytes / 4, (size_t)256 << 20) : 0);
+    hipError_t e = hipMalloc(&q, want);
+    if (e != hipSuccess && want > bytes) {
+      (void)hipGetLastError();
+      e = hipMalloc(&q, want = bytes);
+    }
     if (e != hipSuccess) {
       (void)hipGetLastError();
       return fail(MOE_ERR_OOM, "hipMalloc(%zu): %s", bytes, hipGetErrorString(e));
@@ -88,7 +95,7 @@ int ensure(const DenseCtx &c, size_t bytes, hipStream_t s) {
     else if (w.p)
       (void)hipFree(w.p);  // waits for the launches that use it
     w.p = q;
-    w.cap = bytes;
+    w.cap = want;
     w.captured = false;
   }
   w.captured |= capturing;

@@ -7,6 +7,7 @@
 // sizes take.
 //   dense_calls_test calls [BYTES] < lines   a line a call: its forms; no workspace may be above BYTES
 //   dense_calls_test refusals           calls that must be refused before anything is launched
+//   dense_calls_test growth             the workspace over calls of rising lengths
 //   dense_calls_test draw N SEED        the forms of N drawn calls, each with the cheapest call that takes it
 //   dense_calls_test plant WHAT < lines the same as `calls` with a mistake: must find it
 //   dense_calls_test checks             products that the kernels could not store in their pieces: each must be refused
@@ -381,19 +382,21 @@ hipError_t launch_zero(void *p, size_t bytes, hipStream_t) {
 }  // namespace moe
 
 static bool g_capturing;
-static size_t g_allocations, g_most = ~(size_t)0;
+static size_t g_allocations, g_frees, g_most = ~(size_t)0, g_memory = ~(size_t)0;
 extern "C" {
 hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus *s) {
   *s = g_capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone;
   return hipSuccess;
 }
 hipError_t hipMalloc(void **p, size_t bytes) {
+  if (bytes > g_memory) return hipErrorOutOfMemory;
   if (bytes > g_most) fault("a workspace above the bound");
   *p = (void *)buffer(g_plant == "short" ? bytes - 4096 : bytes, true);
   g_allocations++;
   return hipSuccess;
 }
 hipError_t hipFree(void *p) {
+  g_frees++;
   for (auto b = g_buffers.begin(); b != g_buffers.end(); ++b)
     if (b->at == (uintptr_t)p) return g_buffers.erase(b), hipSuccess;
   fault("a free of what is not allocated");
@@ -595,6 +598,45 @@ int main(int argc, char **argv) {
     expect("a workspace that capture needs", loss(x, t, a, b), MOE_ERR_STATE);
     if (work.p || work.captured) wrong++, printf("a refused call changed the workspace\n");
     printf("refusals %d wrong %d\n", n, wrong);
+    return wrong || g_faults ? 3 : 0;
+  }
+  if (what == "growth") {
+    DenseWork work;
+    moe_ctx ctx{};
+    const size_t H = 256, V = 4096, most = 4000;
+    ctx.d = DenseCtx{nullptr, H, 7.0f, (const uint16_t *)buffer(V * H * 2), V, &work};
+    void *x = (void *)buffer(most * H * 4);
+    int32_t *t = (int32_t *)buffer(most * 4);
+    float *loss = (float *)buffer(most * 4), *lse = (float *)buffer(most * 4);
+    int wrong = 0;
+    auto call = [&](size_t T, int code = MOE_OK) {
+      g_written.clear();
+      if (moe_lm_head_loss_device(&ctx, x, MOE_F32, t, T, V, loss, lse, nullptr) != code) wrong++, printf("%zu tokens: not %d\n", T, code);
+    };
+    auto check = [&](const char *what, bool holds) {
+      if (!holds) wrong++, printf("%s: %zu allocations, %zu frees, %zu bytes\n", what, g_allocations, g_frees, work.cap);
+    };
+    call(1000);
+    const size_t exact = work.cap;
+    check("the first workspace", g_allocations == 1 && g_frees == 0);
+    for (size_t T = 1001; T <= 1200; T++) call(T);
+    check("200 lengths that rise by one", g_allocations <= 3 && g_frees == g_allocations - 1 && work.cap < 2 * exact);
+    const size_t allocations = g_allocations, frees = g_frees, room = work.cap;
+    g_capturing = true;  // within the room a longer call is captured, past it it is refused and nothing changes
+    call(1201);
+    void *held = work.p;
+    call(most, MOE_ERR_STATE);
+    check("under capture", g_allocations == allocations && g_frees == frees && work.p == held && work.captured);
+    g_capturing = false;
+    g_memory = room + room / 8;  // no memory for the room above a length: the length alone
+    for (size_t T = 1210; work.cap == room && T < most; T += 10) call(T);
+    check("little memory", g_allocations == allocations + 1 && g_frees == frees && work.kept.size() == 1 && work.kept[0] == held && work.cap <= g_memory);
+    g_memory = 0;
+    const size_t cap = work.cap;
+    call(most, MOE_ERR_OOM);
+    check("no memory", work.cap == cap && g_frees == frees);
+    call(1200);
+    printf("wrong %d\n", wrong);
     return wrong || g_faults ? 3 : 0;
   }
   if (what == "draw") {

@@ -86,6 +86,12 @@ def test_refusals(calls):
     assert r.returncode == 0, r.stdout
 
 
+def test_workspace_growth(calls):
+    """Lengths that rise by one do not allocate, and wait for the device, each time."""
+    r = subprocess.run([calls, "growth"], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0, r.stdout
+
+
 def test_tiles(tiles):
     r = subprocess.run([tiles], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0, r.stdout.splitlines()[-1]
