@@ -257,6 +257,19 @@ class GpuMoeDispatcher {
                            const moe_ffn_grads &grads, void *stream = nullptr) const {
     moe_check(moe_ffn_backward_device(ctx_, &block, x, x_type, dy, dtype, T, &grads, stream));
   }
+  static size_t act8_bytes(size_t T, size_t cols) {
+    const size_t n = moe_act8_bytes(T, cols);
+    need(n || !T, "cols: a positive multiple of 32");
+    return n;
+  }
+  void act8_pack_device(const void *x, moe_dtype dtype, size_t T, size_t cols, uint8_t *packed, void *stream = nullptr) const {
+    moe_check(moe_act8_pack_device(ctx_, x, dtype, T, cols, packed, stream));
+  }
+  void act8_unpack_device(const uint8_t *packed, size_t T, size_t cols, void *out, moe_dtype dtype, void *stream = nullptr) const {
+    moe_check(moe_act8_unpack_device(ctx_, packed, T, cols, out, dtype, stream));
+  }
+  // Waits for the context's stream.
+  void synchronize() const { moe_check(moe_synchronize(ctx_)); }
 
  private:
   GpuMoeDispatcher(moe_ctx *c, size_t h, size_t i) : ctx_(c), hidden_size_(h), inter_size_(i) {}
