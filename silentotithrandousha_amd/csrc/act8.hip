@@ -10,6 +10,7 @@
 
 #include "act8.hpp"
 #include "dense.hpp"
+#include "kernels.hpp"
 
 namespace moe {
 namespace {
@@ -36,11 +37,8 @@ hipError_t launch_act8_pack(const void *x, bool bf16, size_t n, size_t cols, uin
   if (!blocks) return hipSuccess;
   if (cols % 32) return hipErrorInvalidValue;
   uint8_t *scales = packed + n * cols;
-  if (bf16)
-    k_act8_pack<<<grid_for(blocks), 256, 0, s>>>((const uint16_t *)x, blocks, packed, scales);
-  else
-    k_act8_pack<<<grid_for(blocks), 256, 0, s>>>((const float *)x, blocks, packed, scales);
-  return hipGetLastError();
+  return bf16 ? launch_own(k_act8_pack<uint16_t>, grid_for(blocks), 256, 0, s, (const uint16_t *)x, blocks, packed, scales)
+              : launch_own(k_act8_pack<float>, grid_for(blocks), 256, 0, s, (const float *)x, blocks, packed, scales);
 }
 
 hipError_t launch_act8_unpack(const uint8_t *packed, size_t n, size_t cols, void *out, bool bf16, hipStream_t s) {
@@ -48,11 +46,8 @@ hipError_t launch_act8_unpack(const uint8_t *packed, size_t n, size_t cols, void
   if (!blocks) return hipSuccess;
   if (cols % 32) return hipErrorInvalidValue;
   const uint8_t *scales = packed + n * cols;
-  if (bf16)
-    k_act8_unpack<<<grid_for(blocks), 256, 0, s>>>(packed, scales, blocks, (uint16_t *)out);
-  else
-    k_act8_unpack<<<grid_for(blocks), 256, 0, s>>>(packed, scales, blocks, (float *)out);
-  return hipGetLastError();
+  return bf16 ? launch_own(k_act8_unpack<uint16_t>, grid_for(blocks), 256, 0, s, packed, scales, blocks, (uint16_t *)out)
+              : launch_own(k_act8_unpack<float>, grid_for(blocks), 256, 0, s, packed, scales, blocks, (float *)out);
 }
 
 }  // namespace moe

@@ -306,49 +306,37 @@ __global__ __launch_bounds__(1024) void k_loss(const float2 *stats, int parts, c
 hipError_t launch_rows(DenseRowJobs a, hipStream_t s) {
   const size_t blocks = a.ends();
   if (a.count == 1 && a.d[0].what == ROWS_PLANES)
-    k_planes<<<(unsigned)blocks, 256, 0, s>>>(a.d[0]);
-  else if (blocks)
-    k_rows<<<(unsigned)blocks, 256, 0, s>>>(a);
-  return hipGetLastError();
+    return launch_own(k_planes, (unsigned)blocks, 256, 0, s, a.d[0]);
+  return blocks ? launch_own(k_rows, (unsigned)blocks, 256, 0, s, a) : hipSuccess;
 }
 
 hipError_t launch_sums(DenseSums a, hipStream_t s) {
   const size_t blocks = a.ends();
-  if (blocks) k_sums<<<(unsigned)blocks, 256, 0, s>>>(a);
-  return hipGetLastError();
+  return blocks ? launch_own(k_sums, (unsigned)blocks, 256, 0, s, a) : hipSuccess;
 }
 
 hipError_t launch_dgate(const DgateArgs &a, hipStream_t s) {
   const dim3 grid((a.I + 127) / 128, dense_dgate_parts(a.T));
   if (a.T < 1 || a.I < 8 || a.I % 8 || grid.y > 65535) return hipErrorInvalidValue;
-  if (a.planes == 1)
-    k_dgate<true><<<grid, 256, 0, s>>>(a);
-  else
-    k_dgate<false><<<grid, 256, 0, s>>>(a);
-  return hipGetLastError();
+  return launch_own(a.planes == 1 ? k_dgate<true> : k_dgate<false>, grid, 256, 0, s, a);
 }
 
 hipError_t launch_dloss_scale(const DlossScale &d, hipStream_t s) {
-  k_dloss_scale<<<1, 1024, 0, s>>>(d);
-  return hipGetLastError();
+  return launch_own(k_dloss_scale, 1, 1024, 0, s, d);
 }
 
 hipError_t launch_colsum(const void *x, bool bf16, size_t T, size_t H, float *part, hipStream_t s) {
   const dim3 grid((unsigned)((H + 63) / 64), (unsigned)dense_colsum_parts(T));
   if (!T || !H) return hipSuccess;
-  if (bf16)
-    k_colsum<<<grid, 1024, 0, s>>>((const uint16_t *)x, T, H, part);
-  else
-    k_colsum<<<grid, 1024, 0, s>>>((const float *)x, T, H, part);
-  return hipGetLastError();
+  return bf16 ? launch_own(k_colsum<uint16_t>, grid, 1024, 0, s, (const uint16_t *)x, T, H, part)
+              : launch_own(k_colsum<float>, grid, 1024, 0, s, (const float *)x, T, H, part);
 }
 
 hipError_t launch_loss(const float2 *stats, int parts, const float *picked, const int32_t *targets, size_t T,
                        int vocab, float *loss, float *lse, hipStream_t s) {
   if (!T) return hipSuccess;
   const int lt = T >= 1024 ? 4 : T >= 64 ? 2 : 0;
-  k_loss<<<(unsigned)((T + (1 << lt) - 1) >> lt), 1024, 0, s>>>(stats, parts, picked, targets, T, vocab, lt, loss, lse);
-  return hipGetLastError();
+  return launch_own(k_loss, (unsigned)((T + (1 << lt) - 1) >> lt), 1024, 0, s, stats, parts, picked, targets, T, vocab, lt, loss, lse);
 }
 
 }  // namespace moe

@@ -90,25 +90,21 @@ __global__ __launch_bounds__(64 * kWaves) void k_dense_few(const DenseArgs a) {
 }
 
 template <int ROWS>
-void launch_few(const DenseShape &s, const DenseArgs &a, hipStream_t st) {
+hipError_t launch_few(const DenseShape &s, const DenseArgs &a, hipStream_t st) {
   const unsigned grid = (unsigned)((a.M + ROWS - 1) / ROWS);
-  if (s.epi == DENSE_GATE)
-    k_dense_few<ROWS, DENSE_GATE><<<grid, 64 * kWaves, 0, st>>>(a);
-  else
-    k_dense_few<ROWS, DENSE_STORE><<<grid, 64 * kWaves, 0, st>>>(a);
+  return launch_own(s.epi == DENSE_GATE ? k_dense_few<ROWS, DENSE_GATE> : k_dense_few<ROWS, DENSE_STORE>, grid, 64 * kWaves, 0, st, a);
 }
 
 }  // namespace
 
 hipError_t launch_dense_few(const DenseShape &s, const DenseArgs &a, hipStream_t st) {
   switch (dense_few_rows(s, a)) {
-    case 8: launch_few<8>(s, a, st); break;
-    case 12: launch_few<12>(s, a, st); break;
-    case 16: launch_few<16>(s, a, st); break;
-    case 24: launch_few<24>(s, a, st); break;
+    case 8: return launch_few<8>(s, a, st);
+    case 12: return launch_few<12>(s, a, st);
+    case 16: return launch_few<16>(s, a, st);
+    case 24: return launch_few<24>(s, a, st);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 }  // namespace moe

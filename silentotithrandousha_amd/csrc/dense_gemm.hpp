@@ -672,8 +672,7 @@ hipError_t launch_dense_pair_as(const DenseArgs &a, const DenseArgs &b, hipStrea
   if (e != hipSuccess) return e;
   auto tiles = [](const DenseArgs &a) { return (size_t)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN); };
   if ((tiles(a) + tiles(b)) * 64 * WM * WN >> 32) return hipErrorInvalidValue;  // (a launch counts threads in 32 bits)
-  kernel<<<(unsigned)(tiles(a) + tiles(b)), 64 * WM * WN, bytes, st>>>(DensePair{{a, b}, (int)tiles(a)});
-  return hipGetLastError();
+  return launch_own(kernel, (unsigned)(tiles(a) + tiles(b)), 64 * WM * WN, bytes, st, DensePair{{a, b}, (int)tiles(a)});
 }
 
 template <int BM, int BN, int WM, int WN, int NS, int PL, bool AT, bool BT, int EPI>
@@ -687,8 +686,7 @@ hipError_t launch_dense_as(const DenseArgs &a, hipStream_t st) {
   if (a.b_planes != PL || (a.stack > 1 && (PL > 1 || a.N * a.stack > BN || BN > 64))) return hipErrorInvalidValue;
   if ((EPI == DENSE_GATE || EPI == DENSE_DGATE || EPI == DENSE_DLOGITS) && (PL > 1 ? a.planes == 1 : BN > 64 && a.planes > 1)) return hipErrorInvalidValue;
   if (tiles * 64 * WM * WN >> 32 || a.splits > 65535) return hipErrorInvalidValue;  // (a launch counts threads in 32 bits)
-  kernel<<<dim3((unsigned)tiles, a.splits), 64 * WM * WN, bytes, st>>>(a);
-  return hipGetLastError();
+  return launch_own(kernel, dim3((unsigned)tiles, a.splits), 64 * WM * WN, bytes, st, a);
 }
 
 }  // namespace moe

@@ -11,6 +11,15 @@
 
 namespace moe {
 
+// A launch, and its own error: hipGetLastError behind it would return any that the caller's thread has not read yet.
+template <class... P, class... A>
+hipError_t launch_own(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t s, const A &...a) {
+  return [&](P... p) {
+    void *args[] = {(void *)&p...};
+    return hipLaunchKernel((const void *)kernel, grid, block, args, lds, s);
+  }(a...);
+}
+
 // Raises a kernel's dynamic-LDS limit on the current device once per device. One DynLdsOnce per
 // kernel (a function-local static at the launch site); thread-safe; a failed call is returned
 // and retried by the next launch.

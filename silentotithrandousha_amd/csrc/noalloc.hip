@@ -61,8 +61,7 @@ hipError_t launch_zero(void *p, size_t bytes, hipStream_t s) {
   if (!bytes) return hipSuccess;
   const size_t n16 = bytes / 16, tail = bytes % 16;
   const unsigned blocks = (unsigned)std::min<size_t>((n16 + 255) / 256 + 1, 1024);
-  k_zero<<<blocks, 256, 0, s>>>(reinterpret_cast<uint4 *>(p), n16, tail);
-  return hipGetLastError();
+  return launch_own(k_zero, blocks, 256, 0, s, reinterpret_cast<uint4 *>(p), n16, tail);
 }
 
 }  // namespace moe

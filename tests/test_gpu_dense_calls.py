@@ -1,11 +1,13 @@
 """What a call of the dense operators leaves for the next one: errors, workspaces."""
+import ctypes
+
 import numpy as np
 import pytest
 
 from silentotithrandousha_amd import MOE_BF16, MOE_F32, DeviceBuffer, GatedFfn, MoeError, _ffi
-from silentotithrandousha_amd._ffi import check, lib
+from silentotithrandousha_amd._ffi import LIB_PATH, check, lib
 from tests import dense_ref as ref
-from tests.test_gpu_dense import context, dev, run_loss
+from tests.test_gpu_dense import BlockOnDevice, Out, block_case, context, dev, loss_case, run_loss
 
 pytestmark = pytest.mark.gpu
 
@@ -92,5 +94,36 @@ def test_a_wide_head():
         tol = 2.0 ** -14 + 2.0 ** -20 * np.abs(want)
         ref.assert_close(lse.get(), want, tol, "lse")
         ref.assert_close(loss.get(), want - logits[np.arange(T), targets - (V - 300)], 2 * tol, "loss")
+    finally:
+        d.close()
+
+
+def test_an_error_of_the_caller_is_not_the_calls():
+    """An allocation of the caller's own fails, and the caller has not asked for the error: the calls behind it succeed, and
+    leave it to the caller."""
+    hip = ctypes.CDLL(LIB_PATH)  # (the library's HIP runtime)
+    for name in ("hipMalloc", "hipGetLastError"):
+        getattr(hip, name).restype = ctypes.c_int
+    T, H, V, I = 20, 64, 100, 40  # noqa: E741
+    x, xv, w, wv, targets, dloss = loss_case(MOE_F32, T, H, V)
+    c = block_case(MOE_F32, T, H, I)
+    d = context(H, w)
+    try:
+        xd, td, loss, lse = run_loss(d, x, MOE_F32, targets, V)
+        b, gd, dx, dw = BlockOnDevice(c), dev(dloss), Out((T, H), MOE_F32), Out((V, H), MOE_F32)
+        packed = DeviceBuffer(d.act8_bytes(T, H))
+        hip.hipGetLastError()
+        assert hip.hipMalloc(ctypes.byref(ctypes.c_void_p()), ctypes.c_size_t(2**46)) == 2  # out of memory
+        d.lm_head_loss_device(xd, MOE_F32, td, T, V, loss, lse)
+        d.lm_head_loss_backward_device(xd, MOE_F32, td, lse, gd, T, V, dx, dw)
+        b.forward(d, MOE_F32, x8=packed)
+        b.backward(d, MOE_F32)
+        d.act8_pack_device(xd, MOE_F32, T, H, packed)
+        d.act8_unpack_device(packed, T, H, dx, MOE_F32)
+        assert hip.hipGetLastError() == 2
+        d.synchronize()
+        want = ref.Loss(xv, wv, targets, dloss.astype(np.float64), MOE_F32)
+        ref.assert_close(loss.get(), want.loss, want.loss_tol, "loss")
+        ref.assert_close(dw.get(), want.dw, want.dw_tol, "dw")
     finally:
         d.close()
