@@ -25,7 +25,10 @@ constexpr int kPairs6 = 6;
 constexpr uint32_t kWhereOne = 0x01, kWhereThree = 0x010204, kWhereLeft = 0x100C23, kWhereRight = 0x020934;
 constexpr int dense_last_slot(uint32_t where, int plane) { return 31 - __builtin_clz(where >> 8 * plane & 255); }
 
-// Epilogues.
+// Epilogues. What they leave for the next product (h, d(gate, up), the logits' gradient) is in the activations'
+// type, as the products take it: f32 in three planes, bf16 rounded once more, 2^-8. A second plane of bf16 rows would
+// double the time of the product that reads it; without the rounding a block's results were 0.0017 off (relative, 4096
+// rows), with it 0.0023 to 0.0024.
 enum DenseEpi {
   DENSE_STORE = 0,   // out (+ bias) as f32 or bf16, or added to f32
   DENSE_GATE = 1,    // rows of D are interleaved gate and up: h = act(gate, up) as bf16 planes
