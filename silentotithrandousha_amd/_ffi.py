@@ -9,9 +9,8 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmxfp4moe.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "mxfp4_moe.h")
-# every header of the library's C ABI: the MoE path, the dense operators and the Beaver-triple generator
-HEADER_PATHS = [HEADER_PATH, os.path.join(os.path.dirname(_HERE), "include", "moe_dense.h"),
-                os.path.join(os.path.dirname(_HERE), "include", "beaver32.h")]
+# every header of the library's C ABI: the MoE path, the dense and the serving operators, the Beaver-triple generator
+HEADER_PATHS = [HEADER_PATH, *(os.path.join(os.path.dirname(_HERE), "include", h) for h in ("moe_dense.h", "moe_serve.h", "beaver32.h"))]
 
 MOE_OK = 0
 MOE_ERR_INVALID = 1
@@ -24,6 +23,12 @@ MOE_ERR_IO = 6
 MOE_F32 = 0
 MOE_BF16 = 1
 MOE_MXFP8 = 2
+MOE_MXFP4 = 3
+
+MOE_SCORE_SOFTMAX = 0
+MOE_SCORE_SIGMOID = 1
+MOE_GROUP_MAX = 0
+MOE_GROUP_TOP2 = 1
 
 MOE_OPT_FUSED_DECODE = 1
 MOE_OPT_SPIN_LIMIT = 2
@@ -68,6 +73,17 @@ class GatedFfn(ctypes.Structure):
 class GatedFfnGrads(ctypes.Structure):
     """moe_ffn_grads: the device pointers that a gated block's gradients go to (None: not computed)."""
     _fields_ = [("x", _vp), ("gate_up", _vp), ("gate_up_bias", _vp), ("down", _vp), ("down_bias", _vp)]
+
+
+class Routing(ctypes.Structure):
+    """moe_routing: a rule that chooses experts (bias: a device pointer or None)."""
+    _fields_ = [("score", _int), ("normalize", _int), ("top_k", _sz), ("n_groups", _sz), ("top_groups", _sz), ("group_score", _int),
+                ("scale", _f), ("bias", _vp)]
+
+
+class Sampling(ctypes.Structure):
+    """moe_sampling: the device pointers of the rows' settings (None: 1, off, off, off)."""
+    _fields_ = [("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp)]
 
 
 # name -> (restype, argtypes)
@@ -135,6 +151,12 @@ SIGNATURES = {
     "moe_act8_bytes": (_sz, [_sz, _sz]),
     "moe_act8_pack_device": (_int, [_vp, _vp, _int, _sz, _sz, _vp, _vp]),
     "moe_act8_unpack_device": (_int, [_vp, _vp, _sz, _sz, _vp, _int, _vp]),
+    # include/moe_serve.h
+    "moe_mxfp4_quantize_device": (_int, [_vp, _vp, _int, _sz, _sz, _vp, _vp, _vp]),
+    "moe_mxfp4_matmul_device": (_int, [_vp, _vp, _sz, _sz, _vp, _vp, _int, _vp, _sz, _vp, _int, _vp]),
+    "moe_route_device": (_int, [_vp, ctypes.POINTER(Routing), _vp, _sz, _sz, _vp, _vp, _vp, _vp]),
+    "moe_route_backward_device": (_int, [_vp, ctypes.POINTER(Routing), _vp, _vp, _vp, _sz, _sz, _vp, _vp]),
+    "moe_sample_device": (_int, [_vp, ctypes.POINTER(Sampling), _vp, _sz, _vp, _sz, _sz, _vp, _vp, _vp]),
     # include/beaver32.h
     "beaver32_create": (_int, [_sz, _sz, ctypes.POINTER(_vp)]),
     "beaver32_destroy": (None, [_vp]),

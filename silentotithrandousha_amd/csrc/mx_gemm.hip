@@ -1,0 +1,144 @@
+// Products with a resident MXFP4 matrix: the rows as the product takes them, and its launches.
+#include <algorithm>
+
+#include "act8.hpp"
+#include "mx_gemm.hpp"
+
+namespace moe {
+namespace {
+
+// A wavefront a (tile, step): lane 16 g + j holds block 4 s + g of row j.
+template <int TYPE>
+__global__ __launch_bounds__(256) void k_mx_rows(MxRows r, const void *x, const uint8_t *x_scales, uint8_t *codes, uint8_t *scales) {
+  const uint32_t at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (at >= r.tiles * r.ns) return;
+  const uint32_t tile = at / r.ns, s = at % r.ns, g = lane >> 4, t = tile * 16 + (lane & 15), b = 4 * s + g;
+  const bool live = t < r.tokens && b < r.nb;
+  const size_t block = (size_t)t * r.nb + b;
+  uint8_t *out = codes + (size_t)at * r.terms * r.chunk;
+  uint32_t byte = 0;
+  if constexpr (TYPE == MOE_MXFP4) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (live) {
+      v = ((const uint4 *)x)[block];
+      byte = x_scales[block];
+    }
+    *(uint4 *)(out + lane * 16) = v;
+  } else if constexpr (TYPE == MOE_MXFP8) {
+    uint4 v[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+    if (live) {
+      v[0] = ((const uint4 *)x)[2 * block];
+      v[1] = ((const uint4 *)x)[2 * block + 1];
+      byte = x_scales[block];
+    }
+    // the MFMA's lane of group g takes values 16 g .. of the step and, in its upper half, 64 + 16 g ..
+#pragma unroll
+    for (int h = 0; h < 2; h++) *(uint4 *)(out + (g >> 1) * 1024 + ((2 * (g & 1) + h) * 16 + (lane & 15)) * 16) = v[h];
+  } else {
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = 0.0f;
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float w[8];
+        if constexpr (TYPE == MOE_BF16)
+          act8_load((const uint16_t *)x + block * 32 + 8 * i, w);
+        else
+          act8_load((const float *)x + block * 32 + 8 * i, w);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[8 * i + k] = w[k];
+      }
+    }
+    constexpr int kTerms = TYPE == MOE_BF16 ? 4 : 6;
+    split32_fp6_each<kTerms>(v, [&](int term, const u32x6v &c, uint32_t sb) {
+      if (term == 0) byte = sb;
+      uint8_t *o = out + term * 1536;
+      *(uint4 *)(o + lane * 16) = make_uint4(c[0], c[1], c[2], c[3]);
+      *(uint2 *)(o + 1024 + lane * 8) = make_uint2(c[4], c[5]);
+    });
+  }
+  scales[(((size_t)tile * r.nq + s / 4) * 64 + lane) * 4 + s % 4] = (uint8_t)byte;
+}
+
+// out[t][r] = the sum of the parts in order, and the bias.
+template <bool BF16>
+__global__ __launch_bounds__(256) void k_mx_sum(const float *part, int parts, size_t n, uint32_t rows, const float *bias, void *out) {
+  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (size_t)gridDim.x * 1024) {
+    f32x4 v = *(const f32x4 *)(part + i);
+    for (int p = 1; p < parts; p++) v = v + *(const f32x4 *)(part + p * n + i);
+    if (bias) v = v + *(const f32x4 *)(bias + i % rows);
+    if constexpr (BF16) {
+      uint16_t q[4];
+#pragma unroll
+      for (int x = 0; x < 4; x++) q[x] = __builtin_bit_cast(uint16_t, (__bf16)v[x]);
+      *(uint2 *)((uint16_t *)out + i) = __builtin_bit_cast(uint2, q);
+    } else {
+      *(f32x4 *)((float *)out + i) = v;
+    }
+  }
+}
+
+}  // namespace
+
+MxRows mx_rows(int type, size_t tokens, size_t cols) {
+  MxRows r{};
+  r.type = type;
+  r.tokens = (uint32_t)tokens;
+  r.nb = (uint32_t)(cols / 32);
+  r.ns = (r.nb + 3) / 4;
+  r.nq = (r.ns + 3) / 4;
+  r.tiles = (uint32_t)((tokens + 15) / 16);
+  r.terms = type == MOE_F32 ? 6 : type == MOE_BF16 ? 4 : 1;
+  r.chunk = type == MOE_MXFP4 ? 1024 : type == MOE_MXFP8 ? 2048 : 1536;
+  return r;
+}
+
+hipError_t launch_mx_rows(const MxRows &r, const void *x, const uint8_t *x_scales, uint8_t *codes, uint32_t *scales, hipStream_t s) {
+  const size_t n = (size_t)r.tiles * r.ns;
+  if (!n || n > (size_t)1 << 25) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)((n + 3) / 4));
+  auto go = [&](auto k) { return launch_own(k, grid, dim3(256), 0, s, r, x, x_scales, codes, (uint8_t *)scales); };
+  switch (r.type) {
+    case MOE_F32: return go(k_mx_rows<MOE_F32>);
+    case MOE_BF16: return go(k_mx_rows<MOE_BF16>);
+    case MOE_MXFP8: return go(k_mx_rows<MOE_MXFP8>);
+    case MOE_MXFP4: return go(k_mx_rows<MOE_MXFP4>);
+  }
+  return hipErrorInvalidValue;
+}
+
+namespace {
+
+// the tile of a product by its tokens
+template <int FMT, int TERMS>
+hipError_t by_tokens(const MxGemmArgs &a, hipStream_t s) {
+  if (a.r.tiles >= 64) return launch_mx_shape<MxShape<FMT, TERMS, 16, FMT == 4 ? 16 : 8, 2, 4, FMT == 4 ? 3 : 2>>(a, s);
+  if (a.r.tiles >= 4) return launch_mx_shape<MxShape<FMT, TERMS, 4, 4, 2, 2, 3>>(a, s);
+  return launch_mx_shape<MxShape<FMT, TERMS, 4, 1, 4, 1, 3>>(a, s);
+}
+
+}  // namespace
+
+int mx_gemm_splits(const MxGemmArgs &) { return 1; }
+
+hipError_t launch_mx_gemm(const MxGemmArgs &a, hipStream_t s) {
+  hipError_t e;
+  switch (a.r.type) {
+    case MOE_F32: e = by_tokens<6, 6>(a, s); break;
+    case MOE_BF16: e = by_tokens<6, 4>(a, s); break;
+    case MOE_MXFP8: e = by_tokens<8, 1>(a, s); break;
+    case MOE_MXFP4: e = by_tokens<4, 1>(a, s); break;
+    default: return hipErrorInvalidValue;
+  }
+  return e;
+}
+
+hipError_t launch_mx_sum(const float *part, int parts, size_t n, size_t rows, const float *bias, void *out, bool bf16, hipStream_t s) {
+  if (!n) return hipSuccess;
+  const unsigned grid = (unsigned)std::min<size_t>((n / 4 + 255) / 256, 8192);
+  return bf16 ? launch_own(k_mx_sum<true>, dim3(grid), dim3(256), 0, s, part, parts, n, (uint32_t)rows, bias, out)
+              : launch_own(k_mx_sum<false>, dim3(grid), dim3(256), 0, s, part, parts, n, (uint32_t)rows, bias, out);
+}
+
+}  // namespace moe

@@ -1,0 +1,70 @@
+// Host interface of the kernels behind include/moe_serve.h: MXFP4 quantisation (mx_quant.hip), products with
+// a resident MXFP4 matrix (mx_gemm.hip), routing rules (route_rule.hip), sampling (sample.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/moe_serve.h"
+#include "layout.hpp"
+
+namespace moe {
+
+hipError_t launch_mx4_quantize(const void *x, bool bf16, size_t n, size_t cols, uint8_t *blocks, uint8_t *scales, hipStream_t s);
+
+// What a product makes of its rows: tiles of 16 rows x steps of 128 values as the block-scaled MFMA's B operand
+// takes them. Step s of tile n lies at ((n ns + s) terms) * kRowChunk bytes, one chunk a term: lane l = 16 g + j holds
+// block 4 s + g of row 16 n + j, in planes of 16 (and 8 or 16) bytes a lane. Behind the tiles, a scale word per (tile, 4
+// steps, lane), byte i that of step 4 q + i: the weights' layout (layout.hpp). Several terms share the first one's
+// byte: term t's is 5 t below it, at least 1.
+struct MxRows {
+  int type;     // MOE_F32, MOE_BF16, MOE_MXFP8, MOE_MXFP4
+  uint32_t tokens, nb, ns, nq, tiles;
+  int terms, chunk;  // terms a value, bytes of a chunk
+};
+MxRows mx_rows(int type, size_t tokens, size_t cols);
+inline size_t mx_rows_code_bytes(const MxRows &r) { return (size_t)r.tiles * r.ns * r.terms * r.chunk; }
+inline size_t mx_rows_scale_bytes(const MxRows &r) { return (size_t)r.tiles * r.nq * 256; }
+hipError_t launch_mx_rows(const MxRows &r, const void *x, const uint8_t *x_scales, uint8_t *codes, uint32_t *scales, hipStream_t s);
+
+struct MxGemmArgs {
+  const uint8_t *w;      // resident matrix (layout.hpp)
+  PackDims d;
+  MxRows r;
+  const uint8_t *codes;  // rows (MxRows)
+  const uint32_t *scales;
+  const float *bias;     // [rows] or NULL
+  void *out;             // [tokens][rows]
+  bool bf16;
+  int splits;            // parts of K: out is f32 parts [splits][tokens][rows] then
+  int steps;             // MFMA steps a part
+};
+int mx_gemm_splits(const MxGemmArgs &a);  // parts worth taking
+hipError_t launch_mx_gemm(const MxGemmArgs &a, hipStream_t s);
+// out [n / rows][rows] = the sum of parts [parts][n] in order, + bias
+hipError_t launch_mx_sum(const float *part, int parts, size_t n, size_t rows, const float *bias, void *out, bool bf16, hipStream_t s);
+
+struct RouteRule {
+  int score, normalize, k, groups, top_groups, two;
+  float scale;
+  const float *bias;
+};
+hipError_t launch_route_rule(const RouteRule &r, const float *logits, size_t T, int E, int32_t *idx, float *w, int32_t *counts, hipStream_t s);
+hipError_t launch_route_rule_backward(const RouteRule &r, const float *logits, const int32_t *idx, const float *dw, size_t T, int E, float *dl,
+                                      hipStream_t s);
+
+struct SampleArgs {
+  moe_sampling rule;
+  const float *logits;
+  size_t ld;
+  const float *u;
+  uint32_t T, V;
+  int32_t *tokens;
+  float *logprob;
+  // workspace, sized by sample_workspace
+  void *work;
+};
+size_t sample_workspace(size_t T, size_t V);
+hipError_t launch_sample(const SampleArgs &a, hipStream_t s);
+
+}  // namespace moe

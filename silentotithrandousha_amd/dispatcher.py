@@ -310,6 +310,50 @@ class GpuMoeDispatcher:
     def act8_unpack_device(self, packed, n_tokens, cols, out, dtype, stream=None):
         check(lib().moe_act8_unpack_device(self._ctx, _dpn(packed), n_tokens, cols, _dpn(out), dtype, stream))
 
+    # ---- serving operators (include/moe_serve.h): device pointers (DeviceBuffer or int), enqueued without
+    # synchronisation
+    def mxfp4_quantize_device(self, x, dtype, n_rows, cols, blocks, scales, stream=None):
+        """Rows as MXFP4 in the checkpoint's layout: blocks [n_rows, cols / 32, 16] and scales [n_rows, cols / 32]."""
+        check(lib().moe_mxfp4_quantize_device(self._ctx, _dpn(x), dtype, n_rows, cols, _dpn(blocks), _dpn(scales), stream))
+
+    def mxfp4_dequant_device(self, blocks, scales, n_rows, cols, out, stream=None):
+        """The values (f32) that MXFP4 rows stand for, bit-exact with the reference's decode (weights.rs:350-423)."""
+        check(lib().moe_mxfp4_dequant_device(_dpn(blocks), _dpn(scales), n_rows, cols, _dpn(out),
+                                             lib().moe_stream(self._ctx) if stream is None else stream))
+
+    @staticmethod
+    def mxfp4_packed_size(rows, cols):
+        n = lib().moe_mxfp4_packed_size(rows, cols)
+        if n == 0:
+            raise ValueError("rows must be a multiple of 16 and cols of 32")
+        return n
+
+    def mxfp4_pack_device(self, blocks, scales, rows, cols, packed, stream=None):
+        """A matrix in the checkpoint's layout as the resident form that products read."""
+        check(lib().moe_mxfp4_pack_device(_dpn(blocks), _dpn(scales), rows, cols, _dpn(packed),
+                                          lib().moe_stream(self._ctx) if stream is None else stream))
+
+    def mxfp4_matmul_device(self, packed, rows, cols, bias, x, x_type, x_scales, n_tokens, y, dtype, stream=None):
+        """y [n_tokens, rows] = x W^T + bias with a resident MXFP4 matrix; x_type MOE_F32, MOE_BF16, MOE_MXFP8 or MOE_MXFP4."""
+        check(lib().moe_mxfp4_matmul_device(self._ctx, _dpn(packed), rows, cols, _dpn(bias), _dpn(x), x_type, _dpn(x_scales), n_tokens,
+                                            _dpn(y), dtype, stream))
+
+    def route_device(self, rule, logits, n_tokens, n_experts, idx, weights, counts=None, stream=None):
+        """The experts that a Routing rule chooses from logits [n_tokens, n_experts], their weights, and how often each
+        expert was chosen."""
+        check(lib().moe_route_device(self._ctx, ctypes.byref(rule), _dpn(logits), n_tokens, n_experts, _dpn(idx), _dpn(weights),
+                                     _dpn(counts), stream))
+
+    def route_backward_device(self, rule, logits, idx, dweights, n_tokens, n_experts, dlogits, stream=None):
+        """The gradient of sum(dweights * weights) with respect to the logits."""
+        check(lib().moe_route_backward_device(self._ctx, ctypes.byref(rule), _dpn(logits), _dpn(idx), _dpn(dweights), n_tokens, n_experts,
+                                              _dpn(dlogits), stream))
+
+    def sample_device(self, rule, logits, ld, u, n_tokens, vocab, tokens, logprob=None, stream=None):
+        """A token for each row of logits by a Sampling rule and the random numbers u, and its log probability."""
+        check(lib().moe_sample_device(self._ctx, ctypes.byref(rule), _dpn(logits), ld, _dpn(u), n_tokens, vocab, _dpn(tokens),
+                                      _dpn(logprob), stream))
+
     # ---- path level
     def router_topk(self, layer, x, top_k, want_logits=False, n_experts=None):
         x = _c(x, np.float32).reshape(-1, self.hidden_size)
