@@ -3,15 +3,17 @@
 //
 // With m the row's largest logit, a token's mass is 2^s exp((l - m) / temperature) rounded to a whole number (s = 44, less for a
 // vocabulary above 2^18): sums of masses are whole numbers of 64 bits, exact and the same in any order, so that workgroups can
-// add them up as they come. The exponential takes 64-bit arithmetic (relative error below 2^-44).
+// add them up as they come. The exponential takes 64-bit arithmetic where it has to: a mass is off by less than one.
 //
 // top-k, top-p and min-p each leave a first part of the row's falling order, so the tokens left are those above some
 // logit, and of those equal to it the first few. To find it without sorting, logits are counted (and their masses summed)
 // in 2047 bins of 1/64 of (m - l) / temperature; what lies beyond, 32 temperatures below m, has mass 0 and never matters. The
 // border of top-k or top-p lies in one bin, whose tokens are gathered and searched digit by digit.
 //
-// Launches: largest logits of chunks; masses or bins; masses above the border's bin and the tokens in it; the draw, a
-// workgroup a row. A workgroup takes a chunk of 8192 logits.
+// Launches: largest logits of chunks; masses or bins; the border's tokens (and masses above them); the draw, a workgroup a
+// row. A workgroup takes one or more chunks of 2048 logits. A row with a top-k of up to kFewK counts bins, no masses, and gathers all
+// that top-k leaves; other rows sum masses by bin, and gather the bins that hold a border. What is gathered is sorted in LDS. Should
+// it be more than kList tokens, the draw goes through the row itself.
 #include <algorithm>
 
 #include "device.hpp"
@@ -20,44 +22,33 @@
 namespace moe {
 namespace {
 
-constexpr int kChunk = 8192, kThreads = 256, kEach = kChunk / kThreads;
+constexpr int kThreads = 512, kChunk = 4 * kThreads;  // a thread has four logits of a chunk
+constexpr int kMaxSpan = 4;                            // chunks of a workgroup that looks for the largest logit
 constexpr int kBins = 2048, kTail = kBins - 1;  // bin kTail: mass 0, not counted
-constexpr int kList = 4096;                     // tokens of a border's bins that are gathered
+constexpr int kList = 4096;                     // tokens that are gathered of a row
+constexpr uint32_t kParts = 1024;                // chunks whose masses the draw holds in LDS
+constexpr uint32_t kFewK = 2048;                // top-k up to which all that it leaves is
+
+struct RowState;
 
 // Workspace of a launch over T rows.
 struct Work {
-  float *max;        // [T][chunks] largest logit of a chunk
-  uint32_t *first;   // and its first place
-  uint64_t *mass;    // [T][chunks]
+  uint2 *largest;       // [T][groups] largest logit of kMaxSpan chunks and its first place
+  uint64_t *mass;       // [T][chunks]
   uint64_t *bin_mass;   // [T][kBins]
   uint32_t *bin_count;  // [T][kBins]
   uint2 *list;          // [T][kList] key, place
-  uint32_t *listed;     // [T]
+  RowState *row;        // [T]
 };
-MOE_HD size_t work_layout(Work &w, char *p, size_t T, size_t chunks) {
-  size_t off = 0;
-  auto take = [&](size_t bytes) {
-    char *q = p + off;
-    off += (bytes + 255) / 256 * 256;
-    return q;
-  };
-  w.mass = (uint64_t *)take(T * chunks * 8);
-  w.max = (float *)take(T * chunks * 4);
-  w.first = (uint32_t *)take(T * chunks * 4);
-  w.bin_mass = (uint64_t *)take(T * kBins * 8);
-  w.bin_count = (uint32_t *)take(T * kBins * 4);
-  w.list = (uint2 *)take(T * kList * 8);
-  w.listed = (uint32_t *)take(T * 4);
-  return off;
-}
 
 struct Args {
   moe_sampling rule;
   const float *logits;
   size_t ld;
   const float *u;
-  uint32_t V, chunks;
-  int shift;
+  uint32_t V, chunks, groups;
+  int shift, span;  // span: chunks that a workgroup takes
+
   int32_t *tokens;
   float *logprob;
   Work w;
@@ -70,83 +61,130 @@ __device__ __forceinline__ uint32_t key_of(float l) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
 
+// 2^(i / 32), each its nearest 64-bit number: as many as LDS has pairs of banks, so that lanes reading different ones do not wait
+// for each other.
+constexpr int kPowersOf2 = 32;
+__device__ const double kPowers[kPowersOf2] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0,
+};
+// into LDS, by the workgroup's first lanes
+__device__ __forceinline__ void load_powers(double *s_powers) {
+  if (threadIdx.x < kPowersOf2) s_powers[threadIdx.x] = kPowers[threadIdx.x];
+}
+
 // What a row's settings make of its logits.
 struct Row {
-  float m, bins;  // largest logit; bins a unit of (m - l) / 2
-  double scale;   // log2 e / temperature
-  double unit;    // 2^shift
-  double p, min_p;
+  float m, bins;        // largest logit; bins a unit of (m - l) / 2
+  float lowest;         // a logit whose mass is 0 (or the lowest finite one)
+  double scale;         // 32 log2 e / temperature
+  double least;         // min_p 2^shift
+  double p;
+  const double *table;  // kPowers in LDS
   uint32_t k;
-  bool greedy, by_k, by_p;
-  __device__ __forceinline__ void set(const Args &a, uint32_t t, float largest) {
+  int shift;
+  bool greedy, by_k, by_p, few;
+  __device__ __forceinline__ void set(const Args &a, uint32_t t, float largest, const double *powers) {
+    table = powers;
     m = largest;
     const float temperature = a.rule.temperature ? a.rule.temperature[t] : 1.0f;
     greedy = !(temperature > 0.0f);
     bins = fminf(128.0f / temperature, 3e38f);
-    scale = 1.4426950408889634 / (double)temperature;
-    unit = (double)((uint64_t)1 << a.shift);
+    lowest = fmaxf(m - fminf(40.0f * temperature, 3e38f), -3.4e38f);
+    scale = 32 * 1.4426950408889634 / (double)temperature;
+    shift = a.shift;
     const int kk = a.rule.top_k ? a.rule.top_k[t] : 0;
     by_k = kk > 0 && (uint32_t)kk < a.V;
     k = (uint32_t)kk;
     const float pp = a.rule.top_p ? a.rule.top_p[t] : 1.0f;
     by_p = pp < 1.0f;
+    few = by_k && k <= kFewK;
     p = fmax((double)pp, 0.0);
     const float mp = a.rule.min_p ? a.rule.min_p[t] : 0.0f;
-    min_p = mp > 0.0f ? (double)mp : 0.0;
+    least = mp > 0.0f ? (double)mp * (double)((uint64_t)1 << shift) : 0.0;
   }
   __device__ __forceinline__ bool cut() const { return by_k || by_p; }
-  // exp((l - m) / temperature) as 2^(n + f), n whole and f in [-1/2, 1/2]: the Taylor series of 2^f to the 12th power is
-  // within 2^-52. l is not NaN.
-  __device__ __forceinline__ double weight(float l) const {
-    if (l == m) return 1.0;
-    const double x = fmax(((double)l - (double)m) * scale, -1000.0);
-    const double n = rint(x), f = (x - n) * 0.6931471805599453;
-    double r = 1.0 / 479001600.0;
-    r = fma(r, f, 1.0 / 39916800.0);
-    r = fma(r, f, 1.0 / 3628800.0);
-    r = fma(r, f, 1.0 / 362880.0);
-    r = fma(r, f, 1.0 / 40320.0);
-    r = fma(r, f, 1.0 / 5040.0);
-    r = fma(r, f, 1.0 / 720.0);
-    r = fma(r, f, 1.0 / 120.0);
-    r = fma(r, f, 1.0 / 24.0);
-    r = fma(r, f, 1.0 / 6.0);
-    r = fma(r, f, 0.5);
-    r = fma(r, f, 1.0);
-    r = fma(r, f, 1.0);
-    return r * __builtin_bit_cast(double, (uint64_t)(1023 + (int)n) << 52);
+  // Masses of four logits, and which of them min_p leaves (a largest logit always).
+  // exp((l - m) / temperature) = 2^(k / 32) 2^(t / 32), k whole and t in [-1/2, 1/2]: 2^(k % 32 / 32) from the table, the
+  // second factor its Taylor series to the fifth power, within 2^-48. (Of 12 powers without a table, 161 MB of logits
+  // took 70 us.)
+  __device__ __forceinline__ void masses(const float (&l)[4], uint64_t (&e)[4], bool (&stays)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      // (no logit is so far below that the power is none: those have mass 0, a NaN and -inf with them)
+      const double x = ((double)fmaxf(l[i], lowest) - (double)m) * scale;
+      const double r = x + 6755399441055744.0;  // 1.5 2^52: the low word is x rounded
+      const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, r);
+      const double t = x - (r - 6755399441055744.0);
+      double p = 3.973709984549416e-11;
+      p = fma(p, t, 9.172562701824643e-09);
+      p = fma(p, t, 1.693850972437182e-06);
+      p = fma(p, t, 0.0002345961982022468);
+      p = fma(p, t, 0.02166084939249829);
+      const uint64_t power = __builtin_bit_cast(uint64_t, table[k & 31]) + ((uint64_t)(uint32_t)((k >> 5) + shift) << 52);
+      const double f = __builtin_bit_cast(double, power), w = fma(f, p * t, f);
+      // rounded: the low bits of 2^52 + w
+      e[i] = __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+      stays[i] = least == 0.0 || l[i] == m || w >= least;
+    }
+    if (m == INFINITY)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        stays[i] = l[i] == m;
+        e[i] = stays[i] ? (uint64_t)1 << shift : 0;
+      }
   }
-  __device__ __forceinline__ uint64_t whole(double e) const {  // round(e 2^shift): the low bits of 2^52 + that
-    return __builtin_bit_cast(uint64_t, fma(e, unit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+  __device__ __forceinline__ void left(const float (&l)[4], uint64_t (&e)[4]) const {
+    bool stays[4];
+    masses(l, e, stays);
+#pragma unroll
+    for (int i = 0; i < 4; i++) e[i] = stays[i] ? e[i] : 0;
   }
-  __device__ __forceinline__ uint64_t mass(float l) const { return whole(weight(l)); }
-  // what is left of it by min_p (a largest logit always stays)
+  __device__ __forceinline__ uint64_t mass(float l) const {
+    uint64_t e[4];
+    bool stays[4];
+    masses({l, l, l, l}, e, stays);
+    return e[0];
+  }
   __device__ __forceinline__ uint64_t left(float l) const {
-    const double e = weight(l);
-    return l == m || e >= min_p ? whole(e) : 0;
+    uint64_t e[4];
+    left({l, l, l, l}, e);
+    return e[0];
   }
   __device__ __forceinline__ int bin(float l) const {
     return l == m ? 0 : (int)fminf((0.5f * m - 0.5f * l) * bins, (float)kTail);  // (halves: their difference is finite)
   }
 };
 
-// Four logits of a row from place i, -inf past its end and for a NaN.
-__device__ __forceinline__ float4 load4(const float *row, uint32_t i, uint32_t V) {
+// This thread's four logits of chunk c, as they are and -inf past the row's end; chunks past the last read the last. (What is
+// done with them waits for them: it has to come after the next loads.)
+__device__ __forceinline__ uint32_t place_of(uint32_t c) { return c * kChunk + threadIdx.x * 4; }
+__device__ __forceinline__ float4 load_chunk(const Args &a, const float *row, uint32_t c) {
   struct __attribute__((packed, aligned(4))) four { float v[4]; };
-  float4 r = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-  if (i + 4 <= V) {
+  const uint32_t i = place_of(min(c, a.chunks - 1));
+  if (c + 1 < a.chunks) {
     const four f = *(const four *)(row + i);
-    r = make_float4(f.v[0], f.v[1], f.v[2], f.v[3]);
-  } else {
-    if (i < V) r.x = row[i];
-    if (i + 1 < V) r.y = row[i + 1];
-    if (i + 2 < V) r.z = row[i + 2];
+    return make_float4(f.v[0], f.v[1], f.v[2], f.v[3]);
   }
-  r.x = fmaxf(r.x, -INFINITY);
-  r.y = fmaxf(r.y, -INFINITY);
-  r.z = fmaxf(r.z, -INFINITY);
-  r.w = fmaxf(r.w, -INFINITY);
+  float4 r = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  if (i < a.V) r.x = row[i];
+  if (i + 1 < a.V) r.y = row[i + 1];
+  if (i + 2 < a.V) r.z = row[i + 2];
+  if (i + 3 < a.V) r.w = row[i + 3];
   return r;
+}
+// a NaN counts as -inf
+__device__ __forceinline__ void logits_of(const float4 &v, float (&l)[4]) {
+  l[0] = fmaxf(v.x, -INFINITY);
+  l[1] = fmaxf(v.y, -INFINITY);
+  l[2] = fmaxf(v.z, -INFINITY);
+  l[3] = fmaxf(v.w, -INFINITY);
 }
 
 // The larger logit, of equal ones the first place.
@@ -156,35 +194,45 @@ __device__ __forceinline__ void take_larger(float &m, uint32_t &at, float o, uin
     at = oat;
   }
 }
-// over the workgroup's threads; every thread gets it
-__device__ __forceinline__ void block_largest(float &m, uint32_t &at) {
-  __shared__ float s_m[kThreads / 64];
-  __shared__ uint32_t s_at[kThreads / 64];
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) take_larger(m, at, __shfl_xor(m, x), __shfl_xor(at, x));
-  if ((threadIdx.x & 63) == 0) {
-    s_m[threadIdx.x >> 6] = m;
-    s_at[threadIdx.x >> 6] = at;
-  }
-  __syncthreads();
-  m = s_m[0];
-  at = s_at[0];
-#pragma unroll
-  for (int i = 1; i < kThreads / 64; i++) take_larger(m, at, s_m[i], s_at[i]);
-  __syncthreads();
-}
+// The row's largest logit from those of its groups of chunks, in every wavefront for itself.
 __device__ __forceinline__ void row_largest(const Args &a, uint32_t t, float &m, uint32_t &at) {
   m = -INFINITY;
   at = 0xFFFFFFFFu;
-  for (uint32_t c = threadIdx.x; c < a.chunks; c += kThreads)
-    take_larger(m, at, a.w.max[(size_t)t * a.chunks + c], a.w.first[(size_t)t * a.chunks + c]);
-  block_largest(m, at);
+  for (uint32_t g = threadIdx.x & 63; g < a.groups; g += 64) {
+    const uint2 q = a.w.largest[(size_t)t * a.groups + g];
+    take_larger(m, at, __uint_as_float(q.x), q.y);
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) take_larger(m, at, __shfl_xor(m, x), __shfl_xor(at, x));
 }
 
-__device__ __forceinline__ uint64_t wave_add(uint64_t v) {
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) v += __shfl_xor((unsigned long long)v, x);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, true);
+  return (uint64_t)hi << 32 | lo;
+}
+// the sum of the lanes up to this one
+__device__ __forceinline__ uint64_t wave_run(uint64_t v) {
+  v += dpp64<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v += dpp64<0x112, 0xF>(v);
+  v += dpp64<0x114, 0xF>(v);
+  v += dpp64<0x118, 0xF>(v);
+  v += dpp64<0x142, 0xA>(v);  // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+  v += dpp64<0x143, 0xC>(v);
   return v;
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ uint64_t wave_add(uint64_t v) { return lane_of(wave_run(v), 63); }
+// adds a wavefront's masses to its chunk's
+__device__ __forceinline__ void add_mass(const Args &a, uint32_t t, uint32_t c, uint64_t sum) {
+  const uint64_t some = __ballot(sum != 0);
+  if (!some) return;
+  const bool few = __popcll(some) <= 4;  // (their own additions are sooner done than a sum over lanes)
+  if (!few) sum = wave_add(sum);
+  if (few ? sum != 0 : (threadIdx.x & 63) == 0) atomicAdd((unsigned long long *)a.w.mass + (size_t)t * a.chunks + c, (unsigned long long)sum);
 }
 __device__ __forceinline__ uint64_t block_add(uint64_t v) {
   __shared__ uint64_t s[kThreads / 64];
@@ -200,99 +248,14 @@ __device__ __forceinline__ uint64_t block_add(uint64_t v) {
 // the sum of the threads before this one
 __device__ __forceinline__ uint64_t block_before(uint64_t v) {
   __shared__ uint64_t s[kThreads / 64];
-  uint64_t run = v;
+  const uint64_t run = wave_run(v);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t o = __shfl_up((unsigned long long)run, d);
-    if (lane >= d) run += o;
-  }
   __syncthreads();
   if (lane == 63) s[wave] = run;
   __syncthreads();
   uint64_t before = run - v;
   for (int i = 0; i < wave; i++) before += s[i];
   return before;
-}
-
-__global__ __launch_bounds__(kThreads) void k_sample_max(Args a) {
-  const uint32_t c = blockIdx.x, t = blockIdx.y;
-  const float *row = a.logits + t * a.ld;
-  float4 v[kEach / 4];
-#pragma unroll
-  for (int j = 0; j < kEach / 4; j++) v[j] = load4(row, min(c * kChunk + j * 4 * kThreads + threadIdx.x * 4, a.V), a.V);
-  float m = -INFINITY;
-  uint32_t at = 0xFFFFFFFFu;
-#pragma unroll
-  for (int j = 0; j < kEach / 4; j++) {
-    const uint32_t i = c * kChunk + j * 4 * kThreads + threadIdx.x * 4;
-    // (places rise: an equal logit does not replace one)
-    if (v[j].x > m) m = v[j].x, at = i;
-    if (v[j].y > m) m = v[j].y, at = i + 1;
-    if (v[j].z > m) m = v[j].z, at = i + 2;
-    if (v[j].w > m) m = v[j].w, at = i + 3;
-  }
-  block_largest(m, at);
-  if (threadIdx.x == 0) {
-    a.w.max[(size_t)t * a.chunks + c] = m;
-    a.w.first[(size_t)t * a.chunks + c] = at;
-  }
-  // the row's bins, a part by each of its workgroups
-  for (uint32_t b = c * kThreads + threadIdx.x; b < kBins; b += a.chunks * kThreads) {
-    a.w.bin_mass[(size_t)t * kBins + b] = 0;
-    a.w.bin_count[(size_t)t * kBins + b] = 0;
-  }
-  if (c == 0 && threadIdx.x == 0) a.w.listed[t] = 0;
-}
-
-__global__ __launch_bounds__(kThreads) void k_sample_mass(Args a) {
-  const uint32_t c = blockIdx.x, t = blockIdx.y;
-  __shared__ unsigned long long s_mass[kBins];
-  __shared__ uint32_t s_count[kBins];
-  float m;
-  uint32_t at;
-  row_largest(a, t, m, at);
-  Row r;
-  r.set(a, t, m);
-  if (r.greedy || m == -INFINITY) return;
-  const float *row = a.logits + t * a.ld;
-  const bool cut = r.cut();
-  if (cut) {
-    for (int b = threadIdx.x; b < kBins; b += kThreads) {
-      s_mass[b] = 0;
-      s_count[b] = 0;
-    }
-    __syncthreads();
-  }
-  uint64_t sum = 0;
-  for (int j = 0; j < kEach / 4; j++) {
-    const uint32_t i = c * kChunk + j * 4 * kThreads + threadIdx.x * 4;
-    const float4 v = load4(row, min(i, a.V), a.V);
-    const float l[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int x = 0; x < 4; x++) {
-      if (l[x] == -INFINITY) continue;
-      if (!cut) {
-        sum += r.left(l[x]);
-        continue;
-      }
-      const int b = r.bin(l[x]);
-      if (b == kTail) continue;
-      atomicAdd(s_count + b, 1u);
-      if (r.by_p) atomicAdd(s_mass + b, (unsigned long long)r.mass(l[x]));
-    }
-  }
-  if (!cut) {
-    sum = block_add(sum);
-    if (threadIdx.x == 0) a.w.mass[(size_t)t * a.chunks + c] = sum;
-    return;
-  }
-  __syncthreads();
-  for (int b = threadIdx.x; b < kTail; b += kThreads)
-    if (s_count[b]) {
-      atomicAdd(a.w.bin_count + (size_t)t * kBins + b, s_count[b]);
-      if (r.by_p) atomicAdd((unsigned long long *)a.w.bin_mass + (size_t)t * kBins + b, s_mass[b]);
-    }
 }
 
 // A row's bins as a workgroup holds them: each thread 8 neighbours, their running sums. Bins end at the first whose
@@ -306,13 +269,13 @@ struct Bins {
     uint32_t count;          // before it
     uint64_t mass, through;  // before it, and with it
   };
-  __device__ __forceinline__ void load(const Args &a, uint32_t t) {
+  __device__ __forceinline__ void load(const Args &a, uint32_t t, const Row &r) {
     uint64_t m = 0, n = 0;
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
       const size_t b = (size_t)t * kBins + threadIdx.x * kPer + i;
-      n += a.w.bin_count[b];
-      m += a.w.bin_mass[b];
+      if (r.by_k) n += __hip_atomic_load(a.w.bin_count + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (r.by_p && !r.few) m += __hip_atomic_load(a.w.bin_mass + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       count[i] = (uint32_t)n;
       mass[i] = m;
     }
@@ -350,62 +313,226 @@ struct Bins {
   }
 };
 
-// The bins in which a row's border may lie: that of top-k, and those of top-p for every sum that top-k may leave.
+// The bins in which a row's border may lie, whose tokens are gathered.
 struct Border {
   Bins::Found k;    // of top-k (kTail: it leaves all that has mass)
-  int p_low, p_high;
-  int lowest;       // bins before it are left whole
+  int low, high;    // of top-p, for every sum that top-k may leave; of few: all that top-k may leave
+  uint64_t before;  // the mass before bin `low`
+  bool first;       // no token lies before it
   __device__ __forceinline__ void find(const Bins &b, const Row &r) {
     k = b.first([&](uint32_t n, uint64_t) { return r.by_k && n >= r.k; });
-    p_low = p_high = kTail;
-    lowest = k.bin;
+    before = 0;
+    first = true;
+    low = 0;
+    high = min(k.bin, kTail - 1);
+    if (r.few) return;
+    low = high = kTail;
     if (r.by_p) {
-      const double low = r.p * (double)k.mass, high = r.p * (double)k.through;
-      // (a bin ends the sum if it holds a token before which the sum is not below p: at least the first bin)
-      p_low = min(b.first([&](uint32_t n, uint64_t m) { return n > 0 && (double)m >= low; }).bin, k.bin);
-      p_high = min(b.first([&](uint32_t n, uint64_t m) { return n > 0 && (double)m >= high; }).bin, k.bin);
-      lowest = min(p_low, k.bin);
+      const double least = r.p * (double)k.mass, most = r.p * (double)k.through;
+      // (top-p ends in the first bin through which the sum reaches p; every row leaves one token)
+      const Bins::Found f = b.first([&](uint32_t, uint64_t m) { return m > 0 && (double)m >= least; });
+      low = min(f.bin, k.bin);
+      before = f.mass;
+      first = f.mass == 0;
+      high = min(b.first([&](uint32_t, uint64_t m) { return m > 0 && (double)m >= most; }).bin, k.bin);
     }
   }
-  __device__ __forceinline__ bool holds(int bin) const { return (bin >= p_low && bin <= p_high) || bin == k.bin; }
+  __device__ __forceinline__ int lowest() const { return min(low, k.bin); }  // bins before it are left whole
+  __device__ __forceinline__ bool holds(int bin) const { return (bin >= low && bin <= high) || bin == k.bin; }
 };
 
-__global__ __launch_bounds__(kThreads) void k_sample_border(Args a) {
-  const uint32_t c = blockIdx.x, t = blockIdx.y;
+// What the launches leave each other of a row (a cache line apart from the next row's: every wavefront adds to it).
+struct __attribute__((aligned(256))) RowState {
+  uint2 largest;    // the row's largest logit and its first place
+  uint32_t listed;  // tokens in its list
+  uint32_t done;    // workgroups that have added their bins
+  Border border;
+};
+
+// Clears a row's bins, sums and state, a part by each of the row's workgroups.
+__device__ __forceinline__ void begin_row(const Args &a, uint32_t t) {
+  for (uint32_t b = blockIdx.x * kThreads + threadIdx.x; b < kBins; b += gridDim.x * kThreads) {
+    a.w.bin_mass[(size_t)t * kBins + b] = 0;
+    a.w.bin_count[(size_t)t * kBins + b] = 0;
+  }
+  for (uint32_t c = blockIdx.x * kThreads + threadIdx.x; c < a.chunks; c += gridDim.x * kThreads) a.w.mass[(size_t)t * a.chunks + c] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.w.row[t].listed = a.w.row[t].done = 0;
+}
+
+__global__ __launch_bounds__(kThreads) void k_sample_max(Args a) {
+  __shared__ float s_m[kThreads / 64];
+  __shared__ uint32_t s_at[kThreads / 64];
+  const uint32_t t = blockIdx.y, c0 = blockIdx.x * kMaxSpan;
+  const float *row = a.logits + t * a.ld;
+  float4 v[kMaxSpan];
+#pragma unroll
+  for (int j = 0; j < kMaxSpan; j++) v[j] = load_chunk(a, row, c0 + j);
+  begin_row(a, t);
+  float m = -INFINITY;
+  uint32_t at = 0xFFFFFFFFu;
+#pragma unroll
+  for (int j = 0; j < kMaxSpan; j++) {
+    const uint32_t i = place_of(c0 + j);
+    // (places rise: an equal logit does not replace one)
+    if (v[j].x > m) m = v[j].x, at = i;
+    if (v[j].y > m) m = v[j].y, at = i + 1;
+    if (v[j].z > m) m = v[j].z, at = i + 2;
+    if (v[j].w > m) m = v[j].w, at = i + 3;
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) take_larger(m, at, __shfl_xor(m, x), __shfl_xor(at, x));
+  if ((threadIdx.x & 63) == 0) {
+    s_m[threadIdx.x >> 6] = m;
+    s_at[threadIdx.x >> 6] = at;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < kThreads / 64; i++) take_larger(m, at, s_m[i], s_at[i]);
+    a.w.largest[(size_t)t * a.groups + blockIdx.x] = make_uint2(__float_as_uint(m), at);
+  }
+}
+
+// f(chunk, its four logits) for the workgroup's chunks, two loads ahead.
+template <class F>
+__device__ __forceinline__ void each_chunk(const Args &a, const float *row, const float4 &first, F &&f) {
+  const uint32_t c0 = blockIdx.x * a.span, c1 = min(c0 + a.span, a.chunks);
+  float4 v = first, next = load_chunk(a, row, c0 + 1);
+#pragma unroll 1
+  for (uint32_t c = c0; c < c1; c++) {
+    const float4 after = load_chunk(a, row, c + 2);
+    float l[4];
+    logits_of(v, l);
+    f(c, l);
+    v = next;
+    next = after;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void k_sample_mass(Args a) {
+  const uint32_t t = blockIdx.y;
+  __shared__ unsigned long long s_mass[kBins];
+  __shared__ uint32_t s_count[kBins];
+  __shared__ uint32_t s_done;
+  const float *row = a.logits + t * a.ld;
+  __shared__ double s_powers[kPowersOf2];
+  load_powers(s_powers);
+  const float4 v = load_chunk(a, row, blockIdx.x * a.span);
   float m;
   uint32_t at;
   row_largest(a, t, m, at);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.w.row[t].largest = make_uint2(__float_as_uint(m), at);
   Row r;
-  r.set(a, t, m);
-  if (r.greedy || m == -INFINITY || !r.cut()) return;
-  Bins bins;
-  bins.load(a, t);
-  Border border;
-  border.find(bins, r);
-  const float *row = a.logits + t * a.ld;
-  uint64_t sum = 0;
-  for (int j = 0; j < kEach / 4; j++) {
-    const uint32_t i = c * kChunk + j * 4 * kThreads + threadIdx.x * 4;
-    const float4 v = load4(row, min(i, a.V), a.V);
-    const float l[4] = {v.x, v.y, v.z, v.w};
+  r.set(a, t, m, s_powers);
+  if (r.greedy || m == -INFINITY) return;
+  if (!r.cut()) {
+    __syncthreads();
+    each_chunk(a, row, v, [&](uint32_t c, const float (&l)[4]) {
+      uint64_t e[4];
+      r.left(l, e);
+      add_mass(a, t, c, (e[0] + e[1]) + (e[2] + e[3]));
+    });
+    return;
+  }
+  const bool masses = r.by_p && !r.few;
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    s_mass[b] = 0;
+    s_count[b] = 0;
+  }
+  __syncthreads();
+  each_chunk(a, row, v, [&](uint32_t, const float (&l)[4]) {
+    uint64_t e[4];
+    bool stays[4];
+    if (masses) r.masses(l, e, stays);
 #pragma unroll
     for (int x = 0; x < 4; x++) {
-      if (l[x] == -INFINITY) continue;
       const int b = r.bin(l[x]);
       if (b == kTail) continue;
-      if (b < border.lowest) sum += r.left(l[x]);
-      if (border.holds(b)) {
-        const uint32_t n = atomicAdd(a.w.listed + t, 1u);
-        if (n < kList) a.w.list[(size_t)t * kList + n] = make_uint2(key_of(l[x]), i + x);
-      }
+      if (r.by_k) atomicAdd(s_count + b, 1u);
+      if (masses) atomicAdd(s_mass + b, (unsigned long long)e[x]);
     }
+  });
+  __syncthreads();
+  for (int b = threadIdx.x; b < kTail; b += kThreads) {
+    if (s_count[b]) atomicAdd(a.w.bin_count + (size_t)t * kBins + b, s_count[b]);
+    if (s_mass[b]) atomicAdd((unsigned long long *)a.w.bin_mass + (size_t)t * kBins + b, s_mass[b]);
   }
-  sum = block_add(sum);
-  if (threadIdx.x == 0) a.w.mass[(size_t)t * a.chunks + c] = sum;
+  // the row's last workgroup finds where its border lies
+  wait_mem();
+  __syncthreads();
+  if (threadIdx.x == 0) s_done = atomicAdd(&a.w.row[t].done, 1u);
+  __syncthreads();
+  if (s_done + 1 != gridDim.x) return;
+  Bins bins;
+  bins.load(a, t, r);
+  Border border;
+  border.find(bins, r);
+  if (threadIdx.x == 0) a.w.row[t].border = border;
 }
 
-// The border among the tokens that `each` goes through (each(f): f(key, place) for this thread's share): the largest
-// key at which the count or mass from above reaches a target, digit by digit.
+__device__ __forceinline__ bool row_of(const Args &a, uint32_t t, const double *powers, Row &r, uint32_t &at) {
+  const uint2 q = a.w.row[t].largest;
+  at = q.y;
+  r.set(a, t, __uint_as_float(q.x), powers);
+  return r.m != -INFINITY;
+}
+
+__global__ __launch_bounds__(kThreads) void k_sample_border(Args a) {
+  __shared__ double s_powers[kPowersOf2];
+  __shared__ uint2 s_held[kList];
+  __shared__ uint32_t s_n, s_at;
+  const uint32_t t = blockIdx.y;
+  load_powers(s_powers);
+  if (threadIdx.x == 0) s_n = 0;
+  const float *row = a.logits + t * a.ld;
+  const float4 v = load_chunk(a, row, blockIdx.x * a.span);
+  Row r;
+  uint32_t at;
+  const Border border = a.w.row[t].border;
+  if (!row_of(a, t, s_powers, r, at) || r.greedy || !r.cut()) return;
+  __syncthreads();
+  const int lowest = border.lowest(), most = border.k.bin == kTail ? max(border.high, lowest - 1) : border.k.bin;
+  // The border's tokens are noted in LDS and get their places in the row's list behind the loop: an atomic that waits
+  // for its result held the stream of logits up (206 MB took 68 us).
+  each_chunk(a, row, v, [&](uint32_t c, const float (&l)[4]) {
+    int b[4];
+    bool near = false, whole = false;
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+      b[x] = r.bin(l[x]);
+      near |= b[x] <= most;
+      whole |= b[x] < lowest;
+    }
+    if (!__any(near)) return;  // (few logits are)
+    if (__any(whole)) {
+      uint64_t e[4], sum = 0;
+      r.left(l, e);
+#pragma unroll
+      for (int x = 0; x < 4; x++) sum += b[x] < lowest ? e[x] : 0;
+      add_mass(a, t, c, sum);
+    }
+    uint32_t n = 0;
+#pragma unroll
+    for (int x = 0; x < 4; x++) n += b[x] < kTail && border.holds(b[x]);
+    if (!n) return;
+    uint32_t place = atomicAdd(&s_n, n);
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+      if (b[x] < kTail && border.holds(b[x])) {
+        if (place < kList) s_held[place] = make_uint2(key_of(l[x]), place_of(c) + x);
+        place++;
+      }
+  });
+  __syncthreads();
+  if (s_n == 0) return;
+  if (threadIdx.x == 0) s_at = atomicAdd(&a.w.row[t].listed, s_n);
+  __syncthreads();
+  for (uint32_t i = threadIdx.x, end = min(s_n, kList - min(s_at, (uint32_t)kList)); i < end; i += kThreads)
+    a.w.list[(size_t)t * kList + s_at + i] = s_held[i];
+}
+
+// The largest key at which a sum over the tokens from above reaches a target, digit by digit; `each` goes through this
+// thread's share of the tokens (f(key, place)).
 struct Digits {
   uint32_t key;     // that key
   uint64_t before;  // what lies above it
@@ -421,8 +548,10 @@ struct Digits {
     before = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
       __syncthreads();
-      s_sum[threadIdx.x] = 0;
-      s_ties[threadIdx.x] = 0;
+      if (threadIdx.x < 256) {
+        s_sum[threadIdx.x] = 0;
+        s_ties[threadIdx.x] = 0;
+      }
       __syncthreads();
       each([&](uint32_t k, uint32_t place) {
         if (shift < 24 && (k >> (shift + 8)) != (key >> (shift + 8))) return;
@@ -453,180 +582,308 @@ struct Digits {
   }
 };
 
+// Sorts 2^log n values (n >= 64) in LDS, the largest first: pairs within a wavefront's 64 values pass through
+// registers.
+__device__ __forceinline__ void sort_down(uint64_t *v, uint32_t n) {
+  auto meet = [](uint64_t x, uint32_t i, uint32_t size, uint32_t far) {
+    const uint64_t o = __shfl_xor((unsigned long long)x, (int)far);
+    const bool larger = ((i & far) == 0) == ((i & size) == 0);  // this place takes the larger of the two
+    return larger == (x > o) ? x : o;
+  };
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {  // (n is a multiple of 64: whole wavefronts)
+    uint64_t x = v[i];
+#pragma unroll
+    for (uint32_t size = 2; size <= 64; size <<= 1)
+#pragma unroll
+      for (uint32_t far = size >> 1; far; far >>= 1) x = meet(x, i, size, far);
+    v[i] = x;
+  }
+  __syncthreads();
+  for (uint32_t size = 128; size <= n; size <<= 1)
+    for (uint32_t far = size >> 1; far; ) {
+      if (far >= 64) {
+        for (uint32_t i = threadIdx.x; i < n / 2; i += kThreads) {
+          const uint32_t lo = (i / far) * 2 * far + i % far, hi = lo + far;
+          const uint64_t x = v[lo], y = v[hi];
+          if ((x < y) == ((lo & size) == 0)) {
+            v[lo] = y;
+            v[hi] = x;
+          }
+        }
+        __syncthreads();
+        far >>= 1;
+      } else {
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+          uint64_t x = v[i];
+#pragma unroll
+          for (uint32_t f = 32; f; f >>= 1) x = meet(x, i, size, f);
+          v[i] = x;
+        }
+        __syncthreads();
+        far = 0;
+      }
+    }
+}
+
 __global__ __launch_bounds__(kThreads) void k_sample_draw(Args a) {
+  __shared__ uint64_t s_list[kList];
   const uint32_t t = blockIdx.x;
-  float m;
-  uint32_t at;
-  row_largest(a, t, m, at);
+  // (what the row's list may hold, before it is known how much that is)
+  const uint2 early = a.w.list[(size_t)t * kList + threadIdx.x];
+  const uint32_t n = a.w.row[t].listed;
+  const Border border = a.w.row[t].border;
   Row r;
-  r.set(a, t, m);
-  if (m == -INFINITY || r.greedy) {
+  uint32_t at;
+  __shared__ double s_powers[kPowersOf2];
+  load_powers(s_powers);
+  const bool live = row_of(a, t, s_powers, r, at);
+  if (!live || r.greedy) {
     if (threadIdx.x == 0) {
-      a.tokens[t] = m == -INFINITY ? -1 : (int32_t)at;
-      if (a.logprob) a.logprob[t] = m == -INFINITY ? NAN : 0.0f;
+      a.tokens[t] = live ? (int32_t)at : -1;
+      if (a.logprob) a.logprob[t] = live ? 0.0f : NAN;
     }
     return;
   }
   const float *row = a.logits + t * a.ld;
+  // masses of the chunks, of ordinary vocabularies in LDS
+  __shared__ uint64_t s_mass[kParts];
   uint64_t *mass = a.w.mass + (size_t)t * a.chunks;
+  if (a.chunks <= kParts) {
+    for (uint32_t c = threadIdx.x; c < a.chunks; c += kThreads) s_mass[c] = mass[c];
+    mass = s_mass;
+  }
+  __syncthreads();
   // tokens above `key` are left, and of those equal to it the ones up to `last`
   uint32_t key = 0, last = 0xFFFFFFFFu;
   if (r.cut()) {
-    Bins bins;
-    bins.load(a, t);
-    Border border;
-    border.find(bins, r);
-    const uint32_t n = a.w.listed[t];
-    const uint2 *list = a.w.list + (size_t)t * kList;
-    // the tokens of the border's bins: the list, or the row again if they are too many
-    auto each = [&](auto &&f) {
-      if (n <= kList) {
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) f(list[i].x, list[i].y);
-      } else {
+    if (__builtin_expect(n <= kList, 1)) {
+      uint32_t padded = 64;
+      while (padded < n) padded <<= 1;
+      for (uint32_t i = threadIdx.x; i < padded; i += kThreads) {
+        uint64_t e = 0;  // (behind every token)
+        if (i < n) {
+          const uint2 q = i < kThreads ? early : a.w.list[(size_t)t * kList + i];
+          e = (uint64_t)q.x << 32 | (uint32_t)~q.y;
+        }
+        s_list[i] = e;
+      }
+      __syncthreads();
+      sort_down(s_list, padded);
+      // A thread's neighbours of the list, in order: up to two times four.
+      constexpr int kMost = kList / kThreads;
+      static_assert(kMost == 8, "two groups of four");
+      const uint32_t each = (padded + kThreads - 1) / kThreads, i0 = threadIdx.x * each;
+      uint32_t keys[kMost];
+      uint64_t e[kMost], above = 0, of_k = 0;
+      bool stays[kMost];
+      int bin[kMost];
+      uint32_t rank = 0;  // of the first token of the border of top-k in the list
+#pragma unroll
+      for (int g = 0; g < kMost; g += 4) {
+        float l[4];
+        uint64_t e4[4] = {0, 0, 0, 0};
+        bool stays4[4] = {false, false, false, false};
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          const uint32_t i = i0 + g + x;
+          keys[g + x] = g + x < (int)each && i < n ? (uint32_t)(s_list[i] >> 32) : 0;
+          l[x] = keys[g + x] ? of_key(keys[g + x]) : -INFINITY;
+          bin[g + x] = r.bin(l[x]);
+          rank += bin[g + x] < border.k.bin;
+        }
+        if (g < (int)each) r.masses(l, e4, stays4);
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          e[g + x] = e4[x];
+          stays[g + x] = stays4[x];
+        }
+      }
+      // top-k: a token's place in the row's order
+      const uint32_t of_few = r.few ? 0u : border.k.count - (uint32_t)block_add(rank);  // (tokens before the list, for those of its border)
+      uint64_t Z = r.few ? 0 : border.k.mass;
+#pragma unroll
+      for (int x = 0; x < kMost; x++) {
+        const bool in_k = r.few ? i0 + x < r.k : bin[x] == border.k.bin && of_few + i0 + x < r.k;
+        if (in_k) of_k += e[x];
+        above += e[x];
+      }
+      if (r.by_p) Z += block_add(of_k);
+      const double P = r.p * (double)Z;
+      uint64_t run = border.before + block_before(above);
+      bool keep[kMost];
+      uint32_t kept = 0;
+#pragma unroll
+      for (int x = 0; x < kMost; x++) {
+        const uint32_t i = i0 + x;
+        keep[x] = keys[x] != 0;
+        if (r.by_k && (r.few || bin[x] == border.k.bin)) keep[x] &= of_few + i < r.k;
+        if (r.by_p) keep[x] &= (bin[x] <= border.high && (double)run < P) || (i == 0 && border.first);
+        run += e[x];
+        kept += keep[x];
+        if (keep[x] && stays[x])
+          atomicAdd((unsigned long long *)mass + ~(uint32_t)s_list[i] / kChunk, (unsigned long long)e[x]);
+      }
+      kept = (uint32_t)block_add(kept);  // they are the list's first
+      if (kept) {
+        key = (uint32_t)(s_list[kept - 1] >> 32);
+        last = ~(uint32_t)s_list[kept - 1];
+      }
+    } else {
+      auto each = [&](auto &&f) {
         for (uint32_t i = threadIdx.x; i < a.V; i += kThreads) {
           const float l = fmaxf(row[i], -INFINITY);
-          if (l == -INFINITY) continue;
-          const int b = r.bin(l);
-          if (b != kTail && border.holds(b)) f(key_of(l), i);
+          if (l != -INFINITY) f(key_of(l), i);
         }
-      }
-    };
-    auto in_bin = [&](int bin) {
-      return [&, bin](auto &&f) {
-        each([&](uint32_t k, uint32_t place) {
-          if (r.bin(of_key(k)) == bin) f(k, place);
-        });
       };
-    };
-    uint32_t keep = 0;  // of the tokens equal to `key`
-    bool found = false;
-    uint64_t Z = border.k.through;  // the masses that top-k leaves
-    if (border.k.bin != kTail) {
-      const uint32_t want = r.k - border.k.count;
-      Digits d;
-      d.find(in_bin(border.k.bin), [](uint32_t, uint32_t) { return 1ull; }, [&](uint64_t s) { return s >= want; });
-      key = d.key;
-      keep = want - (uint32_t)d.before;
-      found = true;
-      if (r.by_p) {
-        uint64_t sum = 0;
-        in_bin(border.k.bin)([&](uint32_t k, uint32_t) {
-          if (k > key) sum += r.mass(of_key(k));
-        });
-        Z = border.k.mass + block_add(sum) + keep * r.mass(of_key(key));
-      }
-    }
-    if (r.by_p) {
-      const double P = r.p * (double)Z;
-      const Bins::Found b = bins.first([&](uint32_t c, uint64_t s) { return c > 0 && (double)s >= P; });
-      const int bin = min(b.bin, border.k.bin);
-      if (bin != kTail) {
+      auto sum = [&](auto &&what) {
+        uint64_t s = 0;
+        each([&](uint32_t k, uint32_t place) { s += what(k, place); });
+        return block_add(s);
+      };
+      const uint64_t tokens = sum([](uint32_t, uint32_t) { return 1ull; });
+      uint64_t keep = 0xFFFFFFFFull;  // of the tokens equal to `key`
+      uint64_t Z = 0;
+      if (r.by_k && r.k < tokens) {
         Digits d;
-        d.find(in_bin(bin), [&](uint32_t k, uint32_t) { return r.mass(of_key(k)); },
-               [&](uint64_t s) { return (double)(b.mass + s) >= P; });
+        d.find(each, [](uint32_t, uint32_t) { return 1ull; }, [&](uint64_t s) { return s >= r.k; });
+        key = d.key;
+        keep = r.k - d.before;
+        if (r.by_p) Z = sum([&](uint32_t k, uint32_t) { return k > key ? r.mass(of_key(k)) : 0ull; }) + keep * r.mass(of_key(key));
+      } else if (r.by_p) {
+        Z = sum([&](uint32_t k, uint32_t) { return r.mass(of_key(k)); });
+      }
+      if (r.by_p) {
+        const double P = r.p * (double)Z;
+        Digits d;
+        d.find(each, [&](uint32_t k, uint32_t) { return r.mass(of_key(k)); }, [&](uint64_t s) { return s > 0 && (double)s >= P; });
         // of equal tokens the i-th is left if the sum before it, before + i one, is below P
         const uint64_t one = d.here / max(d.ties, 1u);
-        uint64_t few = d.ties;
+        uint64_t some = d.ties;
         if (one) {
-          const double rest = (P - (double)(b.mass + d.before)) / (double)one;
-          few = rest > 0.0 ? (uint64_t)fmin(ceil(rest), (double)d.ties) : 0;
+          const double rest = (P - (double)d.before) / (double)one;
+          some = rest > 0.0 ? (uint64_t)fmin(ceil(rest), (double)d.ties) : 0;
         }
-        few = max(few, (uint64_t)1);
-        if (!found || d.key > key || (d.key == key && few < keep)) {
+        some = max(some, (uint64_t)1);
+        if (d.key > key || (d.key == key && some < keep)) {
           key = d.key;
-          keep = (uint32_t)few;
+          keep = some;
         }
-        found = true;
       }
+      if (key) {
+        Digits d;  // the keep-th place of those equal to key
+        d.find([&](auto &&f) { each([&](uint32_t k, uint32_t place) { if (k == key) f(~place, place); }); },
+               [](uint32_t, uint32_t) { return 1ull; }, [&](uint64_t s) { return s >= keep; });
+        last = ~d.key;
+      }
+      for (uint32_t c = threadIdx.x; c < a.chunks; c += kThreads) __hip_atomic_store(mass + c, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      wait_mem();
+      __syncthreads();
+      each([&](uint32_t k, uint32_t place) {
+        if (k > key || (k == key && place <= last)) {
+          const uint64_t e = r.left(of_key(k));
+          if (e) atomicAdd((unsigned long long *)mass + place / kChunk, (unsigned long long)e);
+        }
+      });
     }
-    if (found) {
-      Digits d;  // the keep-th place of those equal to key
-      d.find([&](auto &&f) { each([&](uint32_t k, uint32_t place) { if (k == key) f(~place, place); }); },
-             [](uint32_t, uint32_t) { return 1ull; }, [&](uint64_t s) { return s >= keep; });
-      last = ~d.key;
-    }
-    // their masses, beside those of the bins before
-    each([&](uint32_t k, uint32_t place) {
-      if (r.bin(of_key(k)) >= border.lowest && (k > key || (k == key && place <= last)))
-        atomicAdd((unsigned long long *)mass + place / kChunk, (unsigned long long)r.left(of_key(k)));
-    });
-    __threadfence();
+    wait_mem();  // (the sums of chunks are atomics, read as such: no cache has to be written back)
     __syncthreads();
   }
   // the chunk in which the running sum passes u
   __shared__ uint32_t s_chunk;
-  __shared__ uint64_t s_rest;
-  uint64_t total = 0;
-  for (uint32_t c = threadIdx.x; c < a.chunks; c += kThreads) total += __hip_atomic_load(mass + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  total = block_add(total);
-  const double u = fmin(fmax((double)a.u[t], 0.0), 1.0);
-  uint64_t target = min((uint64_t)(u * (double)total), total - 1);
-  uint64_t base = 0;
-  for (uint32_t c0 = 0; c0 < a.chunks; c0 += kThreads) {
-    const uint32_t c = c0 + threadIdx.x;
-    const uint64_t v = c < a.chunks ? __hip_atomic_load(mass + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
-    const uint64_t before = base + block_before(v);
-    if (before <= target && target < before + v) {
-      s_chunk = c;
-      s_rest = target - before;
+  __shared__ uint64_t s_rest, s_total;
+  if (threadIdx.x < 64) {
+    auto of_chunk = [&](uint32_t c) { return c < a.chunks ? __hip_atomic_load(mass + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0; };
+    uint64_t total = 0;
+    for (uint32_t c = threadIdx.x; c < a.chunks; c += 64) total += of_chunk(c);
+    total = wave_add(total);
+    const double u = fmin(fmax((double)a.u[t], 0.0), 1.0);
+    const uint64_t target = min((uint64_t)(u * (double)total), total - 1);
+    uint64_t base = 0;
+    for (uint32_t c0 = 0; c0 < a.chunks; c0 += 64) {
+      const uint64_t v = of_chunk(c0 + threadIdx.x);
+      const uint64_t run = wave_run(v);
+      const uint64_t before = base + run - v;
+      if (before <= target && target < before + v) {
+        s_chunk = c0 + threadIdx.x;
+        s_rest = target - before;
+        s_total = total;
+      }
+      base += lane_of(run, 63);
     }
-    base += block_add(v);
   }
   __syncthreads();
-  // and the token in it, a thread 32 neighbours
-  const uint32_t i0 = s_chunk * kChunk + threadIdx.x * kEach;
+  const uint64_t total = s_total;
+  // and the token in it, a thread 4 neighbours
+  const uint32_t i0 = place_of(s_chunk);
   const uint64_t rest = s_rest;
-  uint64_t masses[kEach], sum = 0;
+  const float4 v = load_chunk(a, row, s_chunk);
+  float l[4];
+  logits_of(v, l);
+  uint64_t e[4];
+  r.left(l, e);
 #pragma unroll
-  for (int j = 0; j < kEach / 4; j++) {
-    const float4 v = load4(row, min(i0 + 4 * j, a.V), a.V);
-    const float l[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int x = 0; x < 4; x++) {
-      const uint32_t k = key_of(l[x]);
-      uint64_t e = 0;
-      if (l[x] != -INFINITY && (k > key || (k == key && i0 + 4 * j + x <= last))) e = r.left(l[x]);
-      masses[4 * j + x] = e;
-      sum += e;
-    }
+  for (int x = 0; x < 4; x++) {
+    const uint32_t k = key_of(l[x]);
+    if (k < key || (k == key && i0 + x > last)) e[x] = 0;
   }
+  const uint64_t sum = (e[0] + e[1]) + (e[2] + e[3]);
   uint64_t before = block_before(sum);
   if (before <= rest && rest < before + sum) {
-    uint32_t found = i0;
-    bool done = false;
-#pragma unroll
-    for (int j = 0; j < kEach; j++) {
-      if (!done && rest < before + masses[j]) {
-        found = i0 + j;
-        done = true;
-      }
-      before += masses[j];
-    }
-    a.tokens[t] = (int32_t)found;
+    uint32_t x = 0;
+    while (x < 3 && rest >= before + e[x]) before += e[x++];
+    a.tokens[t] = (int32_t)(i0 + x);
     if (a.logprob) {
-      const float l = row[found];
-      const double z = l == m ? 0.0 : ((double)l - (double)m) * r.scale * 0.6931471805599453;
-      a.logprob[t] = (float)(z - log((double)total / r.unit));
+      const double z = l[x] == r.m ? 0.0 : ((double)l[x] - (double)r.m) * r.scale * (0.6931471805599453 / 32);
+      a.logprob[t] = (float)(z - log(ldexp((double)total, -r.shift)));
     }
   }
+}
+
+size_t work_layout(Work &w, char *p, size_t T, size_t chunks, size_t groups) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char *q = p + off;
+    off += (bytes + 255) / 256 * 256;
+    return q;
+  };
+  w.row = (RowState *)take(T * sizeof(RowState));
+  w.mass = (uint64_t *)take(T * chunks * 8);
+  w.largest = (uint2 *)take(T * groups * 8);
+  w.bin_mass = (uint64_t *)take(T * kBins * 8);
+  w.bin_count = (uint32_t *)take(T * kBins * 4);
+  w.list = (uint2 *)take(T * kList * 8);
+  return off;
 }
 
 }  // namespace
 
 static uint32_t sample_chunks(size_t V) { return (uint32_t)((V + kChunk - 1) / kChunk); }
+static uint32_t sample_groups(uint32_t chunks) { return (chunks + kMaxSpan - 1) / kMaxSpan; }
 
 size_t sample_workspace(size_t T, size_t V) {
   Work w;
-  return work_layout(w, nullptr, T, sample_chunks(V));
+  return work_layout(w, nullptr, T, sample_chunks(V), sample_groups(sample_chunks(V)));
 }
 
 hipError_t launch_sample(const SampleArgs &s, hipStream_t st) {
   if (!s.T || s.T > 65535 || !s.V || s.V > 1u << 28 || s.ld < s.V) return hipErrorInvalidValue;
-  Args a{s.rule, s.logits, s.ld, s.u, s.V, sample_chunks(s.V), 44, s.tokens, s.logprob, {}};
-  while (a.shift > 62 - 32 && ((uint64_t)s.V << a.shift) > (uint64_t)1 << 62) a.shift--;
-  work_layout(a.w, (char *)s.work, s.T, a.chunks);
-  const dim3 grid(a.chunks, s.T);
-  hipError_t e = launch_own(k_sample_max, grid, kThreads, 0, st, a);
+  Args a{};
+  a.rule = s.rule;
+  a.logits = s.logits;
+  a.ld = s.ld;
+  a.u = s.u;
+  a.V = s.V;
+  a.chunks = sample_chunks(s.V);
+  a.groups = sample_groups(a.chunks);
+  a.shift = 44;
+  while (((uint64_t)s.V << a.shift) > (uint64_t)1 << 62) a.shift--;
+  a.tokens = s.tokens;
+  a.logprob = s.logprob;
+  work_layout(a.w, (char *)s.work, s.T, a.chunks, a.groups);
+  // up to 3 workgroups a CU, each of which adds its bins to the row's once
+  a.span = (int)(((size_t)s.T * a.chunks + 767) / 768);
+  const dim3 grid((a.chunks + a.span - 1) / a.span, s.T);
+  hipError_t e = launch_own(k_sample_max, dim3(a.groups, s.T), kThreads, 0, st, a);
   if (e == hipSuccess) e = launch_own(k_sample_mass, grid, kThreads, 0, st, a);
   if (e == hipSuccess && (s.rule.top_k || s.rule.top_p)) e = launch_own(k_sample_border, grid, kThreads, 0, st, a);
   if (e == hipSuccess) e = launch_own(k_sample_draw, dim3(s.T), kThreads, 0, st, a);
