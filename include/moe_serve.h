@@ -50,8 +50,7 @@ int moe_mxfp4_quantize_device(moe_ctx *ctx, const void *x, int dtype, size_t n_r
  * absolute. A row that holds a value that is not finite, or a scale byte of 255, gives NaN, as does a scale
  * byte of 255 in W; a scale byte of 0 counts as 2^-127. packed, x, y and bias are 16-byte aligned; rows is a
  * multiple of 16, at most 2^24, cols of 32, at most 2^20. Workspace: the rows as the product takes them, 0.53 cols
- * bytes a token for MOE_MXFP4, 1.03 for MOE_MXFP8, 3.03 for MOE_BF16 and 4.53 for MOE_F32, and f32 parts of y
- * for few rows. */
+ * bytes a token for MOE_MXFP4, 1.03 for MOE_MXFP8, 3.03 for MOE_BF16 and 4.53 for MOE_F32. */
 int moe_mxfp4_matmul_device(moe_ctx *ctx, const uint8_t *packed, size_t rows, size_t cols, const float *bias,
                             const void *x, int x_type, const uint8_t *x_scales, size_t n_tokens, void *y, int dtype,
                             void *stream);

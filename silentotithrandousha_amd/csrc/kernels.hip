@@ -907,24 +907,6 @@ __device__ __forceinline__ void decode_block_f32(uint4 raw, uint32_t sbyte, floa
   }
 }
 
-__global__ __launch_bounds__(256) void k_dequant_hf(const uint8_t *blocks, const uint8_t *scales,
-                                                    size_t n_blocks, float *out) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n_blocks) return;
-  const uint4 raw = reinterpret_cast<const uint4 *>(blocks)[i];
-  decode_block_f32(raw, scales[i], out + i * 32);
-}
-
-hipError_t launch_dequant_hf(const uint8_t *blocks, const uint8_t *scales, size_t rows,
-                             size_t cols, float *out, hipStream_t s) {
-  if (cols % 32) return hipErrorInvalidValue;
-  const size_t n = rows * (cols / 32);
-  if (!n) return hipSuccess;
-  hipLaunchKernelGGL(k_dequant_hf, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, blocks,
-                     scales, n, out);
-  return hipGetLastError();
-}
-
 __global__ __launch_bounds__(256) void k_dequant_packed(const uint8_t *packed, PackDims d,
                                                         float *out) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;

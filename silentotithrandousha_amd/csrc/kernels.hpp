@@ -233,6 +233,7 @@ hipError_t launch_gemv(GemvMode mode, const GemvArgs &a, hipStream_t s);
 hipError_t launch_combine(const float *o, const int32_t *pos, const float *w, int T, int k, int H,
                           int skip_nonfinite, const float *resid, float *y, hipStream_t s);
 hipError_t launch_split(const float *x, size_t n_rows, size_t K, uint16_t *xsplit, hipStream_t s);
+// (mx_quant.hip)
 hipError_t launch_dequant_hf(const uint8_t *blocks, const uint8_t *scales, size_t rows,
                              size_t cols, float *out, hipStream_t s);
 hipError_t launch_dequant_packed(const uint8_t *packed, size_t rows, size_t cols, float *out,

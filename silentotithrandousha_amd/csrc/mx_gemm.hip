@@ -1,5 +1,6 @@
 // Products with a resident MXFP4 matrix: the rows as the product takes them, and its launches.
 #include <algorithm>
+#include <cmath>
 
 #include "act8.hpp"
 #include "mx_gemm.hpp"
@@ -61,24 +62,6 @@ __global__ __launch_bounds__(256) void k_mx_rows(MxRows r, const void *x, const 
   scales[(((size_t)tile * r.nq + s / 4) * 64 + lane) * 4 + s % 4] = (uint8_t)byte;
 }
 
-// out[t][r] = the sum of the parts in order, and the bias.
-template <bool BF16>
-__global__ __launch_bounds__(256) void k_mx_sum(const float *part, int parts, size_t n, uint32_t rows, const float *bias, void *out) {
-  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (size_t)gridDim.x * 1024) {
-    f32x4 v = *(const f32x4 *)(part + i);
-    for (int p = 1; p < parts; p++) v = v + *(const f32x4 *)(part + p * n + i);
-    if (bias) v = v + *(const f32x4 *)(bias + i % rows);
-    if constexpr (BF16) {
-      uint16_t q[4];
-#pragma unroll
-      for (int x = 0; x < 4; x++) q[x] = __builtin_bit_cast(uint16_t, (__bf16)v[x]);
-      *(uint2 *)((uint16_t *)out + i) = __builtin_bit_cast(uint2, q);
-    } else {
-      *(f32x4 *)((float *)out + i) = v;
-    }
-  }
-}
-
 }  // namespace
 
 MxRows mx_rows(int type, size_t tokens, size_t cols) {
@@ -110,35 +93,42 @@ hipError_t launch_mx_rows(const MxRows &r, const void *x, const uint8_t *x_scale
 
 namespace {
 
-// the tile of a product by its tokens
+enum Form { FEW, SMALL, MIDDLE, LARGE };
+
+// The form of a product. Few rows, and matrices that fill less than 150 tiles of 64 x 64, split K over a workgroup's wavefronts
+// (mx_few.hip: 1024 bf16 rows over 512 x 2880 22 us, 64 x 64 tiles 28; 128 over 5760 x 2880 22 and 21). Otherwise the tile whose
+// workgroups take least, in units of 2880 bf16 values: a 64 x 64 tile 16 us alone and 12 among others (of which a CU holds
+// several), a 128 x 128 one 25 and 26, a 192 x 256 one 62 (a CU holds one, so the last round counts whole); the other types' times
+// stand in the same ratios within a fifth.
+Form form_of(const MxGemmArgs &a) {
+  auto groups = [&](size_t m, size_t n) { return (double)((a.d.tiles + m - 1) / m * ((a.r.tiles + n - 1) / n)) / 256.0; };
+  if (a.r.tiles <= 4 || groups(4, 4) * 256 < 150) return FEW;
+  const double small = std::max(16.0, 12.0 * groups(4, 4)), middle = std::max(25.0, 26.0 * groups(8, 8)), large = 62.0 * std::ceil(groups(12, 16));
+  return large <= middle && large <= small ? LARGE : middle <= small ? MIDDLE : SMALL;
+}
+
 template <int FMT, int TERMS>
-hipError_t by_tokens(const MxGemmArgs &a, hipStream_t s) {
-  if (a.r.tiles >= 64) return launch_mx_shape<MxShape<FMT, TERMS, 16, FMT == 4 ? 16 : 8, 2, 4, FMT == 4 ? 3 : 2>>(a, s);
-  if (a.r.tiles >= 4) return launch_mx_shape<MxShape<FMT, TERMS, 4, 4, 2, 2, 3>>(a, s);
-  return launch_mx_shape<MxShape<FMT, TERMS, 4, 1, 4, 1, 3>>(a, s);
+hipError_t by_form(Form f, const MxGemmArgs &a, hipStream_t s) {
+  switch (f) {
+    case SMALL: return launch_mx_shape<MxShape<FMT, TERMS, 4, 4, 2, 2, 4>>(a, s);
+    case MIDDLE: return launch_mx_shape<MxShape<FMT, TERMS, 8, 8, 2, 2, 4>>(a, s);
+    case LARGE: return launch_mx_shape<MxShape<FMT, TERMS, 12, 16, 2, 4, FMT == 8 ? 3 : FMT == 4 ? 5 : 4>>(a, s);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 }  // namespace
 
-int mx_gemm_splits(const MxGemmArgs &) { return 1; }
-
 hipError_t launch_mx_gemm(const MxGemmArgs &a, hipStream_t s) {
-  hipError_t e;
+  const Form f = form_of(a);
+  if (f == FEW) return launch_mx_few(a, s);
   switch (a.r.type) {
-    case MOE_F32: e = by_tokens<6, 6>(a, s); break;
-    case MOE_BF16: e = by_tokens<6, 4>(a, s); break;
-    case MOE_MXFP8: e = by_tokens<8, 1>(a, s); break;
-    case MOE_MXFP4: e = by_tokens<4, 1>(a, s); break;
-    default: return hipErrorInvalidValue;
+    case MOE_F32: return by_form<6, 6>(f, a, s);
+    case MOE_BF16: return by_form<6, 4>(f, a, s);
+    case MOE_MXFP8: return by_form<8, 1>(f, a, s);
+    case MOE_MXFP4: return by_form<4, 1>(f, a, s);
   }
-  return e;
-}
-
-hipError_t launch_mx_sum(const float *part, int parts, size_t n, size_t rows, const float *bias, void *out, bool bf16, hipStream_t s) {
-  if (!n) return hipSuccess;
-  const unsigned grid = (unsigned)std::min<size_t>((n / 4 + 255) / 256, 8192);
-  return bf16 ? launch_own(k_mx_sum<true>, dim3(grid), dim3(256), 0, s, part, parts, n, (uint32_t)rows, bias, out)
-              : launch_own(k_mx_sum<false>, dim3(grid), dim3(256), 0, s, part, parts, n, (uint32_t)rows, bias, out);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace moe

@@ -4,10 +4,16 @@
 // three bf16 planes of f32 rows three products at a quarter of the rate.
 //
 // A workgroup of WM x WN wavefronts computes MT x NT16 tiles of 16 x 16. A package is one term of a step of 128 values: the
-// rows' chunks, and with the first term the weights' chunks and both sides' scale words. Packages arrive by LDS-DMA, DEPTH
-// ahead, in rings of slots; every wavefront issues the same number of loads a package, so that one counted wait and one
-// barrier hand a package over. A wavefront holds the weights of its tiles in registers over the terms of a step.
+// rows' chunks, with the first term the weights' chunks, and with every fourth step both sides' scale words. Packages arrive by LDS-DMA in rings
+// of DEPTH slots; every wavefront issues the same number of loads a package, so that one counted wait and one barrier hand a
+// package over. That barrier stands in the middle of the package before it, whose operands are in registers by then: the next
+// one's are read, and the loads that take its slots issued, between the MFMAs of its second half. (With the reads in front of all
+// of a package's MFMAs both wavefronts of a SIMD waited for them together: 4096 bf16 rows over 2880 x 2880 took 68 us, this XX.)
+// The weights' operands stay in registers over the terms of a step.
 #pragma once
+#include <algorithm>
+#include <cmath>
+
 #include "serve.hpp"
 #include "stream.hpp"
 
@@ -23,35 +29,83 @@ struct MxShape {
   static constexpr int kPiecesA = MT, kPiecesB = (NT * kChunk + 1023) / 1024, kPiecesSA = (MT + 3) / 4, kPiecesSB = (NT + 3) / 4;
   static constexpr int per(int n) { return (n + kWaves - 1) / kWaves; }
   static constexpr int kLoadA = per(kPiecesA), kLoadB = per(kPiecesB), kLoadS = per(kPiecesSA + kPiecesSB);
-  static constexpr int loads(int term) { return kLoadB + (term == 0 ? kLoadA + kLoadS : 0); }
-  // rings: packages i .. i + DEPTH are in LDS at once; a step's weights leave it for registers with its first package
-  static constexpr int kSlotsB = kDepth + 1, kSlotsA = (kDepth + TERMS) / TERMS;
+  static constexpr int kRound = 4 * TERMS;  // packages whose scales come in one word
+  static constexpr int loads(int u) { return kLoadB + (u % TERMS == 0 ? kLoadA : 0) + (u % kRound == 0 ? kLoadS : 0); }
+  // rings: packages i + 1 .. i + DEPTH are in LDS while i is multiplied; a step's weights leave it with its first package
+  static constexpr int kSlotsB = kDepth, kSlotsA = (kDepth + TERMS - 1) / TERMS, kSlotsS = (kDepth + kRound - 1) / kRound;
   static constexpr int kBytesA = kPiecesA * 1024, kBytesB = kPiecesB * 1024, kBytesS = (kPiecesSA + kPiecesSB) * 1024;
-  static constexpr int kOffB = kSlotsA * kBytesA, kOffS = kOffB + kSlotsB * kBytesB, kLds = kOffS + kSlotsA * kBytesS;
-  // loads of packages after the one needed that may be outstanding when package (., term) is awaited
-  static constexpr int behind(int term) {
+  static constexpr int kOffB = kSlotsA * kBytesA, kOffS = kOffB + kSlotsB * kBytesB, kRings = kOffS + kSlotsS * kBytesS;
+  // loads that may be outstanding when the package after the round's u-th is awaited: those of the packages behind it
+  static constexpr int behind(int u) {
     int n = 0;
-    for (int j = 1; j < kDepth; j++) n += loads((term + j) % TERMS);
+    for (int j = 2; j < kDepth; j++) n += loads(u + j);
     return n;
   }
   static constexpr int most() {
     int n = 0;
-    for (int t = 0; t < TERMS; t++) n = behind(t) > n ? behind(t) : n;
+    for (int u = 0; u < kRound; u++) n = behind(u) + loads(u + kDepth) > n ? behind(u) + loads(u + kDepth) : n;
     return n;
   }
+  static constexpr int kStage = 16 * (TM * 64 + 16);  // bytes a wavefront's results pass through
+  static constexpr int kLds = kRings > kWaves * kStage ? kRings : kWaves * kStage;
   static_assert(kLds <= 160 * 1024 && most() <= 63 && MT % WM == 0 && NT % WN == 0, "rings");
 };
+
+// A wavefront's tiles to out [tokens][rows]. Lane l of a tile holds token l % 16, rows 4 (l / 16) ..; they pass through LDS so
+// that a token's rows leave in 16-byte pieces side by side (stored as they lie, in pieces of 8 bytes over 16 tokens, 4096 x
+// 5760 results in bf16 took some 25 us more).
+template <class S, class O>
+__device__ __forceinline__ void mx_store(const MxGemmArgs &a, const f32x4 (&acc)[S::TM][S::TN], uint8_t *stage, int lane, uint32_t row0,
+                                         uint32_t t0, const float *bias, O *out) {
+  constexpr int kRow = S::TM * 16 * sizeof(O), kPieces = kRow / 16;
+  const uint32_t R = a.d.rows;
+  f32x4 b[S::TM];
+#pragma unroll
+  for (int i = 0; i < S::TM; i++) {
+    b[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (bias && row0 + i * 16 < R) b[i] = *(const f32x4 *)(bias + row0 + i * 16 + (lane >> 4) * 4);
+  }
+#pragma unroll
+  for (int j = 0; j < S::TN; j++) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < S::TM; i++) {
+      const f32x4 v = acc[i][j] + b[i];
+      uint8_t *to = stage + (lane & 15) * (kRow + 16) + (i * 16 + (lane >> 4) * 4) * sizeof(O);
+      if constexpr (sizeof(O) == 2) {
+        uint16_t q[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) q[x] = __builtin_bit_cast(uint16_t, (__bf16)v[x]);
+        *(uint2 *)to = __builtin_bit_cast(uint2, q);
+      } else {
+        *(f32x4 *)to = v;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int c = 0; c < 16 * kPieces; c += 64) {
+      const int at = c + lane, tok = at / kPieces, piece = at % kPieces;
+      const uint32_t t = t0 + j * 16 + tok, row = row0 + piece * (16 / sizeof(O));
+      if (tok < 16 && t < a.r.tokens && row < R)
+        *(uint4 *)(out + (size_t)t * R + row) = *(const uint4 *)(stage + tok * (kRow + 16) + piece * 16);
+    }
+  }
+}
 
 template <class S>
 __global__ __launch_bounds__(64 * S::kWaves) void k_mx_gemm(MxGemmArgs a) {
   extern __shared__ __align__(1024) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / S::WN, wn = wave % S::WN;
-  const uint32_t nm = (a.d.tiles + S::MT - 1) / S::MT, nn = (a.r.tiles + S::NT - 1) / S::NT;
-  const uint32_t split = blockIdx.x / (nm * nn), tile = blockIdx.x % (nm * nn);
-  const uint32_t m0 = tile % nm * S::MT, n0 = tile / nm * S::NT;
+  // Workgroups go to the 8 XCDs in turn, each of which takes tiles that lie together, in strips of a.strip tiles of rows: what
+  // its CUs read at a time then comes through its L2 once.
+  const uint32_t nm = (a.d.tiles + S::MT - 1) / S::MT, nn = (a.r.tiles + S::NT - 1) / S::NT, all = nm * nn;
+  const uint32_t at = blockIdx.x % 8 * ((all + 7) / 8) + blockIdx.x / 8;
+  if (blockIdx.x / 8 >= (all + 7) / 8 || at >= all) return;
+  const uint32_t strip = at / (nm * a.strip) * a.strip, in = at - strip * nm, wide = min((uint32_t)a.strip, nn - strip);
+  // (uniform, and said to be: the loads' bases are scalar)
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(in / wide) * S::MT, n0 = __builtin_amdgcn_readfirstlane(strip + in % wide) * S::NT;
   const uint32_t nb = a.d.nb, ns = a.d.ns, nq = a.d.nq;
-  const uint32_t s_first = split * a.steps, s_last = min(s_first + a.steps, ns);
   const uint32_t lds0 = str_lds(lds);
 
   // this lane's offsets from the workgroup's first tile (tiles past the matrix read its last one)
@@ -77,24 +131,58 @@ __global__ __launch_bounds__(64 * S::kWaves) void k_mx_gemm(MxGemmArgs a) {
     off_s[i] = min(t, of_a ? m_last : n_last) * nq * 256 + (lane & 15) * 16;
   }
 
-  // package (s, term) into slots sa, sb; steps past the last one load the last again
-  auto issue = [&](uint32_t s, int term, uint32_t sa, uint32_t sb) {
-    s = min(s, s_last - 1);
-    if (term == 0) {
+  // load `piece` of the package of step s and term u % TERMS into slots; steps past the last one load the last again
+  auto issue = [&](int piece, uint32_t s, int u, uint32_t slot_a, uint32_t slot_b, uint32_t slot_s) {
+    s = min(s, ns - 1);
+    if (piece < S::kLoadB) {
+      str_dma16(off_b[piece], xb + ((size_t)s * S::kTerms + u % S::kTerms) * S::kChunk,
+                lds0 + S::kOffB + slot_b * S::kBytesB + min(piece * S::kWaves + wave, S::kPiecesB - 1) * 1024);
+    } else if (piece < S::kLoadB + S::kLoadA) {
+      const int i = piece - S::kLoadB;
       const uint32_t in_tile = min((uint32_t)lane * 16, 256 * nb - 16 - s * 1024);  // (a last step may be short)
+      str_dma16(off_a[i] + in_tile, wa + (size_t)s * 1024, lds0 + slot_a * S::kBytesA + min(i * S::kWaves + wave, S::kPiecesA - 1) * 1024);
+    } else {
+      const int i = piece - S::kLoadB - S::kLoadA, p = min(i * S::kWaves + wave, S::kPiecesSA + S::kPiecesSB - 1);
+      str_dma16(off_s[i], (p < S::kPiecesSA ? wsc : xsc) + (size_t)(s / 4) * 256, lds0 + S::kOffS + slot_s * S::kBytesS + p * 1024);
+    }
+  };
+  auto wait = [&](auto outstanding) {  // for the loads before the last `outstanding` ones, of every wavefront
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(vm_lgkm_wait(decltype(outstanding)::value));
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  };
+  // the operands of a package, of a step, and the scale words of a round
+  auto read_b = [&](uint32_t slot, i32x8 (&B)[S::TN]) {
+    const uint8_t *pb = lds + S::kOffB + slot * S::kBytesB + wn * S::TN * S::kChunk + lane * 16;
 #pragma unroll
-      for (int i = 0; i < S::kLoadA; i++)
-        str_dma16(off_a[i] + in_tile, wa + (size_t)s * 1024, lds0 + sa * S::kBytesA + min(i * S::kWaves + wave, S::kPiecesA - 1) * 1024);
-#pragma unroll
-      for (int i = 0; i < S::kLoadS; i++) {
-        const int p = min(i * S::kWaves + wave, S::kPiecesSA + S::kPiecesSB - 1);
-        str_dma16(off_s[i], (p < S::kPiecesSA ? wsc : xsc) + (size_t)(s / 4) * 256, lds0 + S::kOffS + sa * S::kBytesS + p * 1024);
+    for (int j = 0; j < S::TN; j++) {
+      const uint8_t *p = pb + j * S::kChunk;
+      const uint4 v = *(const uint4 *)p;
+      B[j] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+      if constexpr (S::kFmt == 6) {
+        const uint2 u = *(const uint2 *)(p - lane * 8 + 1024);
+        B[j][4] = (int)u.x, B[j][5] = (int)u.y;
+      } else if constexpr (S::kFmt == 8) {
+        const uint4 u = *(const uint4 *)(p + 1024);
+        B[j][4] = (int)u.x, B[j][5] = (int)u.y, B[j][6] = (int)u.z, B[j][7] = (int)u.w;
       }
     }
+  };
+  auto read_a = [&](uint32_t slot, i32x8 (&A)[S::TM]) {
+    const uint8_t *pa = lds + slot * S::kBytesA + wm * S::TM * 1024 + lane * 16;
 #pragma unroll
-    for (int i = 0; i < S::kLoadB; i++)
-      str_dma16(off_b[i], xb + ((size_t)s * S::kTerms + term) * S::kChunk,
-                lds0 + S::kOffB + sb * S::kBytesB + min(i * S::kWaves + wave, S::kPiecesB - 1) * 1024);
+    for (int i = 0; i < S::TM; i++) {
+      const uint4 v = *(const uint4 *)(pa + i * 1024);
+      A[i] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+    }
+  };
+  auto read_s = [&](uint32_t slot, uint32_t (&sa)[S::TM], uint32_t (&sb)[S::TN]) {
+    const uint8_t *ps = lds + S::kOffS + slot * S::kBytesS + lane * 4;
+#pragma unroll
+    for (int i = 0; i < S::TM; i++) sa[i] = *(const uint32_t *)(ps + (wm * S::TM + i) * 256);
+#pragma unroll
+    for (int j = 0; j < S::TN; j++) sb[j] = *(const uint32_t *)(ps + S::kPiecesSA * 1024 + (wn * S::TN + j) * 256);
   };
 
   f32x4 acc[S::TM][S::TN];
@@ -104,89 +192,82 @@ __global__ __launch_bounds__(64 * S::kWaves) void k_mx_gemm(MxGemmArgs a) {
     for (int j = 0; j < S::TN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
 #pragma unroll
-  for (int d = 0; d < S::kDepth; d++) issue(s_first + d / S::kTerms, d % S::kTerms, d / S::kTerms % S::kSlotsA, d % S::kSlotsB);
-
-  uint32_t slot_a = 0, slot_b = 0;  // of the package at hand
-  uint32_t next_a = S::kDepth / S::kTerms % S::kSlotsA;  // of the step that the next first term belongs to
-  if (S::kDepth % S::kTerms) next_a = (next_a + 1) % S::kSlotsA;
-  for (uint32_t s = s_first; s < s_last; s++) {
-    i32x8 A[S::TM];
-    uint32_t sa[S::TM], sb[S::TN];
-    str_static_for<0, S::kTerms>([&](auto term_) {
-      constexpr int term = decltype(term_)::value;
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      __builtin_amdgcn_s_waitcnt(vm_lgkm_wait(S::behind(term)));
-      __builtin_amdgcn_s_barrier();
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      {  // DEPTH ahead, into the slots of the package before this one
-        constexpr int ahead = (term + S::kDepth) % S::kTerms;
-        issue(s + (term + S::kDepth) / S::kTerms, ahead, next_a, slot_b == 0 ? S::kSlotsB - 1 : slot_b - 1);
-        if (ahead == 0) next_a = next_a + 1 == S::kSlotsA ? 0 : next_a + 1;
+  for (int d = 0; d < S::kDepth; d++)
+#pragma unroll
+    for (int i = 0; i < S::loads(d); i++) issue(i, d / S::kTerms, d, d / S::kTerms, d, d / S::kRound);
+  // (package 0: those of the packages 1 .. DEPTH - 1 may be outstanding)
+  wait(std::integral_constant<int, S::behind(S::kRound - 1) + S::loads(S::kDepth - 1)>{});
+  i32x8 A[2][S::TM], B[2][S::TN];  // of the step and package at hand, and of the next
+  uint32_t sa[S::TM], sb[S::TN], sw[S::TN];
+  read_s(0, sa, sb);
+  read_a(0, A[0]);
+  read_b(0, B[0]);
+  // slots of the next package, step and round; and of the step and round to be loaded next
+  uint32_t slot_b = 1 % S::kSlotsB, slot_a = 1 % S::kSlotsA, slot_s = 1 % S::kSlotsS, next_a = 0, next_s = 0;
+  for (uint32_t s0 = 0; s0 < ns; s0 += 4) {
+    str_static_for<0, S::kRound>([&](auto u_) {
+      constexpr int u = decltype(u_)::value, step = u / S::kTerms, term = u % S::kTerms;
+      const uint32_t s = s0 + step;
+      if (step && s >= ns) return;  // (steps are no multiple of 4)
+      // the rows' scales: of several terms 2^-5 each (a NaN's 255 is the first one's alone: the codes are 0)
+      if constexpr (S::kTerms > 1) {
+#pragma unroll
+        for (int j = 0; j < S::TN; j++) sw[j] = term == 0 ? sb[j] >> 8 * step & 255 : (uint32_t)max((int)sw[j] - 5, 1);
       }
-      if constexpr (term == 0) {
-        const uint8_t *pa = lds + slot_a * S::kBytesA, *ps = lds + S::kOffS + slot_a * S::kBytesS;
-        const int sh = 8 * (s & 3);
+      constexpr int kB = S::kFmt == 4 ? 4 : S::kFmt == 6 ? 2 : 0, kAll = S::TM * S::TN, kHalf = kAll / 2;
+      auto mfma = [&](int p) {
+        const int i = p % S::TM, j = p / S::TM;
+        if constexpr (S::kTerms > 1)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A[step & 1][i], B[u & 1][j], acc[i][j], 4, kB, step, (int)sa[i], 0, (int)sw[j]);
+        else
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A[step & 1][i], B[u & 1][j], acc[i][j], 4, kB, step, (int)sa[i], step, (int)sb[j]);
+      };
 #pragma unroll
-        for (int i = 0; i < S::TM; i++) {
-          const uint4 v = *(const uint4 *)(pa + (wm * S::TM + i) * 1024 + lane * 16);
-          A[i] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
-          sa[i] = *(const uint32_t *)(ps + (wm * S::TM + i) * 256 + lane * 4) >> sh;
-        }
-#pragma unroll
-        for (int j = 0; j < S::TN; j++) sb[j] = *(const uint32_t *)(ps + S::kPiecesSA * 1024 + (wn * S::TN + j) * 256 + lane * 4) >> sh & 255;
+      for (int p = 0; p < kHalf; p++) mfma(p);
+      __builtin_amdgcn_sched_barrier(0);
+      wait(std::integral_constant<int, S::behind(u)>{});
+      if constexpr (term == S::kTerms - 1) {
+        read_a(slot_a, A[step & 1 ^ 1]);
         slot_a = slot_a + 1 == S::kSlotsA ? 0 : slot_a + 1;
-      } else {  // 2^-5 a term (a NaN's 255 is the first one's alone: the codes are 0)
-#pragma unroll
-        for (int j = 0; j < S::TN; j++) sb[j] = (uint32_t)max((int)sb[j] - 5, 1);
       }
-      const uint8_t *pb = lds + S::kOffB + slot_b * S::kBytesB;
+      read_b(slot_b, B[u & 1 ^ 1]);
+      uint32_t sa2[S::TM], sb2[S::TN];
+      if constexpr (u == S::kRound - 1) {
+        read_s(slot_s, sa2, sb2);
+        slot_s = slot_s + 1 == S::kSlotsS ? 0 : slot_s + 1;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      constexpr int ahead = u + S::kDepth;
+      const uint32_t into_b = slot_b == 0 ? S::kSlotsB - 1 : slot_b - 1;
 #pragma unroll
-      for (int j = 0; j < S::TN; j++) {
-        const uint8_t *p = pb + (wn * S::TN + j) * S::kChunk + lane * 16;
-        const uint4 v = *(const uint4 *)p;
-        i32x8 B{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
-        if constexpr (S::kFmt == 6) {
-          const uint2 u = *(const uint2 *)(p - lane * 8 + 1024);
-          B[4] = (int)u.x, B[5] = (int)u.y;
-        } else if constexpr (S::kFmt == 8) {
-          const uint4 u = *(const uint4 *)(p + 1024);
-          B[4] = (int)u.x, B[5] = (int)u.y, B[6] = (int)u.z, B[7] = (int)u.w;
+      for (int p = kHalf; p < kAll || p - kHalf < S::loads(ahead); p++) {
+        if (p < kAll) mfma(p);
+        if (p - kHalf < S::loads(ahead)) {
+          issue(p - kHalf, s0 + ahead / S::kTerms, ahead, next_a, into_b, next_s);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        constexpr int kB = S::kFmt == 4 ? 4 : S::kFmt == 6 ? 2 : 0;
-#pragma unroll
-        for (int i = 0; i < S::TM; i++)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A[i], B, acc[i][j], 4, kB, 0, (int)sa[i], 0, (int)sb[j]);
       }
+      if (ahead % S::kTerms == 0) next_a = next_a + 1 == S::kSlotsA ? 0 : next_a + 1;
+      if (ahead % S::kRound == 0) next_s = next_s + 1 == S::kSlotsS ? 0 : next_s + 1;
       slot_b = slot_b + 1 == S::kSlotsB ? 0 : slot_b + 1;
+      if constexpr (u == S::kRound - 1) {
+#pragma unroll
+        for (int i = 0; i < S::TM; i++) sa[i] = sa2[i];
+#pragma unroll
+        for (int j = 0; j < S::TN; j++) sb[j] = sb2[j];
+      }
     });
   }
-  __builtin_amdgcn_s_waitcnt(vm_wait(0));  // (no load may land once the workgroup's LDS is another's)
 
-  // lane l: token 16 j + l % 16, rows 16 i + 4 (l / 16) ..
-  const uint32_t R = a.d.rows;
-#pragma unroll
-  for (int i = 0; i < S::TM; i++) {
-    const uint32_t mt = m0 + wm * S::TM + i, row = mt * 16 + (lane >> 4) * 4;
-    if (mt >= a.d.tiles) continue;
-    f32x4 b = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (a.bias && a.splits == 1) b = *(const f32x4 *)(a.bias + row);
-#pragma unroll
-    for (int j = 0; j < S::TN; j++) {
-      const uint32_t t = (n0 + wn * S::TN + j) * 16 + (lane & 15);
-      if (t >= a.r.tokens) continue;
-      const f32x4 v = acc[i][j] + b;
-      if (a.splits > 1) {
-        *(f32x4 *)((float *)a.out + ((size_t)split * a.r.tokens + t) * R + row) = v;
-      } else if (a.bf16) {
-        uint16_t q[4];
-#pragma unroll
-        for (int x = 0; x < 4; x++) q[x] = __builtin_bit_cast(uint16_t, (__bf16)v[x]);
-        *(uint2 *)((uint16_t *)a.out + (size_t)t * R + row) = __builtin_bit_cast(uint2, q);
-      } else {
-        *(f32x4 *)((float *)a.out + (size_t)t * R + row) = v;
-      }
-    }
-  }
+  // (no load may land once the workgroup's LDS holds something else, its own results or another's)
+  __builtin_amdgcn_s_waitcnt(vm_wait(0));
+  __syncthreads();
+  uint8_t *stage = lds + wave * S::kStage;
+  const uint32_t row0 = (m0 + wm * S::TM) * 16, t0 = (n0 + wn * S::TN) * 16;
+  if (a.bf16)
+    mx_store<S, uint16_t>(a, acc, stage, lane, row0, t0, a.bias, (uint16_t *)a.out);
+  else
+    mx_store<S, float>(a, acc, stage, lane, row0, t0, a.bias, (float *)a.out);
 }
 
 template <class S>
@@ -194,9 +275,12 @@ hipError_t launch_mx_shape(const MxGemmArgs &a, hipStream_t s) {
   static DynLdsOnce once;
   hipError_t e = ensure_dyn_lds(once, (const void *)k_mx_gemm<S>, S::kLds);
   if (e != hipSuccess) return e;
-  const size_t nm = (a.d.tiles + S::MT - 1) / S::MT, nn = (a.r.tiles + S::NT - 1) / S::NT;
-  if (nm * nn * a.splits > (size_t)1 << 22) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
-  return launch_own(k_mx_gemm<S>, dim3((unsigned)(nm * nn * a.splits)), dim3(64 * S::kWaves), S::kLds, s, a);
+  const size_t nm = (a.d.tiles + S::MT - 1) / S::MT, nn = (a.r.tiles + S::NT - 1) / S::NT, all = nm * nn;
+  if (all > (size_t)1 << 22) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
+  MxGemmArgs b = a;
+  // an XCD's 32 CUs on about as many rows as tokens
+  b.strip = std::max(1, (int)std::lround(std::sqrt(32.0 * S::MT / S::NT)));
+  return launch_own(k_mx_gemm<S>, dim3((unsigned)((all + 7) / 8 * 8)), dim3(64 * S::kWaves), S::kLds, s, b);
 }
 
 }  // namespace moe

@@ -1,4 +1,4 @@
-// Rows quantised to MXFP4: E2M1 codes with one E8M0 scale per 32 values, in the checkpoint's layout.
+// Rows quantised to MXFP4: E2M1 codes with one E8M0 scale per 32 values, in the checkpoint's layout; and such rows read back.
 //
 // e = floor(log2 max |x|) - 2, at least -126: the largest value of a block comes to lie in [4, 8), codes are x 2^-e
 // rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, ties to the even code, at most 6.
@@ -39,7 +39,35 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const S *x, size_t blocks,
   }
 }
 
+// The values of MXFP4 rows, as the reference decodes them (weights.rs:350-371): a code's value times f32_from_bits(byte << 23),
+// so that byte 0 is 0 and byte 255 infinity. A thread takes 4 values and 4 further on, so that a
+// wavefront's stores lie side by side; bound by the bytes written (one thread a block, whose stores lay 128 bytes apart, took 100 us
+// for 23040 x 2880; this 45).
+__global__ __launch_bounds__(256) void k_dequant_hf(const uint16_t *codes, const uint8_t *scales, size_t n, f32x4 *out) {
+  for (size_t i = (size_t)blockIdx.x * 512 + threadIdx.x; i < n; i += (size_t)gridDim.x * 512) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const size_t k = i + 256 * h;
+      if (k >= n) break;
+      const uint32_t w = codes[k];
+      const float sc = __uint_as_float((uint32_t)scales[k / 8] << 23);
+      f32x4 v;
+#pragma unroll
+      for (int x = 0; x < 4; x++) v[x] = canon_nan(e2m1_to_f32(w >> 4 * x & 15u) * sc);
+      __builtin_nontemporal_store(v, out + k);
+    }
+  }
+}
+
 }  // namespace
+
+hipError_t launch_dequant_hf(const uint8_t *blocks, const uint8_t *scales, size_t rows, size_t cols, float *out, hipStream_t s) {
+  if (cols % 32) return hipErrorInvalidValue;
+  const size_t n = rows * (cols / 32) * 8;
+  if (!n) return hipSuccess;
+  const unsigned grid = (unsigned)std::min<size_t>((n + 511) / 512, (size_t)1 << 23);
+  return launch_own(k_dequant_hf, grid, 256, 0, s, (const uint16_t *)blocks, scales, n, (f32x4 *)out);
+}
 
 hipError_t launch_mx4_quantize(const void *x, bool bf16, size_t n, size_t cols, uint8_t *blocks, uint8_t *scales, hipStream_t s) {
   const size_t nb = n * cols / 32;

@@ -36,11 +36,13 @@ struct MxGemmArgs {
   const float *bias;     // [rows] or NULL
   void *out;             // [tokens][rows]
   bool bf16;
-  int splits;            // parts of K: out is f32 parts [splits][tokens][rows] then
-  int steps;             // MFMA steps a part
+  int strip;             // set by the launch
 };
-int mx_gemm_splits(const MxGemmArgs &a);  // parts worth taking
 hipError_t launch_mx_gemm(const MxGemmArgs &a, hipStream_t s);
+// The form for few rows (mx_few.hip).
+hipError_t launch_mx_few(const MxGemmArgs &a, hipStream_t s);
+// The form for few rows (mx_few.hip).
+hipError_t launch_mx_few(const MxGemmArgs &a, hipStream_t s);
 // out [n / rows][rows] = the sum of parts [parts][n] in order, + bias
 hipError_t launch_mx_sum(const float *part, int parts, size_t n, size_t rows, const float *bias, void *out, bool bf16, hipStream_t s);
 

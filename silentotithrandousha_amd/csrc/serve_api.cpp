@@ -92,18 +92,10 @@ int moe_mxfp4_matmul_device(moe_ctx *ctx, const uint8_t *packed, size_t rows, si
   Carve w;
   uint8_t *codes = nullptr;
   uint32_t *scales = nullptr;
-  float *part = nullptr;
   for (int placed = 0; placed < 2; placed++) {
     a.r = mx_rows(x_type, Tc, cols);
     codes = w.take<uint8_t>(mx_rows_code_bytes(a.r));
     scales = w.take<uint32_t>(mx_rows_scale_bytes(a.r) / 4);
-    size_t parts = 0;  // (the last piece may take other parts)
-    for (size_t t0 = 0; t0 < T; t0 += Tc) {
-      a.r = mx_rows(x_type, std::min(Tc, T - t0), cols);
-      const size_t n = mx_gemm_splits(a);
-      if (n > 1) parts = std::max(parts, n * a.r.tokens * rows);
-    }
-    part = parts ? w.take<float>(parts) : nullptr;
     if (!placed) {
       RETURN_IF(ensure(c, w.off, s));
       w = Carve{(char *)c.work->p};
@@ -113,13 +105,9 @@ int moe_mxfp4_matmul_device(moe_ctx *ctx, const uint8_t *packed, size_t rows, si
     a.r = mx_rows(x_type, std::min(Tc, T - t0), cols);
     a.codes = codes;
     a.scales = scales;
-    void *out = (char *)y + t0 * rows * el;
+    a.out = (char *)y + t0 * rows * el;
     HIP_TRY(launch_mx_rows(a.r, (const char *)x + t0 * xb, x_scales ? x_scales + t0 * (cols / 32) : nullptr, codes, scales, s));
-    a.splits = mx_gemm_splits(a);
-    a.steps = (int)((a.d.ns + a.splits - 1) / a.splits);
-    a.out = a.splits > 1 ? (void *)part : out;
     HIP_TRY(launch_mx_gemm(a, s));
-    if (a.splits > 1) HIP_TRY(launch_mx_sum(part, a.splits, (size_t)a.r.tokens * rows, rows, bias, out, a.bf16, s));
   }
   return MOE_OK;
 }
