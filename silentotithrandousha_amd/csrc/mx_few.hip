@@ -1,7 +1,7 @@
 // Products of a few rows with a resident MXFP4 matrix (mx_gemm.hpp's operands and arithmetic): bound by the weights, which a
 // workgroup's 8 wavefronts stream through registers, each every eighth step of K, and by the latency of its loads.
 // There is no barrier before the wavefronts' sums meet in LDS, where they are added in order.
-#include "device.hpp"
+#include "act8.hpp"
 #include "serve.hpp"
 
 namespace moe {
@@ -100,6 +100,129 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_mx_few(MxGemmArgs a) {
   }
 }
 
+// One to a few f32 or bf16 rows, whose terms fit the MFMA's 16 columns (column t TERMS + i: term i of token t): the terms are
+// made by every workgroup for itself, while its weights are on their way. (Made by a launch of their own, one f32 row over 5760 x
+// 2880 took 10.6 us, so 5.1.)
+constexpr int kEarly = 3;  // steps of a wavefront whose weights are asked for first
+constexpr size_t kOneLds = 64 * 1024;
+__host__ __device__ constexpr size_t one_lds(size_t nb, size_t cols) { return (nb + 3) / 4 * 4 * cols * 28 + 8 * 64 * 16 + 1024; }
+
+template <class X, int TERMS>
+__global__ __launch_bounds__(64 * kFewWaves) void k_mx_one(MxGemmArgs a, const X *x) {
+  extern __shared__ __align__(16) uint8_t s_mem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
+  const uint32_t m = blockIdx.x, nb = a.d.nb, ns = a.d.ns, nq = a.d.nq, T = a.r.tokens, cols = T * TERMS, blocks = 4 * ns;
+  f32x4 *s_sum = (f32x4 *)s_mem;                   // [8 wavefronts][64]
+  float *s_col = (float *)(s_mem + 8 * 64 * 16);   // [16 columns][16 rows]
+  uint8_t *s_code = s_mem + 8 * 64 * 16 + 1024;    // [blocks][cols] 24 bytes
+  uint32_t *s_scale = (uint32_t *)(s_code + (size_t)blocks * cols * 24);  // [blocks][cols]
+  const uint8_t *w = a.w + (size_t)m * 256 * nb;
+  const uint32_t *wsc = (const uint32_t *)(a.w + pack_weight_bytes(a.d)) + (size_t)m * nq * 64 + lane;
+  auto weights = [&](uint32_t s) {  // (a last step may be short: its scales are 0)
+    return __builtin_nontemporal_load((const u32x4 *)(w + min((s * 64 + lane) * 16, 256 * nb - 16)));
+  };
+  u32x4 A[kEarly];
+  uint32_t sa[kEarly];
+#pragma unroll
+  for (int i = 0; i < kEarly; i++) {
+    const uint32_t s = min((uint32_t)(wave + i * kFewWaves), ns - 1);
+    A[i] = weights(s);
+    sa[i] = wsc[s / 4 * 64];
+  }
+  // a pair of lanes a block of 32 values (pairs leave together)
+  for (uint32_t k = tid; k < 2 * blocks * T; k += 64 * kFewWaves) {
+    const uint32_t b = k / 2 % blocks, t = k / 2 / blocks, half = k & 1;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = 0.0f;
+    if (b < nb) {
+      float u[8];
+      act8_load(x + (size_t)t * nb * 32 + b * 32 + half * 16, u);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = u[i];
+      act8_load(x + (size_t)t * nb * 32 + b * 32 + half * 16 + 8, u);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[8 + i] = u[i];
+    }
+    float top = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      top = fmaxf(top, fabsf(v[i]));
+      bad |= !isfinite(v[i]);
+    }
+    if (bad) top = INFINITY;
+    top = fmaxf(top, __shfl_xor(top, 1));
+    bad = !isfinite(top);
+    int E = 0;
+    if (top > 0.0f && !bad) frexpf(top, &E);
+    f32x16v lo = {}, hi = {};
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      lo[i] = bad ? 0.0f : v[2 * i];
+      hi[i] = bad ? 0.0f : v[2 * i + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < TERMS; i++) {
+      const int se = split_scale_exp<TERMS>(E, i);
+      const float sc = __builtin_amdgcn_ldexpf(1.0f, se);
+      u32x6v c;
+      asm volatile("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3" : "=&v"(c) : "v"(lo), "v"(hi), "v"(sc));
+      if (i + 1 < TERMS) {  // the residual feeds the next term
+        f32x32v q;
+        asm volatile("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2" : "=&v"(q) : "v"(c), "v"(sc));
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+          lo[n] = lo[n] - q[2 * n];
+          hi[n] = hi[n] - q[2 * n + 1];
+        }
+      }
+      const uint32_t at = b * cols + t * TERMS + i;
+      uint32_t *o = (uint32_t *)(s_code + at * 24 + half * 12);
+      o[0] = c[0];
+      o[1] = c[1];
+      o[2] = c[2];
+      if (!half) s_scale[at] = bad ? 255u : (uint32_t)(se + 127);
+    }
+  }
+  __syncthreads();
+  f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto step = [&](uint32_t s, const u32x4 &A, uint32_t sa) {
+    const uint32_t at = (4 * s + g) * cols + min((uint32_t)col, cols - 1);  // (columns past the last: the last again)
+    const uint2 *p = (const uint2 *)(s_code + at * 24);
+    const uint2 p0 = p[0], p1 = p[1], p2 = p[2];
+    const i32x8 B{(int)p0.x, (int)p0.y, (int)p1.x, (int)p1.y, (int)p2.x, (int)p2.y, 0, 0};
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(i32x8{(int)A.x, (int)A.y, (int)A.z, (int)A.w, 0, 0, 0, 0}, B, acc, 4, 2, 0,
+                                                           (int)(sa >> 8 * (s & 3)), 0, (int)s_scale[at]);
+  };
+#pragma unroll
+  for (int i = 0; i < kEarly; i++)
+    if (wave + i * kFewWaves < ns) step(wave + i * kFewWaves, A[i], sa[i]);
+#pragma unroll 2
+  for (uint32_t s = wave + kEarly * kFewWaves; s < ns; s += kFewWaves) step(s, weights(s), wsc[s / 4 * 64]);
+  s_sum[wave * 64 + lane] = acc;
+  __syncthreads();
+  if (tid < 64) {  // the wavefronts' sums in order, then the terms'
+    f32x4 v = s_sum[tid];
+#pragma unroll
+    for (int k = 1; k < kFewWaves; k++) v = v + s_sum[k * 64 + tid];
+    *(f32x4 *)(s_col + col * 16 + g * 4) = v;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const uint32_t row = tid & 15, t = tid >> 4;
+    if (t < T) {
+      float v = s_col[(t * TERMS + TERMS - 1) * 16 + row];
+#pragma unroll
+      for (int i = TERMS - 2; i >= 0; i--) v = v + s_col[(t * TERMS + i) * 16 + row];
+      if (a.bias) v = v + a.bias[m * 16 + row];
+      const size_t at = (size_t)t * a.d.rows + m * 16 + row;
+      if (a.bf16)
+        ((__bf16 *)a.out)[at] = (__bf16)v;
+      else
+        ((float *)a.out)[at] = v;
+    }
+  }
+}
+
 template <int FMT, int TERMS, int RT, int CT>
 hipError_t launch(const MxGemmArgs &a, hipStream_t s) {
   return launch_own(k_mx_few<FMT, TERMS, RT, CT>, dim3((a.d.tiles + RT - 1) / RT, (a.r.tiles + CT - 1) / CT), dim3(64 * kFewWaves), 0, s, a);
@@ -115,6 +238,19 @@ hipError_t by_tokens(const MxGemmArgs &a, hipStream_t s) {
 }
 
 }  // namespace
+
+bool mx_one_takes(int type, size_t tokens, size_t cols) {
+  if (type != MOE_F32 && type != MOE_BF16) return false;
+  const size_t terms = type == MOE_F32 ? 6 : 4;
+  return tokens * terms <= 16 && one_lds(cols / 32, tokens * terms) <= kOneLds;
+}
+
+hipError_t launch_mx_one(const MxGemmArgs &a, const void *x, hipStream_t s) {
+  const size_t lds = one_lds(a.d.nb, (size_t)a.r.tokens * a.r.terms);
+  if (!mx_one_takes(a.r.type, a.r.tokens, (size_t)a.d.nb * 32) || a.d.tiles >= 1u << 22) return hipErrorInvalidValue;
+  return a.r.type == MOE_F32 ? launch_own(k_mx_one<float, 6>, dim3(a.d.tiles), dim3(64 * kFewWaves), lds, s, a, (const float *)x)
+                             : launch_own(k_mx_one<uint16_t, 4>, dim3(a.d.tiles), dim3(64 * kFewWaves), lds, s, a, (const uint16_t *)x);
+}
 
 hipError_t launch_mx_few(const MxGemmArgs &a, hipStream_t s) {
   if (a.d.tiles >= 1u << 22) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)

@@ -41,8 +41,14 @@ struct MxGemmArgs {
 hipError_t launch_mx_gemm(const MxGemmArgs &a, hipStream_t s);
 // The form for few rows (mx_few.hip).
 hipError_t launch_mx_few(const MxGemmArgs &a, hipStream_t s);
+// One to a few f32 or bf16 rows x, without MxRows (a.codes, a.scales).
+bool mx_one_takes(int type, size_t tokens, size_t cols);
+hipError_t launch_mx_one(const MxGemmArgs &a, const void *x, hipStream_t s);
 // The form for few rows (mx_few.hip).
 hipError_t launch_mx_few(const MxGemmArgs &a, hipStream_t s);
+// One to a few f32 or bf16 rows x, without MxRows (a.codes, a.scales).
+bool mx_one_takes(int type, size_t tokens, size_t cols);
+hipError_t launch_mx_one(const MxGemmArgs &a, const void *x, hipStream_t s);
 // out [n / rows][rows] = the sum of parts [parts][n] in order, + bias
 hipError_t launch_mx_sum(const float *part, int parts, size_t n, size_t rows, const float *bias, void *out, bool bf16, hipStream_t s);
 

@@ -89,6 +89,12 @@ int moe_mxfp4_matmul_device(moe_ctx *ctx, const uint8_t *packed, size_t rows, si
   a.d = pack_dims(rows, cols);
   a.bias = bias;
   a.bf16 = dtype == MOE_BF16;
+  if (mx_one_takes(x_type, T, cols)) {
+    a.r = mx_rows(x_type, T, cols);
+    a.out = y;
+    HIP_TRY(launch_mx_one(a, x, s));
+    return MOE_OK;
+  }
   Carve w;
   uint8_t *codes = nullptr;
   uint32_t *scales = nullptr;

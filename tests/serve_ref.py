@@ -52,9 +52,8 @@ def matmul(x, x_type, w, bias, dtype):
     steps = -(-x.shape[1] // 128)
     tol = (steps * terms + 8) * 2.0 ** -23 * mag
     if x_type == MOE_MXFP8:
-        groups = np.abs(x).reshape(x.shape[0], -1, 8), np.abs(w).reshape(w.shape[0], -1, 8)
-        for t in range(x.shape[0]):
-            tol[t] += 7 * 2.0 ** -13 * (groups[0][t][None] * groups[1]).max(-1).sum(-1)
+        gx, gw = (np.abs(v).reshape(v.shape[0], -1, 8).max(-1) for v in (x, w))  # (no product is above those of these)
+        tol += 7 * 2.0 ** -13 * (gx @ gw.T)
     if terms > 1:
         top = np.abs(x).reshape(x.shape[0], -1, 32).max(-1)
         off = np.where(top < 2.0 ** -99, 2.0 ** -129, 2.0 ** (-29 if x_type == MOE_F32 else -19) * top)
