@@ -60,7 +60,7 @@ int moe_mxfp4_matmul_device(moe_ctx *ctx, const uint8_t *packed, size_t rows, si
 enum moe_score { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID = 1 };
 enum moe_group_score { MOE_GROUP_MAX = 0, MOE_GROUP_TOP2 = 1 };
 
-/* A routing rule. Zeros beside top_k and scale: the path's own (softmax over all experts, the top_k largest). */
+/* A routing rule. With normalize 1, scale 1 and zeros otherwise: the path's own. */
 typedef struct moe_routing {
   int score;         /* of a token's logits: softmax over all experts, or the sigmoid of each */
   int normalize;     /* not 0: the weights are divided by their sum */

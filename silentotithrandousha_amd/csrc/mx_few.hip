@@ -104,8 +104,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_mx_few(MxGemmArgs a) {
 // made by every workgroup for itself, while its weights are on their way. (Made by a launch of their own, one f32 row over 5760 x
 // 2880 took 10.6 us, so 5.1.)
 constexpr int kEarly = 3;  // steps of a wavefront whose weights are asked for first
-constexpr size_t kOneLds = 64 * 1024;
-__host__ __device__ constexpr size_t one_lds(size_t nb, size_t cols) { return (nb + 3) / 4 * 4 * cols * 28 + 8 * 64 * 16 + 1024; }
 
 template <class X, int TERMS>
 __global__ __launch_bounds__(64 * kFewWaves) void k_mx_one(MxGemmArgs a, const X *x) {
@@ -239,14 +237,8 @@ hipError_t by_tokens(const MxGemmArgs &a, hipStream_t s) {
 
 }  // namespace
 
-bool mx_one_takes(int type, size_t tokens, size_t cols) {
-  if (type != MOE_F32 && type != MOE_BF16) return false;
-  const size_t terms = type == MOE_F32 ? 6 : 4;
-  return tokens * terms <= 16 && one_lds(cols / 32, tokens * terms) <= kOneLds;
-}
-
 hipError_t launch_mx_one(const MxGemmArgs &a, const void *x, hipStream_t s) {
-  const size_t lds = one_lds(a.d.nb, (size_t)a.r.tokens * a.r.terms);
+  const size_t lds = mx_one_lds(a.d.nb, (size_t)a.r.tokens * a.r.terms);
   if (!mx_one_takes(a.r.type, a.r.tokens, (size_t)a.d.nb * 32) || a.d.tiles >= 1u << 22) return hipErrorInvalidValue;
   return a.r.type == MOE_F32 ? launch_own(k_mx_one<float, 6>, dim3(a.d.tiles), dim3(64 * kFewWaves), lds, s, a, (const float *)x)
                              : launch_own(k_mx_one<uint16_t, 4>, dim3(a.d.tiles), dim3(64 * kFewWaves), lds, s, a, (const uint16_t *)x);

@@ -64,19 +64,6 @@ __global__ __launch_bounds__(256) void k_mx_rows(MxRows r, const void *x, const 
 
 }  // namespace
 
-MxRows mx_rows(int type, size_t tokens, size_t cols) {
-  MxRows r{};
-  r.type = type;
-  r.tokens = (uint32_t)tokens;
-  r.nb = (uint32_t)(cols / 32);
-  r.ns = (r.nb + 3) / 4;
-  r.nq = (r.ns + 3) / 4;
-  r.tiles = (uint32_t)((tokens + 15) / 16);
-  r.terms = type == MOE_F32 ? 6 : type == MOE_BF16 ? 4 : 1;
-  r.chunk = type == MOE_MXFP4 ? 1024 : type == MOE_MXFP8 ? 2048 : 1536;
-  return r;
-}
-
 hipError_t launch_mx_rows(const MxRows &r, const void *x, const uint8_t *x_scales, uint8_t *codes, uint32_t *scales, hipStream_t s) {
   const size_t n = (size_t)r.tiles * r.ns;
   if (!n || n > (size_t)1 << 25) return hipErrorInvalidValue;

@@ -82,7 +82,6 @@ __device__ __forceinline__ void load_powers(double *s_powers) {
 // What a row's settings make of its logits.
 struct Row {
   float m, bins;        // largest logit; bins a unit of (m - l) / 2
-  float lowest;         // a logit whose mass is 0 (or the lowest finite one)
   double scale;         // 32 log2 e / temperature
   double least;         // min_p 2^shift
   double p;
@@ -96,7 +95,6 @@ struct Row {
     const float temperature = a.rule.temperature ? a.rule.temperature[t] : 1.0f;
     greedy = !(temperature > 0.0f);
     bins = fminf(128.0f / temperature, 3e38f);
-    lowest = fmaxf(m - fminf(40.0f * temperature, 3e38f), -3.4e38f);
     scale = 32 * 1.4426950408889634 / (double)temperature;
     shift = a.shift;
     const int kk = a.rule.top_k ? a.rule.top_k[t] : 0;
@@ -117,8 +115,9 @@ struct Row {
   __device__ __forceinline__ void masses(const float (&l)[4], uint64_t (&e)[4], bool (&stays)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      // (no logit is so far below that the power is none: those have mass 0, a NaN and -inf with them)
-      const double x = ((double)fmaxf(l[i], lowest) - (double)m) * scale;
+      // (from 40 temperatures below the largest logit the mass is 0; a -inf lies there, under an infinite temperature too, where
+      // the product is NaN)
+      const double x = fmax(((double)l[i] - (double)m) * scale, -40.0 * 32 * 1.4426950408889634);
       const double r = x + 6755399441055744.0;  // 1.5 2^52: the low word is x rounded
       const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, r);
       const double t = x - (r - 6755399441055744.0);

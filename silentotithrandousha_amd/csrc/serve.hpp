@@ -22,7 +22,18 @@ struct MxRows {
   uint32_t tokens, nb, ns, nq, tiles;
   int terms, chunk;  // terms a value, bytes of a chunk
 };
-MxRows mx_rows(int type, size_t tokens, size_t cols);
+inline MxRows mx_rows(int type, size_t tokens, size_t cols) {
+  MxRows r{};
+  r.type = type;
+  r.tokens = (uint32_t)tokens;
+  r.nb = (uint32_t)(cols / 32);
+  r.ns = (r.nb + 3) / 4;
+  r.nq = (r.ns + 3) / 4;
+  r.tiles = (uint32_t)((tokens + 15) / 16);
+  r.terms = type == MOE_F32 ? 6 : type == MOE_BF16 ? 4 : 1;
+  r.chunk = type == MOE_MXFP4 ? 1024 : type == MOE_MXFP8 ? 2048 : 1536;
+  return r;
+}
 inline size_t mx_rows_code_bytes(const MxRows &r) { return (size_t)r.tiles * r.ns * r.terms * r.chunk; }
 inline size_t mx_rows_scale_bytes(const MxRows &r) { return (size_t)r.tiles * r.nq * 256; }
 hipError_t launch_mx_rows(const MxRows &r, const void *x, const uint8_t *x_scales, uint8_t *codes, uint32_t *scales, hipStream_t s);
@@ -41,16 +52,14 @@ struct MxGemmArgs {
 hipError_t launch_mx_gemm(const MxGemmArgs &a, hipStream_t s);
 // The form for few rows (mx_few.hip).
 hipError_t launch_mx_few(const MxGemmArgs &a, hipStream_t s);
-// One to a few f32 or bf16 rows x, without MxRows (a.codes, a.scales).
-bool mx_one_takes(int type, size_t tokens, size_t cols);
+// One to a few f32 or bf16 rows x, without MxRows (a.codes, a.scales): those whose terms fit the MFMA's 16 columns and 64 KB of LDS.
+constexpr size_t mx_one_lds(size_t nb, size_t columns) { return (nb + 3) / 4 * 4 * columns * 28 + 8 * 64 * 16 + 1024; }
+inline bool mx_one_takes(int type, size_t tokens, size_t cols) {
+  if (type != MOE_F32 && type != MOE_BF16) return false;
+  const size_t columns = tokens * (type == MOE_F32 ? 6 : 4);
+  return columns <= 16 && mx_one_lds(cols / 32, columns) <= 64 * 1024;
+}
 hipError_t launch_mx_one(const MxGemmArgs &a, const void *x, hipStream_t s);
-// The form for few rows (mx_few.hip).
-hipError_t launch_mx_few(const MxGemmArgs &a, hipStream_t s);
-// One to a few f32 or bf16 rows x, without MxRows (a.codes, a.scales).
-bool mx_one_takes(int type, size_t tokens, size_t cols);
-hipError_t launch_mx_one(const MxGemmArgs &a, const void *x, hipStream_t s);
-// out [n / rows][rows] = the sum of parts [parts][n] in order, + bias
-hipError_t launch_mx_sum(const float *part, int parts, size_t n, size_t rows, const float *bias, void *out, bool bf16, hipStream_t s);
 
 struct RouteRule {
   int score, normalize, k, groups, top_groups, two;

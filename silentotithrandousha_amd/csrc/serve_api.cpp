@@ -125,7 +125,7 @@ int moe_route_device(moe_ctx *ctx, const moe_routing *rule, const float *logits,
   RETURN_IF(check_rule(rule, T, E));
   if (T && (!logits || !idx || !weights)) return fail(MOE_ERR_INVALID, "null logits, idx or weights");
   RETURN_IF(check_aligned({logits, idx, weights, counts}, 4));
-  if (T) RETURN_IF(check_distinct({idx, weights, counts}, {logits, rule->bias}));
+  RETURN_IF(check_distinct({idx, weights, counts}, {logits, rule->bias}));
   if (T || counts)
     HIP_TRY(launch_route_rule(rule_of(*rule), logits, T, (int)E, idx, weights, counts, stream ? (hipStream_t)stream : c.stream));
   return MOE_OK;

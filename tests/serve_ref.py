@@ -59,6 +59,10 @@ def matmul(x, x_type, w, bias, dtype):
         off = np.where(top < 2.0 ** -99, 2.0 ** -129, 2.0 ** (-29 if x_type == MOE_F32 else -19) * top)
         if x_type == MOE_BF16:  # values of bf16 down to 2^-11 of the largest enter exactly
             small = np.abs(x).reshape(*top.shape, 32) < 2.0 ** -11 * top[..., None]
+            # (a block whose largest is below 2^-99: terms have scales of at least 2^-126 and steps of 2^-3 of those, so that a bf16
+            # between 2^-k and 2^(1 - k), whose step is 2^-(k + 7), is off by up to 2^-130 from k = 123 on, whatever the block's
+            # largest; the last term's rounding counted as 2^-129 as for f32)
+            small |= (top < 2.0 ** -99)[..., None]
             tol += (off[..., None] * small).reshape(x.shape) @ np.abs(w).T
         else:
             tol += off.repeat(32, -1) @ np.abs(w).T
@@ -169,7 +173,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
             tokens[t], logprob[t] = order[0], 0.0
             continue
         with np.errstate(invalid="ignore"):
-            z = np.where(row == m, 0.0, (row - m) / tau)
+            z = np.where(row == m, 0.0, np.where(row == -np.inf, -np.inf, (row - m) / tau))
         e = np.exp(z)[order]
         k = V if top_k is None or top_k[t] < 1 else min(int(top_k[t]), V)
         p = 1.0 if top_p is None else float(top_p[t])
