@@ -50,7 +50,9 @@ int moe_mxfp4_quantize_device(moe_ctx *ctx, const void *x, int dtype, size_t n_r
  * absolute. A row that holds a value that is not finite, or a scale byte of 255, gives NaN, as does a scale
  * byte of 255 in W; a scale byte of 0 counts as 2^-127. packed, x, y and bias are 16-byte aligned; rows is a
  * multiple of 16, at most 2^24, cols of 32, at most 2^20. Workspace: the rows as the product takes them, 0.53 cols
- * bytes a token for MOE_MXFP4, 1.03 for MOE_MXFP8, 3.03 for MOE_BF16 and 4.53 for MOE_F32. */
+ * bytes a token for MOE_MXFP4, 1.03 for MOE_MXFP8, 3.03 for MOE_BF16 and 4.53 for MOE_F32, of 65536 tokens at a time (fewer
+ * of above 65536 cols); none for one or two rows of MOE_F32 and up to four of MOE_BF16 of up to 3968 cols (of
+ * fewer such rows up to 16000). */
 int moe_mxfp4_matmul_device(moe_ctx *ctx, const uint8_t *packed, size_t rows, size_t cols, const float *bias,
                             const void *x, int x_type, const uint8_t *x_scales, size_t n_tokens, void *y, int dtype,
                             void *stream);
@@ -103,9 +105,9 @@ typedef struct moe_sampling {
  * 1 and above as the last). tokens [n_tokens]; logprob [n_tokens] (may be NULL): the logarithm of its
  * probability among those left, 0 where the temperature is not above 0. Probabilities are multiples of 2^-44 of the
  * largest (2^-(62 - log2 vocab) for a vocab above 2^18), their sums exact. A NaN logit counts as -inf, infinite ones
- * share the row; a row without a logit above -inf gives token -1, logprob NaN. Workspace: 57 KB a row and
- * 16 bytes for every 8192 logits, of 4096 rows at a time; where more than 4096 logits of a row lie within 1/64 of a temperature at the border of
- * top_k or top_p, the row takes longer. */
+ * share the row; a row without a logit above -inf gives token -1, logprob NaN. Workspace: 57 KB a row and 21 bytes for every
+ * 1024 logits, of 4096 rows at a time. Where more than 4096 logits have to be looked at for a row's border (those within 1/64 of a
+ * temperature of it; of a top-k up to 2048 all that are not surely below its border) the row takes longer. */
 int moe_sample_device(moe_ctx *ctx, const moe_sampling *rule, const float *logits, size_t ld, const float *u, size_t n_tokens,
                       size_t vocab, int32_t *tokens, float *logprob, void *stream);
 

@@ -12,8 +12,14 @@
 //
 // Launches: largest logits of chunks; masses or bins; the border's tokens (and masses above them); the draw, a workgroup a
 // row. A workgroup takes one or more chunks of 2048 logits. A row with a top-k of up to kFewK counts bins, no masses, and gathers all
-// that top-k leaves; other rows sum masses by bin, and gather the bins that hold a border. What is gathered is sorted in LDS. Should
-// it be more than kList tokens, the draw goes through the row itself.
+// that top-k leaves; other rows sum masses by bin, and gather the bins that hold a border. Of a top-k well below the row's pieces
+// of 256 logits even the bins are those of the pieces' largest alone: no piece below the k-th of them holds one of the k, and
+// the second launch gathers from the few that may. What is gathered is sorted in LDS. Should it be more than kList tokens, the draw
+// goes through the row itself.
+//
+// 256 rows of 201088 logits, of which half have a top-k of 20 to 400, half a top-p: 34, 50, 20 and 18 us. The first is bound by its 206
+// MB (6.1 TB/s), the second by the 64-bit arithmetic and LDS atomics of the rows without a small top-k, the third by reads through the
+// last-level cache, the draw by the latency of some 40 steps that wait for each other (11 us for a single row).
 #include <algorithm>
 
 #include "device.hpp"
@@ -28,12 +34,15 @@ constexpr int kBins = 2048, kTail = kBins - 1;  // bin kTail: mass 0, not counte
 constexpr int kList = 4096;                     // tokens that are gathered of a row
 constexpr uint32_t kParts = 1024;                // chunks whose masses the draw holds in LDS
 constexpr uint32_t kFewK = 2048;                // top-k up to which all that it leaves is
+constexpr int kPiece = 256;                      // neighbouring logits whose largest is kept, a wavefront's of a chunk
+constexpr int kPieces = 8 * kThreads;            // of a row, at most
 
 struct RowState;
 
 // Workspace of a launch over T rows.
 struct Work {
   uint2 *largest;       // [T][groups] largest logit of kMaxSpan chunks and its first place
+  float *peak;          // [T][8 chunks] largest logit of a piece
   uint64_t *mass;       // [T][chunks]
   uint64_t *bin_mass;   // [T][kBins]
   uint32_t *bin_count;  // [T][kBins]
@@ -48,7 +57,7 @@ struct Args {
   const float *u;
   uint32_t V, chunks, groups;
   int shift, span;  // span: chunks that a workgroup takes
-
+  bool peaks;       // Work::peak is filled
   int32_t *tokens;
   float *logprob;
   Work w;
@@ -88,7 +97,7 @@ struct Row {
   const double *table;  // kPowers in LDS
   uint32_t k;
   int shift;
-  bool greedy, by_k, by_p, few;
+  bool greedy, by_k, by_p, few, direct;
   __device__ __forceinline__ void set(const Args &a, uint32_t t, float largest, const double *powers) {
     table = powers;
     m = largest;
@@ -103,9 +112,15 @@ struct Row {
     const float pp = a.rule.top_p ? a.rule.top_p[t] : 1.0f;
     by_p = pp < 1.0f;
     few = by_k && k <= kFewK;
+    direct = takes_direct(a, kk);
     p = fmax((double)pp, 0.0);
     const float mp = a.rule.min_p ? a.rule.min_p[t] : 0.0f;
     least = mp > 0.0f ? (double)mp * (double)((uint64_t)1 << shift) : 0.0;
+  }
+  // A row whose top-k is up to half of its pieces is gathered without counting its logits: pieces whose largest is below the k-th largest of those
+  // hold none of the k. (Above that, most pieces hold one, and the list of tokens above that border grows.)
+  static __device__ __forceinline__ bool takes_direct(const Args &a, int k) {
+    return a.peaks && k > 0 && (uint32_t)k <= kFewK && (uint32_t)k * 2 <= a.chunks * (kChunk / kPiece) && (uint32_t)k < a.V;
   }
   __device__ __forceinline__ bool cut() const { return by_k || by_p; }
   // Masses of four logits, and which of them min_p leaves (a largest logit always).
@@ -369,6 +384,14 @@ __global__ __launch_bounds__(kThreads) void k_sample_max(Args a) {
   begin_row(a, t);
   float m = -INFINITY;
   uint32_t at = 0xFFFFFFFFu;
+  if (a.peaks) {
+#pragma unroll
+    for (int j = 0; j < kMaxSpan; j++) {
+      const float peak = wave_fmax_dpp(fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(fmaxf(v[j].z, v[j].w), -INFINITY)));
+      if ((threadIdx.x & 63) == 0 && c0 + j < a.chunks)
+        a.w.peak[((size_t)t * a.chunks + c0 + j) * (kChunk / kPiece) + (threadIdx.x >> 6)] = peak;
+    }
+  }
 #pragma unroll
   for (int j = 0; j < kMaxSpan; j++) {
     const uint32_t i = place_of(c0 + j);
@@ -408,6 +431,104 @@ __device__ __forceinline__ void each_chunk(const Args &a, const float *row, cons
   }
 }
 
+// Gives the lanes of N masks places behind `n` of a list, with one atomic a wavefront: to(i, place) in the lanes of mask i.
+template <int N, class F>
+__device__ __forceinline__ void append(const uint64_t (&takes)[N], uint32_t *n, F &&to) {
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < N; i++) all += __popcll(takes[i]);
+  if (!all) return;
+  uint32_t at = 0;
+  if ((threadIdx.x & 63) == 0) at = atomicAdd(n, all);
+  at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    if (takes[i] >> (threadIdx.x & 63) & 1) to(i, at + __popcll(takes[i] & ((1ull << (threadIdx.x & 63)) - 1)));
+    at += __popcll(takes[i]);
+  }
+}
+
+// Into the row's list, of this workgroup's chunks: all tokens whose bin is up to that in which the k-th largest of the row's
+// pieces lies, read from the pieces that hold one.
+__device__ __forceinline__ void gather_few(const Args &a, uint32_t t, const Row &r, const float *row, uint32_t *s_count) {
+  __shared__ uint32_t s_some;
+  __shared__ uint16_t s_piece[kPieces];
+  constexpr int kMine = kPieces / kThreads, kOfChunk = kChunk / kPiece;
+  const uint32_t pieces = a.chunks * kOfChunk, lane = threadIdx.x & 63;
+  int bin[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; i++) {
+    const uint32_t p = i * kThreads + threadIdx.x;
+    bin[i] = p < pieces ? r.bin(a.w.peak[(size_t)t * pieces + p]) : kTail;
+  }
+  for (int b = threadIdx.x; b < kBins; b += kThreads) s_count[b] = 0;
+  if (threadIdx.x == 0) s_some = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kMine; i++)
+    if (bin[i] < kTail) atomicAdd(s_count + bin[i], 1u);
+  __syncthreads();
+  Bins bins;
+  uint32_t sum = 0;
+#pragma unroll
+  for (int i = 0; i < Bins::kPer; i++) {
+    bins.count[i] = sum += s_count[threadIdx.x * Bins::kPer + i];
+    bins.mass[i] = 0;
+  }
+  bins.before_count = (uint32_t)block_before(sum);
+  bins.before_mass = 0;
+#pragma unroll
+  for (int i = 0; i < Bins::kPer; i++) bins.count[i] += bins.before_count;
+  const int most = min(bins.first([&](uint32_t c, uint64_t) { return c >= r.k; }).bin, kTail - 1);
+  const uint32_t first = blockIdx.x * a.span * kOfChunk, last = first + a.span * kOfChunk;
+  {
+    uint64_t takes[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+      const uint32_t p = i * kThreads + threadIdx.x;
+      takes[i] = __ballot(bin[i] <= most && p >= first && p < last);
+    }
+    append(takes, &s_some, [&](int i, uint32_t at) { s_piece[at] = (uint16_t)(i * kThreads + threadIdx.x); });
+  }
+  __syncthreads();
+  // a wavefront a piece, several under way
+  constexpr int kAhead = 8, kWaves = kThreads / 64;
+  const uint32_t some = s_some;
+  for (uint32_t p0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); p0 < some; p0 += kAhead * kWaves) {
+    struct __attribute__((packed, aligned(4))) four { float v[4]; };
+    four f[kAhead];
+    uint32_t place[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const uint32_t p = p0 + j * kWaves;
+      place[j] = s_piece[min(p, some - 1)] * kPiece + lane * 4;
+      f[j] = four{{-INFINITY, -INFINITY, -INFINITY, -INFINITY}};
+      if (p >= some) continue;
+      if (place[j] + 4 <= a.V) {
+        f[j] = *(const four *)(row + place[j]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+          if (place[j] + x < a.V) f[j].v[x] = row[place[j] + x];
+      }
+    }
+    uint64_t takes[4 * kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      float l[4];
+      logits_of(make_float4(f[j].v[0], f[j].v[1], f[j].v[2], f[j].v[3]), l);
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        f[j].v[x] = l[x];
+        takes[4 * j + x] = __ballot(r.bin(l[x]) <= most);
+      }
+    }
+    append(takes, &a.w.row[t].listed, [&](int i, uint32_t at) {
+      if (at < kList) a.w.list[(size_t)t * kList + at] = make_uint2(key_of(f[i / 4].v[i % 4]), place[i / 4] + i % 4);
+    });
+  }
+}
+
 __global__ __launch_bounds__(kThreads) void k_sample_mass(Args a) {
   const uint32_t t = blockIdx.y;
   __shared__ unsigned long long s_mass[kBins];
@@ -424,6 +545,10 @@ __global__ __launch_bounds__(kThreads) void k_sample_mass(Args a) {
   Row r;
   r.set(a, t, m, s_powers);
   if (r.greedy || m == -INFINITY) return;
+  if (r.direct) {
+    gather_few(a, t, r, row, s_count);
+    return;
+  }
   if (!r.cut()) {
     __syncthreads();
     each_chunk(a, row, v, [&](uint32_t c, const float (&l)[4]) {
@@ -481,6 +606,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_border(Args a) {
   __shared__ uint2 s_held[kList];
   __shared__ uint32_t s_n, s_at;
   const uint32_t t = blockIdx.y;
+  if (a.peaks && Row::takes_direct(a, a.rule.top_k[t])) return;
   load_powers(s_powers);
   if (threadIdx.x == 0) s_n = 0;
   const float *row = a.logits + t * a.ld;
@@ -630,12 +756,13 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(Args a) {
   // (what the row's list may hold, before it is known how much that is)
   const uint2 early = a.w.list[(size_t)t * kList + threadIdx.x];
   const uint32_t n = a.w.row[t].listed;
-  const Border border = a.w.row[t].border;
+  Border border = a.w.row[t].border;
   Row r;
   uint32_t at;
   __shared__ double s_powers[kPowersOf2];
   load_powers(s_powers);
   const bool live = row_of(a, t, s_powers, r, at);
+  if (r.direct) border.low = 0, border.high = kTail, border.before = 0, border.first = true;  // (k is of other rows)
   if (!live || r.greedy) {
     if (threadIdx.x == 0) {
       a.tokens[t] = live ? (int32_t)at : -1;
@@ -848,6 +975,7 @@ size_t work_layout(Work &w, char *p, size_t T, size_t chunks, size_t groups) {
   w.row = (RowState *)take(T * sizeof(RowState));
   w.mass = (uint64_t *)take(T * chunks * 8);
   w.largest = (uint2 *)take(T * groups * 8);
+  w.peak = (float *)take(T * chunks * (kChunk / kPiece) * 4);
   w.bin_mass = (uint64_t *)take(T * kBins * 8);
   w.bin_count = (uint32_t *)take(T * kBins * 4);
   w.list = (uint2 *)take(T * kList * 8);
@@ -874,13 +1002,18 @@ hipError_t launch_sample(const SampleArgs &s, hipStream_t st) {
   a.V = s.V;
   a.chunks = sample_chunks(s.V);
   a.groups = sample_groups(a.chunks);
+  // (All launches of 257 rows of 201088 with a top-k of 50: 128 us if their logits are counted and read again for the border's tokens,
+  // 75 by pieces; with one of 390, 136 and 106; 8 rows 28 and 25. A single row takes 28 and 30.)
+  a.peaks = s.rule.top_k && a.chunks * (kChunk / kPiece) <= kPieces && (size_t)s.T * a.chunks >= 768;
   a.shift = 44;
   while (((uint64_t)s.V << a.shift) > (uint64_t)1 << 62) a.shift--;
   a.tokens = s.tokens;
   a.logprob = s.logprob;
   work_layout(a.w, (char *)s.work, s.T, a.chunks, a.groups);
-  // up to 3 workgroups a CU, each of which adds its bins to the row's once
-  a.span = (int)(((size_t)s.T * a.chunks + 767) / 768);
+  // Workgroups add their bins to the row's once, which costs as much as some chunks: 3 a CU, and up to 6 while a workgroup keeps
+  // 8 chunks (256 rows of 201088 mixed: 3 a CU 59 and 32 us, 6 a CU 50 and 20; 254 rows of 32003: 13 and 12, or 20 and 15).
+  const size_t all = (size_t)s.T * a.chunks;
+  a.span = (int)std::max((all + 1535) / 1536, std::min<size_t>((all + 767) / 768, 8));
   const dim3 grid((a.chunks + a.span - 1) / a.span, s.T);
   hipError_t e = launch_own(k_sample_max, dim3(a.groups, s.T), kThreads, 0, st, a);
   if (e == hipSuccess) e = launch_own(k_sample_mass, grid, kThreads, 0, st, a);

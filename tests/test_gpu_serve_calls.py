@@ -307,6 +307,30 @@ def test_sample_flat_rows(d, V, which):  # noqa: F811
     check_sample(d, logits, rng.random(T).astype(np.float32), **f)
 
 
+@pytest.mark.parametrize("V", [2048, 20000, 32003, 300000])
+@pytest.mark.parametrize("k", [1, 4, 30, 60, 580])
+def test_sample_few_of_many(d, k, V):  # noqa: F811
+    """top-k below and above half of the row's pieces of 256 logits: ordinary rows, rows whose largest lie side by side, whose
+    pieces are nearly all masked, whose logits are equal or few values."""
+    rng = np.random.default_rng([21, k, V])
+    T = 8
+    logits = (rng.standard_normal((T, V)) * 3).astype(np.float32)
+    logits[1] = np.sort(logits[1])
+    logits[2, 700:] = -np.inf
+    logits[3, :] = -np.inf
+    logits[3, 5::256] = np.linspace(0, 3, len(logits[3, 5::256]))
+    logits[4] = 1.0
+    logits[5] = np.round(logits[5])
+    logits[6, rng.random(V) < 0.5] = np.nan
+    logits[7] *= 1e-4
+    logits = np.tile(logits, (-(-800 // (T * -(-V // 2048))), 1))  # enough rows that their pieces are looked at
+    T = len(logits)
+    u = rng.random(T).astype(np.float32)
+    check_sample(d, logits, u, top_k=np.full(T, k, np.int32))
+    check_sample(d, logits, u, top_k=np.where(np.arange(T) % 2 == 0, k, 0).astype(np.int32), top_p=np.full(T, 0.813, np.float32),
+                 temperature=rng.uniform(0.4, 1.6, T).astype(np.float32), min_p=np.full(T, 0.01, np.float32))
+
+
 @pytest.mark.parametrize("temperature", [1e-4, 0.05, 30.0, 1e6, 1e30, np.inf])
 def test_sample_far_temperatures(d, temperature):  # noqa: F811
     rng = np.random.default_rng(18)
