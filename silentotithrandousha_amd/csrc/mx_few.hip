@@ -1,6 +1,8 @@
 // Products of a few rows with a resident MXFP4 matrix (mx_gemm.hpp's operands and arithmetic): bound by the weights, which a
 // workgroup's 8 wavefronts stream through registers, each every eighth step of K, and by the latency of its loads.
-// There is no barrier before the wavefronts' sums meet in LDS, where they are added in order.
+// There is no barrier before the wavefronts' sums meet in LDS, where they are added in order. (One f32 row over 5760 x 2880: 4.7 us for
+// 8.8 MB, of which the stream is 1.3 and the rest a launch's and a load's latency. K split over workgroups instead, with a launch that
+// adds the parts, was slower.)
 #include "act8.hpp"
 #include "serve.hpp"
 

@@ -16,7 +16,8 @@ __device__ __forceinline__ float quad_xor(float v) {
   return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), XOR == 1 ? 0xB1 : 0x4E, 0xF, 0xF, true));
 }
 
-// Four lanes a block of 32 values (which leave together).
+// Four lanes a block of 32 values (which leave together): a lane reads 16 bytes of bf16, or 32 of f32, and writes 4. Bound by memory:
+// 23040 x 2880 bf16 (133 MB read, 35 written) take 25 us, 6.7 TB/s; one row 1.9 us, the latency of its loads.
 template <class S>
 __global__ __launch_bounds__(256) void k_mx4_quantize(const S *x, size_t blocks, uint8_t *codes, uint8_t *scales) {
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i / 4 < blocks; i += (size_t)gridDim.x * 256) {

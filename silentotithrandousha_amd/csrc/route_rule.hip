@@ -6,6 +6,10 @@
 // keys are first taken in f32, each within 2^-19 of the row's largest score (and 2^-24 of itself), and the choice stands if no two
 // keys that it compares are closer than 2^-18 of that. Else (a token in some hundreds) it is made again with keys of 64 bits.
 // Without a bias or groups the logits' order is the scores', exactly. Weights are of 64 bits until their rounding.
+//
+// 16384 tokens of 256 experts (8 of 4 of 8 groups, sigmoid, bias): 34 us, the gradient 13, where their bytes take 11. Bound by
+// instructions that wait for each other, 4 wavefronts a SIMD (97 registers, the 64-bit choice's): k times a largest key over the
+// wavefront, its lane and its place, one after the other. 512 workgroups in place of 256: 40 us.
 #include <algorithm>
 
 #include "device.hpp"

@@ -1,5 +1,5 @@
 // C++ host mirror of the reference's GpuMoeDispatcher (src/gpu/moe_dispatch.rs:36-684) over
-// the C ABI of libmxfp4moe.so (include/mxfp4_moe.h, moe_dense.h). Header-only; link -lmxfp4moe.
+// the C ABI of libmxfp4moe.so (include/mxfp4_moe.h, moe_dense.h, moe_serve.h). Header-only; link -lmxfp4moe.
 //
 // Same method names, argument meaning and error behaviour as the Rust type:
 //   * the constructor is the only fallible call and returns Result<GpuMoeDispatcher>
@@ -21,6 +21,7 @@
 #include <vector>
 
 #include "../../include/moe_dense.h"
+#include "../../include/moe_serve.h"
 #include "../../include/mxfp4_moe.h"
 
 namespace silentot {
@@ -267,6 +268,33 @@ class GpuMoeDispatcher {
   }
   void act8_unpack_device(const uint8_t *packed, size_t T, size_t cols, void *out, moe_dtype dtype, void *stream = nullptr) const {
     moe_check(moe_act8_unpack_device(ctx_, packed, T, cols, out, dtype, stream));
+  }
+  // The serving operators (include/moe_serve.h), likewise.
+  void mxfp4_quantize_device(const void *x, moe_dtype dtype, size_t n_rows, size_t cols, uint8_t *blocks, uint8_t *scales,
+                             void *stream = nullptr) const {
+    moe_check(moe_mxfp4_quantize_device(ctx_, x, dtype, n_rows, cols, blocks, scales, stream));
+  }
+  static size_t mxfp4_packed_size(size_t rows, size_t cols) { return moe_mxfp4_packed_size(rows, cols); }
+  void mxfp4_pack_device(const uint8_t *blocks, const uint8_t *scales, size_t rows, size_t cols, uint8_t *packed,
+                         void *stream = nullptr) const {
+    moe_check(moe_mxfp4_pack_device(blocks, scales, rows, cols, packed, stream ? stream : moe_stream(ctx_)));
+  }
+  // x_type: a moe_dtype, or MOE_MXFP4.
+  void mxfp4_matmul_device(const uint8_t *packed, size_t rows, size_t cols, const float *bias, const void *x, int x_type,
+                           const uint8_t *x_scales, size_t T, void *y, moe_dtype dtype, void *stream = nullptr) const {
+    moe_check(moe_mxfp4_matmul_device(ctx_, packed, rows, cols, bias, x, x_type, x_scales, T, y, dtype, stream));
+  }
+  void route_device(const moe_routing &rule, const float *logits, size_t T, size_t n_experts, int32_t *idx, float *weights,
+                    int32_t *counts = nullptr, void *stream = nullptr) const {
+    moe_check(moe_route_device(ctx_, &rule, logits, T, n_experts, idx, weights, counts, stream));
+  }
+  void route_backward_device(const moe_routing &rule, const float *logits, const int32_t *idx, const float *dweights, size_t T,
+                             size_t n_experts, float *dlogits, void *stream = nullptr) const {
+    moe_check(moe_route_backward_device(ctx_, &rule, logits, idx, dweights, T, n_experts, dlogits, stream));
+  }
+  void sample_device(const moe_sampling &rule, const float *logits, size_t ld, const float *u, size_t T, size_t vocab,
+                     int32_t *tokens, float *logprob = nullptr, void *stream = nullptr) const {
+    moe_check(moe_sample_device(ctx_, &rule, logits, ld, u, T, vocab, tokens, logprob, stream));
   }
   // Waits for the context's stream.
   void synchronize() const { moe_check(moe_synchronize(ctx_)); }
