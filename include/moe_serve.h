@@ -9,7 +9,7 @@
  *
  * All calls take device pointers and are asynchronous on `stream` (a hipStream_t, NULL = the context's
  * stream). Matrices are contiguous, rows first, unless a stride is given. No output may overlap an input or
- * another output. Results depend on the arguments' values and on nothing else. What lies behind the last row
+ * another output. Results depend on the arguments' values and shapes, and on nothing else. What lies behind the last row
  * of an output is left as it was. n_tokens is at most 2^20.
  */
 #ifndef MOE_SERVE_H

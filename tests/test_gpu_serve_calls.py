@@ -380,6 +380,75 @@ def test_sample_keeps_nothing_between_calls(d):  # noqa: F811
     assert np.array_equal(a[0][p], b[0]) and np.array_equal(a[1][p], b[1])
 
 
+# ------------------------------------------------------------------ offsets past 32 bits
+
+
+class Large:
+    """A buffer of zeros, written and read in parts."""
+
+    def __init__(self, n):
+        self.buf = DeviceBuffer(n)
+        self.ptr, self.n = self.buf.ptr, n
+        check(lib().moe_memset_device(self.ptr, 0, n))
+
+    def put(self, at, a):
+        a = np.ascontiguousarray(a)
+        check(lib().moe_memcpy_h2d(self.ptr + at, a.ctypes.data, a.nbytes))
+
+    def get(self, at, shape, dtype):
+        a = np.empty(shape, dtype)
+        check(lib().moe_memcpy_d2h(a.ctypes.data, self.ptr + at, a.nbytes))
+        return a
+
+
+def test_quantize_past_32_bits(d):  # noqa: F811
+    T, C = 2**17 + 3, 2**15
+    x = np.random.default_rng(22).standard_normal((2, C)).astype(np.float32)
+    stored, v = dense_ref.store(x, MOE_BF16)
+    src, blocks, scales = Large(T * C * 2), Large(T * C // 2), Large(T * C // 32)
+    src.put((T - 2) * C * 2, stored)
+    d.mxfp4_quantize_device(src, MOE_BF16, T, C, blocks, scales)
+    d.synchronize()
+    want = ref.mx4(v)
+    assert np.array_equal(blocks.get((T - 2) * C // 2, (2, C // 32, 16), np.uint8), want[0])
+    assert np.array_equal(scales.get((T - 2) * C // 32, (2, C // 32), np.uint8), want[1])
+    assert (scales.get((T - 3) * C // 32, (C // 32,), np.uint8) == 1).all()
+
+
+def test_matmul_past_32_bits(d):  # noqa: F811
+    """More than one piece of tokens, more than 4 GB of results."""
+    T, R, C = 66000, 16416, 32
+    blocks, scales = weights(23, R, C)
+    packed = resident(d, blocks, scales)
+    x = np.random.default_rng(23).standard_normal((T, C)).astype(np.float32)
+    y = Large(T * R * 4)
+    d.mxfp4_matmul_device(packed, R, C, None, dev(x), MOE_F32, None, T, y, MOE_F32)
+    d.synchronize()
+    for t in (0, 40000, 65400, 65535, 65536, T - 1):
+        want, tol = ref.matmul(x[t:t + 1], MOE_F32, ref.mx4_values(blocks, scales), np.zeros(R), MOE_F32)
+        assert (np.abs(y.get(t * R * 4, (1, R), np.float32) - want) <= tol).all(), t
+
+
+def test_sample_past_32_bits(d):  # noqa: F811
+    T, V = 2100, 2**19 + 1
+    rng = np.random.default_rng(24)
+    last = (rng.standard_normal((2, V)) * 3).astype(np.float32)
+    logits = Large(T * V * 4)
+    logits.put((T - 2) * V * 4, last)
+    u = rng.random(T).astype(np.float32)
+    for top_k, top_p in ((0, 1.0), (50, 1.0), (0, 0.9)):
+        k, p = np.zeros(T, np.int32), np.ones(T, np.float32)
+        k[-2:], p[-2:] = top_k, top_p
+        bufs = [dev(k), dev(p), dev(u)]
+        tokens = Out((T,), np.int32)
+        d.sample_device(Sampling(None, bufs[0].ptr, bufs[1].ptr, None), logits, V, bufs[2], T, V, tokens)
+        d.synchronize()
+        got = tokens.get()
+        want, _, room = ref.sample(last, u[-2:], top_k=k[-2:], top_p=p[-2:])
+        assert (room > 2.0 ** -40).all() and np.array_equal(got[-2:], want)
+        assert (np.abs(got[:-2] - u[:-2].astype(np.float64) * V) <= 1).all()  # (equal logits)
+
+
 # ------------------------------------------------------------------ streams, graphs, workspaces, together
 
 
