@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from oracle import orc
-from silentotithrandousha_amd import (MOE_BF16, MOE_F32, MOE_MXFP4, MOE_MXFP8, MOE_SCORE_SIGMOID, DeviceBuffer, GpuMoeDispatcher, MoeError,
+from silentotithrandousha_amd import (MOE_BF16, MOE_F32, MOE_MXFP4, MOE_MXFP8, MOE_SCORE_SIGMOID, MOE_SCORE_SOFTMAX, DeviceBuffer, GpuMoeDispatcher, MoeError,
                                       Routing, Sampling, _ffi)
 from silentotithrandousha_amd import synthetic as syn
 from silentotithrandousha_amd._ffi import check, lib
@@ -200,6 +200,44 @@ def test_route_keys_closer_than_f32(d):  # noqa: F811
         for t in other:
             assert np.abs(key[t][idx[t]] - key[t][want[0][t]]).max() < 2.0 ** -50 or kw.get("groups"), (kw, t)
         assert len(other) <= 2, kw
+
+
+@pytest.mark.parametrize("E,kw", [(256, dict(k=8, groups=8, top_groups=4, two=True)), (256, dict(k=5)), (250, dict(k=32)), (128, dict(k=6, groups=4, top_groups=2)),
+                                  (128, dict(k=3, groups=16, top_groups=16)), (96, dict(k=4, groups=3, top_groups=2, two=True)), (72, dict(k=9, groups=8, top_groups=3)),
+                                  (64, dict(k=8, groups=2, top_groups=1, scale=2.5)), (40, dict(k=2, normalize=False)), (2, dict(k=2)), (7, dict(k=1))])
+@pytest.mark.parametrize("score", [MOE_SCORE_SOFTMAX, MOE_SCORE_SIGMOID])
+def test_route_many(d, score, E, kw):  # noqa: F811
+    """Many tokens with a bias: ordinary ones, masked, equal, infinite and with keys closer than an f32 tells apart, side by side."""
+    rng = np.random.default_rng([25, E, score])
+    T, n = 4097, 241
+    x = (rng.standard_normal((n, E)) * 1.5).astype(np.float32)
+    x[5:40][rng.random((35, E)) < 0.6] = -np.inf
+    x[40] = -np.inf
+    x[41] = np.nan
+    x[42, ::3] = np.inf
+    x[43:60] = x[43]
+    x[60:80] = np.round(x[60:80])
+    bias = (rng.standard_normal(E) * 0.1).astype(np.float32)
+    bias[E // 2:] = bias[0]
+    near = (1.0 - ref.scores(x[100:101], score)[0]).astype(np.float32)  # all keys of rows 100 .. nearly the same
+    x[100:120] = x[100] + (rng.standard_normal((20, E)) * 1e-6).astype(np.float32)
+    for b in (bias, near):
+        if b is bias and E > 6:
+            b[3], b[4] = np.nan, -np.inf
+        keep = dev(b)
+        r = rule(score=score, bias=keep, **kw)
+        want = ref.route(x, r, b)
+        at = rng.integers(0, n, T)
+        at[:n] = np.arange(n)
+        idx, w, count = route(d, r, x[at])
+        key = ref.scores(x, score) + b.astype(np.float64)
+        other = np.nonzero((idx != want[0][at]).any(1))[0]
+        for t in other:  # (two libraries' exponentials differ in the last bit of 64)
+            assert np.abs(key[at[t]][idx[t]] - key[at[t]][want[0][at[t]]]).max() < 2.0 ** -50, t
+        assert len(other) <= T // 100
+        same = np.setdiff1d(np.arange(T), other)
+        assert (np.abs(w - want[1][at])[same] <= 2.0 ** -24 * np.abs(want[1][at])[same] * 1.001 + 1e-45).all()
+        assert np.array_equal(count, np.bincount(idx[idx >= 0], minlength=E))
 
 
 def test_route_is_the_paths_own(d):  # noqa: F811
