@@ -7,7 +7,7 @@
 // keys that it compares are closer than 2^-18 of that. Else (a token in some hundreds) it is made again with keys of 64 bits.
 // Without a bias or groups the logits' order is the scores', exactly. Weights are of 64 bits until their rounding.
 //
-// 16384 tokens of 256 experts (8 of 4 of 8 groups, sigmoid, bias): 23 us, the gradient 13, where their bytes take 11. Bound by
+// 16384 tokens of 256 experts (8 of 4 of 8 groups, sigmoid, bias): 23 us, the gradient 8.4, where their bytes take 11. Bound by
 // instructions at 4 wavefronts a SIMD (some 100 registers, the 64-bit choice's), and by the last wavefronts that make a 64-bit choice.
 // One token a wavefront (k_route_rule: 690 VALU and 440 SALU instructions a token, k times a largest key over the wavefront, its lane and
 // its place) took 33.
@@ -587,12 +587,14 @@ __global__ __launch_bounds__(1024) void k_route_pairs(RouteRule r, const float *
 //   d / d s_j = scale / S dw_j - (normalised) sum_i dw_i w_i / S,
 //   sigmoid: d l_j = d s_j s_j (1 - s_j);  softmax: d l_e = s_e (d s_e - sum_j d s_j s_j).
 // Of a normalised softmax that sum is 0, and S stands for its denominator, too: as for a sigmoid, the chosen experts' logits are
-// all that is read, and the other gradients are 0.
-template <int Q>
+// all that is read, and the other gradients are 0: the chosen ones' go to their places through LDS (13 us for 16384 tokens of 256 experts
+// if every lane looks for its own among all, with 64-bit sums, so 8.4). An expert that idx names twice gets their sum.
+template <int Q, bool DENSE>  // DENSE: a softmax without normalisation, all of whose experts have a gradient
 __global__ __launch_bounds__(256) void k_route_rule_backward(RouteRule r, const float *logits, const int32_t *idx, const float *dw, uint32_t T,
                                                              int E, float *dl) {
+  __shared__ float s_out[4][64 * Q];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const bool dense = r.score == MOE_SCORE_SOFTMAX && !r.normalize;
+  float *s_row = s_out[wave];
   const uint32_t step = gridDim.x * 4;
   for (uint32_t t = blockIdx.x * 4 + wave; t < T; t += step) {
     int e = -1;
@@ -616,7 +618,7 @@ __global__ __launch_bounds__(256) void k_route_rule_backward(RouteRule r, const 
       rest = lg < 0.0f ? y : x * y;
     } else {
       m = lg;
-      if (dense) {
+      if constexpr (DENSE) {
         load_logits<Q>(logits + (size_t)t * E, E, lane, l);
 #pragma unroll
         for (int q = 0; q < Q; q++) {
@@ -626,7 +628,7 @@ __global__ __launch_bounds__(256) void k_route_rule_backward(RouteRule r, const 
       }
       m = wave_largest(m);
       sc = lg == -INFINITY ? 0.0 : lg == m ? 1.0 : exp64((double)lg - (double)m);
-      if (dense) {
+      if constexpr (DENSE) {
         sum = 0.0;
 #pragma unroll
         for (int q = 0; q < Q; q++) {
@@ -643,35 +645,51 @@ __global__ __launch_bounds__(256) void k_route_rule_backward(RouteRule r, const 
       const double S = slots_sum64(sc), inv = S > 0.0 ? 1.0 / S : 0.0;
       ds = (d - slots_sum64(d * sc) * inv) * inv;
     }
-    if (!dense) {
+    struct __attribute__((packed, aligned(4))) some { float v[Q]; };
+    some o;
+    bool twice = true;
+    if constexpr (!DENSE) {
       ds = ds * sc * rest;
 #pragma unroll
-      for (int q = 0; q < Q; q++) g[q] = 0.0;
+      for (int q = 0; q < Q; q++) s_row[lane * Q + q] = 0.0f;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (e >= 0) s_row[e] = __int_as_float(lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      twice = __any(e >= 0 && __float_as_int(s_row[max(e, 0)]) != lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (e >= 0) s_row[e] = (float)ds;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int q = 0; q < Q; q++) {
+        o.v[q] = s_row[lane * Q + q];
+        g[q] = 0.0;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     } else {
       const double mean = slots_sum64(ds * sc);
 #pragma unroll
       for (int q = 0; q < Q; q++) g[q] = g[q] * sum * -mean;
       ds = ds * sc;
     }
-    for (int j = 0; j < r.k; j++) {
-      const int ej = __builtin_amdgcn_readlane(e, j);
-      const double v = lane64(ds, j);
-      if (ej < 0) continue;
+    if (twice) {
+      for (int j = 0; j < r.k; j++) {
+        const int ej = __builtin_amdgcn_readlane(e, j);
+        const double v = lane64(ds, j);
+        if (ej < 0) continue;
 #pragma unroll
-      for (int q = 0; q < Q; q++)
-        if (q == ej % Q && lane == ej / Q) g[q] = g[q] + v;
-    }
-    struct __attribute__((packed, aligned(4))) some { float v[Q]; };
-    float *out = dl + (size_t)t * E + lane * Q;
-    if (lane * Q + Q <= E) {
-      some o;
+        for (int q = 0; q < Q; q++)
+          if (q == ej % Q && lane == ej / Q) g[q] = g[q] + v;
+      }
 #pragma unroll
       for (int q = 0; q < Q; q++) o.v[q] = (float)g[q];
+    }
+    float *out = dl + (size_t)t * E + lane * Q;
+    if (lane * Q + Q <= E) {
       *(some *)out = o;
     } else {
 #pragma unroll
       for (int q = 0; q < Q; q++)
-        if (lane * Q + q < E) out[q] = (float)g[q];
+        if (lane * Q + q < E) out[q] = o.v[q];
     }
   }
 }
@@ -709,11 +727,12 @@ hipError_t launch_route_rule_backward(const RouteRule &r, const float *logits, c
   if (!T) return hipSuccess;
   const unsigned grid = (unsigned)std::min<size_t>((T + 3) / 4, 4096);
   auto go = [&](auto k) { return launch_own(k, grid, 256, 0, s, r, logits, idx, dw, (uint32_t)T, E, dl); };
-  return E <= 64    ? go(k_route_rule_backward<1>)
-         : E <= 128 ? go(k_route_rule_backward<2>)
-         : E <= 256 ? go(k_route_rule_backward<4>)
-         : E <= 512 ? go(k_route_rule_backward<8>)
-                    : go(k_route_rule_backward<16>);
+  auto by_score = [&](auto dense, auto other) { return r.score == MOE_SCORE_SOFTMAX && !r.normalize ? go(dense) : go(other); };
+  return E <= 64    ? by_score(k_route_rule_backward<1, true>, k_route_rule_backward<1, false>)
+         : E <= 128 ? by_score(k_route_rule_backward<2, true>, k_route_rule_backward<2, false>)
+         : E <= 256 ? by_score(k_route_rule_backward<4, true>, k_route_rule_backward<4, false>)
+         : E <= 512 ? by_score(k_route_rule_backward<8, true>, k_route_rule_backward<8, false>)
+                    : by_score(k_route_rule_backward<16, true>, k_route_rule_backward<16, false>);
 }
 
 }  // namespace moe
