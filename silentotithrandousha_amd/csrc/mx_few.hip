@@ -66,7 +66,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_mx_few(MxGemmArgs a) {
     constexpr int kB = FMT == 4 ? 4 : FMT == 6 ? 2 : 0;
 #pragma unroll
     for (int t = 0; t < TERMS; t++) {
-      if (t)
+      if (t && FMT == 6)
 #pragma unroll
         for (int j = 0; j < CT; j++) sb[j] = (uint32_t)max((int)sb[j] - 5, 1);
 #pragma unroll
@@ -251,7 +251,7 @@ hipError_t launch_mx_few(const MxGemmArgs &a, hipStream_t s) {
   switch (a.r.type) {
     case MOE_F32: return by_tokens<6, 6>(a, s);
     case MOE_BF16: return by_tokens<6, 4>(a, s);
-    case MOE_MXFP8: return by_tokens<8, 1>(a, s);
+    case MOE_MXFP8: return by_tokens<8, 2>(a, s);
     case MOE_MXFP4: return by_tokens<4, 1>(a, s);
   }
   return hipErrorInvalidValue;

@@ -1,6 +1,6 @@
 // Product of rows with a resident MXFP4 matrix on v_mfma_scale_f32_16x16x128_f8f6f4: D[r][t] = sum W[r][k] x[t][k],
-// A = the weights as stored (tile16, layout.hpp), B = the rows as MxRows (serve.hpp): MXFP4 and MXFP8 rows as they are, bf16
-// and f32 rows as 4 and 6 E2M3 terms whose sum they are. A decoded to bf16 would cost more issue slots than the products save, and
+// A = the weights as stored (tile16, layout.hpp), B = the rows as MxRows (serve.hpp): MXFP4 rows as they are, MXFP8 rows as their larger and
+// their smaller codes, bf16 and f32 rows as 4 and 6 E2M3 terms whose sum they are. A decoded to bf16 would cost more issue slots than the products save, and
 // three bf16 planes of f32 rows three products at a quarter of the rate.
 //
 // A workgroup of WM x WN wavefronts computes MT x NT16 tiles of 16 x 16. A package is one term of a step of 128 values: the
@@ -211,15 +211,15 @@ __global__ __launch_bounds__(64 * S::kWaves) void k_mx_gemm(MxGemmArgs a) {
       constexpr int u = decltype(u_)::value, step = u / S::kTerms, term = u % S::kTerms;
       const uint32_t s = s0 + step;
       if (step && s >= ns) return;  // (steps are no multiple of 4)
-      // the rows' scales: of several terms 2^-5 each (a NaN's 255 is the first one's alone: the codes are 0)
-      if constexpr (S::kTerms > 1) {
+      // the rows' scales: of E2M3 terms 2^-5 each (a NaN's 255 is the first one's alone: the codes are 0)
+      if constexpr (S::kFmt == 6) {
 #pragma unroll
         for (int j = 0; j < S::TN; j++) sw[j] = term == 0 ? sb[j] >> 8 * step & 255 : (uint32_t)max((int)sw[j] - 5, 1);
       }
       constexpr int kB = S::kFmt == 4 ? 4 : S::kFmt == 6 ? 2 : 0, kAll = S::TM * S::TN, kHalf = kAll / 2;
       auto mfma = [&](int p) {
         const int i = p % S::TM, j = p / S::TM;
-        if constexpr (S::kTerms > 1)
+        if constexpr (S::kFmt == 6)
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A[step & 1][i], B[u & 1][j], acc[i][j], 4, kB, step, (int)sa[i], 0, (int)sw[j]);
         else
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A[step & 1][i], B[u & 1][j], acc[i][j], 4, kB, step, (int)sa[i], step, (int)sb[j]);

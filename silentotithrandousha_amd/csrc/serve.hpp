@@ -15,8 +15,8 @@ hipError_t launch_mx4_quantize(const void *x, bool bf16, size_t n, size_t cols, 
 // What a product makes of its rows: tiles of 16 rows x steps of 128 values as the block-scaled MFMA's B operand
 // takes them. Step s of tile n lies at ((n ns + s) terms) * kRowChunk bytes, one chunk a term: lane l = 16 g + j holds
 // block 4 s + g of row 16 n + j, in planes of 16 (and 8 or 16) bytes a lane. Behind the tiles, a scale word per (tile, 4
-// steps, lane), byte i that of step 4 q + i: the weights' layout (layout.hpp). Several terms share the first one's
-// byte: term t's is 5 t below it, at least 1.
+// steps, lane), byte i that of step 4 q + i: the weights' layout (layout.hpp). All terms share the
+// byte: an E2M3 term t's is 5 t below it, at least 1.
 struct MxRows {
   int type;     // MOE_F32, MOE_BF16, MOE_MXFP8, MOE_MXFP4
   uint32_t tokens, nb, ns, nq, tiles;
@@ -30,7 +30,7 @@ inline MxRows mx_rows(int type, size_t tokens, size_t cols) {
   r.ns = (r.nb + 3) / 4;
   r.nq = (r.ns + 3) / 4;
   r.tiles = (uint32_t)((tokens + 15) / 16);
-  r.terms = type == MOE_F32 ? 6 : type == MOE_BF16 ? 4 : 1;
+  r.terms = type == MOE_F32 ? 6 : type == MOE_BF16 ? 4 : type == MOE_MXFP8 ? 2 : 1;
   r.chunk = type == MOE_MXFP4 ? 1024 : type == MOE_MXFP8 ? 2048 : 1536;
   return r;
 }
