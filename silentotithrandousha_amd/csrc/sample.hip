@@ -1005,8 +1005,7 @@ hipError_t launch_sample(const SampleArgs &s, hipStream_t st) {
   // (All launches of 257 rows of 201088 with a top-k of 50: 128 us if their logits are counted and read again for the border's tokens,
   // 75 by pieces; with one of 390, 136 and 106; 8 rows 28 and 25. A single row takes 28 and 30.)
   a.peaks = s.rule.top_k && a.chunks * (kChunk / kPiece) <= kPieces && (size_t)s.T * a.chunks >= 768;
-  a.shift = 44;
-  while (((uint64_t)s.V << a.shift) > (uint64_t)1 << 62) a.shift--;
+  a.shift = sample_shift(s.V);
   a.tokens = s.tokens;
   a.logprob = s.logprob;
   work_layout(a.w, (char *)s.work, s.T, a.chunks, a.groups);

@@ -70,6 +70,12 @@ hipError_t launch_route_rule(const RouteRule &r, const float *logits, size_t T, 
 hipError_t launch_route_rule_backward(const RouteRule &r, const float *logits, const int32_t *idx, const float *dw, size_t T, int E, float *dl,
                                       hipStream_t s);
 
+// Bits of the largest logit's mass in a row of V: 44, fewer where the sum of V such masses would pass 2^62 (V at most 2^28).
+constexpr int sample_shift(size_t V) {
+  int s = 44;
+  while (V > (size_t)1 << (62 - s)) s--;
+  return s;
+}
 struct SampleArgs {
   moe_sampling rule;
   const float *logits;

@@ -5,7 +5,7 @@ import pytest
 
 from silentotithrandousha_amd import MOE_BF16, MOE_F32, MOE_MXFP8
 from tests import dense_ref, serve_ref as ref
-from tests.test_gpu_serve import d, matmul, resident, weights  # noqa: F401
+from tests.test_gpu_serve import d, matmul, resident, sample, weights  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,45 @@ def test_mxfp8_products_are_exact(d, T, R, C, dtype):  # noqa: F811
     tol = (2 * -(-C // 128) + 8) * 2.0 ** -23 * mag + 2.0 ** -23 * (np.abs(want) + np.abs(bias)) + (dense_ref.u(dtype) + 2.0 ** -24) * np.abs(want)
     got = matmul(d, resident(d, blocks, scales), R, C, bias, codes, MOE_MXFP8, x_scales, T, dtype)
     assert (np.abs(got - want) <= tol).all(), np.max(np.abs(got - want) / tol)
+
+
+# ------------------------------------------------------------------ sampling
+
+
+def check_wide(d, logits, u, **s):  # noqa: F811
+    """Rows whose masses sum up to nearly as much as 64 bits hold. A mass is a multiple of 2^-s of the largest, s at least 34, off by half
+    of that: sums over V of them by at most 2^-s-1 V, relative to a sum of nearly V 2^-35, and each border by as much."""
+    s = {k: np.asarray(v, np.int32 if k == "top_k" else np.float32) for k, v in s.items()}
+    u = np.asarray(u, np.float32)
+    got, lp = sample(d, logits, u, **s)
+    want, wlp, room = ref.sample(logits, u, **s)
+    assert (room > 2.0 ** -33).all(), "a draw too near a border for the test"
+    assert np.array_equal(got, want), (got, want)
+    assert (np.abs(lp - wlp) <= 2.0 ** -24 * np.abs(wlp) * 1.001 + 2.0 ** -33).all(), (lp, wlp)
+
+
+U = [0.0101, 0.3337, 0.5003, 0.9871]
+
+
+@pytest.mark.parametrize("V", [2**18 + 1, 2**20 - 1, 2**20, 2**20 + 1, 1200000, 2**21 + 3])
+@pytest.mark.parametrize("rows", ["equal", "near", "hot"])
+def test_sample_flat_wide_rows(d, V, rows):  # noqa: F811
+    """Equal logits, logits within 1e-3, and ordinary ones under a temperature of 1e30: all tokens' masses count."""
+    rng = np.random.default_rng([51, V])
+    u = U if V <= 2**20 else U[V % 2::2]
+    T = len(u)
+    x = np.full((T, V), 1.25, np.float32)
+    if rows != "equal":
+        x = (x + rng.standard_normal((T, V)) * (2e-4 if rows == "near" else 1)).astype(np.float32)
+    s = dict(temperature=np.full(T, 1e30)) if rows == "hot" else {}
+    check_wide(d, x, u, **s)
+    check_wide(d, x, u, min_p=np.full(T, 0.5), **s)
+    check_wide(d, x, u, top_p=np.full(T, 0.6), **s)
+    check_wide(d, x, u, top_k=np.full(T, V - 5000), **s)
+
+
+def test_sample_flat_rows_of_16_million(d):  # noqa: F811
+    V = 2**24 + 7
+    x = (np.float32(-3.5) + np.random.default_rng(52).standard_normal((1, V)) * 1e-4).astype(np.float32)
+    check_wide(d, x, [0.87654])
+    check_wide(d, x, [0.41234], top_p=[0.6])
