@@ -30,6 +30,7 @@ namespace {
 
 constexpr int kThreads = 512, kChunk = 4 * kThreads;  // a thread has four logits of a chunk
 constexpr int kMaxSpan = 4;                            // chunks of a workgroup that looks for the largest logit
+static_assert(kThreads == 512 && kMaxSpan * kChunk == kSampleSpan, "sample_rows");
 constexpr int kBins = 2048, kTail = kBins - 1;  // bin kTail: mass 0, not counted
 constexpr int kList = 4096;                     // tokens that are gathered of a row
 constexpr uint32_t kParts = 1024;                // chunks whose masses the draw holds in LDS
@@ -993,7 +994,7 @@ size_t sample_workspace(size_t T, size_t V) {
 }
 
 hipError_t launch_sample(const SampleArgs &s, hipStream_t st) {
-  if (!s.T || s.T > 65535 || !s.V || s.V > 1u << 28 || s.ld < s.V) return hipErrorInvalidValue;
+  if (!s.T || s.T > sample_rows(s.V) || !s.V || s.V > 1u << 28 || s.ld < s.V) return hipErrorInvalidValue;
   Args a{};
   a.rule = s.rule;
   a.logits = s.logits;

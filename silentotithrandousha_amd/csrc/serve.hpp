@@ -76,6 +76,13 @@ constexpr int sample_shift(size_t V) {
   while (V > (size_t)1 << (62 - s)) s--;
   return s;
 }
+// Logits of a row that a workgroup of 512 threads takes in the launch that looks for the largest, and rows at once: a launch has less than
+// 2^32 threads.
+constexpr size_t kSampleSpan = 4 * 2048;
+constexpr size_t sample_rows(size_t V) {
+  const size_t rows = (((size_t)1 << 23) - 1) / ((V + kSampleSpan - 1) / kSampleSpan);
+  return rows < 4096 ? rows : 4096;
+}
 struct SampleArgs {
   moe_sampling rule;
   const float *logits;

@@ -13,7 +13,6 @@ using namespace moe;
 namespace {
 
 constexpr size_t kMaxRows = (size_t)1 << 24;     // of a matrix
-constexpr size_t kSampleRows = 4096;             // rows of logits at once
 constexpr size_t kMatmulTokens = 65536;          // tokens of a product at once
 
 int check_cols(size_t cols) {
@@ -157,7 +156,7 @@ int moe_sample_device(moe_ctx *ctx, const moe_sampling *rule, const float *logit
   RETURN_IF(check_aligned({logits, u, tokens, logprob, rule->temperature, rule->top_k, rule->top_p, rule->min_p}, 4));
   RETURN_IF(check_distinct({tokens, logprob}, {logits, u, rule->temperature, rule->top_k, rule->top_p, rule->min_p}));
   const hipStream_t s = stream ? (hipStream_t)stream : c.stream;
-  const size_t Tc = std::min(T, kSampleRows);
+  const size_t Tc = std::min(T, sample_rows(vocab));
   RETURN_IF(ensure(c, sample_workspace(Tc, vocab), s));
   for (size_t t0 = 0; t0 < T; t0 += Tc) {
     auto at = [&](auto *p) { return p ? p + t0 : nullptr; };

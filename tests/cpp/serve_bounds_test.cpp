@@ -1,5 +1,6 @@
 // The bounds of include/moe_serve.h's calls at the ends of what it allows, over the launches that serve_calls_test.cpp notes.
 //   serve_bounds_test shift   a row's masses sum up within 64 bits, and have as many bits as that leaves
+//   serve_bounds_test rows    rows of the widest vocabularies go in launches of less than 2^32 threads, each row once
 #define main serve_calls_main
 #include "serve_calls_test.cpp"
 #undef main
@@ -27,6 +28,22 @@ void shift() {
   for (int i = 0; i < 100000; i++) one(1 + rng() % ((size_t)1 << 28));
 }
 
+void rows() {
+  // (sizes whose logits no card holds: a bound of the call alone)
+  for (size_t V : {(size_t)1, (size_t)8192, (size_t)201088, (size_t)1 << 23, (size_t)1 << 24, ((size_t)1 << 24) + 1, ((size_t)1 << 28) - 1, (size_t)1 << 28})
+    for (size_t T : {(size_t)1, (size_t)255, (size_t)256, (size_t)257, (size_t)4096, (size_t)4097, (size_t)20000}) {
+      const moe_sampling r{};
+      int32_t *tokens = device<int32_t>(T * 4);
+      if (moe_sample_device(&g_ctx, &r, device<float>(T * V * 4), V, device<float>(T * 4), T, V, tokens, nullptr, nullptr)) fault(g_error.c_str());
+      for (auto &w : g_buffers[(uintptr_t)tokens].written) {
+        const size_t n = (w.second - w.first) / 4, groups = (V + 8191) / 8192;
+        check(n <= 4096 && groups * n * 512 < (size_t)1 << 32, "a launch's threads", V, n);
+      }
+      whole(tokens, T * 4);
+      check(V > (size_t)1 << 23 || g_buffers[(uintptr_t)tokens].written.size() == (T + 4095) / 4096, "pieces of an ordinary call", V, T);
+    }
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -35,6 +52,8 @@ int main(int argc, char **argv) {
   const std::string what = argc > 1 ? argv[1] : "";
   if (what == "shift")
     shift();
+  else if (what == "rows")
+    rows();
   else
     return 2;
   printf("wrong %d, faults %ld\n", wrong, g_faults);

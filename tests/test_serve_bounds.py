@@ -18,3 +18,7 @@ def run(bounds, what):
 
 def test_masses_of_a_row_fit_64_bits(bounds):
     run(bounds, "shift")
+
+
+def test_launches_of_wide_rows(bounds):
+    run(bounds, "rows")
