@@ -13,7 +13,9 @@ using namespace moe;
 namespace {
 
 constexpr size_t kMaxRows = (size_t)1 << 24;     // of a matrix
-constexpr size_t kMatmulTokens = 65536;          // tokens of a product at once
+// tokens of a product at once, and values of theirs: 19 GB as terms of f32 rows at most, within 2^25 wavefronts' steps and 32-bit offsets
+// in 16 tiles
+constexpr size_t kMatmulTokens = 65536, kMatmulValues = (size_t)1 << 32;
 
 int check_cols(size_t cols) {
   if (!cols || cols % 32 || cols > kMaxInter) return fail(MOE_ERR_INVALID, "cols %zu must be a positive multiple of 32, at most %zu", cols, kMaxInter);
@@ -80,9 +82,7 @@ int moe_mxfp4_matmul_device(moe_ctx *ctx, const uint8_t *packed, size_t rows, si
   const size_t el = dtype == MOE_F32 ? 4 : 2;
   // bytes of a row of x
   const size_t xb = x_type == MOE_F32 ? 4 * cols : x_type == MOE_BF16 ? 2 * cols : x_type == MOE_MXFP8 ? cols : cols / 2;
-  // tokens at once: those of 2^25 wavefronts' steps and 32-bit offsets within 16 tiles
-  const size_t most = std::min<size_t>(kMatmulTokens, std::max<size_t>(16, ((size_t)1 << 29) / ((cols + 127) / 128) / 16 * 16));
-  const size_t Tc = std::min(T, most);
+  const size_t Tc = std::min({T, kMatmulTokens, kMatmulValues / cols / 16 * 16});
   MxGemmArgs a{};
   a.w = packed;
   a.d = pack_dims(rows, cols);

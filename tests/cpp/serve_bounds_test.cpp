@@ -1,6 +1,7 @@
 // The bounds of include/moe_serve.h's calls at the ends of what it allows, over the launches that serve_calls_test.cpp notes.
 //   serve_bounds_test shift   a row's masses sum up within 64 bits, and have as many bits as that leaves
 //   serve_bounds_test rows    rows of the widest vocabularies go in launches of less than 2^32 threads, each row once
+//   serve_bounds_test terms   a product's workspace: fewer tokens at a time of above 65536 columns
 #define main serve_calls_main
 #include "serve_calls_test.cpp"
 #undef main
@@ -44,6 +45,25 @@ void rows() {
     }
 }
 
+void terms() {
+  for (size_t cols : {(size_t)1 << 20, ((size_t)1 << 20) - 32, (size_t)100000, (size_t)65536 + 32, (size_t)65536, (size_t)2880})
+    for (size_t T : {(size_t)65536, (size_t)65537, (size_t)40000, (size_t)5000})
+      for (int type : {(int)MOE_F32, (int)MOE_BF16, (int)MOE_MXFP8, (int)MOE_MXFP4}) {
+        const PackDims d = pack_dims(16, cols);
+        void *y = buffer(T * 64);
+        g_work = DenseWork{};
+        if (moe_mxfp4_matmul_device(&g_ctx, device(pack_weight_bytes(d) + pack_scale_bytes(d)), 16, cols, nullptr, buffer(T * cols * 4), type,
+                                    device(T * cols / 32), T, y, MOE_F32, nullptr))
+          fault(g_error.c_str());
+        whole(y, T * 64);
+        size_t largest = 0;
+        for (auto &w : g_buffers[(uintptr_t)y].written) largest = std::max(largest, (w.second - w.first) / 64);
+        check(largest * cols <= (size_t)1 << 32 && largest <= 65536, "tokens at a time", cols, largest);
+        check(cols > 65536 || largest == std::min<size_t>(T, 65536), "pieces of an ordinary call", cols, largest);
+        check(g_work.cap < (size_t)20 << 30, "workspace", cols, g_work.cap);
+      }
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -54,6 +74,8 @@ int main(int argc, char **argv) {
     shift();
   else if (what == "rows")
     rows();
+  else if (what == "terms")
+    terms();
   else
     return 2;
   printf("wrong %d, faults %ld\n", wrong, g_faults);

@@ -22,3 +22,7 @@ def test_masses_of_a_row_fit_64_bits(bounds):
 
 def test_launches_of_wide_rows(bounds):
     run(bounds, "rows")
+
+
+def test_workspace_of_wide_products(bounds):
+    run(bounds, "terms")
