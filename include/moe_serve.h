@@ -78,8 +78,9 @@ typedef struct moe_routing {
  * (may be NULL): how often each was chosen. Equal scores go to the lower index, for groups as well. Without a bias
  * the order of experts is that of their logits; otherwise scores are compared in 64 bits. An expert whose logit is
  * -inf or NaN is never chosen: slots without an expert hold idx -1, weight 0. (A group with one expert left has
- * that one's score, a group with none is taken last.) Infinite logits share a softmax among them. Weights whose
- * sum is 0 are uniform if normalised. All pointers 4-byte aligned. n_tokens 0 zeroes counts. */
+ * that one's score, a group with none is taken last.) Infinite logits share a softmax among them; a score of a
+ * softmax below 2^-1075 is 0. Weights whose sum is 0 are uniform if normalised (and have no gradient); those of a sigmoid's
+ * finite logits, however far below 0, are what the formula says. All pointers 4-byte aligned. n_tokens 0 zeroes counts. */
 int moe_route_device(moe_ctx *ctx, const moe_routing *rule, const float *logits, size_t n_tokens, size_t n_experts,
                      int32_t *idx, float *weights, int32_t *counts, void *stream);
 /* Gradient of sum(dweights * weights) with respect to the logits, dlogits [n_tokens, n_experts], for the choice idx that

@@ -95,6 +95,12 @@ __device__ __forceinline__ double sigmoid64(double l) {
   return (l < 0.0 ? e : 1.0) * inverse64(1.0 + e);
 }
 
+// Normalised weights stay the same if all scores are divided by one number. Where every chosen score lies below e^kFar, their 64-bit
+// numbers lose bits and their sum's inverse leaves the range: there they are divided by the largest of them, which leaves
+// e^(l - the largest chosen logit) of a softmax, and of a sigmoid, which is e^l to the last bit there. A softmax score below
+// 2^-1075 (e^kGone) counts as 0.
+constexpr double kFar = -600.0, kLeast = 0x1p-865 /* a little more than e^kFar */, kGone = -745.1332191019412;
+
 // The logits of a lane's experts, -inf past the last one and for a NaN.
 template <int Q>
 __device__ __forceinline__ void load_logits(const float *row, int E, int lane, float (&l)[Q]) {
@@ -355,9 +361,18 @@ __global__ __launch_bounds__(rule_threads(Q)) void k_route_rule(RouteRule r, con
     double sc = 0.0;
     if (r.score == MOE_SCORE_SIGMOID) {
       if (slot >= 0) sc = sigmoid64((double)logit);
+      if (r.normalize && !__any((double)logit >= kFar)) {
+        const double top = (double)wave_largest(logit);
+        sc = slot >= 0 ? exp64((double)logit - top) : 0.0;
+      }
     } else {
       if (slot >= 0) sc = logit == m ? 1.0 : exp64((double)logit - (double)m);
-      if (!r.normalize) {
+      if (r.normalize) {
+        if (!__any(slot >= 0 && sc > kLeast)) {
+          const double top = (double)wave_largest(logit);
+          sc = slot >= 0 && top - (double)m >= kGone ? exp64((double)logit - top) : 0.0;
+        }
+      } else {
         double s[Q], sum = 0.0;
 #pragma unroll
         for (int q = 0; q < Q; q++) {
@@ -565,6 +580,12 @@ __global__ __launch_bounds__(1024) void k_route_pairs(RouteRule r, const float *
     double sc = 0.0;
     if (slot >= 0) sc = r.score == MOE_SCORE_SIGMOID ? sigmoid64((double)logit) : logit == m ? 1.0 : exp64((double)logit - (double)m);
     if (r.normalize) {
+      const bool sigmoid = r.score == MOE_SCORE_SIGMOID;
+      const uint64_t near = __ballot(slot >= 0 && (sigmoid ? (double)logit >= kFar : sc > kLeast));
+      if (!(uint32_t)near || !(uint32_t)(near >> 32)) {
+        const double top = (double)half_max(logit);
+        if (!(uint32_t)(near >> 32 * half)) sc = slot >= 0 && (sigmoid || top - (double)m >= kGone) ? exp64((double)logit - top) : 0.0;
+      }
       const double run = row_sum64(sc), s0 = lane64(run, 15) + lane64(run, 31), s1 = lane64(run, 47) + lane64(run, 63), total = half ? s1 : s0;
       const uint32_t n = __popc((uint32_t)(__ballot(slot >= 0) >> 32 * half));
       sc = total > 0.0 ? sc / total : 1.0 / max(n, 1u);
@@ -587,7 +608,8 @@ __global__ __launch_bounds__(1024) void k_route_pairs(RouteRule r, const float *
 //   d / d s_j = scale / S dw_j - (normalised) sum_i dw_i w_i / S,
 //   sigmoid: d l_j = d s_j s_j (1 - s_j);  softmax: d l_e = s_e (d s_e - sum_j d s_j s_j).
 // Of a normalised softmax that sum is 0, and S stands for its denominator, too: as for a sigmoid, the chosen experts' logits are
-// all that is read, and the other gradients are 0: the chosen ones' go to their places through LDS (13 us for 16384 tokens of 256 experts
+// all that is read (under a bias the others' largest as well, 10.0 us for 8.8 of the case below: it tells whether the chosen scores count as 0),
+// and the other gradients are 0: the chosen ones' go to their places through LDS (13 us for 16384 tokens of 256 experts
 // if every lane looks for its own among all, with 64-bit sums, so 8.4). An expert that idx names twice gets their sum.
 template <int Q, bool DENSE>  // DENSE: a softmax without normalisation, all of whose experts have a gradient
 __global__ __launch_bounds__(256) void k_route_rule_backward(RouteRule r, const float *logits, const int32_t *idx, const float *dw, uint32_t T,
@@ -616,6 +638,10 @@ __global__ __launch_bounds__(256) void k_route_rule_backward(RouteRule r, const 
       const double x = exp64(-fabs((double)lg)), y = inverse64(1.0 + x);
       sc = lg == -INFINITY ? 0.0 : lg < 0.0f ? x * y : y;
       rest = lg < 0.0f ? y : x * y;
+      if (r.normalize && !__any((double)lg >= kFar)) {
+        const double top = (double)wave_largest(lg);
+        sc = lg == -INFINITY ? 0.0 : exp64((double)lg - top);
+      }
     } else {
       m = lg;
       if constexpr (DENSE) {
@@ -628,6 +654,13 @@ __global__ __launch_bounds__(256) void k_route_rule_backward(RouteRule r, const 
       }
       m = wave_largest(m);
       sc = lg == -INFINITY ? 0.0 : lg == m ? 1.0 : exp64((double)lg - (double)m);
+      if (!DENSE && r.bias) {  // (under a bias all chosen scores may be 0: their weights are uniform, whatever the logits)
+        float all[Q], top = -INFINITY;
+        load_logits<Q>(logits + (size_t)t * E, E, lane, all);
+#pragma unroll
+        for (int q = 0; q < Q; q++) top = fmaxf(top, all[q]);
+        if ((double)m - (double)wave_largest(top) < kGone) sc = 0.0;
+      }
       if constexpr (DENSE) {
         sum = 0.0;
 #pragma unroll

@@ -3,9 +3,9 @@ hold what f32 sums lose and nothing else."""
 import numpy as np
 import pytest
 
-from silentotithrandousha_amd import MOE_BF16, MOE_F32, MOE_MXFP8
+from silentotithrandousha_amd import MOE_BF16, MOE_F32, MOE_MXFP8, MOE_SCORE_SIGMOID, MOE_SCORE_SOFTMAX
 from tests import dense_ref, serve_ref as ref
-from tests.test_gpu_serve import d, matmul, resident, sample, weights  # noqa: F401
+from tests.test_gpu_serve import Out, d, dev, matmul, resident, route, rule, sample, weights  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,86 @@ def test_sample_flat_rows_of_16_million(d):  # noqa: F811
     x = (np.float32(-3.5) + np.random.default_rng(52).standard_normal((1, V)) * 1e-4).astype(np.float32)
     check_wide(d, x, [0.87654])
     check_wide(d, x, [0.41234], top_p=[0.6])
+
+
+# ------------------------------------------------------------------ routing: scores that 64 bits hold badly or not at all
+
+
+def log_form(z, idx, dw, rule):
+    """(weights, dlogits, its magnitude) by logarithms of the scores. A softmax whose chosen scores all lie below 2^-1075: uniform, and
+    without a gradient."""
+    T, k = idx.shape
+    sigmoid = rule.score == MOE_SCORE_SIGMOID
+    if sigmoid:
+        ls, rest = np.minimum(z, 0) - np.log1p(np.exp(-np.abs(z))), np.exp(np.minimum(-z, 0) - np.log1p(np.exp(-np.abs(z))))
+    else:
+        top = z.max(1, keepdims=True)
+        ls = z - top - np.log(np.exp(z - top).sum(1, keepdims=True))
+    live = idx >= 0
+    at = np.where(live, idx, 0)
+    lw = np.where(live, np.take_along_axis(ls, at, 1), -np.inf)
+    gone = np.zeros(T, bool)
+    if rule.normalize:
+        best = lw.max(1, keepdims=True)
+        gone = (best[:, 0] < np.log(2) * -1075) & (not sigmoid)
+        w = np.exp(lw - best)
+        w[gone] = live[gone]
+        w = w / w.sum(1, keepdims=True)
+    else:
+        w = np.exp(lw)
+    w = w * rule.scale
+    g = dw * w
+    size = np.abs(g)
+    if rule.normalize:
+        part = w / rule.scale
+        g, size = g - part * g.sum(1, keepdims=True), size + part * size.sum(1, keepdims=True)
+    out, mag = np.zeros_like(z), np.zeros_like(z)
+    for t in range(T):
+        for j in range(k):
+            if live[t, j] and not gone[t]:
+                f = rest[t, idx[t, j]] if sigmoid else 1.0
+                out[t, idx[t, j]] += g[t, j] * f
+                mag[t, idx[t, j]] += size[t, j] * f
+    if not sigmoid and not rule.normalize:
+        s = np.exp(ls)
+        out -= s * g.sum(1, keepdims=True)
+        mag += s * size.sum(1, keepdims=True)
+    return w, out, mag
+
+
+FAR = [[-720, -720.5, -719.25], [-600.5, -601, -640], [-599.5, -640, -720], [-650, -700, -743], [-744.5, -745.5, -746], [-800, -900, -801],
+       [-1e9, -1e9, -1e9], [-1e30, -1e30, -1.5e30], [-1e30, -3e38, -1e9], [-20, -700, -1], [3, -700, -1e30], [-590, -720.5, -1e30], [-708, -709.5, -710]]
+
+
+@pytest.mark.parametrize("T", [13, 70, 4099])
+@pytest.mark.parametrize("E", [8, 200, 520])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("score", [MOE_SCORE_SOFTMAX, MOE_SCORE_SIGMOID])
+def test_route_far_scores(d, score, biased, E, T):  # noqa: F811
+    """Rows whose chosen logits all lie far below 0 (sigmoid) or below a logit that is not chosen (softmax): a masked token, a token under
+    a strong bias. Weights and gradient are finite and what the formula says."""
+    rng = np.random.default_rng([61, E, T])
+    k = 3
+    places = [E // 2, E // 2 + 1, E - 1]
+    logits = np.full((T, E), -np.inf, np.float32)
+    logits[:, places] = np.array(FAR, np.float32)[np.arange(T) % len(FAR)]
+    bias = None
+    if biased:  # the largest logit of a softmax, 0, is not among the chosen
+        bias = np.ones(E, np.float32)
+        bias[1] = -9
+        if score == MOE_SCORE_SOFTMAX:
+            logits[:, 1] = np.maximum(0, logits[:, places].max(1) + 1)
+    b = dev(bias)
+    dw = rng.standard_normal((T, k)).astype(np.float32)
+    for normalize in (True, False):
+        r = rule(score=score, k=k, normalize=normalize, scale=2.5, bias=b)
+        idx, w, _ = route(d, r, logits)
+        assert np.array_equal(np.sort(idx, 1), np.broadcast_to(places, (T, k)))
+        dl = Out((T, E), np.float32)
+        keep = [dev(logits), dev(idx), dev(dw)]
+        d.route_backward_device(r, *keep, T, E, dl)
+        d.synchronize()
+        want, grad, mag = log_form(logits.astype(np.float64), idx, dw.astype(np.float64), r)
+        # (logarithms of up to 1000 are off by 2^-43, their exponentials by as much)
+        assert (np.abs(w - want) <= (2.0 ** -24 + 2.0 ** -40) * np.abs(want) + 1e-45).all(), normalize
+        assert (np.abs(dl.get() - grad) <= 2.0 ** -24 * np.abs(grad) + 2.0 ** -38 * mag + 1e-45).all(), normalize
