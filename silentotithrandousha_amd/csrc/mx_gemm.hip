@@ -117,12 +117,13 @@ Form form_of(const MxGemmArgs &a) {
   return large <= middle && large <= small ? LARGE : middle <= small ? MIDDLE : SMALL;
 }
 
-// (64 x 64 tiles of MXFP8 rows with 4 slots, two steps, 13.0 us for those 128 rows, with 6 12.6; 192 x 256 ones with 3 or 4 the same)
+// (MXFP8 rows' slots, two to a step: 64 x 64 tiles with 4 13.0 us for those 128 rows, with 6 12.6; 128 x 128 ones, of which a CU holds one
+// with 4 and two with 3, 46.6 and 40.4 us for 2000 rows over 2880 x 2880; 192 x 256 ones with 3 or 4 the same)
 template <int FMT, int TERMS>
 hipError_t by_form(Form f, const MxGemmArgs &a, hipStream_t s) {
   switch (f) {
     case SMALL: return launch_mx_shape<MxShape<FMT, TERMS, 4, 4, 2, 2, FMT == 8 ? 6 : 4>>(a, s);
-    case MIDDLE: return launch_mx_shape<MxShape<FMT, TERMS, 8, 8, 2, 2, 4>>(a, s);
+    case MIDDLE: return launch_mx_shape<MxShape<FMT, TERMS, 8, 8, 2, 2, FMT == 8 ? 3 : 4>>(a, s);
     case LARGE: return launch_mx_shape<MxShape<FMT, TERMS, 12, 16, 2, 4, FMT == 8 ? 3 : FMT == 4 ? 5 : 4>>(a, s);
     default: return hipErrorInvalidValue;
   }
