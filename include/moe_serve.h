@@ -42,16 +42,17 @@ int moe_mxfp4_quantize_device(moe_ctx *ctx, const void *x, int dtype, size_t n_r
  * (moe_mxfp4_pack_device), y of type dtype (MOE_F32 or MOE_BF16). Rows x [n_tokens, cols] by x_type:
  *   MOE_F32: of a block of 32 values those down to 2^-5 of its largest magnitude enter exactly, none is off
  *     by more than 2^-29 of that;
- *   MOE_BF16: those down to 2^-11 exactly, none is off by more than 2^-19 of the largest;
+ *   MOE_BF16: exactly (weights of 2^128 and above are infinite, as in f32);
  *   MOE_MXFP8: moe_act8_pack_device's codes, their scales at x_scales, or behind the codes if that is NULL;
  *   MOE_MXFP4: blocks as moe_mxfp4_quantize_device writes them, their scales at x_scales.
- * Products are exact, sums f32. Blocks of f32 or bf16 rows whose largest magnitude is below 2^-99 keep 2^-129
- * absolute. A row that holds a value that is not finite, or a scale byte of 255, gives NaN, as does a scale
- * byte of 255 in W; a scale byte of 0 counts as 2^-127. packed, x, y and bias are 16-byte aligned; rows is a
- * multiple of 16, at most 2^24, cols of 32, at most 2^20. Workspace: the rows as the product takes them, 0.53 cols
- * bytes a token for MOE_MXFP4, 2.03 for MOE_MXFP8, 3.03 for MOE_BF16 and 4.53 for MOE_F32, of 65536 tokens at a time (fewer
- * of above 65536 cols); none for one or two rows of MOE_F32 and up to four of MOE_BF16 of up to 3968 cols (of
- * fewer such rows up to 16000). */
+ * Products are exact, sums f32. Blocks of f32 rows whose largest magnitude is below 2^-99 keep 2^-129 absolute. A row that
+ * holds a value that is not finite, or a scale byte of 255, gives NaN, as does a scale byte of 255 in W; a scale byte of 0
+ * counts as 2^-127. packed, x, y and bias are 16-byte aligned; rows is a multiple of 16, at most 2^24, cols of 32, at most
+ * 2^20. Workspace: the rows as the product takes them, 0.53 cols bytes a token for MOE_MXFP4, 2.03 for MOE_MXFP8, 2 for
+ * MOE_BF16 and 4.53 for MOE_F32, of 65536 tokens at a time (fewer of above 65536 cols); none for one row of MOE_F32 of up to
+ * 10624 cols, two of up to 5248, and up to 16 rows of MOE_BF16 of 48 KB in all (each 2 cols, rounded up to 256, and 16
+ * bytes). (moe_mxfp4_matvec_device takes one f32 row as well, exact to 2^-16 of it: 4.8 us over 5760 x 2880, where this
+ * takes 5.1.) */
 int moe_mxfp4_matmul_device(moe_ctx *ctx, const uint8_t *packed, size_t rows, size_t cols, const float *bias,
                             const void *x, int x_type, const uint8_t *x_scales, size_t n_tokens, void *y, int dtype,
                             void *stream);

@@ -4,6 +4,7 @@
 // 8.8 MB, of which the stream is 1.3 and the rest a launch's and a load's latency. K split over workgroups instead, with a launch that
 // adds the parts, was slower.)
 #include "act8.hpp"
+#include "mx_gemm.hpp"
 #include "serve.hpp"
 
 namespace moe {
@@ -14,7 +15,7 @@ constexpr int kFewWaves = 8;
 // RT row tiles a workgroup, CT tiles of 16 tokens.
 template <int FMT, int TERMS, int RT, int CT>
 __global__ __launch_bounds__(64 * kFewWaves) void k_mx_few(MxGemmArgs a) {
-  constexpr int kChunk = FMT == 4 ? 1024 : FMT == 6 ? 1536 : 2048;
+  constexpr int kChunk = FMT == 4 || FMT == 16 ? 1024 : FMT == 6 ? 1536 : 2048;
   __shared__ f32x4 s_sum[kFewWaves][RT * CT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
   const uint32_t m0 = blockIdx.x * RT, n0 = blockIdx.y * CT, nb = a.d.nb, ns = a.d.ns, nq = a.d.nq;
@@ -39,7 +40,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_mx_few(MxGemmArgs a) {
 #pragma unroll
     for (int j = 0; j < CT; j++) {
       const uint32_t n = min(n0 + j, a.r.tiles - 1);
-      sb[j] = a.scales[((size_t)n * nq + s / 4) * 64 + lane];
+      if constexpr (FMT != 16) sb[j] = a.scales[((size_t)n * nq + s / 4) * 64 + lane];
       row[j] = a.codes + ((size_t)n * ns + s) * TERMS * kChunk + lane * 16;
     }
     i32x8 B[TERMS][CT];
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_mx_few(MxGemmArgs a) {
 #pragma unroll
     for (int i = 0; i < RT; i++) sa[i] >>= sh;
 #pragma unroll
-    for (int j = 0; j < CT; j++) sb[j] = sb[j] >> sh & 255;
+    for (int j = 0; j < CT; j++) sb[j] = FMT == 16 ? 0 : sb[j] >> sh & 255;
     constexpr int kB = FMT == 4 ? 4 : FMT == 6 ? 2 : 0;
 #pragma unroll
     for (int t = 0; t < TERMS; t++) {
@@ -70,11 +71,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_mx_few(MxGemmArgs a) {
 #pragma unroll
         for (int j = 0; j < CT; j++) sb[j] = (uint32_t)max((int)sb[j] - 5, 1);
 #pragma unroll
-      for (int i = 0; i < RT; i++)
+      for (int i = 0; i < RT; i++) {
+        if constexpr (FMT == 16) {
+          const bf16x8 w = mx_weights8(A[i][t], sa[i] & 255);
+#pragma unroll
+          for (int j = 0; j < CT; j++)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, as_bf16x8(make_uint4(B[t][j][0], B[t][j][1], B[t][j][2], B[t][j][3])), acc[i][j], 0, 0, 0);
+          continue;
+        }
 #pragma unroll
         for (int j = 0; j < CT; j++)
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(i32x8{(int)A[i].x, (int)A[i].y, (int)A[i].z, (int)A[i].w, 0, 0, 0, 0},
                                                                        B[t][j], acc[i][j], 4, kB, 0, (int)sa[i], 0, (int)sb[j]);
+      }
     }
   }
 #pragma unroll
@@ -102,13 +111,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_mx_few(MxGemmArgs a) {
   }
 }
 
-// One to a few f32 or bf16 rows, whose terms fit the MFMA's 16 columns (column t TERMS + i: term i of token t): the terms are
-// made by every workgroup for itself, while its weights are on their way. (Made by a launch of their own, one f32 row over 5760 x
+// One or two f32 rows, whose terms fit the MFMA's 16 columns (column t TERMS + i: term i of token t): the terms are made by every
+// workgroup for itself, while its weights are on their way. (Made by a launch of their own, one f32 row over 5760 x
 // 2880 took 10.6 us, so 5.1.)
 constexpr int kEarly = 3;  // steps of a wavefront whose weights are asked for first
 
-template <class X, int TERMS>
-__global__ __launch_bounds__(64 * kFewWaves) void k_mx_one(MxGemmArgs a, const X *x) {
+__global__ __launch_bounds__(64 * kFewWaves) void k_mx_one(MxGemmArgs a, const float *x) {
+  constexpr int TERMS = 6;
   extern __shared__ __align__(16) uint8_t s_mem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
   const uint32_t m = blockIdx.x, nb = a.d.nb, ns = a.d.ns, nq = a.d.nq, T = a.r.tokens, cols = T * TERMS, blocks = 4 * ns;
@@ -223,6 +232,81 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_mx_one(MxGemmArgs a, const X
   }
 }
 
+// Up to 16 bf16 rows that fit 64 KB of LDS, where every workgroup puts them while its weights are on their way: 16 bytes a thread, those
+// with a value that is not finite as NaN. One row over 201088 x 2880, whose weights are 308 MB, takes 49 us, 6.3 TB/s, over 5760 x 2880 4.5, eight
+// rows 84 and 6. Two tiles of rows a workgroup share what it puts there, where there are tiles enough. (In terms: 70, 4.5, 133 and 9. Read
+// by each wavefront from memory, 64 bytes a lane in 16 rows, one row took 67 and 5.1, eight 75 and 6.8.)
+template <int RT>
+__global__ __launch_bounds__(64 * kFewWaves) void k_mx_bf16(MxGemmArgs a, const uint16_t *x) {
+  extern __shared__ __align__(16) uint8_t s_mem[];
+  f32x4(*s_sum)[RT][64] = (f32x4(*)[RT][64])s_mem;  // [8 wavefronts]
+  uint8_t *s_x = s_mem + kFewWaves * RT * 1024;     // [tokens] of 16 ns pieces of 16 bytes and one more
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
+  const uint32_t m0 = blockIdx.x * RT, nb = a.d.nb, ns = a.d.ns, nq = a.d.nq, T = a.r.tokens, stride = (16 * ns + 1) * 16;
+  const uint32_t *wsc = (const uint32_t *)(a.w + pack_weight_bytes(a.d));
+  u32x4 A[kEarly][RT];
+  uint32_t sa[kEarly][RT];
+  auto weights = [&](uint32_t s0) {
+#pragma unroll
+    for (int e = 0; e < kEarly; e++) {
+      const uint32_t s = min(s0 + e * kFewWaves, ns - 1);
+#pragma unroll
+      for (int i = 0; i < RT; i++) {
+        const uint32_t m = min(m0 + i, a.d.tiles - 1);
+        A[e][i] = __builtin_nontemporal_load((const u32x4 *)(a.w + (size_t)m * 256 * nb + min((s * 64 + lane) * 16, 256 * nb - 16)));
+        sa[e][i] = wsc[((size_t)m * nq + s / 4) * 64 + lane];
+      }
+    }
+  };
+  weights(wave);
+  for (uint32_t t = 0; t < T; t++)
+    for (uint32_t c = tid; c < 16 * ns; c += 64 * kFewWaves) {  // (a last step may be short)
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (c < 4 * nb) v = ((const uint4 *)x)[(size_t)t * 4 * nb + c];
+      *(uint4 *)(s_x + t * stride + c * 16) = mx_not_finite(v) ? make_uint4(kNan2, kNan2, kNan2, kNan2) : v;
+    }
+  __syncthreads();
+  f32x4 acc[RT][2];  // (one chain of MFMAs would be twice as long)
+#pragma unroll
+  for (int i = 0; i < RT; i++) acc[i][0] = acc[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint8_t *row = s_x + min((uint32_t)col, T - 1) * stride + g * 64;  // (columns past the last: the last again)
+  for (uint32_t s0 = wave;;) {
+#pragma unroll
+    for (int e = 0; e < kEarly; e++) {
+      const uint32_t s = s0 + e * kFewWaves;
+      if (s >= ns) break;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const bf16x8 v = *(const bf16x8 *)(row + s * 256 + k * 16);
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+          acc[i][k & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_weights8(A[e][i][k], sa[e][i] >> 8 * (s & 3) & 255), v, acc[i][k & 1], 0, 0, 0);
+      }
+    }
+    s0 += kEarly * kFewWaves;
+    if (s0 >= ns) break;
+    weights(s0);
+  }
+#pragma unroll
+  for (int i = 0; i < RT; i++) s_sum[wave][i][lane] = acc[i][0] + acc[i][1];
+  __syncthreads();
+  if (wave >= RT) return;
+  f32x4 v = s_sum[0][wave][lane];
+#pragma unroll
+  for (int w = 1; w < kFewWaves; w++) v = v + s_sum[w][wave][lane];
+  const uint32_t m = m0 + wave, at = m * 16 + g * 4;
+  if (m >= a.d.tiles || (uint32_t)col >= T) return;
+  if (a.bias) v = v + *(const f32x4 *)(a.bias + at);
+  if (a.bf16) {
+    uint16_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) q[i] = __builtin_bit_cast(uint16_t, (__bf16)v[i]);
+    *(uint2 *)((uint16_t *)a.out + (size_t)col * a.d.rows + at) = __builtin_bit_cast(uint2, q);
+  } else {
+    *(f32x4 *)((float *)a.out + (size_t)col * a.d.rows + at) = v;
+  }
+}
+
 template <int FMT, int TERMS, int RT, int CT>
 hipError_t launch(const MxGemmArgs &a, hipStream_t s) {
   return launch_own(k_mx_few<FMT, TERMS, RT, CT>, dim3((a.d.tiles + RT - 1) / RT, (a.r.tiles + CT - 1) / CT), dim3(64 * kFewWaves), 0, s, a);
@@ -240,17 +324,21 @@ hipError_t by_tokens(const MxGemmArgs &a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_mx_one(const MxGemmArgs &a, const void *x, hipStream_t s) {
-  const size_t lds = mx_one_lds(a.d.nb, (size_t)a.r.tokens * a.r.terms);
   if (!mx_one_takes(a.r.type, a.r.tokens, (size_t)a.d.nb * 32) || a.d.tiles >= 1u << 22) return hipErrorInvalidValue;
-  return a.r.type == MOE_F32 ? launch_own(k_mx_one<float, 6>, dim3(a.d.tiles), dim3(64 * kFewWaves), lds, s, a, (const float *)x)
-                             : launch_own(k_mx_one<uint16_t, 4>, dim3(a.d.tiles), dim3(64 * kFewWaves), lds, s, a, (const uint16_t *)x);
+  if (a.r.type == MOE_BF16) {
+    auto go = [&](auto k, unsigned rt) {
+      return launch_own(k, dim3((a.d.tiles + rt - 1) / rt), dim3(64 * kFewWaves), mx_one_rows(a.d.nb, a.r.tokens) + kFewWaves * rt * 1024, s, a, (const uint16_t *)x);
+    };
+    return a.d.tiles < 1024 ? go(k_mx_bf16<1>, 1) : go(k_mx_bf16<2>, 2);
+  }
+  return launch_own(k_mx_one, dim3(a.d.tiles), dim3(64 * kFewWaves), mx_one_lds(a.d.nb, (size_t)a.r.tokens * 6), s, a, (const float *)x);
 }
 
 hipError_t launch_mx_few(const MxGemmArgs &a, hipStream_t s) {
   if (a.d.tiles >= 1u << 22) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   switch (a.r.type) {
     case MOE_F32: return by_tokens<6, 6>(a, s);
-    case MOE_BF16: return by_tokens<6, 4>(a, s);
+    case MOE_BF16: return by_tokens<16, 4>(a, s);
     case MOE_MXFP8: return by_tokens<8, 2>(a, s);
     case MOE_MXFP4: return by_tokens<4, 1>(a, s);
   }

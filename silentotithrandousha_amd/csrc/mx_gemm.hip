@@ -23,7 +23,7 @@ __device__ __forceinline__ void e4m3_halves(const uint4 &codes, uint4 &large, ui
 }
 
 // A wavefront a (tile, step): lane 16 g + j holds block 4 s + g of row j, so that a block's scale and all its terms are one lane's, and
-// stores lie side by side. Bound by memory where there are many rows: 4096 x 2880 bf16 (24 MB read, 36 written) take 11.5 us, 5.2 TB/s;
+// stores lie side by side. Bound by memory where there are many rows: 4096 x 2880 bf16 (24 MB read, 24 written) take 10 us, 4.8 TB/s;
 // few rows wait for their loads and the chain of terms (333 x 1056 f32 5.4 us). Terms made within the product instead would be made
 // by every workgroup along the weights' rows, 15 to 30 of them.
 template <int TYPE>
@@ -58,6 +58,16 @@ __global__ __launch_bounds__(256) void k_mx_rows(MxRows r, const void *x, const 
       *(uint4 *)o = large;
       *(uint4 *)(o + 2048) = small;
     }
+  } else if constexpr (TYPE == MOE_BF16) {
+    uint4 v[4] = {};
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = ((const uint4 *)x)[4 * block + i];
+    }
+    const bool bad = mx_not_finite(v[0]) || mx_not_finite(v[1]) || mx_not_finite(v[2]) || mx_not_finite(v[3]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) *(uint4 *)(out + i * 1024 + lane * 16) = bad ? make_uint4(kNan2, kNan2, kNan2, kNan2) : v[i];
+    return;
   } else {
     float v[32];
 #pragma unroll
@@ -66,16 +76,12 @@ __global__ __launch_bounds__(256) void k_mx_rows(MxRows r, const void *x, const 
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         float w[8];
-        if constexpr (TYPE == MOE_BF16)
-          act8_load((const uint16_t *)x + block * 32 + 8 * i, w);
-        else
-          act8_load((const float *)x + block * 32 + 8 * i, w);
+        act8_load((const float *)x + block * 32 + 8 * i, w);
 #pragma unroll
         for (int k = 0; k < 8; k++) v[8 * i + k] = w[k];
       }
     }
-    constexpr int kTerms = TYPE == MOE_BF16 ? 4 : 6;
-    split32_fp6_each<kTerms>(v, [&](int term, const u32x6v &c, uint32_t sb) {
+    split32_fp6_each<6>(v, [&](int term, const u32x6v &c, uint32_t sb) {
       if (term == 0) byte = sb;
       uint8_t *o = out + term * 1536;
       *(uint4 *)(o + lane * 16) = make_uint4(c[0], c[1], c[2], c[3]);
@@ -105,15 +111,21 @@ namespace {
 
 enum Form { FEW, SMALL, MIDDLE, LARGE };
 
-// The form of a product. Few rows, and matrices that fill less than 150 tiles of 64 x 64, split K over a workgroup's wavefronts
-// (mx_few.hip: 1024 bf16 rows over 512 x 2880 22 us, 64 x 64 tiles 28; 128 over 5760 x 2880 22 and 21). Otherwise the tile whose
-// workgroups take least, in units of 2880 bf16 values: a 64 x 64 tile 16 us alone and 12 among others (of which a CU holds
-// several), a 128 x 128 one 25 and 26, a 192 x 256 one 62 (a CU holds one, so the last round counts whole); the other types' times
-// stand in the same ratios within a fifth.
+// The form of a product. Few rows, and matrices that fill few tiles of 64 x 64, split K over a workgroup's wavefronts (mx_few.hip: 1024 bf16
+// rows over 512 x 2880, 128 tiles, 17.5 us, 64 x 64 tiles 23.7; over 5760 x 2880 128 rows, 180 tiles, 15.0 and 18.8, 192 rows, 270 tiles, 21.4
+// and 21.1, but 128 MXFP8 rows 14.5 and 12.3). Otherwise the tile whose workgroups take least, in units of 2880 values: a 64 x 64 tile alone
+// and among others (of which a CU holds several), a 128 x 128 one the same, a 192 x 256 one (a CU holds one, so the last round counts
+// whole). bf16 rows take times of their own (their barriers come four to a step); the other types' stand in the same ratios within a fifth.
+struct FormTimes {
+  double few_tiles, small_alone, small, middle_alone, middle, large;
+};
+constexpr FormTimes kOfBf16{260, 16.5, 8.1, 30, 29, 52}, kOfOthers{150, 16, 12, 25, 26, 62};
 Form form_of(const MxGemmArgs &a) {
+  const FormTimes &f = a.r.type == MOE_BF16 ? kOfBf16 : kOfOthers;
   auto groups = [&](size_t m, size_t n) { return (double)((a.d.tiles + m - 1) / m * ((a.r.tiles + n - 1) / n)) / 256.0; };
-  if (a.r.tiles <= 4 || groups(4, 4) * 256 < 150) return FEW;
-  const double small = std::max(16.0, 12.0 * groups(4, 4)), middle = std::max(25.0, 26.0 * groups(8, 8)), large = 62.0 * std::ceil(groups(12, 16));
+  if (a.r.tiles <= 4 || groups(4, 4) * 256 < f.few_tiles) return FEW;
+  const double small = std::max(f.small_alone, f.small * groups(4, 4)), middle = std::max(f.middle_alone, f.middle * groups(8, 8)),
+               large = f.large * std::ceil(groups(12, 16));
   return large <= middle && large <= small ? LARGE : middle <= small ? MIDDLE : SMALL;
 }
 
@@ -136,7 +148,7 @@ hipError_t launch_mx_gemm(const MxGemmArgs &a, hipStream_t s) {
   if (f == FEW) return launch_mx_few(a, s);
   switch (a.r.type) {
     case MOE_F32: return by_form<6, 6>(f, a, s);
-    case MOE_BF16: return by_form<6, 4>(f, a, s);
+    case MOE_BF16: return by_form<16, 4>(f, a, s);
     case MOE_MXFP8: return by_form<8, 2>(f, a, s);
     case MOE_MXFP4: return by_form<4, 1>(f, a, s);
   }

@@ -1,16 +1,20 @@
-// Product of rows with a resident MXFP4 matrix on v_mfma_scale_f32_16x16x128_f8f6f4: D[r][t] = sum W[r][k] x[t][k],
-// A = the weights as stored (tile16, layout.hpp), B = the rows as MxRows (serve.hpp): MXFP4 rows as they are, MXFP8 rows as their larger and
-// their smaller codes, bf16 and f32 rows as 4 and 6 E2M3 terms whose sum they are. A decoded to bf16 would cost more issue slots than the products save, and
-// three bf16 planes of f32 rows three products at a quarter of the rate.
+// Product of rows with a resident MXFP4 matrix: D[r][t] = sum W[r][k] x[t][k], A = the weights as stored (tile16, layout.hpp), B = the rows
+// as MxRows (serve.hpp).
+//
+// On v_mfma_scale_f32_16x16x128_f8f6f4: MXFP4 rows as they are, MXFP8 rows as their larger and their smaller codes, f32 rows as 6
+// E2M3 terms whose sum they are to 2^-29 of their block's largest (three bf16 planes would hold them whole and take twice as long).
+// On v_mfma_f32_16x16x32_bf16: bf16 rows as they are, the weights decoded in registers, four conversions for 8 values that meet all of a
+// wavefront's row tiles. (As 4 E2M3 terms, whose products take as long, what is below 2^-11 of a block's largest lost bits, and the terms
+// cost half as many bytes again: 4096 rows over 2880 x 2880 73 us, so 64.)
 //
 // A workgroup of WM x WN wavefronts computes MT x NT16 tiles of 16 x 16. A package is one term of a step of 128 values: the
 // rows' chunks, with the first term the weights' chunks, and with every fourth step both sides' scale words. Packages arrive by LDS-DMA in rings
 // of DEPTH slots; every wavefront issues the same number of loads a package, so that one counted wait and one barrier hand a
 // package over. That barrier stands in the middle of the package before it, whose operands are in registers by then: the next
 // one's are read, and the loads that take its slots issued, between the MFMAs of its second half. (With the reads in front of all
-// of a package's MFMAs both wavefronts of a SIMD waited for them together: 4096 bf16 rows over 2880 x 2880 took 68 us, this 66.)
+// of a package's MFMAs both wavefronts of a SIMD waited for them together: 4096 bf16 rows in terms 68 us, so 66.)
 // The weights' operands stay in registers over the terms of a step. What bounds the 192 x 256 tile: its MFMAs, issued at some 60 % of their
-// rate (4096 x 2880 x 2880 in bf16 66 us, 4.1 PFLOP/s of terms; MXFP4 rows over 5760 x 2880 44 us, 3.0 PFLOP/s, of which some 10 us a
+// rate (4096 x 2880 x 2880 in bf16 60 us, 1.14 PFLOP/s; MXFP4 rows over 5760 x 2880 44 us, 3.0 PFLOP/s, of which some 10 us a
 // tile are its first loads and its results, which no other workgroup of the CU covers).
 #pragma once
 #include <algorithm>
@@ -21,14 +25,26 @@
 
 namespace moe {
 
-// FMT: the rows' format (4 E2M1, 6 E2M3, 8 E4M3).
+// a row's weights of 8 values in bf16 (E2M1 times a power of two, exactly; of 2^128 and above infinite as in f32); a scale byte of 255
+// is NaN
+__device__ __forceinline__ bf16x8 mx_weights8(uint32_t codes, uint32_t scale_byte) {
+  return decode8(codes, __uint_as_float(scale_byte == 255 ? 0x7FC00000u : scale_byte << 23));
+}
+// whether one of 8 bf16 values is infinite or NaN: its exponent's carry
+__device__ __forceinline__ bool mx_not_finite(const uint4 &v) {
+  auto carry = [](uint32_t w) { return (w & 0x7F807F80u) + 0x00800080u; };
+  return ((carry(v.x) | carry(v.y) | carry(v.z) | carry(v.w)) & 0x80008000u) != 0;
+}
+constexpr uint32_t kNan2 = 0x7FC07FC0u;  // two bf16
+
+// FMT: the rows' format (4 E2M1, 6 E2M3, 8 E4M3, 16 bf16: TERMS are the four eighths of a block).
 template <int FMT, int TERMS, int MT_, int NT_, int WM_, int WN_, int DEPTH_>
 struct MxShape {
   static constexpr int kFmt = FMT, kTerms = TERMS, MT = MT_, NT = NT_, WM = WM_, WN = WN_, kDepth = DEPTH_;
   static constexpr int kWaves = WM * WN, TM = MT / WM, TN = NT / WN;
-  static constexpr int kChunk = FMT == 4 ? 1024 : FMT == 6 ? 1536 : 2048;
+  static constexpr int kChunk = FMT == 4 || FMT == 16 ? 1024 : FMT == 6 ? 1536 : 2048;
   // 1 KB pieces of a package, and those a wavefront loads (the last ones again where they do not divide)
-  static constexpr int kPiecesA = MT, kPiecesB = (NT * kChunk + 1023) / 1024, kPiecesSA = (MT + 3) / 4, kPiecesSB = (NT + 3) / 4;
+  static constexpr int kPiecesA = MT, kPiecesB = (NT * kChunk + 1023) / 1024, kPiecesSA = (MT + 3) / 4, kPiecesSB = FMT == 16 ? 0 : (NT + 3) / 4;
   static constexpr int per(int n) { return (n + kWaves - 1) / kWaves; }
   static constexpr int kLoadA = per(kPiecesA), kLoadB = per(kPiecesB), kLoadS = per(kPiecesSA + kPiecesSB);
   static constexpr int kRound = 4 * TERMS;  // packages whose scales come in one word
@@ -184,7 +200,7 @@ __global__ __launch_bounds__(64 * S::kWaves) void k_mx_gemm(MxGemmArgs a) {
 #pragma unroll
     for (int i = 0; i < S::TM; i++) sa[i] = *(const uint32_t *)(ps + (wm * S::TM + i) * 256);
 #pragma unroll
-    for (int j = 0; j < S::TN; j++) sb[j] = *(const uint32_t *)(ps + S::kPiecesSA * 1024 + (wn * S::TN + j) * 256);
+    for (int j = 0; j < S::TN; j++) sb[j] = S::kPiecesSB ? *(const uint32_t *)(ps + S::kPiecesSA * 1024 + (wn * S::TN + j) * 256) : 0;
   };
 
   f32x4 acc[S::TM][S::TN];
@@ -217,9 +233,14 @@ __global__ __launch_bounds__(64 * S::kWaves) void k_mx_gemm(MxGemmArgs a) {
         for (int j = 0; j < S::TN; j++) sw[j] = term == 0 ? sb[j] >> 8 * step & 255 : (uint32_t)max((int)sw[j] - 5, 1);
       }
       constexpr int kB = S::kFmt == 4 ? 4 : S::kFmt == 6 ? 2 : 0, kAll = S::TM * S::TN, kHalf = kAll / 2;
+      bf16x8 w[S::kFmt == 16 ? S::TM : 1];
       auto mfma = [&](int p) {
         const int i = p % S::TM, j = p / S::TM;
-        if constexpr (S::kFmt == 6)
+        if constexpr (S::kFmt == 16) {
+          if (j == 0) w[i] = mx_weights8((uint32_t)A[step & 1][i][term], sa[i] >> 8 * step & 255);
+          const i32x8 &b = B[u & 1][j];
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], as_bf16x8(make_uint4(b[0], b[1], b[2], b[3])), acc[i][j], 0, 0, 0);
+        } else if constexpr (S::kFmt == 6)
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A[step & 1][i], B[u & 1][j], acc[i][j], 4, kB, step, (int)sa[i], 0, (int)sw[j]);
         else
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A[step & 1][i], B[u & 1][j], acc[i][j], 4, kB, step, (int)sa[i], step, (int)sb[j]);

@@ -12,11 +12,11 @@ namespace moe {
 
 hipError_t launch_mx4_quantize(const void *x, bool bf16, size_t n, size_t cols, uint8_t *blocks, uint8_t *scales, hipStream_t s);
 
-// What a product makes of its rows: tiles of 16 rows x steps of 128 values as the block-scaled MFMA's B operand
-// takes them. Step s of tile n lies at ((n ns + s) terms) * kRowChunk bytes, one chunk a term: lane l = 16 g + j holds
-// block 4 s + g of row 16 n + j, in planes of 16 (and 8 or 16) bytes a lane. Behind the tiles, a scale word per (tile, 4
-// steps, lane), byte i that of step 4 q + i: the weights' layout (layout.hpp). All terms share the
-// byte: an E2M3 term t's is 5 t below it, at least 1.
+// What a product makes of its rows: tiles of 16 rows x steps of 128 values as the MFMA's B operand takes them. Step s of tile n lies
+// at ((n ns + s) terms) * chunk bytes, one chunk a term: lane l = 16 g + j holds block 4 s + g of row 16 n + j, in planes of 16
+// (and 8 or 16) bytes a lane; bf16 rows' chunk is four planes of 8 values a lane. Behind the tiles (but of bf16 rows), a scale word per
+// (tile, 4 steps, lane), byte i that of step 4 q + i: the weights' layout (layout.hpp). All terms share the byte: an E2M3 term t's
+// is 5 t below it, at least 1.
 struct MxRows {
   int type;     // MOE_F32, MOE_BF16, MOE_MXFP8, MOE_MXFP4
   uint32_t tokens, nb, ns, nq, tiles;
@@ -30,12 +30,12 @@ inline MxRows mx_rows(int type, size_t tokens, size_t cols) {
   r.ns = (r.nb + 3) / 4;
   r.nq = (r.ns + 3) / 4;
   r.tiles = (uint32_t)((tokens + 15) / 16);
-  r.terms = type == MOE_F32 ? 6 : type == MOE_BF16 ? 4 : type == MOE_MXFP8 ? 2 : 1;
-  r.chunk = type == MOE_MXFP4 ? 1024 : type == MOE_MXFP8 ? 2048 : 1536;
+  r.terms = type == MOE_F32 ? 6 : type == MOE_MXFP8 ? 2 : 1;
+  r.chunk = type == MOE_MXFP4 ? 1024 : type == MOE_MXFP8 ? 2048 : type == MOE_BF16 ? 4096 : 1536;
   return r;
 }
 inline size_t mx_rows_code_bytes(const MxRows &r) { return (size_t)r.tiles * r.ns * r.terms * r.chunk; }
-inline size_t mx_rows_scale_bytes(const MxRows &r) { return (size_t)r.tiles * r.nq * 256; }
+inline size_t mx_rows_scale_bytes(const MxRows &r) { return r.type == MOE_BF16 ? 0 : (size_t)r.tiles * r.nq * 256; }
 hipError_t launch_mx_rows(const MxRows &r, const void *x, const uint8_t *x_scales, uint8_t *codes, uint32_t *scales, hipStream_t s);
 
 struct MxGemmArgs {
@@ -52,12 +52,12 @@ struct MxGemmArgs {
 hipError_t launch_mx_gemm(const MxGemmArgs &a, hipStream_t s);
 // The form for few rows (mx_few.hip).
 hipError_t launch_mx_few(const MxGemmArgs &a, hipStream_t s);
-// One to a few f32 or bf16 rows x, without MxRows (a.codes, a.scales): those whose terms fit the MFMA's 16 columns and 64 KB of LDS.
+// Few rows x without MxRows (a.codes, a.scales): bf16 rows, or the terms of f32 rows, that fit the MFMA's 16 columns and 64 KB of LDS.
+constexpr size_t mx_one_rows(size_t nb, size_t tokens) { return ((nb + 3) / 4 * 16 + 1) * 16 * tokens; }
 constexpr size_t mx_one_lds(size_t nb, size_t columns) { return (nb + 3) / 4 * 4 * columns * 28 + 8 * 64 * 16 + 1024; }
 inline bool mx_one_takes(int type, size_t tokens, size_t cols) {
-  if (type != MOE_F32 && type != MOE_BF16) return false;
-  const size_t columns = tokens * (type == MOE_F32 ? 6 : 4);
-  return columns <= 16 && mx_one_lds(cols / 32, columns) <= 64 * 1024;
+  if (type == MOE_BF16) return tokens <= 16 && mx_one_rows(cols / 32, tokens) + 16 * 1024 <= 64 * 1024;
+  return type == MOE_F32 && tokens <= 2 && mx_one_lds(cols / 32, 6 * tokens) <= 64 * 1024;
 }
 hipError_t launch_mx_one(const MxGemmArgs &a, const void *x, hipStream_t s);
 

@@ -51,6 +51,86 @@ def test_mxfp8_products_are_exact(d, T, R, C, dtype):  # noqa: F811
     assert (np.abs(got - want) <= tol).all(), np.max(np.abs(got - want) / tol)
 
 
+# ------------------------------------------------------------------ bf16 rows
+
+
+BF16_FORMS = FORMS + [(700, 2064, 160), (2000, 2880, 96), (5, 80, 1056), (16, 5760, 2880), (2, 16, 32), (1, 32768, 96), (4, 64, 8224), (17, 16, 96)]
+
+
+def bf16_rows(x):
+    """(bits, values)"""
+    return dense_ref.store(np.asarray(x, np.float32), MOE_BF16)
+
+
+@pytest.mark.parametrize("dtype", [MOE_F32, MOE_BF16])
+@pytest.mark.parametrize("T,R,C", BF16_FORMS)
+def test_bf16_rows_enter_as_they_are(d, T, R, C, dtype):  # noqa: F811
+    """Beside each block's one huge value, whose weight is 0, its neighbours of all sizes count in full: what is left are an f32 sum's
+    roundings, 8 an MFMA (4 MFMAs a step of 128), then the joins' and the output's."""
+    rng = np.random.default_rng([44, T, R, C])
+    x = rng.standard_normal((T, C)) * 2.0 ** rng.integers(-12, 3, (T, C))
+    at = 32 * np.arange(C // 32) + rng.integers(0, 32, C // 32)
+    x[:, at] = rng.choice([-1.0, 1.0], (T, C // 32)) * 2.0 ** rng.integers(8, 60, (T, C // 32))
+    stored, x = bf16_rows(x)
+    blocks, scales = weights(45, R, C)
+    byte = blocks.reshape(R, -1)
+    byte[:, at // 2] &= np.where(at % 2, 0x0F, 0xF0).astype(np.uint8)
+    w = ref.mx4_values(blocks, scales)
+    assert (w[:, at] == 0).all()
+    bias = rng.standard_normal(R).astype(np.float32)
+    want, mag = x @ w.T + bias, np.abs(x) @ np.abs(w).T
+    tol = (4 * -(-C // 128) + 8) * 2.0 ** -23 * mag + 2.0 ** -23 * (np.abs(want) + np.abs(bias)) + (dense_ref.u(dtype) + 2.0 ** -24) * np.abs(want)
+    got = matmul(d, resident(d, blocks, scales), R, C, bias, stored, MOE_BF16, None, T, dtype)
+    assert (np.abs(got - want) <= tol).all(), np.max(np.abs(got - want) / tol)
+
+
+@pytest.mark.parametrize("T", [16, 64, 333])
+def test_bf16_products_of_far_numbers(d, T):  # noqa: F811
+    """One value by one weight, exactly, from the smallest numbers of either to the largest: results below the normal numbers may be 0, above
+    the largest infinite."""
+    C = 32
+    R = 16 * 8 if T < 333 else 16 * 129
+    byte = np.array([0, 1, 2, 3, 127, 240, 252, 253])[np.arange(R) // 16 % 8].astype(np.uint8)
+    blocks = np.zeros((R, 1, 16), np.uint8)
+    blocks[:, 0, 3] = np.arange(R) % 16 << 4  # value 7
+    scales = byte[:, None]
+    numbers = [2.0 ** -133, 3 * 2.0 ** -133, 127 * 2.0 ** -133, 2.0 ** -126, 255 * 2.0 ** -133, 2.0 ** -100, 2.0 ** -20, 1.0, -1.9921875, 2.0 ** 50, 255 * 2.0 ** 120, -(2.0 ** -130)]
+    v = np.resize(np.array(numbers), T)
+    x = np.zeros((T, C))
+    x[:, 7] = v
+    x[:, 8] = 2.0 ** 90  # its weights are 0
+    stored, x = bf16_rows(x)
+    assert np.array_equal(x[:, 7], v)
+    got = matmul(d, resident(d, blocks, scales), R, C, None, stored, MOE_BF16, None, T, MOE_F32)
+    w = ref.mx4_values(blocks, scales)[:, 7]
+    want = v[:, None] * w
+    over = (np.abs(w) >= 2.0 ** 128)[None, :] | (np.abs(want) >= 2.0 ** 128)
+    assert not np.isfinite(got[over]).any()
+    small = np.abs(want) < 2.0 ** -126
+    assert np.array_equal(got[~over & ~small], want[~over & ~small])
+    assert (np.abs(got - want)[small & ~over] <= np.abs(want)[small & ~over]).all()
+
+
+@pytest.mark.parametrize("T,R", [(1, 16), (16, 48), (33, 32), (333, 2064), (1100, 2064), (2000, 2880), (3900, 3008)])
+def test_bf16_rows_that_are_not_finite(d, T, R):  # noqa: F811
+    """NaN, whatever the signs of what an infinity meets, and nothing of it in the other rows."""
+    C = 160
+    blocks = np.full((R, C // 32, 16), 0x22, np.uint8)  # all weights are 1
+    scales = np.full((R, C // 32), 127, np.uint8)
+    scales[5, 1] = 255
+    rng = np.random.default_rng([46, T])
+    x = np.abs(rng.integers(1, 5, (T, C))).astype(np.float64)
+    bad = {0: np.inf, T - 1: -np.inf, T // 2: np.nan}
+    clean = x.copy()
+    for t, v in bad.items():
+        x[t, rng.integers(0, C)] = v
+    got = matmul(d, resident(d, blocks, scales), R, C, None, bf16_rows(x)[0], MOE_BF16, None, T, MOE_F32)
+    want = np.broadcast_to(clean.sum(1)[:, None], (T, R)).copy()
+    want[list(bad)] = np.nan
+    want[:, 5] = np.nan
+    assert np.array_equal(got, want, equal_nan=True)
+
+
 # ------------------------------------------------------------------ sampling
 
 
