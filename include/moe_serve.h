@@ -105,11 +105,11 @@ typedef struct moe_sampling {
  * first in the vocabulary's order at which the sum of their probabilities passes u[t] (in [0, 1); below counts as 0,
  * 1 and above as the last). tokens [n_tokens]; logprob [n_tokens] (may be NULL): the logarithm of its
  * probability among those left, 0 where the temperature is not above 0. Probabilities are multiples of 2^-44 of the
- * largest (2^-(62 - log2 vocab) for a vocab above 2^18), their sums exact. A NaN logit counts as -inf, infinite ones
+ * largest (2^-(62 - log2 vocab), the logarithm rounded up, for a vocab above 2^18), their sums exact. A NaN logit counts as -inf, infinite ones
  * share the row; a row without a logit above -inf gives token -1, logprob NaN. Workspace: 57 KB a row and 21 bytes for every
  * 1024 logits, of 4096 rows at a time (fewer of a vocab above 2^23). Where more than 4096 logits have to be looked at for a
  * row's border (those within 1/64 of a temperature of it; of a top-k up to 2048 all that are not surely below its border) the
- * row takes longer. */
+ * row takes longer: of 201088 logits 1 to 2.6 ms. */
 int moe_sample_device(moe_ctx *ctx, const moe_sampling *rule, const float *logits, size_t ld, const float *u, size_t n_tokens,
                       size_t vocab, int32_t *tokens, float *logprob, void *stream);
 

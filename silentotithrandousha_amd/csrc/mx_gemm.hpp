@@ -37,7 +37,7 @@ __device__ __forceinline__ bool mx_not_finite(const uint4 &v) {
 }
 constexpr uint32_t kNan2 = 0x7FC07FC0u;  // two bf16
 
-// FMT: the rows' format (4 E2M1, 6 E2M3, 8 E4M3, 16 bf16: TERMS are the four eighths of a block).
+// FMT: the rows' format (4 E2M1, 6 E2M3, 8 E4M3, 16 bf16: TERMS are the four quarters of a block).
 template <int FMT, int TERMS, int MT_, int NT_, int WM_, int WN_, int DEPTH_>
 struct MxShape {
   static constexpr int kFmt = FMT, kTerms = TERMS, MT = MT_, NT = NT_, WM = WM_, WN = WN_, kDepth = DEPTH_;

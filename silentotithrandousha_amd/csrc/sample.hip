@@ -15,7 +15,8 @@
 // that top-k leaves; other rows sum masses by bin, and gather the bins that hold a border. Of a top-k well below the row's pieces
 // of 256 logits even the bins are those of the pieces' largest alone: no piece below the k-th of them holds one of the k, and
 // the second launch gathers from the few that may. What is gathered is sorted in LDS. Should it be more than kList tokens, the draw
-// goes through the row itself.
+// goes through the row itself, a workgroup a row: 201088 logits of deviation 1 under a temperature of 4 and a top-p of 0.6 take 0.98 ms (64 such
+// rows 1.8), all equal 2.6 ms.
 //
 // 256 rows of 201088 logits, of which half have a top-k of 20 to 400, half a top-p: 34, 50, 20 and 18 us. The first is bound by its 206
 // MB (6.1 TB/s), the second by the 64-bit arithmetic and LDS atomics of the rows without a small top-k, the third by reads through the
