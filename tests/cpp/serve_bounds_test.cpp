@@ -2,6 +2,7 @@
 //   serve_bounds_test shift   a row's masses sum up within 64 bits, and have as many bits as that leaves
 //   serve_bounds_test rows    rows of the widest vocabularies go in launches of less than 2^32 threads, each row once
 //   serve_bounds_test terms   a product's workspace: fewer tokens at a time of above 65536 columns
+//   serve_bounds_test alone   which products need no workspace, and so may be captured first
 #define main serve_calls_main
 #include "serve_calls_test.cpp"
 #undef main
@@ -64,6 +65,27 @@ void terms() {
       }
 }
 
+void alone() {
+  g_capturing = true;
+  auto one = [](int type, size_t T, size_t cols, bool none) {
+    g_work = DenseWork{};
+    const PackDims d = pack_dims(16, cols);
+    void *y = buffer(T * 64);
+    const int rc = moe_mxfp4_matmul_device(&g_ctx, device(pack_weight_bytes(d) + pack_scale_bytes(d)), 16, cols, nullptr, buffer(T * cols * 4), type,
+                                           device(T * cols), T, y, MOE_F32, nullptr);
+    check(rc == (none ? MOE_OK : MOE_ERR_STATE) && !g_work.p, "a product's workspace", T, cols);
+    if (none) whole(y, T * 64);
+  };
+  one(MOE_F32, 1, 32, true), one(MOE_F32, 1, 10624, true), one(MOE_F32, 2, 5248, true);
+  one(MOE_F32, 1, 10624 + 32, false), one(MOE_F32, 2, 5248 + 32, false), one(MOE_F32, 3, 32, false);
+  // rows of 2 cols, rounded up to 256, and 16 bytes: 48 KB in all
+  for (size_t T = 1; T <= 16; T++)
+    for (size_t cols = 32; cols <= 32768; cols += 32) one(MOE_BF16, T, cols, T * ((2 * cols + 255) / 256 * 256 + 16) <= 48 * 1024);
+  one(MOE_BF16, 17, 32, false);
+  one(MOE_MXFP8, 1, 32, false), one(MOE_MXFP4, 1, 32, false);
+  g_capturing = false;
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -76,6 +98,8 @@ int main(int argc, char **argv) {
     rows();
   else if (what == "terms")
     terms();
+  else if (what == "alone")
+    alone();
   else
     return 2;
   printf("wrong %d, faults %ld\n", wrong, g_faults);

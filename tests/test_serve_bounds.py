@@ -26,3 +26,7 @@ def test_launches_of_wide_rows(bounds):
 
 def test_workspace_of_wide_products(bounds):
     run(bounds, "terms")
+
+
+def test_products_without_a_workspace(bounds):
+    run(bounds, "alone")
